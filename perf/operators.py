@@ -98,8 +98,9 @@ def draw(rng):
         sequences = _log_between(rng, 1, max(1, min(128, most // longest)))
         new = 1
         if kind == "append":
+            sequences = min(sequences, max(1, most // (8 * page)))
             if rng.random() < 0.5:
-                new = _log_between(rng, 1, max(1, min(longest, 8192 // sequences)))
+                new = _log_between(rng, 1, max(1, min(longest, most // (8 * sequences))))
             case["interleaved"] = rng.random() < 0.3
         else:
             if rng.random() < 0.35:
