@@ -100,7 +100,7 @@ def draw(rng):
         if kind == "append":
             sequences = min(sequences, max(1, most // (8 * page)))
             if rng.random() < 0.5:
-                new = _log_between(rng, 1, max(1, min(longest, most // (8 * sequences))))
+                new = _log_between(rng, 1, max(1, min(longest, most // (20 * sequences))))
             case["interleaved"] = rng.random() < 0.3
         else:
             if rng.random() < 0.35:
