@@ -33,7 +33,7 @@ extern "C" {
 
 #define QM_OK                 0
 #define QM_ERR_NULL          -1 /* a required pointer is NULL                               */
-#define QM_ERR_SHAPE         -2 /* m, n or k negative, k odd, or a size overflows int32     */
+#define QM_ERR_SHAPE         -2 /* m, n or k negative, k odd, a size overflows int32, or a size the call does not take */
 #define QM_ERR_CONFIG        -3 /* cfg id unknown, or that config cannot run this shape     */
 #define QM_ERR_LAUNCH        -4 /* the HIP runtime refused the launch (see qm_last_hip_error) */
 #define QM_ERR_ALIGN         -5 /* C is not 4-byte aligned (a 16-bit output: 2-byte)         */
@@ -245,6 +245,92 @@ int qm_quantize_pack_i4(const void *x, int in_dtype, void *dst_packed, float *sc
 size_t qm_linear_workspace_bytes(int m, int n, int k, int in_dtype, int weight_align);
 int qm_linear_i4(const void *x, int in_dtype, const void *B, void *D, int m, int n, int k, const float *col_scale,
                  const void *bias, int out_dtype, void *stream, void *workspace, size_t workspace_bytes);
+
+/*
+ * 16-bit activations times packed int4 weights with a scale per group of K (no counterpart in the reference, whose
+ * activations are int4 too):
+ *   D[m][n] = round16( sum_g scale[n][g] * sum_{k in g} x[m][k] * B[n][k]  + bias[n] )
+ * x is [m, k] fp16 or bf16 (dtype: QM_IN_F16, QM_IN_BF16) with rows `x_stride` elements apart, B [n, k / 2] bytes as
+ * everywhere in this interface, scale [n, ceil(k / group)] row-major, float32 (scale_dtype = QM_IN_F32) or of x's type; groups
+ * are runs of `group` consecutive k, a multiple of 32, the last one shorter where k is no multiple of it.  bias is [n] of x's type or NULL,
+ * D [m, n] of x's type.  Sums are IEEE single precision, the weights take part as the integers they are; one rounding, at
+ * the end.  k is even (k == 0: D is the bias, or zero).  D must not overlap x.
+ *   workspace  16-byte aligned device memory of qm_gemm_grouped_workspace_bytes(...) bytes, used in stream order by the
+ *              kernels of this call only (align: the alignment in bytes that x, its rows and B share); QM_ERR_SCRATCH
+ *              with less, and nothing is enqueued
+ */
+size_t qm_gemm_grouped_workspace_bytes(int m, int n, int k, int group, int align);
+int qm_gemm_grouped_i4(const void *x, int dtype, long long x_stride, const void *B, const void *scale, int scale_dtype, int group,
+                       const void *bias, void *D, int m, int n, int k, void *stream, void *workspace, size_t workspace_bytes);
+
+/*
+ * A paged cache of keys and values in 8 bits, and attention over it (no counterpart in the reference).  A page holds
+ * `page_size` tokens of every head, as int8 codes with one float32 scale per page, head and side: the value is
+ * code * scale.  Codes of the values lie with the tokens of a channel together, which is the order the product with the
+ * attention weights reads them in.
+ *   k            [pages, kv_heads, page_size, head_dim]  int8, 16-byte aligned
+ *   v            [pages, kv_heads, head_dim, page_size]  int8, 16-byte aligned
+ *   scales       [pages, kv_heads, 2]                    float32, 8-byte aligned: of the keys, of the values
+ *   block_table  [sequences, table_width] int32: the page of tokens i * page_size to (i + 1) * page_size - 1 of a sequence; an
+ *                entry outside 0 .. pages - 1 is no page: what would be stored there is dropped, and attention passes over its tokens
+ *   lengths      [sequences] int32: tokens of a sequence, the new ones included (below 1: none)
+ *   query_start  [sequences + 1] int32: the new tokens of sequence s are rows query_start[s] to query_start[s + 1] - 1 of the
+ *                packed tensors; NULL: every sequence has tokens / sequences of them.  They are the last tokens of their
+ *                sequence: the last row is at position lengths[s] - 1.  Rows in front of position 0 are padding.
+ * page_size is 16, 32, 64 or 128; head_dim 64, 96, 128, 192 or 256.  All pointers are device pointers; what the last three hold is
+ * looked at by the kernels only, and no value of theirs makes one read or write outside the tensors.
+ */
+typedef struct qm_kv_cache {
+    void *k, *v;
+    float *scales;
+    int pages, kv_heads, page_size, head_dim;
+    const int *block_table, *lengths, *query_start;
+    int sequences, table_width;
+} qm_kv_cache;
+
+/*
+ * New keys and values into the cache, the keys rotated to their positions on the way; the queries, rotated, in the same call.
+ * Rotation of a head at position p, for pair i of rotary_pairs: (a, b) -> (a c - b s, b c + a s) with c = cos[p][i], s = sin[p][i]
+ * ([positions, rotary_pairs] float32); (a, b) are elements i and i + rotary_pairs, or 2i and 2i + 1 with interleaved = 1; further
+ * elements stay as they are; rotary_pairs = 0: no rotation.  A position at or past `positions` gives NaN.
+ * Storing, for each page, head and side, in single precision, every operation rounded by itself:
+ *   scale' = max(scale, amax * (1 / 127)), amax over the new tokens of the page; scale counts as 0 in a page
+ *            whose first token is new, which begins anew: all its other codes become 0
+ *   code   = clamp(rint(value * (1 / scale')), -127, 127); the codes that the page held become rint(code * (scale / scale')).
+ *            0 where scale' is below 2^-100.  Values that are not finite make scale' infinite or NaN, and attention to the page NaN.
+ * k and v are [tokens, kv_heads, head_dim] fp16 or bf16, q [tokens, heads, head_dim] or NULL, each with strides of its own (in
+ * elements) between tokens and between heads; q_out is [tokens, heads, head_dim] without gaps (rows of padding: 0) and may not overlap q.
+ * No two sequences may be given the same page to write to.  max_query: the most new tokens a sequence has, for the choice of the grid only: any
+ * value gives the same results.
+ */
+typedef struct qm_kv_new {
+    const void *k, *v, *q;
+    void *q_out;
+    long long k_token_stride, k_head_stride, v_token_stride, v_head_stride, q_token_stride, q_head_stride;
+    const float *cos, *sin;
+    int tokens, heads, dtype, rotary_pairs, positions, interleaved, max_query;
+} qm_kv_new;
+int qm_kv_append_i8(const qm_kv_cache *cache, const qm_kv_new *fresh, void *stream);
+
+/*
+ * Attention of the new tokens over the cache:
+ *   out[t][h] = sum_j softmax_j( scale * q[t][h] . key_j ) value_j
+ * over the tokens j of t's sequence with j <= position of t (causal = 1; else all lengths[s]) and, with window > 0, j > position - window.
+ * Heads of q share those of the cache in equal runs (heads a multiple of kv_heads).  A row that attends to nothing is 0.  Sums and softmax are
+ * in single precision.  q [tokens, heads, head_dim] fp16 or bf16 with strides in elements; out [tokens, heads, head_dim] of
+ * its type.  max_query and max_length: the most new tokens, and the most tokens, that a sequence has: for the choice of the
+ * grid only, any values give a right result.
+ *   workspace  16-byte aligned device memory of qm_kv_attend_workspace_bytes(...) bytes, used in stream order by the kernels of this
+ *              call only; QM_ERR_SCRATCH with less, and nothing is enqueued
+ */
+size_t qm_kv_attend_workspace_bytes(const qm_kv_cache *cache, int tokens, int heads, int max_query, int max_length);
+int qm_kv_attend_i8(const qm_kv_cache *cache, const void *q, int dtype, long long q_token_stride, long long q_head_stride, void *out,
+                    int tokens, int heads, float scale, int causal, int window, int max_query, int max_length, void *stream,
+                    void *workspace, size_t workspace_bytes);
+
+/* Pages back as fp16 or bf16 values: k and v [count, kv_heads, page_size, head_dim], both with the channels of a token together.
+ * page_ids is [count] int32 on the device; an id that is no page gives NaN.  Only k, v, scales and the sizes of `cache` are used. */
+int qm_kv_read_i8(const qm_kv_cache *cache, const int *page_ids, int count, int dtype, void *k, void *v, void *stream);
 
 /*
  * Optional: everything a first launch on the current device would otherwise do once -- the

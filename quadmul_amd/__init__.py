@@ -24,7 +24,7 @@ import torch
 
 __all__ = [
     "QuadmulError", "library", "library_path", "gemm", "gemm_cfg", "gemm_static", "gemm_scaled", "pack_int4", "unpack_int4",
-    "config_has_scaled", "quantize_pack",
+    "config_has_scaled", "quantize_pack", "quantize_groups", "gemm_grouped",
     "num_configs", "config_name", "config_names", "config_id", "select_config", "select_config_ex", "config_supports",
     "CFG_AUTO", "version", "init",
 ]
@@ -41,7 +41,22 @@ ABI_SYMBOLS = (
     "qm_gemm_i4_ws", "qm_gemm_i4_static", "qm_gemm_i4_scaled_ws", "qm_gemm_i4_scaled_bias_ws", "qm_gemm_workspace_bytes", "qm_gemm_recode_bytes", "qm_recode_config", "qm_quantize_pack_i4", "qm_select_config", "qm_select_config_ex", "qm_num_configs", "qm_config_name",
     "qm_config_supports", "qm_pack_i4", "qm_unpack_i4", "qm_status_string", "qm_last_hip_error", "qm_version", "qm_init",
     "qm_debug_set_operand_limit", "qm_linear_workspace_bytes", "qm_linear_i4",
+    "qm_gemm_grouped_workspace_bytes", "qm_gemm_grouped_i4", "qm_kv_append_i8", "qm_kv_attend_workspace_bytes", "qm_kv_attend_i8", "qm_kv_read_i8",
 )
+
+
+class KvCache(ctypes.Structure):
+    """``qm_kv_cache`` of include/qm_abi.h."""
+    _fields_ = ([(f, ctypes.c_void_p) for f in ("k", "v", "scales")] + [(f, ctypes.c_int) for f in ("pages", "kv_heads", "page_size", "head_dim")]
+                + [(f, ctypes.c_void_p) for f in ("block_table", "lengths", "query_start")] + [(f, ctypes.c_int) for f in ("sequences", "table_width")])
+
+
+class KvNew(ctypes.Structure):
+    """``qm_kv_new`` of include/qm_abi.h."""
+    _fields_ = ([(f, ctypes.c_void_p) for f in ("k", "v", "q", "q_out")]
+                + [(f, ctypes.c_longlong) for f in ("k_token_stride", "k_head_stride", "v_token_stride", "v_head_stride", "q_token_stride", "q_head_stride")]
+                + [(f, ctypes.c_void_p) for f in ("cos", "sin")]
+                + [(f, ctypes.c_int) for f in ("tokens", "heads", "dtype", "rotary_pairs", "positions", "interleaved", "max_query")])
 
 
 class QuadmulError(RuntimeError):
@@ -117,11 +132,24 @@ def library() -> ctypes.CDLL:
     lib.qm_version.restype = ctypes.c_char_p
     lib.qm_debug_set_operand_limit.argtypes = [ctypes.c_longlong]
     lib.qm_debug_set_operand_limit.restype = ctypes.c_longlong
+    ll, size, cache = ctypes.c_longlong, ctypes.c_size_t, ctypes.POINTER(KvCache)
+    lib.qm_gemm_grouped_workspace_bytes.argtypes = [ci, ci, ci, ci, ci]
+    lib.qm_gemm_grouped_workspace_bytes.restype = size
+    lib.qm_gemm_grouped_i4.argtypes = [vp, ci, ll, vp, vp, ci, ci, vp, vp, ci, ci, ci, vp, vp, size]
+    lib.qm_gemm_grouped_i4.restype = ci
+    lib.qm_kv_append_i8.argtypes = [cache, ctypes.POINTER(KvNew), vp]
+    lib.qm_kv_append_i8.restype = ci
+    lib.qm_kv_attend_workspace_bytes.argtypes = [cache, ci, ci, ci, ci]
+    lib.qm_kv_attend_workspace_bytes.restype = size
+    lib.qm_kv_attend_i8.argtypes = [cache, vp, ci, ll, ll, vp, ci, ci, ctypes.c_float, ci, ci, ci, ci, vp, vp, size]
+    lib.qm_kv_attend_i8.restype = ci
+    lib.qm_kv_read_i8.argtypes = [cache, vp, ci, ci, vp, vp, vp]
+    lib.qm_kv_read_i8.restype = ci
     _lib = lib
     return lib
 
 
-_EXT_FUNCTIONS = ("linear", "pack", "quantize_pack", "unpack")
+_EXT_FUNCTIONS = ("gemm_grouped", "kv_append", "kv_attend", "kv_read", "linear", "pack", "quantize_pack", "unpack")
 _ext = None  # the extension module, once looked for
 
 
@@ -138,6 +166,10 @@ def _extension():
         quadmul = types.SimpleNamespace(**dict.fromkeys(_EXT_FUNCTIONS, lambda *args: None))
     _ext = quadmul
     return _ext
+
+
+def _has_extension() -> bool:
+    return not isinstance(_extension() if _ext is None else _ext, types.SimpleNamespace)
 
 
 def _native(name: str, *args):
@@ -306,6 +338,56 @@ def quantize_pack(x: torch.Tensor):
         st = library().qm_quantize_pack_i4(x.data_ptr(), kind, packed.data_ptr(), scales.data_ptr(), rows, k, _stream_ptr(x))
     _check(st, "qm_quantize_pack_i4")
     return packed, scales
+
+
+def quantize_groups(weight: torch.Tensor, group_size: int = 128, scale_dtype: Optional[torch.dtype] = None):
+    """A float weight ``[n, k]`` (float16, bfloat16 or float32, on the GPU, ``k`` a multiple of ``group_size``) as
+    :func:`gemm_grouped` takes it: ``(packed int8 [n, k/2], scales [n, k/group_size])``, every group of consecutive k quantised as
+    :func:`quantize_pack` quantises a row. ``scale_dtype``: float32 (default), float16 or bfloat16; the integers are those of the
+    float32 scale whatever it is rounded to."""
+    if weight.dim() != 2 or group_size < 32 or group_size % 32 or weight.shape[1] % group_size:
+        raise QuadmulError("quantize_groups: expects [n, k] with k a multiple of the group size, and that of 32")
+    n, k = weight.shape
+    packed, scales = quantize_pack(weight.reshape(-1, group_size).contiguous())
+    scales = scales.reshape(n, k // group_size)
+    return packed.reshape(n, k // 2), scales if scale_dtype is None else scales.to(scale_dtype)
+
+
+def gemm_grouped(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, group_size: int, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``y[m, n] = round16(sum_g weight_scale[n, g] * sum_{k in g} x[m, k] * weight[n, k] + bias[n])``: 16-bit activations times packed
+    int4 weights with a scale per group of ``group_size`` consecutive k (no counterpart in the reference, whose activations are int4).
+
+    ``x`` [m, k] float16 or bfloat16, rows at any distance; ``weight`` [n, k/2] int8 or uint8; ``weight_scale`` [n, ceil(k/group_size)], float32
+    or ``x``'s type; ``group_size`` a multiple of 32; ``bias`` [n] of ``x``'s type. Sums are in float32 and rounded once. From one row (a token) to
+    thousands. Not differentiable."""
+    y = _native("gemm_grouped", x, weight, weight_scale, group_size, bias)
+    if y is not None:
+        return y
+    kinds = {torch.float16: 1, torch.bfloat16: 2, torch.float32: 3}
+    tensors = [t for t in (x, weight, weight_scale, bias) if t is not None]
+    if not (all(t.is_cuda and t.device == x.device for t in tensors) and all(t.dim() == 2 for t in tensors[:3])):
+        raise QuadmulError("gemm_grouped: x, weight and weight_scale must be 2-D GPU tensors on one device")
+    (m, k), n = x.shape, weight.shape[0]
+    if x.dtype not in (torch.float16, torch.bfloat16) or weight_scale.dtype not in (torch.float32, x.dtype):
+        raise QuadmulError("gemm_grouped: x must be float16 or bfloat16, the scales float32 or of x's type")
+    if k % 2 or not _is_byte(weight) or not weight.is_contiguous() or weight.shape[1] != k // 2:
+        raise QuadmulError("gemm_grouped: the weight must be a contiguous [n, k / 2] int8 or uint8 tensor, k even")
+    if group_size < 32 or group_size % 32 or not weight_scale.is_contiguous() or weight_scale.shape != (n, -(-k // group_size)):
+        raise QuadmulError("gemm_grouped: the group size must be a multiple of 32, the scales a contiguous [n, ceil(k / group)] tensor")
+    if bias is not None and not (bias.dtype == x.dtype and bias.is_contiguous() and bias.numel() == n):
+        raise QuadmulError(f"gemm_grouped: the bias must be a contiguous vector of {n} elements of x's type")
+    if (k > 1 and x.stride(1) != 1) or (m > 1 and x.stride(0) < k):
+        x = x.contiguous()
+    stride = x.stride(0) if m > 1 else k
+    y = torch.empty((m, n), dtype=x.dtype, device=x.device)
+    low = x.data_ptr() | weight.data_ptr() | (2 * stride)
+    need = library().qm_gemm_grouped_workspace_bytes(m, n, k, group_size, low & -low if low & 15 else 16)
+    scratch = torch.empty((need,), dtype=torch.uint8, device=x.device) if need else None
+    with torch.cuda.device(x.device):
+        st = library().qm_gemm_grouped_i4(x.data_ptr(), kinds[x.dtype], stride, weight.data_ptr(), weight_scale.data_ptr(), kinds[weight_scale.dtype], group_size,
+                                          None if bias is None else bias.data_ptr(), y.data_ptr(), m, n, k, _stream_ptr(x), scratch.data_ptr() if need else None, need)
+    _check(st, "qm_gemm_grouped_i4")
+    return y
 
 
 def config_has_scaled(cfg: int) -> bool:

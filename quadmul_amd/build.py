@@ -119,7 +119,9 @@ def build_lib(jobs: int = 8, verbose: bool = False) -> str:
                                "`pytest tests -m gpu` before trusting any result and add the compiler to VALIDATED_COMPILERS")
         print(f"quadmul_amd.build: WARNING: {msg}; run `pytest tests -m gpu` before trusting results", file=sys.stderr)
     units = [("qm_dispatch.o", [f'-DQM_COMPILER_VERSION="{ver}"', "-mllvm", "-amdgpu-kernarg-preload-count=16", "-c", os.path.join(CSRC, "qm_dispatch.hip")]),
-             ("qm_scratch.o", ["-c", os.path.join(CSRC, "qm_scratch.hip")])]
+             ("qm_scratch.o", ["-c", os.path.join(CSRC, "qm_scratch.hip")]),
+             ("qm_grouped.o", ["-c", os.path.join(CSRC, "qm_grouped.hip")]),
+             ("qm_kv.o", ["-c", os.path.join(CSRC, "qm_kv.hip")])]
     # (the units with the scaled-output kernels, 6 and up, take longest: they go first)
     units = [(f"qm_tile6_inst_{out}.o", [f"-DQM_TILE6_OUT={out}", "-c", os.path.join(CSRC, "qm_tile6_inst.hip")]) for out in (0, 1, 2)] + units
     units = [(f"qm_tile_inst_{tu}.o", [f"-DQM_TU={tu}", "-c", os.path.join(CSRC, "qm_tile_inst.hip")])

@@ -11,6 +11,7 @@
 #include <torch/library.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
@@ -220,6 +221,163 @@ torch::Tensor unpack(torch::Tensor packed)
     return out;
 }
 
+// 16-bit activations times packed int4 weights with a scale per group of K (include/qm_abi.h: qm_gemm_grouped_i4): a new [m, n]
+// tensor of x's type. x may have any distance between its rows.
+int float16_type(const torch::Tensor &t, const char *what)
+{
+    TORCH_CHECK(t.scalar_type() == torch::kFloat16 || t.scalar_type() == torch::kBFloat16, what, " must be float16 or bfloat16");
+    return t.scalar_type() == torch::kFloat16 ? QM_IN_F16 : QM_IN_BF16;
+}
+
+void check_grouped(const torch::Tensor &x, const torch::Tensor &weight, const torch::Tensor &weight_scale, int64_t group, const c10::optional<torch::Tensor> &bias)
+{
+    TORCH_CHECK(x.dim() == 2 && weight.dim() == 2 && weight_scale.dim() == 2, "quadmul.gemm_grouped: x, weight and weight_scale must be 2-D");
+    const int64_t m = x.size(0), k = x.size(1), n = weight.size(0);
+    TORCH_CHECK(m <= INT32_MAX && n <= INT32_MAX && k <= INT32_MAX, "quadmul.gemm_grouped: m, n, k must fit in int32");
+    TORCH_CHECK(is_byte(weight) && weight.is_contiguous() && k % 2 == 0 && weight.size(1) == k / 2,
+                "quadmul.gemm_grouped: the weight must be a contiguous [n, k / 2] int8 or uint8 tensor (packed int4), k = ", k, " even");
+    TORCH_CHECK(group >= 32 && group <= INT32_MAX && group % 32 == 0, "quadmul.gemm_grouped: the group size must be a multiple of 32, got ", group);
+    TORCH_CHECK(weight_scale.is_contiguous() && weight_scale.size(0) == n && weight_scale.size(1) == (k + group - 1) / group &&
+                    (weight_scale.scalar_type() == torch::kFloat32 || weight_scale.scalar_type() == x.scalar_type()),
+                "quadmul.gemm_grouped: the scales must be a contiguous [n, ceil(k / group)] tensor of float32 or of x's type");
+    TORCH_CHECK(x.device() == weight.device() && x.device() == weight_scale.device(), "quadmul.gemm_grouped: all tensors must be on the same device");
+    TORCH_CHECK(!bias.has_value() || (bias->device() == x.device() && bias->scalar_type() == x.scalar_type() && bias->is_contiguous() && bias->numel() == n),
+                "quadmul.gemm_grouped: the bias must be a contiguous vector of ", n, " elements of x's type on x's device");
+}
+
+torch::Tensor gemm_grouped(torch::Tensor x, torch::Tensor weight, torch::Tensor weight_scale, int64_t group, c10::optional<torch::Tensor> bias)
+{
+    TORCH_CHECK(x.is_cuda(), "quadmul.gemm_grouped: expects GPU tensors");
+    const int type = float16_type(x, "quadmul.gemm_grouped: x");
+    check_grouped(x, weight, weight_scale, group, bias);
+    const int64_t m = x.size(0), k = x.size(1), n = weight.size(0);
+    c10::OptionalDeviceGuard guard(x.device());
+    if ((k > 1 && x.stride(1) != 1) || (m > 1 && x.stride(0) < k)) x = x.contiguous();
+    auto y = torch::empty({m, n}, x.options());
+    const int64_t stride = m > 1 ? x.stride(0) : k;
+    const uintptr_t low = reinterpret_cast<uintptr_t>(x.data_ptr()) | reinterpret_cast<uintptr_t>(weight.data_ptr()) | (uintptr_t)(2 * stride);
+    const size_t need = qm_gemm_grouped_workspace_bytes((int)m, (int)n, (int)k, (int)group, low & 15 ? (int)(low & (~low + 1)) : 16);
+    torch::Tensor scratch;
+    if (need > 0) scratch = torch::empty({(int64_t)need}, x.options().dtype(torch::kUInt8));
+    check_status(qm_gemm_grouped_i4(x.data_ptr(), type, stride, weight.data_ptr(), weight_scale.data_ptr(), weight_scale.scalar_type() == torch::kFloat32 ? QM_IN_F32 : type,
+                                    (int)group, bias.has_value() ? bias->data_ptr() : nullptr, y.data_ptr(), (int)m, (int)n, (int)k, stream_of(x),
+                                    need > 0 ? scratch.data_ptr() : nullptr, need),
+                 "quadmul.gemm_grouped");
+    return y;
+}
+
+// The paged cache in 8 bits: three tensors (codes of the keys and of the values, scales) and what says where a sequence's tokens
+// are in them, checked and put together for the C interface.
+qm_kv_cache kv_cache(const char *what, const torch::Tensor &k, const torch::Tensor &v, const torch::Tensor &scales)
+{
+    TORCH_CHECK(k.is_cuda() && k.device() == v.device() && k.device() == scales.device(), what, ": the cache must be GPU tensors on one device");
+    TORCH_CHECK(k.dim() == 4 && v.dim() == 4 && k.scalar_type() == torch::kInt8 && v.scalar_type() == torch::kInt8 && k.is_contiguous() && v.is_contiguous(), what,
+                ": the codes must be contiguous int8 tensors, [pages, kv_heads, page_size, head_dim] of the keys and [pages, kv_heads, head_dim, page_size] of the values");
+    const int64_t pages = k.size(0), heads = k.size(1), page = k.size(2), dim = k.size(3);
+    TORCH_CHECK(v.size(0) == pages && v.size(1) == heads && v.size(2) == dim && v.size(3) == page, what,
+                ": the codes of the values must be [pages, kv_heads, head_dim, page_size], of the same sizes as the keys'");
+    TORCH_CHECK(scales.scalar_type() == torch::kFloat32 && scales.is_contiguous() && scales.dim() == 3 && scales.size(0) == pages && scales.size(1) == heads &&
+                    scales.size(2) == 2, what, ": the scales must be a contiguous float32 tensor [pages, kv_heads, 2]");
+    TORCH_CHECK(page == 16 || page == 32 || page == 64 || page == 128, what, ": the page size must be 16, 32, 64 or 128, got ", page);
+    TORCH_CHECK(dim == 64 || dim == 96 || dim == 128 || dim == 192 || dim == 256, what, ": the head dimension must be 64, 96, 128, 192 or 256, got ", dim);
+    TORCH_CHECK(pages <= INT32_MAX && heads >= 1 && heads <= 4096, what, ": at most 2^31 - 1 pages, and 1 to 4096 heads");
+    qm_kv_cache c{};
+    c.k = k.data_ptr(), c.v = v.data_ptr(), c.scales = scales.data_ptr<float>();
+    c.pages = (int)pages, c.kv_heads = (int)heads, c.page_size = (int)page, c.head_dim = (int)dim;
+    return c;
+}
+
+void kv_sequences(const char *what, qm_kv_cache &c, const torch::Tensor &k, const torch::Tensor &table, const torch::Tensor &lengths,
+                  const c10::optional<torch::Tensor> &start, int64_t tokens)
+{
+    const auto ints = [&](const torch::Tensor &t, int64_t dims) { return t.device() == k.device() && t.scalar_type() == torch::kInt32 && t.dim() == dims && t.is_contiguous(); };
+    TORCH_CHECK(ints(table, 2) && ints(lengths, 1) && table.size(0) == lengths.size(0), what,
+                ": block_table [sequences, width] and lengths [sequences] must be contiguous int32 tensors on the cache's device");
+    const int64_t sequences = lengths.size(0);
+    TORCH_CHECK(!start.has_value() || (ints(*start, 1) && start->size(0) == sequences + 1), what,
+                ": query_start must be a contiguous int32 tensor of sequences + 1 elements on the cache's device");
+    TORCH_CHECK(sequences <= INT32_MAX && table.size(1) <= INT32_MAX && tokens <= INT32_MAX, what, ": sizes must fit in int32");
+    TORCH_CHECK(tokens == 0 || (sequences > 0 && (start.has_value() || tokens % sequences == 0)), what,
+                ": ", tokens, " tokens of ", sequences, " sequences need a query_start");
+    c.block_table = table.data_ptr<int>(), c.lengths = lengths.data_ptr<int>(), c.query_start = start.has_value() ? start->data_ptr<int>() : nullptr;
+    c.sequences = (int)sequences, c.table_width = (int)table.size(1);
+}
+
+int clamped(int64_t v) { return (int)std::min<int64_t>(std::max<int64_t>(v, 0), INT32_MAX); }
+
+c10::optional<torch::Tensor> kv_append(torch::Tensor k, torch::Tensor v, torch::Tensor cache_k, torch::Tensor cache_v, torch::Tensor scales, torch::Tensor block_table,
+                                       torch::Tensor lengths, c10::optional<torch::Tensor> query_start, c10::optional<torch::Tensor> q, c10::optional<torch::Tensor> cos,
+                                       c10::optional<torch::Tensor> sin, bool interleaved, int64_t max_query)
+{
+    const char *const what = "quadmul.kv_append";
+    qm_kv_cache c = kv_cache(what, cache_k, cache_v, scales);
+    const int type = float16_type(k, "quadmul.kv_append: the keys");
+    const auto row = [&](const torch::Tensor &t) { return t.device() == cache_k.device() && t.scalar_type() == k.scalar_type() && t.dim() == 3 && t.size(2) == c.head_dim && (t.stride(2) == 1 || t.numel() == 0); };
+    TORCH_CHECK(row(k) && row(v) && k.sizes() == v.sizes() && k.size(1) == c.kv_heads, what, ": keys and values must be [tokens, ", c.kv_heads, ", ", c.head_dim,
+                "] of one type on the cache's device, the last dimension contiguous");
+    const int64_t tokens = k.size(0);
+    kv_sequences(what, c, cache_k, block_table, lengths, query_start, tokens);
+    TORCH_CHECK(!q.has_value() || (row(*q) && q->size(0) == tokens && q->size(1) >= 1 && q->size(1) <= INT32_MAX), what, ": the queries must be [", tokens, ", heads, ",
+                c.head_dim, "] of the keys' type on the cache's device, the last dimension contiguous");
+    TORCH_CHECK(cos.has_value() == sin.has_value(), what, ": cos and sin go together");
+    if (cos.has_value()) {
+        const auto table = [&](const torch::Tensor &t) { return t.device() == cache_k.device() && t.scalar_type() == torch::kFloat32 && t.dim() == 2 && t.is_contiguous(); };
+        TORCH_CHECK(table(*cos) && table(*sin) && cos->sizes() == sin->sizes() && 2 * cos->size(1) <= c.head_dim && cos->size(0) <= INT32_MAX, what,
+                    ": cos and sin must be contiguous float32 tensors [positions, at most ", c.head_dim / 2, "] on the cache's device");
+    }
+    c10::OptionalDeviceGuard guard(cache_k.device());
+    c10::optional<torch::Tensor> out;
+    qm_kv_new n{};
+    if (q.has_value()) {
+        out = torch::empty({tokens, q->size(1), q->size(2)}, q->options());
+        n.q = q->data_ptr(), n.q_out = out->data_ptr(), n.heads = (int)q->size(1), n.q_token_stride = q->stride(0), n.q_head_stride = q->stride(1);
+    }
+    n.k = k.data_ptr(), n.v = v.data_ptr();
+    n.k_token_stride = k.stride(0), n.k_head_stride = k.stride(1), n.v_token_stride = v.stride(0), n.v_head_stride = v.stride(1);
+    if (cos.has_value()) n.cos = cos->data_ptr<float>(), n.sin = sin->data_ptr<float>(), n.rotary_pairs = (int)cos->size(1), n.positions = (int)cos->size(0);
+    n.tokens = (int)tokens, n.dtype = type, n.interleaved = interleaved ? 1 : 0, n.max_query = clamped(max_query);
+    check_status(qm_kv_append_i8(&c, &n, stream_of(cache_k)), what);
+    return out;
+}
+
+torch::Tensor kv_attend(torch::Tensor q, torch::Tensor cache_k, torch::Tensor cache_v, torch::Tensor scales, torch::Tensor block_table, torch::Tensor lengths,
+                        c10::optional<torch::Tensor> query_start, c10::optional<double> scale, bool causal, int64_t window, int64_t max_query, int64_t max_length)
+{
+    const char *const what = "quadmul.kv_attend";
+    qm_kv_cache c = kv_cache(what, cache_k, cache_v, scales);
+    const int type = float16_type(q, "quadmul.kv_attend: the queries");
+    TORCH_CHECK(q.device() == cache_k.device() && q.dim() == 3 && q.size(2) == c.head_dim && (q.stride(2) == 1 || q.numel() == 0), what, ": the queries must be [tokens, heads, ", c.head_dim,
+                "] on the cache's device, the last dimension contiguous");
+    const int64_t tokens = q.size(0), heads = q.size(1);
+    TORCH_CHECK(heads >= 1 && heads <= 65535 && heads % c.kv_heads == 0, what, ": the heads of the queries must be a multiple of the cache's ", c.kv_heads, ", got ", heads);
+    TORCH_CHECK(window >= 0, what, ": the window must be 0 (none) or more tokens");
+    kv_sequences(what, c, cache_k, block_table, lengths, query_start, tokens);
+    c10::OptionalDeviceGuard guard(cache_k.device());
+    auto out = torch::empty({tokens, heads, (int64_t)c.head_dim}, q.options());
+    const int most = clamped(max_query), longest = clamped(max_length);
+    const size_t need = qm_kv_attend_workspace_bytes(&c, (int)tokens, (int)heads, most, longest);
+    torch::Tensor scratch;
+    if (need > 0) scratch = torch::empty({(int64_t)need}, q.options().dtype(torch::kUInt8));
+    check_status(qm_kv_attend_i8(&c, q.data_ptr(), type, q.stride(0), q.stride(1), out.data_ptr(), (int)tokens, (int)heads,
+                                 scale.has_value() ? (float)*scale : (float)(1.0 / std::sqrt((double)c.head_dim)), causal ? 1 : 0, clamped(window), most, longest,
+                                 stream_of(cache_k), need > 0 ? scratch.data_ptr() : nullptr, need),
+                 what);
+    return out;
+}
+
+std::tuple<torch::Tensor, torch::Tensor> kv_read(torch::Tensor cache_k, torch::Tensor cache_v, torch::Tensor scales, torch::Tensor pages, bool bf16)
+{
+    const char *const what = "quadmul.kv_read";
+    const qm_kv_cache c = kv_cache(what, cache_k, cache_v, scales);
+    TORCH_CHECK(pages.device() == cache_k.device() && pages.scalar_type() == torch::kInt32 && pages.dim() == 1 && pages.is_contiguous() && pages.size(0) <= INT32_MAX, what,
+                ": the pages must be a contiguous int32 vector on the cache's device");
+    c10::OptionalDeviceGuard guard(cache_k.device());
+    const auto options = cache_k.options().dtype(bf16 ? torch::kBFloat16 : torch::kFloat16);
+    auto k = torch::empty({pages.size(0), c.kv_heads, c.page_size, c.head_dim}, options), v = torch::empty_like(k);
+    check_status(qm_kv_read_i8(&c, pages.data_ptr<int>(), (int)pages.size(0), bf16 ? QM_IN_BF16 : QM_IN_F16, k.data_ptr(), v.data_ptr(), stream_of(cache_k)), what);
+    return {k, v};
+}
+
 // Dispatcher-visible form of the same op (schema + mutation annotation), so that callers
 // under torch.compile / export can keep `torch.ops.quadmul.gemm(a, b, c, m, n, k)` in the
 // graph.  The reference has only the pybind function (extension.cpp:26-29), which a tracer
@@ -242,6 +400,49 @@ std::tuple<torch::Tensor, torch::Tensor> quantize_pack_meta(const torch::Tensor 
 }
 std::tuple<torch::Tensor, torch::Tensor> quantize_pack_op(const torch::Tensor &x) { return quantize_pack(x); }
 
+torch::Tensor gemm_grouped_op(const torch::Tensor &x, const torch::Tensor &weight, const torch::Tensor &weight_scale, int64_t group, const c10::optional<torch::Tensor> &bias)
+{
+    return gemm_grouped(x, weight, weight_scale, group, bias);
+}
+torch::Tensor gemm_grouped_meta(const torch::Tensor &x, const torch::Tensor &weight, const torch::Tensor &weight_scale, int64_t group, const c10::optional<torch::Tensor> &bias)
+{
+    float16_type(x, "quadmul.gemm_grouped: x");
+    check_grouped(x, weight, weight_scale, group, bias);
+    return torch::empty({x.size(0), weight.size(0)}, x.options());
+}
+
+// (two schemas: an operator whose result is None has no schema that every tracer takes)
+void kv_append_op(const torch::Tensor &k, const torch::Tensor &v, torch::Tensor &cache_k, torch::Tensor &cache_v, torch::Tensor &scales, const torch::Tensor &block_table,
+                  const torch::Tensor &lengths, const c10::optional<torch::Tensor> &query_start, const c10::optional<torch::Tensor> &cos,
+                  const c10::optional<torch::Tensor> &sin, bool interleaved, int64_t max_query)
+{
+    kv_append(k, v, cache_k, cache_v, scales, block_table, lengths, query_start, c10::nullopt, cos, sin, interleaved, max_query);
+}
+void kv_append_meta(const torch::Tensor &, const torch::Tensor &, torch::Tensor &, torch::Tensor &, torch::Tensor &, const torch::Tensor &, const torch::Tensor &,
+                    const c10::optional<torch::Tensor> &, const c10::optional<torch::Tensor> &, const c10::optional<torch::Tensor> &, bool, int64_t) {}
+torch::Tensor kv_append_rotate_op(const torch::Tensor &q, const torch::Tensor &k, const torch::Tensor &v, torch::Tensor &cache_k, torch::Tensor &cache_v, torch::Tensor &scales,
+                                  const torch::Tensor &block_table, const torch::Tensor &lengths, const c10::optional<torch::Tensor> &query_start,
+                                  const c10::optional<torch::Tensor> &cos, const c10::optional<torch::Tensor> &sin, bool interleaved, int64_t max_query)
+{
+    return *kv_append(k, v, cache_k, cache_v, scales, block_table, lengths, query_start, q, cos, sin, interleaved, max_query);
+}
+torch::Tensor kv_append_rotate_meta(const torch::Tensor &q, const torch::Tensor &, const torch::Tensor &, torch::Tensor &, torch::Tensor &, torch::Tensor &, const torch::Tensor &,
+                                    const torch::Tensor &, const c10::optional<torch::Tensor> &, const c10::optional<torch::Tensor> &, const c10::optional<torch::Tensor> &, bool, int64_t)
+{
+    return torch::empty(q.sizes(), q.options());
+}
+torch::Tensor kv_attend_op(const torch::Tensor &q, const torch::Tensor &cache_k, const torch::Tensor &cache_v, const torch::Tensor &scales, const torch::Tensor &block_table,
+                           const torch::Tensor &lengths, const c10::optional<torch::Tensor> &query_start, c10::optional<double> scale, bool causal, int64_t window,
+                           int64_t max_query, int64_t max_length)
+{
+    return kv_attend(q, cache_k, cache_v, scales, block_table, lengths, query_start, scale, causal, window, max_query, max_length);
+}
+torch::Tensor kv_attend_meta(const torch::Tensor &q, const torch::Tensor &, const torch::Tensor &, const torch::Tensor &, const torch::Tensor &, const torch::Tensor &,
+                             const c10::optional<torch::Tensor> &, c10::optional<double>, bool, int64_t, int64_t, int64_t)
+{
+    return torch::empty(q.sizes(), q.options());
+}
+
 }  // namespace
 
 TORCH_LIBRARY(quadmul, m)
@@ -249,18 +450,33 @@ TORCH_LIBRARY(quadmul, m)
     m.def("gemm(Tensor a, Tensor b, Tensor(c!) c, int m, int n, int k) -> ()");
     m.def("gemm_scaled(Tensor a, Tensor b, Tensor(d!) d, int m, int n, int k, Tensor? row_scale, Tensor? col_scale) -> ()");
     m.def("quantize_pack(Tensor x) -> (Tensor, Tensor)");
+    m.def("gemm_grouped(Tensor x, Tensor weight, Tensor weight_scale, int group_size, Tensor? bias) -> Tensor");
+    m.def("kv_append(Tensor k, Tensor v, Tensor(a!) cache_k, Tensor(b!) cache_v, Tensor(c!) scales, Tensor block_table, Tensor lengths, Tensor? query_start, "
+          "Tensor? cos, Tensor? sin, bool interleaved, int max_query) -> ()");
+    m.def("kv_append_rotate(Tensor q, Tensor k, Tensor v, Tensor(a!) cache_k, Tensor(b!) cache_v, Tensor(c!) scales, Tensor block_table, Tensor lengths, "
+          "Tensor? query_start, Tensor? cos, Tensor? sin, bool interleaved, int max_query) -> Tensor");
+    m.def("kv_attend(Tensor q, Tensor cache_k, Tensor cache_v, Tensor scales, Tensor block_table, Tensor lengths, Tensor? query_start, float? scale, bool causal, "
+          "int window, int max_query, int max_length) -> Tensor");
 }
 TORCH_LIBRARY_IMPL(quadmul, CUDA, m)
 {
     m.impl("gemm", &gemm_op);
     m.impl("gemm_scaled", &gemm_scaled_op);
     m.impl("quantize_pack", &quantize_pack_op);
+    m.impl("gemm_grouped", &gemm_grouped_op);
+    m.impl("kv_append", &kv_append_op);
+    m.impl("kv_append_rotate", &kv_append_rotate_op);
+    m.impl("kv_attend", &kv_attend_op);
 }
 TORCH_LIBRARY_IMPL(quadmul, Meta, m)
 {
     m.impl("gemm", &gemm_meta);
     m.impl("gemm_scaled", &gemm_scaled_meta);
     m.impl("quantize_pack", &quantize_pack_meta);
+    m.impl("gemm_grouped", &gemm_grouped_meta);
+    m.impl("kv_append", &kv_append_meta);
+    m.impl("kv_append_rotate", &kv_append_rotate_meta);
+    m.impl("kv_attend", &kv_attend_meta);
 }
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
@@ -273,6 +489,15 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
     using nogil = py::call_guard<py::gil_scoped_release>;
     m.def("linear", &linear, "W4A4 linear layer: quantise + pack the rows of x, GEMM with scaled 16-bit float output, bias", py::arg("x"), py::arg("weight"),
           py::arg("out_features"), py::arg("weight_scale"), py::arg("bias"), py::arg("bf16"), nogil());
+    m.def("gemm_grouped", &gemm_grouped, "16-bit activations x packed int4 weights with a scale per group of K", py::arg("x"), py::arg("weight"), py::arg("weight_scale"),
+          py::arg("group_size"), py::arg("bias") = py::none(), nogil());
+    m.def("kv_append", &kv_append, "New keys and values into the paged 8-bit cache, rotated on the way; returns the rotated queries", py::arg("k"), py::arg("v"),
+          py::arg("cache_k"), py::arg("cache_v"), py::arg("scales"), py::arg("block_table"), py::arg("lengths"), py::arg("query_start") = py::none(), py::arg("q") = py::none(),
+          py::arg("cos") = py::none(), py::arg("sin") = py::none(), py::arg("interleaved") = false, py::arg("max_query") = 0, nogil());
+    m.def("kv_attend", &kv_attend, "Attention over the paged 8-bit cache", py::arg("q"), py::arg("cache_k"), py::arg("cache_v"), py::arg("scales"), py::arg("block_table"),
+          py::arg("lengths"), py::arg("query_start") = py::none(), py::arg("scale") = py::none(), py::arg("causal") = true, py::arg("window") = 0, py::arg("max_query") = 0,
+          py::arg("max_length") = 0, nogil());
+    m.def("kv_read", &kv_read, "Pages of the 8-bit cache as 16-bit floats", py::arg("cache_k"), py::arg("cache_v"), py::arg("scales"), py::arg("pages"), py::arg("bf16"), nogil());
     m.def("pack", &pack, nogil(), "Pack a [rows, K] int8 tensor of int4 values into [rows, K/2] bytes on the GPU");
     m.def("quantize_pack", &quantize_pack, nogil(), "Per-row symmetric int4 quantisation of a [rows, K] float tensor, packed; returns (packed, scales)");
     m.def("unpack", &unpack, nogil(), "Unpack [rows, K/2] bytes into a [rows, K] int8 tensor on the GPU");

@@ -125,7 +125,7 @@ static int check_gemm_args(const void *A, const void *B, void *C, int m, int n, 
     return QM_OK;
 }
 
-static int fail_launch(hipError_t e)
+int fail_launch(hipError_t e)
 {
     g_last_hip_error = (int)e;
     return QM_ERR_LAUNCH;

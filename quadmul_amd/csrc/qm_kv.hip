@@ -1,0 +1,114 @@
+// C entries of the paged 8-bit cache (include/qm_abi.h): argument checks and launches.
+#include <algorithm>
+#include <climits>
+
+#include "qm_launch.hpp"
+#include "qm_kv.hpp"
+#include "qm_attend.hpp"
+
+#define QM_EXPORT extern "C" __attribute__((visibility("default")))
+
+namespace qm {
+
+static bool dim_ok(int dim) { return dim == 64 || dim == 96 || dim == 128 || dim == 192 || dim == 256; }
+
+// What every call checks of the cache; `tables`: the call looks at the sequences too.
+static int check_cache(const qm_kv_cache *c, bool tables)
+{
+    if (!c) return QM_ERR_NULL;
+    if (c->pages < 0 || c->kv_heads < 1 || c->kv_heads > 4096 || !dim_ok(c->head_dim)) return QM_ERR_SHAPE;
+    if (c->page_size != 16 && c->page_size != 32 && c->page_size != 64 && c->page_size != 128) return QM_ERR_SHAPE;
+    if (c->pages > 0 && (!c->k || !c->v || !c->scales)) return QM_ERR_NULL;
+    if ((((uintptr_t)c->k | (uintptr_t)c->v) & 15) || ((uintptr_t)c->scales & 7)) return QM_ERR_ALIGN;
+    if (!tables) return QM_OK;
+    if (c->sequences < 0 || c->table_width < 0) return QM_ERR_SHAPE;
+    if (c->sequences > 0 && (!c->lengths || (c->table_width > 0 && !c->block_table))) return QM_ERR_NULL;
+    if (((uintptr_t)c->block_table | (uintptr_t)c->lengths | (uintptr_t)c->query_start) & 3) return QM_ERR_ALIGN;
+    return QM_OK;
+}
+static int check_tokens(const qm_kv_cache *c, int tokens)
+{
+    if (tokens < 0 || (tokens > 0 && c->sequences == 0)) return QM_ERR_SHAPE;
+    return !c->query_start && c->sequences > 0 && tokens % c->sequences != 0 ? QM_ERR_SHAPE : QM_OK;
+}
+static KvArgs kv_args(const qm_kv_cache *c, int tokens)
+{
+    return {static_cast<int8_t *>(c->k), static_cast<int8_t *>(c->v), c->scales, c->block_table, c->lengths, c->query_start, c->pages, c->kv_heads,
+            c->page_size, c->head_dim, c->sequences, c->table_width, tokens, c->sequences > 0 ? tokens / c->sequences : 0};
+}
+// The most new tokens of a sequence: what the caller says, inside what is possible.
+static int most_new(const qm_kv_cache *c, int tokens, int max_query)
+{
+    const int most = c->query_start ? tokens : tokens / std::max(c->sequences, 1);
+    return std::max(1, c->query_start && max_query > 0 ? std::min(max_query, most) : most);
+}
+
+}  // namespace qm
+
+using namespace qm;
+
+QM_EXPORT int qm_kv_append_i8(const qm_kv_cache *cache, const qm_kv_new *fresh, void *stream)
+{
+    int st = check_cache(cache, true);
+    if (st != QM_OK) return st;
+    if (!fresh) return QM_ERR_NULL;
+    const qm_kv_new &n = *fresh;
+    if (n.dtype != QM_IN_F16 && n.dtype != QM_IN_BF16) return QM_ERR_DTYPE;
+    if ((st = check_tokens(cache, n.tokens)) != QM_OK) return st;
+    if (n.rotary_pairs < 0 || n.rotary_pairs > cache->head_dim / 2 || n.positions < 0 || (n.q && n.heads < 1)) return QM_ERR_SHAPE;
+    if (n.tokens == 0) return QM_OK;
+    if (!n.k || !n.v || (n.q && !n.q_out) || (n.rotary_pairs > 0 && (!n.cos || !n.sin))) return QM_ERR_NULL;
+    if ((((uintptr_t)n.k | (uintptr_t)n.v | (uintptr_t)n.q | (uintptr_t)n.q_out) & 1) || (((uintptr_t)n.cos | (uintptr_t)n.sin) & 3)) return QM_ERR_ALIGN;
+    const KvArgs c = kv_args(cache, n.tokens);
+    const KvNewArgs f{static_cast<const uint16_t *>(n.k), static_cast<const uint16_t *>(n.v), static_cast<const uint16_t *>(n.q), static_cast<uint16_t *>(n.q_out),
+                      n.k_token_stride, n.k_head_stride, n.v_token_stride, n.v_head_stride, n.q_token_stride, n.q_head_stride, n.cos, n.sin, n.heads,
+                      n.rotary_pairs, n.positions, n.interleaved ? 1 : 0};
+    const int most = most_new(cache, n.tokens, n.max_query), slots = std::min((most + c.page - 2) / c.page + 1, 4096);
+    const long long items = n.q ? (long long)most * n.heads * (c.dim / 2) : 0;
+    const int q_slots = (int)std::min<long long>((items + 2 * c.kv_heads * 256 - 1) / (2 * c.kv_heads * 256), 4096);
+    const dim3 grid(slots + q_slots, 2 * c.kv_heads, std::min(c.sequences, 65535));
+    hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    const auto kernel = n.dtype == QM_IN_F16 ? &kv_append_kernel<QM_IN_F16> : &kv_append_kernel<QM_IN_BF16>;
+    const hipError_t e = enqueue(kernel, grid, dim3(256), (size_t)c.page * c.dim, s, c, f, slots);
+    return e == hipSuccess ? QM_OK : fail_launch(e);
+}
+
+QM_EXPORT size_t qm_kv_attend_workspace_bytes(const qm_kv_cache *, int, int, int, int) { return 0; }
+
+QM_EXPORT int qm_kv_attend_i8(const qm_kv_cache *cache, const void *q, int dtype, long long q_token_stride, long long q_head_stride, void *out, int tokens,
+                              int heads, float scale, int causal, int window, int max_query, int max_length, void *stream, void *workspace,
+                              size_t workspace_bytes)
+{
+    int st = check_cache(cache, true);
+    if (st != QM_OK) return st;
+    if (dtype != QM_IN_F16 && dtype != QM_IN_BF16) return QM_ERR_DTYPE;
+    if ((st = check_tokens(cache, tokens)) != QM_OK) return st;
+    if (heads < 1 || heads > 65535 || heads % cache->kv_heads != 0 || window < 0) return QM_ERR_SHAPE;
+    if (tokens == 0) return QM_OK;
+    if (!q || !out) return QM_ERR_NULL;
+    if ((((uintptr_t)q | (uintptr_t)out) & 1) || ((uintptr_t)workspace & 15)) return QM_ERR_ALIGN;
+    if (workspace_bytes < qm_kv_attend_workspace_bytes(cache, tokens, heads, max_query, max_length)) return QM_ERR_SCRATCH;
+    const KvArgs c = kv_args(cache, tokens);
+    const AttendArgs a{static_cast<const uint16_t *>(q), static_cast<uint16_t *>(out), q_token_stride, q_head_stride, heads, causal ? 1 : 0, window, scale};
+    hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    const auto kernel = dtype == QM_IN_F16 ? &kv_attend_kernel<QM_IN_F16> : &kv_attend_kernel<QM_IN_BF16>;
+    const hipError_t e = enqueue(kernel, dim3(std::min(tokens, 1 << 20), heads), dim3(256), 0, s, c, a);
+    return e == hipSuccess ? QM_OK : fail_launch(e);
+}
+
+QM_EXPORT int qm_kv_read_i8(const qm_kv_cache *cache, const int *page_ids, int count, int dtype, void *k, void *v, void *stream)
+{
+    const int st = check_cache(cache, false);
+    if (st != QM_OK) return st;
+    if (dtype != QM_IN_F16 && dtype != QM_IN_BF16) return QM_ERR_DTYPE;
+    if (count < 0) return QM_ERR_SHAPE;
+    if (count == 0) return QM_OK;
+    if (!page_ids || !k || !v) return QM_ERR_NULL;
+    if (((uintptr_t)page_ids & 3) || (((uintptr_t)k | (uintptr_t)v) & 15)) return QM_ERR_ALIGN;
+    if (cache->pages == 0) return QM_ERR_SHAPE;
+    hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    const auto kernel = dtype == QM_IN_F16 ? &kv_read_kernel<QM_IN_F16> : &kv_read_kernel<QM_IN_BF16>;
+    const hipError_t e = enqueue(kernel, dim3(std::min(count, 1 << 20), cache->kv_heads), dim3(256), 0, s, kv_args(cache, 0), page_ids, count,
+                                 static_cast<uint16_t *>(k), static_cast<uint16_t *>(v));
+    return e == hipSuccess ? QM_OK : fail_launch(e);
+}

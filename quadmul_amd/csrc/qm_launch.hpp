@@ -79,6 +79,9 @@ inline hipError_t device_cus(int *cus)
     return hipSuccess;
 }
 
+// QM_ERR_LAUNCH, with the error kept for qm_last_hip_error (qm_dispatch.hip).
+int fail_launch(hipError_t e);
+
 // The tile kernel on 6-bit floats (qm_tile6_inst.hip).
 hipError_t launch_tile6_i32(const GemmArgs &p, const Fp6Operand &a, hipStream_t s, int opt);
 hipError_t launch_tile6_f16(const GemmArgs &p, const Fp6Operand &a, hipStream_t s, int opt);
