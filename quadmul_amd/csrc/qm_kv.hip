@@ -73,7 +73,33 @@ QM_EXPORT int qm_kv_append_i8(const qm_kv_cache *cache, const qm_kv_new *fresh, 
     return e == hipSuccess ? QM_OK : fail_launch(e);
 }
 
-QM_EXPORT size_t qm_kv_attend_workspace_bytes(const qm_kv_cache *, int, int, int, int) { return 0; }
+// How a call's work is dealt out: tiles of 16 rows, and the 64-token steps of a sequence in splits.
+namespace {
+struct AttendPlan {
+    int tiles, splits, per;
+    size_t bytes;
+};
+}
+static AttendPlan attend_plan(const qm_kv_cache *c, int tokens, int heads, int max_query, int max_length)
+{
+    AttendPlan p{1, 1, 1, 0};
+    if (tokens == 0 || c->sequences == 0) return p;
+    const long long most = std::min<long long>((long long)c->table_width * c->page_size, INT_MAX - 2 * ATTEND_STEP);
+    const long long length = max_length > 0 ? std::min<long long>(max_length, most) : most;
+    const int steps = (int)((length + ATTEND_STEP - 1) / ATTEND_STEP);
+    p.tiles = (int)std::min<long long>(((long long)most_new(c, tokens, max_query) * (heads / c->kv_heads) + 15) / 16, 65536);
+    const long long groups = (long long)c->sequences * c->kv_heads * p.tiles;
+    p.splits = (int)std::max<long long>(1, std::min<long long>((2048 + groups - 1) / groups, steps / 8));
+    p.per = std::max(1, (steps + p.splits - 1) / p.splits);
+    if (p.splits > 1) p.bytes = ((size_t)p.splits * (c->head_dim + 1) + 1) * tokens * heads * sizeof(float);
+    return p;
+}
+
+QM_EXPORT size_t qm_kv_attend_workspace_bytes(const qm_kv_cache *cache, int tokens, int heads, int max_query, int max_length)
+{
+    if (check_cache(cache, true) != QM_OK || check_tokens(cache, tokens) != QM_OK || heads < 1 || heads % cache->kv_heads != 0) return 0;
+    return attend_plan(cache, tokens, heads, max_query, max_length).bytes;
+}
 
 QM_EXPORT int qm_kv_attend_i8(const qm_kv_cache *cache, const void *q, int dtype, long long q_token_stride, long long q_head_stride, void *out, int tokens,
                               int heads, float scale, int causal, int window, int max_query, int max_length, void *stream, void *workspace,
@@ -83,16 +109,17 @@ QM_EXPORT int qm_kv_attend_i8(const qm_kv_cache *cache, const void *q, int dtype
     if (st != QM_OK) return st;
     if (dtype != QM_IN_F16 && dtype != QM_IN_BF16) return QM_ERR_DTYPE;
     if ((st = check_tokens(cache, tokens)) != QM_OK) return st;
-    if (heads < 1 || heads > 65535 || heads % cache->kv_heads != 0 || window < 0) return QM_ERR_SHAPE;
+    if (heads < 1 || heads > 65535 || heads % cache->kv_heads != 0 || window < 0 || (long long)tokens * heads > INT_MAX) return QM_ERR_SHAPE;
     if (tokens == 0) return QM_OK;
     if (!q || !out) return QM_ERR_NULL;
     if ((((uintptr_t)q | (uintptr_t)out) & 1) || ((uintptr_t)workspace & 15)) return QM_ERR_ALIGN;
-    if (workspace_bytes < qm_kv_attend_workspace_bytes(cache, tokens, heads, max_query, max_length)) return QM_ERR_SCRATCH;
-    const KvArgs c = kv_args(cache, tokens);
-    const AttendArgs a{static_cast<const uint16_t *>(q), static_cast<uint16_t *>(out), q_token_stride, q_head_stride, heads, causal ? 1 : 0, window, scale};
+    const AttendPlan p = attend_plan(cache, tokens, heads, max_query, max_length);
+    if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes)) return QM_ERR_SCRATCH;
+    const AttendArgs a{static_cast<const uint16_t *>(q), static_cast<uint16_t *>(out), static_cast<float *>(workspace), q_token_stride, q_head_stride, heads,
+                       causal ? 1 : 0, window > 1 << 30 ? 0 : window, scale * 1.4426950408889634f, p.splits, p.tiles, p.per};
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-    const auto kernel = dtype == QM_IN_F16 ? &kv_attend_kernel<QM_IN_F16> : &kv_attend_kernel<QM_IN_BF16>;
-    const hipError_t e = enqueue(kernel, dim3(std::min(tokens, 1 << 20), heads), dim3(256), 0, s, c, a);
+    const KvArgs c = kv_args(cache, tokens);
+    const hipError_t e = dtype == QM_IN_F16 ? launch_attend_f16(c, a, s) : launch_attend_bf16(c, a, s);
     return e == hipSuccess ? QM_OK : fail_launch(e);
 }
 
