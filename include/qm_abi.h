@@ -323,7 +323,7 @@ int qm_kv_append_i8(const qm_kv_cache *cache, const qm_kv_new *fresh, void *stre
  *   workspace  16-byte aligned device memory of qm_kv_attend_workspace_bytes(...) bytes, used in stream order by the kernels of this
  *              call only; QM_ERR_SCRATCH with less, and nothing is enqueued
  */
-size_t qm_kv_attend_workspace_bytes(const qm_kv_cache *cache, int tokens, int heads, int max_query, int max_length);
+size_t qm_kv_attend_workspace_bytes(const qm_kv_cache *cache, int tokens, int heads, int window, int max_query, int max_length);
 int qm_kv_attend_i8(const qm_kv_cache *cache, const void *q, int dtype, long long q_token_stride, long long q_head_stride, void *out,
                     int tokens, int heads, float scale, int causal, int window, int max_query, int max_length, void *stream,
                     void *workspace, size_t workspace_bytes);

@@ -139,7 +139,7 @@ def library() -> ctypes.CDLL:
     lib.qm_gemm_grouped_i4.restype = ci
     lib.qm_kv_append_i8.argtypes = [cache, ctypes.POINTER(KvNew), vp]
     lib.qm_kv_append_i8.restype = ci
-    lib.qm_kv_attend_workspace_bytes.argtypes = [cache, ci, ci, ci, ci]
+    lib.qm_kv_attend_workspace_bytes.argtypes = [cache, ci, ci, ci, ci, ci]
     lib.qm_kv_attend_workspace_bytes.restype = size
     lib.qm_kv_attend_i8.argtypes = [cache, vp, ci, ll, ll, vp, ci, ci, ctypes.c_float, ci, ci, ci, ci, vp, vp, size]
     lib.qm_kv_attend_i8.restype = ci

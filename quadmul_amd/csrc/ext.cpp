@@ -355,7 +355,7 @@ torch::Tensor kv_attend(torch::Tensor q, torch::Tensor cache_k, torch::Tensor ca
     c10::OptionalDeviceGuard guard(cache_k.device());
     auto out = torch::empty({tokens, heads, (int64_t)c.head_dim}, q.options());
     const int most = clamped(max_query), longest = clamped(max_length);
-    const size_t need = qm_kv_attend_workspace_bytes(&c, (int)tokens, (int)heads, most, longest);
+    const size_t need = qm_kv_attend_workspace_bytes(&c, (int)tokens, (int)heads, clamped(window), most, longest);
     torch::Tensor scratch;
     if (need > 0) scratch = torch::empty({(int64_t)need}, q.options().dtype(torch::kUInt8));
     check_status(qm_kv_attend_i8(&c, q.data_ptr(), type, q.stride(0), q.stride(1), out.data_ptr(), (int)tokens, (int)heads,

@@ -21,11 +21,17 @@ namespace qm {
 struct AttendArgs {
     const uint16_t *q;
     uint16_t *out;
-    float *part;  // several splits: partial results, splits x rows of dim values, then as many lse, then the splits of each row in use
     long long q_token, q_head;
     int heads, causal, window;
-    float scale;      // times log2(e)
-    int splits, tiles, per;  // splits of a sequence's steps, tiles of rows side by side, steps of a split (more where the splits are too few)
+    float scale;   // times log2(e)
+    int tiles;     // of rows, side by side
+    int rows;      // of a tile that are used at most
+    // all sequences' steps one after the other cut into as many equal parts (0: a sequence to a workgroup), for each tile and head, and what
+    // is left where a sequence is cut: a part's end of one and beginning of another, 16 rows of dim values and their lse each; and the
+    // first part of each sequence and their number
+    int parts;
+    float *part, *lse;
+    int2 *cuts;
 };
 
 constexpr int ATTEND_STEP = 64;   // tokens
@@ -51,40 +57,111 @@ __device__ __forceinline__ h8 half8_of_codes(const uint32_t a, const uint32_t b)
 __device__ __forceinline__ float across_groups_max(float v) { v = fmaxf(v, __shfl_xor(v, 16)); return fmaxf(v, __shfl_xor(v, 32)); }
 __device__ __forceinline__ float across_groups_sum(float v) { v += __shfl_xor(v, 16); return v + __shfl_xor(v, 32); }
 
-// The steps that a tile of rows first .. last (new tokens) has to look at.
+// The steps that rows first .. last (new tokens) have to look at.
 struct AttendRange {
-    int begin, steps, per, active;
+    int begin, steps;
 };
 __device__ __forceinline__ AttendRange attend_range(const KvArgs &c, const AttendArgs &a, const KvSequence &q, const int first, const int last)
 {
     const long long most = min((long long)c.width * c.page, 0x7FFFFFFFll - 2 * ATTEND_STEP);
-    int end = q.begin + last < 0 || c.pages == 0 ? 0 : a.causal ? q.begin + last + 1 : q.length;
+    int end = q.begin + last < 0 || c.pages == 0 || c.width == 0 ? 0 : a.causal ? q.begin + last + 1 : q.length;
     end = (int)min((long long)end, most);
     const int from = a.window > 0 ? max(q.begin + first - a.window + 1, 0) : 0;
-    const int begin = from / ATTEND_STEP, steps = end > from ? (end + ATTEND_STEP - 1) / ATTEND_STEP - begin : 0;
-    const int per = max(a.per, (steps + a.splits - 1) / a.splits);
-    return {begin, steps, per, (steps + per - 1) / per};
+    const int begin = from / ATTEND_STEP;
+    return {begin, end > from ? (end + ATTEND_STEP - 1) / ATTEND_STEP - begin : 0};
 }
 
-// blockIdx.x: a split, and a tile of rows; blockIdx.y: a head of the cache; blockIdx.z: a sequence. The waves take turns at the steps of their split.
-template <int T, int D, int NW>
+// Where part `number` of all sequences' steps begins: in sequence s (-1: past the last one), at the step `at` of it; `per` steps to a part, and
+// the sequence's own begin at step number `before`. A wave finds it by itself, a lane to a sequence: the lengths are in device
+// memory, and the parts are to be equally long whatever they are.
+struct AttendCut {
+    int s, per;
+    long long before;
+};
+__device__ __forceinline__ int attend_steps(const KvArgs &c, const AttendArgs &a, const KvSequence &q)
+{
+    // (a sequence that sees nothing has its rows of zeros: one step)
+    return q.count > 0 ? max(attend_range(c, a, q, 0, q.count - 1).steps, 1) : 0;
+}
+__device__ __forceinline__ AttendCut attend_cut(const KvArgs &c, const AttendArgs &a, const int number)
+{
+    const int lane = threadIdx.x & 63;
+    const auto steps_of = [&](const int s) {
+        const int i = min(s, c.sequences - 1), n = c.lengths[i], from = c.start[i], to = c.start[i + c.packed], length = max(n, 0);
+        const int lo = c.packed ? min(max(from, 0), c.tokens) : i * c.per, hi = c.packed ? min(max(to, lo), c.tokens) : lo + c.per;
+        return s < c.sequences ? attend_steps(c, a, KvSequence{lo, hi - lo, length - (hi - lo), length}) : 0;
+    };
+    const auto up_to_lane = [&](long long v) {
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const long long w = __shfl_up(v, d);
+            if (lane >= d) v += w;
+        }
+        return v;
+    };
+    long long total = 0, up = 0;
+    int steps = 0;
+    for (int base = 0; base < c.sequences; base += 64) {
+        steps = steps_of(base + lane);
+        up = up_to_lane(steps);
+        total += __shfl(up, 63);
+    }
+    const int per = (int)min((total + a.parts - 1) / a.parts, 0x7FFFFFFFll);
+    const long long from = (long long)number * per;
+    long long before = 0;
+    for (int base = 0; base < c.sequences; base += 64) {
+        if (c.sequences > 64) {
+            steps = steps_of(base + lane);
+            up = up_to_lane(steps);
+        }
+        const unsigned long long past = __ballot(before + up > from);
+        if (past != 0) {
+            const int at = __builtin_ctzll(past);
+            return {base + at, per, before + __shfl(up - steps, at)};
+        }
+        before += __shfl(up, 63);
+    }
+    return {-1, 1, 0};
+}
+
+// blockIdx.x: a head of the cache, and a sequence or (CUT) a part of all sequences; blockIdx.y: a tile of rows. The waves take turns at the steps.
+// (Workgroups are dealt to the XCDs in turn: with the heads side by side each has as many long and short sequences as the others.)
+template <int T, int D, int NW, bool CUT>
 __global__ __launch_bounds__(NW * 64, D > 128 ? 1 : 2) void kv_attend_kernel(const KvArgs c, const AttendArgs a)
 {
     constexpr int J = D / 32, DT = D / 16, KW = D / 16;  // products of 32 channels; tiles of 16 channels; words of a lane's part of a key
     constexpr int LD = D + 4;
     __shared__ float joined[NW / 2][16][LD];
     __shared__ float stats[NW][3][16];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
-    const int head = blockIdx.y, shared = a.heads / c.kv_heads, split = blockIdx.x % a.splits;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
+    const int head = blockIdx.x % c.kv_heads, shared = a.heads / c.kv_heads, number = blockIdx.x / c.kv_heads;
     const int page_shift = __builtin_ctz(c.page), page_mask = c.page - 1;
 
-    for (int s = blockIdx.z; s < c.sequences; s += gridDim.z) {
+    AttendCut cut{number, 1, 0};
+    if constexpr (CUT) {
+        cut = attend_cut(c, a, number);
+        cut.s = __builtin_amdgcn_readfirstlane(cut.s), cut.per = __builtin_amdgcn_readfirstlane(cut.per);
+        if (cut.s < 0) return;
+    }
+    const long long part_begin = (long long)number * cut.per, part_end = part_begin + cut.per;
+    long long before = cut.before;
+    for (int s = cut.s; s < c.sequences && (!CUT || before < part_end); s += CUT ? 1 : gridDim.x / c.kv_heads) {
         const KvSequence q = kv_sequence(c, s);
-        const int rows = q.count * shared;
-        for (int tile = blockIdx.x / a.splits; tile * 16 < rows; tile += a.tiles) {
+        const int rows = q.count * shared, all_steps = CUT ? attend_steps(c, a, q) : 1;
+        const bool begins = !CUT || before >= part_begin, ends = !CUT || before + all_steps <= part_end;
+        const int from = begins ? 0 : (int)(part_begin - before), to = ends ? all_steps : (int)(part_end - before);
+        if (CUT && begins && rows > 0 && blockIdx.y == 0 && head == 0 && threadIdx.x == 0)
+            a.cuts[s] = int2{number, (int)((before + all_steps - 1) / cut.per) - number + 1};
+        before += all_steps;
+        const int begin0 = CUT ? attend_range(c, a, q, 0, q.count - 1).begin : 0;
+        for (int tile = blockIdx.y; tile * 16 < rows; tile += gridDim.y) {
             const int first = tile * 16 / shared, last = min(tile * 16 + 15, rows - 1) / shared;
             const AttendRange range = attend_range(c, a, q, first, last);
-            if (split > 0 && split >= range.active) continue;
+            // (a tile that the hint did not promise is done in one piece, by the part that its sequence begins in)
+            const bool whole_range = (begins && ends) || tile >= a.tiles || min(rows - tile * 16, 16) > a.rows;
+            if (whole_range && !begins) continue;
+            const int step0 = whole_range ? range.begin : max(begin0 + from, range.begin);
+            const int step1 = whole_range ? range.begin + range.steps : min(begin0 + to, range.begin + range.steps);
             const int row = min(tile * 16 + r, rows - 1), token = row / shared;
             const bool mine = tile * 16 + r < rows;
             const size_t out_row = (size_t)(q.row0 + token) * a.heads + head * shared + row % shared;
@@ -103,7 +180,7 @@ __global__ __launch_bounds__(NW * 64, D > 128 ? 1 : 2) void kv_attend_kernel(con
 #pragma unroll
                 for (int j = 0; j < J; ++j) {
                     const int d = j * 32 + 32 <= D / 64 * 64 ? (j / 2) * 64 + 16 * g + 8 * (j & 1) : j * 32 + 8 * g;
-                    const v4i w = mine ? (v4i)*reinterpret_cast<const v4i_half_aligned *>(x + d) : v4i{};
+                    const v4i w = *reinterpret_cast<const v4i_half_aligned *>(x + d);  // (a row past the last one repeats it)
                     if constexpr (T == QM_IN_F16) query[j] = __builtin_bit_cast(h8, w);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
@@ -124,7 +201,6 @@ __global__ __launch_bounds__(NW * 64, D > 128 ? 1 : 2) void kv_attend_kernel(con
                 }
             }
 
-            const int step0 = range.begin + split * range.per, step1 = min(step0 + range.per, range.begin + range.steps);
             struct Pages {
                 int key, value;  // of this lane's row of the keys and of its sixteen tokens; -1: none
             };
@@ -166,13 +242,15 @@ __global__ __launch_bounds__(NW * 64, D > 128 ? 1 : 2) void kv_attend_kernel(con
 
             v4f out[DT] = {};
             float top = ATTEND_LOW, high = ATTEND_LOW, total = 0.0f;
-            Pages now{-1, -1}, next{-1, -1};
             int step = step0 + wave;
+            Pages now{-1, -1}, next{-1, -1};
             if (step < step1) {
                 now = pages(step);
+                next = pages(min(step + NW, step1 - 1));
                 load_keys(step, now);
                 load_values(step, now);
-                if (step + NW < step1) next = pages(step + NW);
+#pragma unroll
+                for (int j = 0; j < J; ++j) asm volatile("" : "+v"(query[j]));  // waited for here, not in the loop behind the values
             }
             for (; step < step1; step += NW) {
                 v4f score[4];
@@ -186,6 +264,7 @@ __global__ __launch_bounds__(NW * 64, D > 128 ? 1 : 2) void kv_attend_kernel(con
                 const float by = key_scale * factor;
                 const float vs = fabsf(value_scale) < 0x1p-126f ? 0.0f : value_scale;
                 const bool there = now.value >= 0;
+                const Pages then = pages(min(step + 2 * NW, step1 - 1));  // (in front of the keys: what is waited for last is loaded last)
                 if (step + NW < step1) load_keys(step + NW, next);
 
                 const int token0 = step * ATTEND_STEP + 16 * g;
@@ -196,11 +275,19 @@ __global__ __launch_bounds__(NW * 64, D > 128 ? 1 : 2) void kv_attend_kernel(con
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         score[t][i] *= by;
-                        if (!whole) {
-                            const int j = token0 + 4 * t + i;
-                            if (!(there && j <= limit && j > below)) score[t][i] = -INFINITY;
-                        }
                         most = fmaxf(most, score[t][i]);
+                    }
+                }
+                if (!whole) {
+                    most = -INFINITY;
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int j = token0 + 4 * t + i;
+                            score[t][i] = (there & (j <= limit) & (j > below)) ? score[t][i] : -INFINITY;
+                            most = fmaxf(most, score[t][i]);
+                        }
                     }
                 }
                 const float size = vs == 0.0f ? -INFINITY : __builtin_amdgcn_logf(fabsf(vs));
@@ -215,7 +302,8 @@ __global__ __launch_bounds__(NW * 64, D > 128 ? 1 : 2) void kv_attend_kernel(con
                 // vs * 2^(top - high + lift): by two factors, for the power alone may leave the float range (the product does only where the
                 // weight is below 2^-118 of the largest)
                 const float root = __builtin_amdgcn_exp2f(0.5f * fminf(top - high + ATTEND_LIFT, 126.0f - size));
-                const float weigh = vs == 0.0f ? 0.0f : vs * root * root;
+                // (sixteen tokens that a mask hides count 0 whatever the scale of their page is)
+                const float weigh = vs == 0.0f || most == -INFINITY ? 0.0f : vs * root * root;
                 h8 weight[2];
 #pragma unroll
                 for (int t = 0; t < 4; ++t) {
@@ -223,8 +311,7 @@ __global__ __launch_bounds__(NW * 64, D > 128 ? 1 : 2) void kv_attend_kernel(con
                     for (int i = 0; i < 4; ++i) {
                         const float p = __builtin_amdgcn_exp2f(score[t][i] - top);
                         total += p;
-                        // (what a mask hides is 0 whatever the scale of its page is)
-                        weight[t / 2][(t & 1) * 4 + i] = (_Float16)(!whole && p == 0.0f ? 0.0f : p * weigh);
+                        weight[t / 2][(t & 1) * 4 + i] = (_Float16)(p * weigh);
                     }
                 }
 #pragma unroll
@@ -233,11 +320,8 @@ __global__ __launch_bounds__(NW * 64, D > 128 ? 1 : 2) void kv_attend_kernel(con
                     for (int u = 0; u < 2; ++u)
                         out[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(half8_of_codes(values[t][2 * u], values[t][2 * u + 1]), weight[u], out[t], 0, 0, 0);
                 }
-                if (step + NW < step1) {
-                    load_values(step + NW, next);
-                    now = next;
-                    if (step + 2 * NW < step1) next = pages(step + 2 * NW);
-                }
+                if (step + NW < step1) load_values(step + NW, next);
+                now = next, next = then;
             }
 
             // the waves' results into one
@@ -269,7 +353,7 @@ __global__ __launch_bounds__(NW * 64, D > 128 ? 1 : 2) void kv_attend_kernel(con
             if (wave == 0 && mine) {
                 // (the sum is 0 where nothing is seen)
                 const float root = __builtin_amdgcn_exp2f(0.5f * (h1 - t1 - ATTEND_LIFT)), by = root / sum;
-                if (a.splits == 1) {
+                if (whole_range) {
                     uint16_t *const to = a.out + out_row * D + 4 * g;
 #pragma unroll
                     for (int t = 0; t < DT; ++t) {
@@ -277,60 +361,61 @@ __global__ __launch_bounds__(NW * 64, D > 128 ? 1 : 2) void kv_attend_kernel(con
                         *reinterpret_cast<v2i_half_aligned *>(to + 16 * t) = v2i{(int)round16_pair<T>(v[0], v[1]), (int)round16_pair<T>(v[2], v[3])};
                     }
                 } else {
-                    const size_t all = (size_t)c.tokens * a.heads;
-                    float *const to = a.part + (split * all + out_row) * D + 4 * g;
+                    const size_t at = ((size_t)(tile * c.kv_heads + head) * (2 * a.parts) + 2 * number + (begins ? 1 : 0)) * 16 + r;
+                    float *const to = a.part + at * D + 4 * g;
 #pragma unroll
                     for (int t = 0; t < DT; ++t) *reinterpret_cast<v4f *>(to + 16 * t) = sum == 0.0f ? v4f{} : out[t] * root * by;
-                    float *const lse = a.part + a.splits * all * D;
-                    if (g == 0) lse[split * all + out_row] = sum == 0.0f ? -INFINITY : t1 + __builtin_amdgcn_logf(sum);
-                    if (g == 0 && split == 0) reinterpret_cast<int *>(lse + a.splits * all)[out_row] = range.active;
+                    if (g == 0) a.lse[at] = sum == 0.0f ? -INFINITY : t1 + __builtin_amdgcn_logf(sum);
                 }
             }
         }
     }
 }
 
-// The splits of a row into one: a workgroup to a row, its waves take turns at the splits, always in the same order.
-template <int T, int D>
-__global__ __launch_bounds__(256) void kv_join_kernel(const float *part, uint16_t *out, const int rows, const int splits)
+// The parts of a sequence's rows into one, always in the same order. blockIdx.x: a row of a tile; blockIdx.y: a tile and a head; blockIdx.z: a
+// sequence. A part to a wave at a time; bound by the latency of three dependent loads.
+template <int T, int D, int NW>
+__global__ __launch_bounds__(NW * 64) void kv_join_kernel(const KvArgs c, const AttendArgs a)
 {
     constexpr int PER = (D + 63) / 64;
-    __shared__ float sums[4][D], weights[4];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const float *const lse = part + (size_t)splits * rows * D;
-    for (int row = blockIdx.x; row < rows; row += gridDim.x) {
-        const int active = min(reinterpret_cast<const int *>(lse + (size_t)splits * rows)[row], splits);
-        float top = -INFINITY;
-        for (int s = lane; s < active; s += 64) top = fmaxf(top, lse[(size_t)s * rows + row]);
+    __shared__ float sums[NW][D], weights[NW];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, s = blockIdx.z, shared = a.heads / c.kv_heads;
+    const int2 cut = a.cuts[s];
+    const KvSequence q = kv_sequence(c, s);
+    const int tile = blockIdx.y / c.kv_heads, head = blockIdx.y % c.kv_heads, row = tile * 16 + blockIdx.x, rows = q.count * shared;
+    if (row >= rows || cut.y <= 1 || min(rows - tile * 16, 16) > a.rows) return;
+    // part i of the sequence: it begins in the second half of its first one, and goes on in the first halves of the others
+    const auto place = [&](const int i) { return ((size_t)blockIdx.y * (2 * a.parts) + 2 * (cut.x + i) + (i == 0 ? 1 : 0)) * 16 + blockIdx.x; };
+    float top = -INFINITY;
+    for (int i = lane; i < cut.y; i += 64) top = fmaxf(top, a.lse[place(i)]);
 #pragma unroll
-        for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
-        if (top == -INFINITY) top = 0.0f;
-        float v[PER] = {}, sum = 0.0f;
+    for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+    if (top == -INFINITY) top = 0.0f;
+    float v[PER] = {}, sum = 0.0f;
 #pragma unroll 4
-        for (int s = wave; s < active; s += 4) {
-            const float w = __builtin_amdgcn_exp2f(lse[(size_t)s * rows + row] - top);
-            const float *const x = part + ((size_t)s * rows + row) * D + lane;
-            sum += w;
-#pragma unroll
-            for (int e = 0; e < PER; ++e)
-                if (D % 64 == 0 || lane + 64 * e < D) v[e] += w * x[64 * e];
-        }
-        __syncthreads();
-        if (lane == 0) weights[wave] = sum;
+    for (int i = wave; i < cut.y; i += NW) {
+        const size_t at = place(i);
+        const float w = __builtin_amdgcn_exp2f(a.lse[at] - top);
+        sum += w;
 #pragma unroll
         for (int e = 0; e < PER; ++e)
-            if (D % 64 == 0 || lane + 64 * e < D) sums[wave][lane + 64 * e] = v[e];
-        __syncthreads();
-        if ((int)threadIdx.x < D) {
-            const int d = threadIdx.x;
-            const float all = weights[0] + weights[1] + weights[2] + weights[3];
-            const float x = sums[0][d] + sums[1][d] + sums[2][d] + sums[3][d];
-            out[(size_t)row * D + d] = round16<T>(all == 0.0f ? 0.0f : x / all);
-        }
+            if (D % 64 == 0 || lane + 64 * e < D) v[e] += w * a.part[at * D + lane + 64 * e];
+    }
+    if (lane == 0) weights[wave] = sum;
+#pragma unroll
+    for (int e = 0; e < PER; ++e)
+        if (D % 64 == 0 || lane + 64 * e < D) sums[wave][lane + 64 * e] = v[e];
+    __syncthreads();
+    if ((int)threadIdx.x < D) {
+        const int d = threadIdx.x;
+        float all = 0.0f, x = 0.0f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) all += weights[w], x += sums[w][d];
+        a.out[((size_t)(q.row0 + row / shared) * a.heads + head * shared + row % shared) * D + d] = round16<T>(all == 0.0f ? 0.0f : x / all);
     }
 }
 
-// One launch of attention, and one that joins the splits where there are several.
+// One launch of attention, and one that joins the parts where sequences are cut.
 hipError_t launch_attend_f16(const KvArgs &c, const AttendArgs &a, hipStream_t s);
 hipError_t launch_attend_bf16(const KvArgs &c, const AttendArgs &a, hipStream_t s);
 

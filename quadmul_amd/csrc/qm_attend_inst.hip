@@ -9,12 +9,11 @@ namespace qm {
 template <int D>
 static hipError_t launch(const KvArgs &c, const AttendArgs &a, hipStream_t s)
 {
-    constexpr int NW = 4;
-    const dim3 grid(a.splits * a.tiles, c.kv_heads, std::min(c.sequences, 65535));
-    const hipError_t e = enqueue(&kv_attend_kernel<QM_ATTEND_TYPE, D, NW>, grid, dim3(NW * 64), 0, s, c, a);
-    if (e != hipSuccess || a.splits == 1) return e;
-    const int rows = c.tokens * a.heads;
-    return enqueue(&kv_join_kernel<QM_ATTEND_TYPE, D>, dim3(std::min(rows, 1 << 20)), dim3(256), 0, s, a.part, a.out, rows, a.splits);
+    constexpr int NW = D > 128 ? 4 : 8;  // (with eight the registers of the wider heads do not fit)
+    if (a.parts == 0) return enqueue(&kv_attend_kernel<QM_ATTEND_TYPE, D, NW, false>, dim3(std::min(c.sequences, 1 << 18) * c.kv_heads, a.tiles), dim3(NW * 64), 0, s, c, a);
+    const hipError_t e = enqueue(&kv_attend_kernel<QM_ATTEND_TYPE, D, 4, true>, dim3(a.parts * c.kv_heads, a.tiles), dim3(256), 0, s, c, a);
+    if (e != hipSuccess) return e;
+    return enqueue(&kv_join_kernel<QM_ATTEND_TYPE, D, 8>, dim3(a.rows, a.tiles * c.kv_heads, c.sequences), dim3(512), 0, s, c, a);
 }
 
 #if QM_ATTEND_TYPE == QM_IN_F16

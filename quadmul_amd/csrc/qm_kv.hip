@@ -33,8 +33,8 @@ static int check_tokens(const qm_kv_cache *c, int tokens)
 }
 static KvArgs kv_args(const qm_kv_cache *c, int tokens)
 {
-    return {static_cast<int8_t *>(c->k), static_cast<int8_t *>(c->v), c->scales, c->block_table, c->lengths, c->query_start, c->pages, c->kv_heads,
-            c->page_size, c->head_dim, c->sequences, c->table_width, tokens, c->sequences > 0 ? tokens / c->sequences : 0};
+    return {static_cast<int8_t *>(c->k), static_cast<int8_t *>(c->v), c->scales, c->block_table, c->lengths, c->query_start ? c->query_start : c->lengths, c->pages,
+            c->kv_heads, c->page_size, c->head_dim, c->sequences, c->table_width, tokens, c->sequences > 0 ? tokens / c->sequences : 0, c->query_start ? 1 : 0};
 }
 // The most new tokens of a sequence: what the caller says, inside what is possible.
 static int most_new(const qm_kv_cache *c, int tokens, int max_query)
@@ -73,32 +73,44 @@ QM_EXPORT int qm_kv_append_i8(const qm_kv_cache *cache, const qm_kv_new *fresh, 
     return e == hipSuccess ? QM_OK : fail_launch(e);
 }
 
-// How a call's work is dealt out: tiles of 16 rows, and the 64-token steps of a sequence in splits.
+// How a call's work is dealt out: tiles of 16 rows; to a tile and a head a workgroup for each sequence, or all sequences' 64-token
+// steps cut into equal parts and joined by a second launch.
 namespace {
 struct AttendPlan {
-    int tiles, splits, per;
-    size_t bytes;
+    int tiles, rows, parts;
+    size_t part_bytes, lse_bytes, bytes;
 };
 }
-static AttendPlan attend_plan(const qm_kv_cache *c, int tokens, int heads, int max_query, int max_length)
+static AttendPlan attend_plan(const qm_kv_cache *c, int tokens, int heads, int max_query, int max_length, int window)
 {
-    AttendPlan p{1, 1, 1, 0};
+    AttendPlan p{1, 16, 0, 0, 0, 0};
     if (tokens == 0 || c->sequences == 0) return p;
     const long long most = std::min<long long>((long long)c->table_width * c->page_size, INT_MAX - 2 * ATTEND_STEP);
-    const long long length = max_length > 0 ? std::min<long long>(max_length, most) : most;
+    long long length = max_length > 0 ? std::min<long long>(max_length, most) : most;
+    const int fresh = most_new(c, tokens, max_query);
+    if (window > 0) length = std::min<long long>(length, (long long)window + fresh + ATTEND_STEP);
     const int steps = (int)((length + ATTEND_STEP - 1) / ATTEND_STEP);
-    p.tiles = (int)std::min<long long>(((long long)most_new(c, tokens, max_query) * (heads / c->kv_heads) + 15) / 16, 65536);
-    const long long groups = (long long)c->sequences * c->kv_heads * p.tiles;
-    p.splits = (int)std::max<long long>(1, std::min<long long>((2048 + groups - 1) / groups, steps / 8));
-    p.per = std::max(1, (steps + p.splits - 1) / p.splits);
-    if (p.splits > 1) p.bytes = ((size_t)p.splits * (c->head_dim + 1) + 1) * tokens * heads * sizeof(float);
+    const long long rows = (long long)fresh * (heads / c->kv_heads);
+    p.tiles = (int)std::min<long long>((rows + 15) / 16, 4096);
+    p.rows = (int)std::min<long long>(rows, 16);
+    const long long groups = (long long)p.tiles * c->kv_heads;
+    // The second launch costs 5 us, a step of a wave 2 to 3.5, a sequence in one workgroup has its waves go through an eighth of its
+    // steps one by one. 32 sequences and 8 heads (256 workgroups): 2048 tokens each 31 us in one piece, 36 cut; 6000 tokens 78 and
+    // 82; lengths from 1 to 8192 62 and 41; one sequence of 2048 tokens 15 and 11, of 1024 11 and 11.
+    if (steps <= 16 || (steps <= 32 && groups * c->sequences >= 128) || c->sequences > 256) return p;
+    // two workgroups of four waves to a CU; a step to a wave at least
+    p.parts = (int)std::max<long long>(1, std::min<long long>(512 / groups, (long long)steps * c->sequences / 4));
+    const auto up = [](size_t v) { return (v + 255) / 256 * 256; };
+    p.part_bytes = (size_t)groups * p.parts * 2 * 16 * c->head_dim * sizeof(float);
+    p.lse_bytes = up((size_t)groups * p.parts * 2 * 16 * sizeof(float));
+    p.bytes = p.part_bytes + p.lse_bytes + c->sequences * sizeof(int2);
     return p;
 }
 
-QM_EXPORT size_t qm_kv_attend_workspace_bytes(const qm_kv_cache *cache, int tokens, int heads, int max_query, int max_length)
+QM_EXPORT size_t qm_kv_attend_workspace_bytes(const qm_kv_cache *cache, int tokens, int heads, int window, int max_query, int max_length)
 {
     if (check_cache(cache, true) != QM_OK || check_tokens(cache, tokens) != QM_OK || heads < 1 || heads % cache->kv_heads != 0) return 0;
-    return attend_plan(cache, tokens, heads, max_query, max_length).bytes;
+    return attend_plan(cache, tokens, heads, max_query, max_length, window).bytes;
 }
 
 QM_EXPORT int qm_kv_attend_i8(const qm_kv_cache *cache, const void *q, int dtype, long long q_token_stride, long long q_head_stride, void *out, int tokens,
@@ -113,10 +125,12 @@ QM_EXPORT int qm_kv_attend_i8(const qm_kv_cache *cache, const void *q, int dtype
     if (tokens == 0) return QM_OK;
     if (!q || !out) return QM_ERR_NULL;
     if ((((uintptr_t)q | (uintptr_t)out) & 1) || ((uintptr_t)workspace & 15)) return QM_ERR_ALIGN;
-    const AttendPlan p = attend_plan(cache, tokens, heads, max_query, max_length);
+    const AttendPlan p = attend_plan(cache, tokens, heads, max_query, max_length, window);
     if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes)) return QM_ERR_SCRATCH;
-    const AttendArgs a{static_cast<const uint16_t *>(q), static_cast<uint16_t *>(out), static_cast<float *>(workspace), q_token_stride, q_head_stride, heads,
-                       causal ? 1 : 0, window > 1 << 30 ? 0 : window, scale * 1.4426950408889634f, p.splits, p.tiles, p.per};
+    uint8_t *const scratch = static_cast<uint8_t *>(workspace);
+    const AttendArgs a{static_cast<const uint16_t *>(q), static_cast<uint16_t *>(out), q_token_stride, q_head_stride, heads, causal ? 1 : 0,
+                       window > 1 << 30 ? 0 : window, scale * 1.4426950408889634f, p.tiles, p.rows, p.parts, reinterpret_cast<float *>(scratch),
+                       reinterpret_cast<float *>(scratch + p.part_bytes), reinterpret_cast<int2 *>(scratch + p.part_bytes + p.lse_bytes)};
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     const KvArgs c = kv_args(cache, tokens);
     const hipError_t e = dtype == QM_IN_F16 ? launch_attend_f16(c, a, s) : launch_attend_bf16(c, a, s);

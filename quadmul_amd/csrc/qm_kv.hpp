@@ -10,7 +10,8 @@ struct KvArgs {
     float *scales;
     const int *table, *lengths, *start;
     int pages, kv_heads, page, dim, sequences, width, tokens;
-    int per;  // new tokens of every sequence where start is null
+    int per;     // new tokens of every sequence where there is no start
+    int packed;  // 1: there is; 0: `start` is `lengths`, so that it can be read all the same
 };
 
 // A sequence's new tokens: rows row0 .. row0 + count - 1, of which row0 + i is at position begin + i (padding where that
@@ -18,19 +19,24 @@ struct KvArgs {
 struct KvSequence {
     int row0, count, begin, length;
 };
+// Integers that are the same for a whole wave come through the scalar cache: one round trip for the three of them, where vector loads behind
+// the test for `start` made three.
+typedef const __attribute__((address_space(4))) int *scalar_ints;
+__device__ __forceinline__ scalar_ints scalars(const int *p) { return (scalar_ints)(uintptr_t)p; }
 __device__ __forceinline__ KvSequence kv_sequence(const KvArgs &c, const int s)
 {
-    const int length = max(c.lengths[s], 0);
-    const int lo = c.start != nullptr ? min(max(c.start[s], 0), c.tokens) : s * c.per;
-    const int hi = c.start != nullptr ? min(max(c.start[s + 1], lo), c.tokens) : lo + c.per;
+    const int n = scalars(c.lengths)[s], from = scalars(c.start)[s], to = scalars(c.start)[s + c.packed];
+    const int length = max(n, 0);
+    const int lo = c.packed ? min(max(from, 0), c.tokens) : s * c.per;
+    const int hi = c.packed ? min(max(to, lo), c.tokens) : lo + c.per;
     return {lo, hi - lo, length - (hi - lo), length};
 }
-// The page of a sequence's tokens number * page and up, -1 for none.
+// The page of a sequence's tokens number * page and up, -1 for none. The load is made whatever the number is, at a place inside the table (a
+// table without entries has none: the callers have left before): a branch round it would be waited for by itself.
 __device__ __forceinline__ int kv_page(const KvArgs &c, const int s, const int number)
 {
-    if (number >= c.width) return -1;
-    const int id = c.table[(size_t)s * c.width + number];
-    return id >= 0 && id < c.pages ? id : -1;
+    const int id = c.table[(size_t)s * c.width + min(number, c.width - 1)];
+    return ((number < c.width) & (id >= 0) & (id < c.pages)) ? id : -1;
 }
 
 struct KvNewArgs {
@@ -108,7 +114,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const KvArgs c, const Kv
             continue;
         }
         const int head = blockIdx.y >> 1, side = blockIdx.y & 1, first = max(q.begin, 0);
-        if (q.count == 0 || q.length <= first) continue;
+        if (q.count == 0 || q.length <= first || c.width == 0) continue;
         const int pairs = side ? 0 : f.pairs, steps = side ? c.page : 1;  // a channel's step from token to token, in codes, is 1 or dim
         const uint16_t *const x = side ? f.v + head * f.v_head : f.k + head * f.k_head;
         const long long token = side ? f.v_token : f.k_token;

@@ -119,7 +119,7 @@ def attend(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor, scales
         raise QuadmulError(f"attend: the heads of the queries must be a multiple of the cache's {c.kv_heads}, the window 0 or more tokens")
     max_query, max_length, window = (min(max(i, 0), 2 ** 31 - 1) for i in (max_query, max_length, window))
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    need = library().qm_kv_attend_workspace_bytes(ctypes.byref(c), tokens, heads, max_query, max_length)
+    need = library().qm_kv_attend_workspace_bytes(ctypes.byref(c), tokens, heads, window, max_query, max_length)
     scratch = torch.empty((need,), dtype=torch.uint8, device=q.device) if need else None
     with torch.cuda.device(q.device):
         st = library().qm_kv_attend_i8(ctypes.byref(c), q.data_ptr(), _KINDS[q.dtype], q.stride(0), q.stride(1), out.data_ptr(), tokens, heads,
