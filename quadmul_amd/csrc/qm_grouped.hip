@@ -10,9 +10,26 @@
 
 namespace qm {
 
+template <int T, int S, int MODE>
+static hipError_t launch_skinny_mode(const GroupedArgs &p, hipStream_t s)
+{
+    constexpr int NW = 8;
+    const auto go = [&](auto kernel, int nt) { return enqueue(kernel, dim3((p.N + 16 * nt - 1) / (16 * nt)), dim3(NW * 64), 0, s, p); };
+    if (p.M <= 16) return p.N <= 6144 ? go(&gemm_grouped_skinny_kernel<T, S, MODE, 1, 1, NW>, 1) : go(&gemm_grouped_skinny_kernel<T, S, MODE, 1, 2, NW>, 2);
+    if (p.M <= 32) return go(&gemm_grouped_skinny_kernel<T, S, MODE, 2, 2, NW>, 2);
+    return go(&gemm_grouped_skinny_kernel<T, S, MODE, 4, 2, NW>, 2);
+}
 template <int T, int S>
 static hipError_t launch_grouped(const GroupedArgs &p, hipStream_t s)
 {
+    if (p.K > 0 && p.K % 32 == 0 && ((uintptr_t)p.B & 15) == 0 && p.M <= 64) {
+        switch (group_mode(p.group)) {
+        case 1: return launch_skinny_mode<T, S, 1>(p, s);
+        case 2: return launch_skinny_mode<T, S, 2>(p, s);
+        case 4: return launch_skinny_mode<T, S, 4>(p, s);
+        default: return launch_skinny_mode<T, S, 0>(p, s);
+        }
+    }
     const int rows = (p.M + GROUPED_ROWS - 1) / GROUPED_ROWS;
     return enqueue(&gemm_grouped_any_kernel<T, S>, dim3((p.N + 3) / 4, std::min(rows, 65535)), dim3(256), 0, s, p);
 }
