@@ -1,6 +1,7 @@
 // C entries of the GEMM on 16-bit activations and int4 weights with group scales (include/qm_abi.h): argument checks,
 // choice of kernel, launch.
 #include <algorithm>
+#include <atomic>
 
 #include "../../include/qm_abi.h"
 #include "qm_launch.hpp"
@@ -10,35 +11,77 @@
 
 namespace qm {
 
+// Which kernel runs, and what it needs.
+enum GroupedKernel { GROUPED_ANY, GROUPED_ROWS16, GROUPED_SKINNY };
+struct GroupedPlan {
+    GroupedKernel kernel;
+    int ways, chunk, runs;  // waves to a tile of columns; blocks of 32 of K in a run, runs
+    size_t bytes;
+};
+static GroupedPlan grouped_plan(int m, int n, int k, int align)
+{
+    GroupedPlan p{GROUPED_ANY, 1, 0, 1, 0};
+    if (k == 0 || k % 32 != 0 || align < 16 || m > 64) return p;
+    if (m > 16) { p.kernel = GROUPED_SKINNY; return p; }
+    p.kernel = GROUPED_ROWS16;
+    // what a workgroup holds of x: 128 KiB, beside the sums; one workgroup to a CU
+    const int blocks = k / 32, most = (128 << 10) / (64 * (m | 1) + 64) / 8 * 8;
+    p.runs = (blocks + most - 1) / most;
+    p.chunk = ((blocks + p.runs - 1) / p.runs + 3) / 4 * 4;
+    p.runs = (blocks + p.chunk - 1) / p.chunk;
+    if (p.runs > 1) p.bytes = (size_t)p.runs * m * n * sizeof(float);
+    while (p.ways < GROUPED_WAVES && (long long)((n + 15) / 16) * p.runs * p.ways < 3072) p.ways *= 2;
+    return p;
+}
+
 template <int T, int S, int MODE>
-static hipError_t launch_skinny_mode(const GroupedArgs &p, hipStream_t s)
+static hipError_t launch_mode(GroupedArgs p, const GroupedPlan &plan, hipStream_t s)
 {
     constexpr int NW = 8;
     const auto go = [&](auto kernel, int nt) { return enqueue(kernel, dim3((p.N + 16 * nt - 1) / (16 * nt)), dim3(NW * 64), 0, s, p); };
-    if (p.M <= 16) return p.N <= 6144 ? go(&gemm_grouped_skinny_kernel<T, S, MODE, 1, 1, NW>, 1) : go(&gemm_grouped_skinny_kernel<T, S, MODE, 1, 2, NW>, 2);
-    if (p.M <= 32) return go(&gemm_grouped_skinny_kernel<T, S, MODE, 2, 2, NW>, 2);
-    return go(&gemm_grouped_skinny_kernel<T, S, MODE, 4, 2, NW>, 2);
+    if (plan.kernel == GROUPED_SKINNY) return p.M <= 32 ? go(&gemm_grouped_skinny_kernel<T, S, MODE, 2, 2, NW, 2>, 2) : go(&gemm_grouped_skinny_kernel<T, S, MODE, 4, 2, NW, 2>, 2);
+    p.chunk = plan.chunk, p.ways = plan.ways;
+    const int tiles = GROUPED_WAVES / plan.ways, groups = ((p.N + 15) / 16 + tiles - 1) / tiles;
+    const size_t lds = (size_t)plan.chunk * (64 * (p.M | 1) + 64);
+    static std::atomic<bool> known[QM_MAX_DEVICES] = {};
+    const auto kernel = &gemm_grouped_rows_kernel<T, S, MODE>;
+    if (const hipError_t e = ensure_dynamic_lds(kernel, 128 << 10, known); e != hipSuccess) return e;
+    return enqueue(kernel, dim3(std::min(groups, std::max(1, 256 / plan.runs)), plan.runs), dim3(GROUPED_WAVES * 64), lds, s, p);
 }
 template <int T, int S>
-static hipError_t launch_grouped(const GroupedArgs &p, hipStream_t s)
+static hipError_t launch_grouped(GroupedArgs p, const GroupedPlan &plan, hipStream_t s)
 {
-    if (p.K > 0 && p.K % 32 == 0 && ((uintptr_t)p.B & 15) == 0 && p.M <= 64) {
-        switch (group_mode(p.group)) {
-        case 1: return launch_skinny_mode<T, S, 1>(p, s);
-        case 2: return launch_skinny_mode<T, S, 2>(p, s);
-        case 4: return launch_skinny_mode<T, S, 4>(p, s);
-        default: return launch_skinny_mode<T, S, 0>(p, s);
-        }
+    if (plan.kernel == GROUPED_ANY) {
+        const int rows = (p.M + GROUPED_ROWS - 1) / GROUPED_ROWS;
+        return enqueue(&gemm_grouped_any_kernel<T, S>, dim3((p.N + 3) / 4, std::min(rows, 65535)), dim3(256), 0, s, p);
     }
-    const int rows = (p.M + GROUPED_ROWS - 1) / GROUPED_ROWS;
-    return enqueue(&gemm_grouped_any_kernel<T, S>, dim3((p.N + 3) / 4, std::min(rows, 65535)), dim3(256), 0, s, p);
+    hipError_t e;
+    switch (group_mode(p.group)) {
+    case 1: e = launch_mode<T, S, 1>(p, plan, s); break;
+    case 2: e = launch_mode<T, S, 2>(p, plan, s); break;
+    case 4: e = launch_mode<T, S, 4>(p, plan, s); break;
+    default: e = launch_mode<T, S, 0>(p, plan, s); break;
+    }
+    if (e != hipSuccess || plan.runs == 1) return e;
+    return enqueue(&gemm_grouped_join_kernel<T>, dim3((unsigned)std::min<size_t>(((size_t)p.M * p.N + 255) / 256, 4096)), dim3(256), 0, s, p, plan.runs);
 }
 
 }  // namespace qm
 
 using namespace qm;
 
-QM_EXPORT size_t qm_gemm_grouped_workspace_bytes(int, int, int, int, int) { return 0; }
+static int grouped_align(const void *x, long long x_stride, const void *B)
+{
+    (void)x;
+    const uintptr_t low = (uintptr_t)B;
+    return x_stride >= (1ll << 31) / 128 ? 1 : low & 15 ? (int)(low & (~low + 1)) : 16;  // (32-bit offsets of rows of x)
+}
+
+QM_EXPORT size_t qm_gemm_grouped_workspace_bytes(int m, int n, int k, int group, int align)
+{
+    if (m <= 0 || n <= 0 || k <= 0 || (k & 1) || group < 32 || group % 32 != 0) return 0;
+    return grouped_plan(m, n, k, align).bytes;
+}
 
 QM_EXPORT int qm_gemm_grouped_i4(const void *x, int dtype, long long x_stride, const void *B, const void *scale, int scale_dtype, int group,
                                  const void *bias, void *D, int m, int n, int k, void *stream, void *workspace, size_t workspace_bytes)
@@ -49,12 +92,14 @@ QM_EXPORT int qm_gemm_grouped_i4(const void *x, int dtype, long long x_stride, c
     if (m == 0 || n == 0) return QM_OK;
     if (!D || (k > 0 && (!x || !B || !scale))) return QM_ERR_NULL;
     if ((((uintptr_t)x | (uintptr_t)D | (uintptr_t)bias) & 1) || ((uintptr_t)scale & (scale_dtype == QM_IN_F32 ? 3 : 1)) || ((uintptr_t)workspace & 15)) return QM_ERR_ALIGN;
-    if (workspace_bytes < qm_gemm_grouped_workspace_bytes(m, n, k, group, 0)) return QM_ERR_SCRATCH;
+    const GroupedPlan plan = grouped_plan(m, n, k, grouped_align(x, m > 1 ? x_stride : 0, B));
+    if (plan.bytes > 0 && (!workspace || workspace_bytes < plan.bytes)) return QM_ERR_SCRATCH;
     const GroupedArgs p{static_cast<const uint16_t *>(x), static_cast<const uint8_t *>(B), scale, static_cast<const uint16_t *>(bias),
-                        static_cast<uint16_t *>(D), x_stride, m, n, k, group, (int)(((long long)k + group - 1) / group)};
+                        static_cast<uint16_t *>(D), m > 1 ? x_stride : k, m, n, k, group, (int)(((long long)k + group - 1) / group), 1, 0,
+                        plan.bytes > 0 ? static_cast<float *>(workspace) : nullptr};
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     hipError_t e;
-    if (dtype == QM_IN_F16) e = scale_dtype == QM_IN_F32 ? launch_grouped<QM_IN_F16, QM_IN_F32>(p, s) : launch_grouped<QM_IN_F16, QM_IN_F16>(p, s);
-    else e = scale_dtype == QM_IN_F32 ? launch_grouped<QM_IN_BF16, QM_IN_F32>(p, s) : launch_grouped<QM_IN_BF16, QM_IN_BF16>(p, s);
+    if (dtype == QM_IN_F16) e = scale_dtype == QM_IN_F32 ? launch_grouped<QM_IN_F16, QM_IN_F32>(p, plan, s) : launch_grouped<QM_IN_F16, QM_IN_F16>(p, plan, s);
+    else e = scale_dtype == QM_IN_F32 ? launch_grouped<QM_IN_BF16, QM_IN_F32>(p, plan, s) : launch_grouped<QM_IN_BF16, QM_IN_BF16>(p, plan, s);
     return e == hipSuccess ? QM_OK : fail_launch(e);
 }

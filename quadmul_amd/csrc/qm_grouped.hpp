@@ -13,6 +13,9 @@ struct GroupedArgs {
     uint16_t *D;
     long long x_stride;
     int M, N, K, group, groups;
+    int ways = 1;           // up to 16 rows: waves that share a tile of columns
+    int chunk = 0;          // K in runs of so many blocks of 32, each summed by workgroups of its own ...
+    float *part = nullptr;  // ... which leave their sums here, [runs, M, N], where there are several
 };
 
 // Any even K at any address: a wave to a column and four rows, a lane to a byte of B at a time, two elements of each
@@ -46,6 +49,8 @@ __global__ __launch_bounds__(256) void gemm_grouped_any_kernel(const GroupedArgs
     }
 }
 
+typedef uint32_t u32_half_aligned __attribute__((aligned(2)));
+
 // ---- on the matrix cores ------------------------------------------------------------------------------------------------------------
 //
 // D^T is not formed: x is the first operand of v_mfma_f32_16x16x32_{f16,bf16} and the weights the second, so that a lane ends up with
@@ -62,16 +67,19 @@ __global__ __launch_bounds__(256) void gemm_grouped_any_kernel(const GroupedArgs
 // columns share and which goes in front of their own: in float32, where it costs 2^-24 of 136 |sum of 32 x|.
 template <int T>
 struct GroupedWeights;
+// (v & mask) ^ put in one instruction: a nibble taken out, s turned into s + 8 (its sign bit over) and the exponent put above it
+__device__ __forceinline__ uint32_t and_xor(const uint32_t v, const uint32_t mask, const uint32_t put) { return __builtin_amdgcn_bitop3_b32(v, mask, put, 0x6A); }
 template <>
 struct GroupedWeights<QM_IN_F16> {
     typedef h8 frag;
     static constexpr bool OFFSET = false;
     static __device__ __forceinline__ frag of(const uint32_t w)
     {
-        const uint32_t t = w ^ 0x88888888u, t8 = t >> 8;
+        const uint32_t w8 = w >> 8;
         const h2 low = {(_Float16)-1032.0f, (_Float16)-1032.0f}, high = {(_Float16)-72.0f, (_Float16)-72.0f}, sixteenth = {(_Float16)0.0625f, (_Float16)0.0625f};
-        const auto pair = [](const uint32_t v, const uint32_t mask) { return __builtin_bit_cast(h2, (v & mask) | 0x64006400u); };
-        const h2 a = pair(t, 0x000F000Fu) + low, b = pair(t, 0x00F000F0u) * sixteenth + high, c = pair(t8, 0x000F000Fu) + low, d = pair(t8, 0x00F000F0u) * sixteenth + high;
+        const auto lower = [](const uint32_t v) { return __builtin_bit_cast(h2, and_xor(v, 0x000F000Fu, 0x64086408u)); };
+        const auto upper = [](const uint32_t v) { return __builtin_bit_cast(h2, and_xor(v, 0x00F000F0u, 0x64806480u)); };
+        const h2 a = lower(w) + low, b = upper(w) * sixteenth + high, c = lower(w8) + low, d = upper(w8) * sixteenth + high;
         return frag{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
     }
     static __device__ __forceinline__ v4f mfma(const frag a, const frag b, const v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
@@ -82,9 +90,8 @@ struct GroupedWeights<QM_IN_BF16> {
     static constexpr bool OFFSET = true;
     static __device__ __forceinline__ frag of(const uint32_t w)
     {
-        const uint32_t t = w ^ 0x88888888u;
-        const auto pair = [](const uint32_t v) { return (int)((v & 0x000F000Fu) | 0x43004300u); };
-        return __builtin_bit_cast(frag, (v4i{pair(t), pair(t >> 4), pair(t >> 8), pair(t >> 12)}));
+        const auto pair = [](const uint32_t v) { return (int)and_xor(v, 0x000F000Fu, 0x43084308u); };
+        return __builtin_bit_cast(frag, (v4i{pair(w), pair(w >> 4), pair(w >> 8), pair(w >> 12)}));
     }
     static __device__ __forceinline__ frag offset() { return __builtin_bit_cast(frag, (v4i{(int)0xC308C308u, (int)0xC308C308u, (int)0xC308C308u, (int)0xC308C308u})); }  // -136
     static __device__ __forceinline__ v4f mfma(const frag a, const frag b, const v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
@@ -109,136 +116,449 @@ __device__ __forceinline__ void turn_blocks(uint32_t (&w)[4])
     swap16(w[2], w[3]);
 }
 
-// How many scales four blocks have: groups of whole 128 (1), of 64 (2), of 32 (4), any other multiple of 32 (0).
-constexpr int group_mode(const int group) { return group % 128 == 0 ? 1 : group == 64 ? 2 : group == 32 ? 4 : 0; }
-
-// The scales of four blocks from block `block` on of one column: scale[i] belongs to block + i.
-template <int S, int MODE>
-__device__ __forceinline__ void load_scales(float (&scale)[4], const void *row, const int block, const int group, const int groups)
+// The same from loads in which four lanes side by side have the four blocks of a column, its 64 bytes: the memory pipeline takes 16 bytes of neighbours
+// together and of lanes 16 apart each by itself, four times as many accesses (a third of the time of 13 x 8192 x 28672). Lane 4 n + j has dwords 0..3 of block
+// j of column n; afterwards lane 16 c + 4 b + a has dword c of blocks 0..3 of column 4 a + b.
+__device__ __forceinline__ void gather_blocks(uint32_t (&w)[4])
 {
-    if constexpr (MODE == 1) {
-        const float s = element<S>(row, (size_t)min(block * 32 / group, groups - 1));
-        scale[0] = scale[1] = scale[2] = scale[3] = s;
-    } else {
+    turn_blocks(w);
+    const bool odd = threadIdx.x & 1, upper = threadIdx.x & 2;
+    const auto swap = [](uint32_t &a, uint32_t &b, const bool second, const auto neighbour) {
+        constexpr int CTRL = decltype(neighbour)::value;
+        const uint32_t to_a = __builtin_amdgcn_update_dpp(0, (int)b, CTRL, 0xF, 0xF, false), to_b = __builtin_amdgcn_update_dpp(0, (int)a, CTRL, 0xF, 0xF, false);
+        a = second ? to_a : a;
+        b = second ? b : to_b;
+    };
+    const std::integral_constant<int, 0xB1> next{};  // lanes 1 0 3 2
+    const std::integral_constant<int, 0x4E> over{};  // lanes 2 3 0 1
+    swap(w[0], w[1], odd, next);
+    swap(w[2], w[3], odd, next);
+    swap(w[0], w[2], upper, over);
+    swap(w[1], w[3], upper, over);
+}
+__device__ __forceinline__ int gathered_column(const int r) { return (r & 3) * 4 + (r >> 2); }
+
+// How many scales four blocks have: groups of 128 and its doubles (1), of 64 (2), of 32 (4); any other multiple of 32 (0).
+constexpr int group_mode(const int group) { return group % 128 == 0 && (group & (group - 1)) == 0 ? 1 : group == 64 ? 2 : group == 32 ? 4 : 0; }
+
+// Memory that a wave reads through a descriptor: a lane's offset and a shared one to a load, without arithmetic, and zeros past the end.
+struct Bytes {
+    __amdgpu_buffer_rsrc_t at;
+    __device__ __forceinline__ Bytes(const void *p, const size_t size)
+        : at(__builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, (int)(uint32_t)min(size, (size_t)0xFFFFFFFFu), 0x00020000))
+    {
+    }
+    __device__ __forceinline__ v4i load16(const uint32_t lane, const uint32_t shared) const { return __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(at, lane, shared, 0)); }
+    __device__ __forceinline__ v2i load8(const uint32_t lane, const uint32_t shared) const { return __builtin_bit_cast(v2i, __builtin_amdgcn_raw_buffer_load_b64(at, lane, shared, 0)); }
+    __device__ __forceinline__ uint32_t load4(const uint32_t lane, const uint32_t shared) const { return __builtin_amdgcn_raw_buffer_load_b32(at, lane, shared, 0); }
+    __device__ __forceinline__ uint32_t load2(const uint32_t lane, const uint32_t shared) const { return (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(at, lane, shared, 0); }
+};
+
+// The scales of four blocks of one column, as they are loaded: at(i) belongs to block i of the four. `to`: bytes to the lane's column. One load where
+// groups are 32 or 64; they are turned into floats when they are used, for a conversion waits for its load. 
+template <int S, int MODE>
+struct GroupedScales {
+    static constexpr bool WIDE = S == QM_IN_F32;
+    static constexpr int SB = WIDE ? 4 : 2, COUNT = MODE == 0 ? 4 : MODE, WORDS = WIDE ? COUNT : MODE == 0 ? 4 : (MODE + 1) / 2;
+    uint32_t raw[WORDS];
+    __device__ __forceinline__ void load(const Bytes &scales, const uint32_t to, const int block, const int group)
+    {
+        if constexpr (MODE == 0) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int at = MODE == 2 ? (block + i) / 2 : MODE == 4 ? block + i : (block + i) * 32 / group;
-            scale[i] = element<S>(row, (size_t)min(at, groups - 1));
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t at = (uint32_t)((block + i) * 32 / group * SB);
+                raw[i] = WIDE ? scales.load4(to, at) : scales.load2(to, at);
+            }
+        } else {
+            const uint32_t at = (uint32_t)((MODE == 1 ? block / 4 >> (__builtin_ctz(group) - 7) : block / (4 / COUNT)) * SB);
+            if constexpr (WORDS == 4) {
+                const v4i v = scales.load16(to, at);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) raw[i] = (uint32_t)v[i];
+            } else if constexpr (WORDS == 2) {
+                const v2i v = scales.load8(to, at);
+                raw[0] = (uint32_t)v[0], raw[1] = (uint32_t)v[1];
+            } else {
+                raw[0] = SB * COUNT == 4 ? scales.load4(to, at) : scales.load2(to, at);
+            }
         }
+    }
+    // one by one, the last of a row for those past it: a load that ends outside the memory gives zeros for all of a word
+    __device__ __forceinline__ void load_end(const Bytes &scales, const uint32_t to, const int block, const int group, const int groups)
+    {
+        const auto one = [&](const int i) {
+            const uint32_t at = (uint32_t)(min(MODE == 1 ? block / 4 >> (__builtin_ctz(group) - 7) : MODE == 0 ? (block + i) * 32 / group : block / (4 / COUNT) + i, groups - 1) * SB);
+            return WIDE ? scales.load4(to, at) : scales.load2(to, at);
+        };
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) raw[i] = WIDE || MODE < 2 ? one(i) : one(2 * i) | one(2 * i + 1) << 16;
+    }
+    __device__ __forceinline__ float at(const int i) const
+    {
+        const int k = MODE == 1 ? 0 : MODE == 2 ? i / 2 : i;
+        if constexpr (WIDE) return __builtin_bit_cast(float, raw[k]);
+        else if constexpr (MODE == 0 || MODE == 1) return float_of<S>((uint16_t)raw[k]);
+        else return float_of<S>((uint16_t)(raw[k / 2] >> (16 * (k & 1))));
+    }
+};
+
+// 32-bit offsets of lanes from addresses that the wave shares: no arithmetic of the lanes for a load.
+template <class V>
+__device__ __forceinline__ V at_offset(const uint8_t *base, const uint32_t offset) { return *reinterpret_cast<const V *>(base + offset); }
+
+// The scales of Q quads of one column, as they are loaded: at(i, run) belongs to block `run` of quad i.
+template <int S, int MODE, int Q>
+struct GroupedScaleSet {
+    static constexpr bool WIDE = S == QM_IN_F32;
+    static constexpr int SB = WIDE ? 4 : 2, COUNT = MODE == 0 ? 4 : MODE, ALL = Q * COUNT, WORDS = WIDE || MODE == 0 ? ALL : ALL / 2;
+    uint32_t raw[WORDS];
+    // scale number i of the set, whose first block is number `block` of the row
+    static __device__ __forceinline__ int index(const int block, const int i, const int group)
+    {
+        if constexpr (MODE == 0) return (block + i) * 32 / group;
+        else if constexpr (MODE == 1) return (block / 4 + i) >> (__builtin_ctz(group) - 7);
+        else return block / (4 / COUNT) + i;
+    }
+    __device__ __forceinline__ void load(const Bytes &scales, const uint32_t to, const int block, const int group, const int groups)
+    {
+        // one after the other in memory, and none of them past the end of the row: a load that ends outside the memory gives zeros for all of a word
+        const int first = index(block, 0, group);
+        if (MODE != 0 && (MODE != 1 || group == 128) && first + ALL <= groups) {
+#pragma unroll
+            for (int w = 0; w < WORDS; w += 4) {
+                const uint32_t at = (uint32_t)(first * SB + w * 4);
+                if constexpr (WORDS == 2) {
+                    const v2i v = scales.load8(to, at);
+                    raw[0] = (uint32_t)v[0], raw[1] = (uint32_t)v[1];
+                } else {
+                    const v4i v = scales.load16(to, at);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) raw[w + e] = (uint32_t)v[e];
+                }
+            }
+        } else {
+            const auto one = [&](const int i) {
+                const uint32_t at = (uint32_t)(min(index(block, i, group), groups - 1) * SB);
+                return WIDE ? scales.load4(to, at) : scales.load2(to, at);
+            };
+#pragma unroll
+            for (int i = 0; i < WORDS; ++i) raw[i] = WORDS == ALL ? one(i) : one(2 * i) | one(2 * i + 1) << 16;
+        }
+    }
+    // (what turns a loaded scale into a float stays where this is called: moved up to the load, it would wait for it)
+    __device__ __forceinline__ void arrive()
+    {
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) asm("" : "+v"(raw[i]));
+    }
+    __device__ __forceinline__ float at(const int quad, const int run) const
+    {
+        const int i = MODE == 1 ? quad : MODE == 2 ? quad * 2 + run / 2 : quad * 4 + run;
+        if constexpr (WIDE) return __builtin_bit_cast(float, raw[i]);
+        else if constexpr (WORDS == ALL) return float_of<S>((uint16_t)raw[i]);
+        else return float_of<S>((uint16_t)(raw[i / 2] >> (16 * (i & 1))));
+    }
+};
+
+// Up to 16 rows. A workgroup has a run of K (all of it where that fits) of x in its LDS, in the order that the first operand wants it, paired, and goes
+// through tiles of columns. A wave has 16 columns and an equal share of the run's quads (four blocks, 64 bytes of each column): `ways` waves share a
+// tile, and their sums meet in the LDS. Bound by the weights' way from HBM: eight quads of a wave are in flight, from the next tile too;
+// and by what a quad costs of the vector pipeline: about 70 instructions a kilobyte, of which 30 make floats of the weights; 6 TB/s leave it 90.
+// (With x from the L2 by each wave for itself, 4 KiB of x for a KiB or two of weights, 13 x 8192 x 28672 took 52 us; with x put into the LDS
+// by 832 workgroups 45.)
+constexpr int GROUPED_WAVES = 16;
+template <int T, int S, int MODE>
+__global__ __launch_bounds__(GROUPED_WAVES * 64, 4) void gemm_grouped_rows_kernel(const GroupedArgs p)
+{
+    typedef GroupedWeights<T> W;
+    typedef typename W::frag frag;
+    // SET: quads that are loaded at a time, one set ahead; PER: blocks of one scale
+    constexpr int NW = GROUPED_WAVES, SET = MODE == 1 || MODE == 2 ? 4 : 2, RING = 2, PER = MODE == 1 ? 4 : MODE == 2 ? 2 : 1;
+    typedef GroupedScaleSet<S, MODE, SET> Scales;
+    extern __shared__ v4i staged[];
+    __shared__ v4f sums[NW][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, c = lane >> 4;
+    const int block0 = blockIdx.y * p.chunk, blocks = min(p.chunk, p.K / 32 - block0), quads = (blocks + 3) / 4;
+    const int pitch = p.M | 1;                                                           // rows of 16 bytes for eight k
+    v4f *const offsets = reinterpret_cast<v4f *>(staged + (size_t)p.chunk * 4 * pitch);  // -136 times the sums of x, for each scale and four rows
+
+    // the waves' tiles, side by side; a wave's turns: sets of four quads of one tile after the other
+    const int abreast = NW / p.ways, groups = ((p.N + 15) / 16 + abreast - 1) / abreast;
+    const int each = (quads + p.ways - 1) / p.ways, quad0 = min(wave % p.ways * each, quads), quad1 = min(quad0 + each, quads);
+    const int sets = (quad1 - quad0 + SET - 1) / SET, mine = ((int)blockIdx.x < groups ? (groups - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0);
+    const auto column0 = [&](const int group) { return (group * abreast + wave / p.ways) * 16; };
+    // (columns past the last one, and blocks past the end of K in the last row, are zeros past the end)
+    const uint32_t w_at = (lane >> 2) * (uint32_t)(p.K / 2) + 16 * (lane & 3), s_at = gathered_column(r) * (uint32_t)(p.groups * Scales::SB);
+    const size_t w_all = (size_t)p.N * (p.K / 2), s_all = (size_t)p.N * p.groups * Scales::SB;
+    struct Set {
+        v4i w[SET];
+        Scales s;
+    };
+    int load_group = blockIdx.x, load_quad = quad0;
+    const auto load = [&](Set &to) {
+        const int n0 = column0(load_group);
+        const size_t w_from = min((size_t)n0 * (p.K / 2) + (size_t)block0 * 16, w_all), s_from = min((size_t)n0 * p.groups * Scales::SB, s_all);
+        const Bytes weights(p.B + w_from, w_all - w_from), scales(static_cast<const uint8_t *>(p.scale) + s_from, s_all - s_from);
+#pragma unroll
+        for (int i = 0; i < SET; ++i) to.w[i] = weights.load16(w_at, (load_quad + i) * 64);
+        to.s.load(scales, s_at, block0 + load_quad * 4, p.group, p.groups);
+        load_quad += SET;
+        if (load_quad >= quad1) load_quad = quad0, load_group += gridDim.x;
+    };
+
+    // x first, for it is waited for first (four loads of a thread at a time); the weights are in flight while it is put in place
+    constexpr int BATCH = 4, THREADS = NW * 64;
+    const int units = quads * 16, all = units * p.M;
+    v4i x[BATCH];
+    const auto get = [&](const int from) {
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+            const int at = min(from + i * THREADS + (int)threadIdx.x, all - 1), m = at / units, k = min(at - m * units, blocks * 4 - 1);
+            if (from + i * THREADS < all) x[i] = *reinterpret_cast<const v4i_half_aligned *>(p.x + m * p.x_stride + (size_t)(block0 * 4 + k) * 8);
+        }
+    };
+    const auto put_in_place = [&](const int from) {
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+            const int at = from + i * THREADS + (int)threadIdx.x, m = at / units, k = at - m * units;
+            if (at < all) staged[k * pitch + m] = k < blocks * 4 ? paired(x[i]) : v4i{};
+        }
+    };
+    get(0);
+    Set ring[RING];
+    const int turns = mine * sets;
+#pragma unroll
+    for (int i = 0; i < RING - 1; ++i)
+        if (i < turns) load(ring[i]);
+    put_in_place(0);
+    for (int from = BATCH * THREADS; from < all; from += BATCH * THREADS) {
+        get(from);
+        put_in_place(from);
+    }
+    __syncthreads();
+    const v4i *const my_x = staged + c * pitch + min(r, p.M - 1);
+    const auto x_frag = [&](const int block) { return __builtin_bit_cast(frag, my_x[block * 4 * pitch]); };
+    if constexpr (W::OFFSET) {
+        for (int i = wave; i < quads * 4 / PER; i += NW) {
+            v4f sum = {};
+#pragma unroll
+            for (int j = 0; j < PER; ++j) sum = W::mfma(x_frag(i * PER + j), W::offset(), sum);
+            if (r == 0) offsets[i * 4 + c] = sum;
+        }
+        __syncthreads();
+    }
+
+    v4f total = {};
+    const auto use = [&](Set &in, const int quad) {
+        in.s.arrive();
+#pragma unroll
+        for (int q = 0; q < SET; ++q) {
+            if (quad + q >= quad1) break;
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = (uint32_t)in.w[q][i];
+            gather_blocks(w);
+#pragma unroll
+            for (int run = 0; run < 4; run += PER) {
+                v4f part = {};
+                if constexpr (W::OFFSET) part = offsets[((quad + q) * 4 + run) / PER * 4 + c];
+#pragma unroll
+                for (int i = run; i < run + PER; ++i) part = W::mfma(x_frag((quad + q) * 4 + i), W::of(w[i]), part);
+                total += part * in.s.at(q, run);
+            }
+        }
+    };
+    const auto put = [&](const int m, const int column, const float v) {
+        if (m >= p.M || column >= p.N) return;
+        if (p.part != nullptr) p.part[((size_t)blockIdx.y * p.M + m) * p.N + column] = v;
+        else p.D[(size_t)m * p.N + column] = round16<T>(p.bias != nullptr ? v + float_of<T>(p.bias[column]) : v);
+    };
+    const auto finish = [&](const int group) {
+        if (p.ways == 1) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) put(4 * c + i, column0(group) + gathered_column(r), total[i]);
+        } else {
+            __syncthreads();  // (the group before is read)
+            sums[wave][lane] = total;
+            __syncthreads();
+            for (int i = threadIdx.x; i < abreast * 256; i += THREADS) {
+                const int tile = i >> 8, column = i & 15, m = (i >> 4) & 15;
+                float v = 0.0f;
+                for (int w = 0; w < p.ways; ++w) v += sums[tile * p.ways + w][gathered_column(column) + 16 * (m >> 2)][m & 3];  // (its own inverse)
+                put(m, (group * abreast + tile) * 16 + column, v);
+            }
+        }
+        total = v4f{};
+    };
+    int group = blockIdx.x, quad = quad0;
+    for (int done = 0; done < turns; done += RING) {
+#pragma unroll
+        for (int i = 0; i < RING; ++i) {
+            if (done + i >= turns) break;
+            if (done + i + RING - 1 < turns) load(ring[(i + RING - 1) % RING]);
+            use(ring[i], quad);
+            quad += SET;
+            if (quad >= quad1) {
+                finish(group);
+                quad = quad0, group += gridDim.x;
+            }
+        }
+    }
+    if (sets == 0)  // (a share of nothing: the others wait for it)
+        for (; group < groups; group += gridDim.x) finish(group);
+}
+
+// The sums of the runs of K into one, always in the same order.
+template <int T>
+__global__ __launch_bounds__(256) void gemm_grouped_join_kernel(const GroupedArgs p, const int runs)
+{
+    const size_t all = (size_t)p.M * p.N;
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (size_t)gridDim.x * 256) {
+        float v = 0.0f;
+#pragma unroll 8
+        for (int run = 0; run < runs; ++run) v += p.part[run * all + i];
+        p.D[i] = round16<T>(p.bias != nullptr ? v + float_of<T>(p.bias[i % p.N]) : v);
     }
 }
 
-// Up to 16 MT rows: a workgroup has 16 NT columns, its waves take turns at 256 elements of K (one line of every row of B) and their sums meet in the
-// LDS. x comes from the L2, where the workgroups share it. Bound by the weights' way from HBM: two turns of every wave are in
-// flight.
-template <int T, int S, int MODE, int MT, int NT, int NW>
+// Up to 16 MT rows: a workgroup has 16 NT columns, its waves take turns at 256 elements of K (one line of every row of B) in two halves, and
+// their sums meet in the LDS. Bound by the weights' way from HBM: the next DEPTH - 1 halves of every wave are in flight. What a half needs of x
+// (from the L2, where the workgroups share it) is loaded with its weights: loads are waited for in their order, and x loaded when it is needed, in
+// 53 us instead of 31 for 13 x 8192 x 28672, would have all weights asked for before it waited for too.
+template <int T, int S, int MODE, int MT, int NT, int NW, int DEPTH>
 __global__ __launch_bounds__(NW * 64, 2) void gemm_grouped_skinny_kernel(const GroupedArgs p)
 {
     typedef GroupedWeights<T> W;
     typedef typename W::frag frag;
     __shared__ v4f sums[NW][MT * NT][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, c = lane >> 4;
-    const int blocks = p.K / 32, turns = (blocks + 7) / 8, n0 = blockIdx.x * 16 * NT;
+    const int blocks = p.K / 32, quads = (blocks + 3) / 4, n0 = blockIdx.x * 16 * NT;
+    typedef GroupedScales<S, MODE> Scales;
 
-    const uint8_t *row[NT];
-    const uint8_t *scales[NT];
-    constexpr int SB = S == QM_IN_F32 ? 4 : 2;
+    const uint8_t *const weights = p.B + (size_t)n0 * (p.K / 2);
+    const size_t s_from = (size_t)n0 * p.groups * Scales::SB;
+    const Bytes scales(static_cast<const uint8_t *>(p.scale) + s_from, (size_t)p.N * p.groups * Scales::SB - s_from);
+    uint32_t w_at[NT], s_at[NT], x_at[MT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        const int n = min(n0 + 16 * t + r, p.N - 1);
-        row[t] = p.B + (size_t)n * (p.K / 2);
-        scales[t] = static_cast<const uint8_t *>(p.scale) + (size_t)n * p.groups * SB;
+        const uint32_t n = min(16 * t + r, p.N - 1 - n0);
+        w_at[t] = n * (uint32_t)(p.K / 2), s_at[t] = n * (uint32_t)(p.groups * Scales::SB);
     }
-    const uint16_t *x[MT];
 #pragma unroll
-    for (int t = 0; t < MT; ++t) x[t] = p.x + min(16 * t + r, p.M - 1) * p.x_stride + 8 * c;
+    for (int t = 0; t < MT; ++t) x_at[t] = (uint32_t)(min(16 * t + r, p.M - 1) * p.x_stride * 2) + 16 * c;
+    const uint8_t *const x = reinterpret_cast<const uint8_t *>(p.x);
 
-    struct Turn {
-        v4i w[NT][2];
-        float s[NT][2][4];
+    struct Half {
+        v4i x[MT][4];
+        v4i w[NT];
+        Scales s[NT];
     };
-    const auto load = [&](Turn &to, const int turn) {
+    // a wave's i-th half is at four blocks number ..; `quads` or more for none
+    const int turns = (quads + 1) / 2, shift = ((blockIdx.x >> 3) * 5 & 15) * turns >> 4;
+    const auto quad = [&](const int i) {
+        const int turn = wave + NW * (i >> 1), at = turn + shift;
+        return turn < turns ? (at < turns ? at : at - turns) * 2 + (i & 1) : quads;
+    };
+    const auto more = [&](const int i) { return wave + NW * (i >> 1) < turns; };
+    const auto load = [&](Half &to, const int at) {
+        const bool whole = at * 4 + 4 <= blocks;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int block = min(at * 4 + i, blocks - 1);
+#pragma unroll
+            for (int t = 0; t < MT; ++t) to.x[t][i] = at_offset<v4i_half_aligned>(x + (size_t)block * 64, x_at[t]);
+        }
+        const uint32_t mine = whole ? 16 * c : 16 * min(c, blocks - 1 - at * 4);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                to.w[t][h] = *reinterpret_cast<const v4i *>(row[t] + (size_t)min(turn * 8 + 4 * h + c, blocks - 1) * 16);
-                load_scales<S, MODE>(to.s[t][h], scales[t], turn * 8 + 4 * h, p.group, p.groups);
-            }
+            to.w[t] = at_offset<v4i>(weights + (size_t)at * 64, w_at[t] + mine);
+            if (whole) to.s[t].load(scales, s_at[t], at * 4, p.group);
+            else to.s[t].load_end(scales, s_at[t], at * 4, p.group, p.groups);
         }
     };
     v4f total[MT][NT] = {};
-    const auto use = [&](Turn &in, const int turn) {
+    const auto use = [&](Half &in, const int at) {
+        v4i xs[MT][4];
+        uint32_t w[NT][4];
+        // (what turns a loaded scale into a float stays here: moved up to the load, it would wait for it and everything before it)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int block = turn * 8 + 4 * h;
-            if (block >= blocks) break;
-            v4i xs[MT][4];
+        for (int t = 0; t < NT; ++t) {
+#pragma unroll
+            for (int i = 0; i < Scales::WORDS; ++i) asm("" : "+v"(in.s[t].raw[i]));
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+#pragma unroll
+            for (int t = 0; t < MT; ++t) xs[t][i] = paired(in.x[t][i]);
+        }
+        if (at * 4 + 4 > blocks) {  // past the end of K: zeros of x, whatever the weights are
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
 #pragma unroll
-                for (int t = 0; t < MT; ++t) xs[t][i] = paired(*reinterpret_cast<const v4i_half_aligned *>(x[t] + (size_t)min(block + i, blocks - 1) * 32));
+                for (int t = 0; t < MT; ++t) xs[t][i] = at * 4 + i < blocks ? xs[t][i] : v4i{};
             }
-            uint32_t w[NT][4];
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[t][i] = (uint32_t)in.w[t][i];
+            turn_blocks(w[t]);
+        }
+        constexpr int PER = MODE == 1 ? 4 : MODE == 2 ? 2 : 1;  // blocks of one scale
+#pragma unroll
+        for (int run = 0; run < 4; run += PER) {
+            v4f part[MT][NT];
+#pragma unroll
+            for (int a = 0; a < MT; ++a) {
+                v4f begin = {};
+                if constexpr (W::OFFSET) {
+#pragma unroll
+                    for (int i = run; i < run + PER; ++i) begin = W::mfma(__builtin_bit_cast(frag, xs[a][i]), W::offset(), begin);
+                }
+#pragma unroll
+                for (int t = 0; t < NT; ++t) part[a][t] = begin;
+            }
+#pragma unroll
+            for (int i = run; i < run + PER; ++i) {
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    const frag four_bits = W::of(w[t][i]);
+#pragma unroll
+                    for (int a = 0; a < MT; ++a) part[a][t] = W::mfma(__builtin_bit_cast(frag, xs[a][i]), four_bits, part[a][t]);
+                }
+            }
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
+                const float scale = in.s[t].at(run);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) w[t][i] = (uint32_t)in.w[t][h][i];
-                turn_blocks(w[t]);
-            }
-            constexpr int PER = MODE == 1 ? 4 : MODE == 2 ? 2 : 1;  // blocks of one scale
-#pragma unroll
-            for (int run = 0; run < 4; run += PER) {
-                v4f part[MT][NT];
-#pragma unroll
-                for (int a = 0; a < MT; ++a) {
-                    v4f begin = {};
-                    if constexpr (W::OFFSET) {
-#pragma unroll
-                        for (int i = run; i < run + PER; ++i)
-                            if (block + i < blocks) begin = W::mfma(__builtin_bit_cast(frag, xs[a][i]), W::offset(), begin);
-                    }
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) part[a][t] = begin;
-                }
-#pragma unroll
-                for (int i = run; i < run + PER; ++i) {
-                    if (block + i >= blocks) break;
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) {
-                        const frag weights = W::of(w[t][i]);
-#pragma unroll
-                        for (int a = 0; a < MT; ++a) part[a][t] = W::mfma(__builtin_bit_cast(frag, xs[a][i]), weights, part[a][t]);
-                    }
-                }
-                if (block + run < blocks) {
-#pragma unroll
-                    for (int a = 0; a < MT; ++a) {
-#pragma unroll
-                        for (int t = 0; t < NT; ++t) total[a][t] += part[a][t] * in.s[t][h][run];
-                    }
-                }
+                for (int a = 0; a < MT; ++a) total[a][t] += part[a][t] * scale;
             }
         }
     };
 
-    // two turns ahead, in three sets of registers
-    Turn one, two, three;
-    int turn = wave;
-    if (turn < turns) load(one, turn);
-    if (turn + NW < turns) load(two, turn + NW);
-    while (turn < turns) {
-        if (turn + 2 * NW < turns) load(three, turn + 2 * NW);
-        use(one, turn);
-        turn += NW;
-        if (turn >= turns) break;
-        if (turn + 2 * NW < turns) load(one, turn + 2 * NW);
-        use(two, turn);
-        turn += NW;
-        if (turn >= turns) break;
-        if (turn + 2 * NW < turns) load(two, turn + 2 * NW);
-        use(three, turn);
-        turn += NW;
+    // (no load of the loop behind a condition: what comes out of one is widened, and so waited for, where the branches meet)
+    Half halves[DEPTH];
+    int first = 0;
+    const auto get = [&](Half &to, const int i) { load(to, min(quad(i), quads - 1)); };
+    const auto put = [&](Half &in, const int i) {
+        const int at = quad(i);
+        if (at < quads) use(in, at);
+    };
+#pragma unroll
+    for (int i = 0; i < DEPTH - 1; ++i) get(halves[i], i);
+    for (; more(first + 2 * DEPTH - 2); first += DEPTH) {
+#pragma unroll
+        for (int i = 0; i < DEPTH; ++i) {
+            get(halves[(i + DEPTH - 1) % DEPTH], first + i + DEPTH - 1);
+            put(halves[i], first + i);
+        }
+    }
+    // the last DEPTH - 1 to 2 DEPTH - 2 halves
+#pragma unroll
+    for (int i = 0; i < 2 * DEPTH - 2; ++i) {
+        if (!more(first + i)) break;
+        if (i < DEPTH - 1) get(halves[(i + DEPTH - 1) % DEPTH], first + i + DEPTH - 1);
+        put(halves[i % DEPTH], first + i);
     }
 
 #pragma unroll
