@@ -292,7 +292,7 @@ typedef struct qm_kv_cache {
  * New keys and values into the cache, the keys rotated to their positions on the way; the queries, rotated, in the same call.
  * Rotation of a head at position p, for pair i of rotary_pairs: (a, b) -> (a c - b s, b c + a s) with c = cos[p][i], s = sin[p][i]
  * ([positions, rotary_pairs] float32); (a, b) are elements i and i + rotary_pairs, or 2i and 2i + 1 with interleaved = 1; further
- * elements stay as they are; rotary_pairs = 0: no rotation.  A position at or past `positions` gives NaN.
+ * elements stay as they are; rotary_pairs = 0: no rotation, else positions is 1 or more.  A position at or past `positions` gives NaN.
  * Storing, for each page, head and side, in single precision, every operation rounded by itself:
  *   scale' = max(scale, amax * (1 / 127)), amax over the new tokens of the page; scale counts as 0 in a page
  *            whose first token is new, which begins anew: all its other codes become 0

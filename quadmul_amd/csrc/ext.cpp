@@ -322,8 +322,8 @@ c10::optional<torch::Tensor> kv_append(torch::Tensor k, torch::Tensor v, torch::
     TORCH_CHECK(cos.has_value() == sin.has_value(), what, ": cos and sin go together");
     if (cos.has_value()) {
         const auto table = [&](const torch::Tensor &t) { return t.device() == cache_k.device() && t.scalar_type() == torch::kFloat32 && t.dim() == 2 && t.is_contiguous(); };
-        TORCH_CHECK(table(*cos) && table(*sin) && cos->sizes() == sin->sizes() && 2 * cos->size(1) <= c.head_dim && cos->size(0) <= INT32_MAX, what,
-                    ": cos and sin must be contiguous float32 tensors [positions, at most ", c.head_dim / 2, "] on the cache's device");
+        TORCH_CHECK(table(*cos) && table(*sin) && cos->sizes() == sin->sizes() && 2 * cos->size(1) <= c.head_dim && cos->size(0) >= 1 && cos->size(0) <= INT32_MAX, what,
+                    ": cos and sin must be contiguous float32 tensors [1 position or more, at most ", c.head_dim / 2, "] on the cache's device");
     }
     c10::OptionalDeviceGuard guard(cache_k.device());
     c10::optional<torch::Tensor> out;

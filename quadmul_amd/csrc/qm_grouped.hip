@@ -12,7 +12,7 @@
 namespace qm {
 
 // Which kernel runs, and what it needs.
-enum GroupedKernel { GROUPED_ANY, GROUPED_ROWS16, GROUPED_SKINNY };
+enum GroupedKernel { GROUPED_ANY, GROUPED_ROWS16, GROUPED_TILE };
 struct GroupedPlan {
     GroupedKernel kernel;
     int ways, chunk, runs;  // waves to a tile of columns; blocks of 32 of K in a run, runs
@@ -21,8 +21,19 @@ struct GroupedPlan {
 static GroupedPlan grouped_plan(int m, int n, int k, int align)
 {
     GroupedPlan p{GROUPED_ANY, 1, 0, 1, 0};
-    if (k == 0 || k % 32 != 0 || align < 16 || m > 64) return p;
-    if (m > 16) { p.kernel = GROUPED_SKINNY; return p; }
+    if (k == 0 || k % 32 != 0 || align < 16) return p;
+    if (m > 16 && n > 65535 * 64) return p;  // (the grid's limit)
+    if (m > 16) {
+        p.kernel = GROUPED_TILE;
+        const int quads = (k / 32 + 3) / 4;
+        // a workgroup to a CU at least, of eight steps of K or more
+        const long long tiles = (long long)((m + (m > 64 ? 127 : m > 32 ? 63 : 31)) / (m > 64 ? 128 : m > 32 ? 64 : 32)) * ((n + 127) / 128);
+        p.runs = (int)std::max<long long>(1, std::min<long long>(256 / tiles, quads / 8));
+        p.chunk = (quads + p.runs - 1) / p.runs * 4;
+        p.runs = (k / 32 + p.chunk - 1) / p.chunk;
+        if (p.runs > 1) p.bytes = (size_t)p.runs * m * n * sizeof(float);
+        return p;
+    }
     p.kernel = GROUPED_ROWS16;
     // what a workgroup holds of x: 128 KiB, beside the sums; one workgroup to a CU
     const int blocks = k / 32, most = (128 << 10) / (64 * (m | 1) + 64) / 8 * 8;
@@ -37,10 +48,14 @@ static GroupedPlan grouped_plan(int m, int n, int k, int align)
 template <int T, int S, int MODE>
 static hipError_t launch_mode(GroupedArgs p, const GroupedPlan &plan, hipStream_t s)
 {
-    constexpr int NW = 8;
-    const auto go = [&](auto kernel, int nt) { return enqueue(kernel, dim3((p.N + 16 * nt - 1) / (16 * nt)), dim3(NW * 64), 0, s, p); };
-    if (plan.kernel == GROUPED_SKINNY) return p.M <= 32 ? go(&gemm_grouped_skinny_kernel<T, S, MODE, 2, 2, NW, 2>, 2) : go(&gemm_grouped_skinny_kernel<T, S, MODE, 4, 2, NW, 2>, 2);
     p.chunk = plan.chunk, p.ways = plan.ways;
+    if (plan.kernel == GROUPED_TILE) {
+        const auto go = [&](auto kernel, int bm, int bn) { return enqueue(kernel, dim3((p.M + bm - 1) / bm, (p.N + bn - 1) / bn, plan.runs), dim3(256), 0, s, p); };
+        // (with a scale to every one or two blocks the registers of 128 columns do not fit)
+        if (p.M > 64 && MODE == 1) return go(&gemm_grouped_tile_kernel<T, S, MODE, 2, 4, 4>, 128, 128);
+        if (p.M > 64) return go(&gemm_grouped_tile_kernel<T, S, MODE, 2, 4, 2>, 128, 64);
+        return p.M > 32 ? go(&gemm_grouped_tile_kernel<T, S, MODE, 1, 4, 2>, 64, 128) : go(&gemm_grouped_tile_kernel<T, S, MODE, 1, 2, 2>, 32, 128);
+    }
     const int tiles = GROUPED_WAVES / plan.ways, groups = ((p.N + 15) / 16 + tiles - 1) / tiles;
     const size_t lds = (size_t)plan.chunk * (64 * (p.M | 1) + 64);
     static std::atomic<bool> known[QM_MAX_DEVICES] = {};
@@ -74,7 +89,7 @@ static int grouped_align(const void *x, long long x_stride, const void *B)
 {
     (void)x;
     const uintptr_t low = (uintptr_t)B;
-    return x_stride >= (1ll << 31) / 128 ? 1 : low & 15 ? (int)(low & (~low + 1)) : 16;  // (32-bit offsets of rows of x)
+    return x_stride >= (1ll << 31) / 512 ? 1 : low & 15 ? (int)(low & (~low + 1)) : 16;  // (32-bit offsets of rows of x)
 }
 
 QM_EXPORT size_t qm_gemm_grouped_workspace_bytes(int m, int n, int k, int group, int align)

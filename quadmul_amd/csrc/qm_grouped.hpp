@@ -49,8 +49,6 @@ __global__ __launch_bounds__(256) void gemm_grouped_any_kernel(const GroupedArgs
     }
 }
 
-typedef uint32_t u32_half_aligned __attribute__((aligned(2)));
-
 // ---- on the matrix cores ------------------------------------------------------------------------------------------------------------
 //
 // D^T is not formed: x is the first operand of v_mfma_f32_16x16x32_{f16,bf16} and the weights the second, so that a lane ends up with
@@ -154,63 +152,11 @@ struct Bytes {
     __device__ __forceinline__ uint32_t load2(const uint32_t lane, const uint32_t shared) const { return (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(at, lane, shared, 0); }
 };
 
-// The scales of four blocks of one column, as they are loaded: at(i) belongs to block i of the four. `to`: bytes to the lane's column. One load where
-// groups are 32 or 64; they are turned into floats when they are used, for a conversion waits for its load. 
-template <int S, int MODE>
-struct GroupedScales {
-    static constexpr bool WIDE = S == QM_IN_F32;
-    static constexpr int SB = WIDE ? 4 : 2, COUNT = MODE == 0 ? 4 : MODE, WORDS = WIDE ? COUNT : MODE == 0 ? 4 : (MODE + 1) / 2;
-    uint32_t raw[WORDS];
-    __device__ __forceinline__ void load(const Bytes &scales, const uint32_t to, const int block, const int group)
-    {
-        if constexpr (MODE == 0) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t at = (uint32_t)((block + i) * 32 / group * SB);
-                raw[i] = WIDE ? scales.load4(to, at) : scales.load2(to, at);
-            }
-        } else {
-            const uint32_t at = (uint32_t)((MODE == 1 ? block / 4 >> (__builtin_ctz(group) - 7) : block / (4 / COUNT)) * SB);
-            if constexpr (WORDS == 4) {
-                const v4i v = scales.load16(to, at);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) raw[i] = (uint32_t)v[i];
-            } else if constexpr (WORDS == 2) {
-                const v2i v = scales.load8(to, at);
-                raw[0] = (uint32_t)v[0], raw[1] = (uint32_t)v[1];
-            } else {
-                raw[0] = SB * COUNT == 4 ? scales.load4(to, at) : scales.load2(to, at);
-            }
-        }
-    }
-    // one by one, the last of a row for those past it: a load that ends outside the memory gives zeros for all of a word
-    __device__ __forceinline__ void load_end(const Bytes &scales, const uint32_t to, const int block, const int group, const int groups)
-    {
-        const auto one = [&](const int i) {
-            const uint32_t at = (uint32_t)(min(MODE == 1 ? block / 4 >> (__builtin_ctz(group) - 7) : MODE == 0 ? (block + i) * 32 / group : block / (4 / COUNT) + i, groups - 1) * SB);
-            return WIDE ? scales.load4(to, at) : scales.load2(to, at);
-        };
-#pragma unroll
-        for (int i = 0; i < WORDS; ++i) raw[i] = WIDE || MODE < 2 ? one(i) : one(2 * i) | one(2 * i + 1) << 16;
-    }
-    __device__ __forceinline__ float at(const int i) const
-    {
-        const int k = MODE == 1 ? 0 : MODE == 2 ? i / 2 : i;
-        if constexpr (WIDE) return __builtin_bit_cast(float, raw[k]);
-        else if constexpr (MODE == 0 || MODE == 1) return float_of<S>((uint16_t)raw[k]);
-        else return float_of<S>((uint16_t)(raw[k / 2] >> (16 * (k & 1))));
-    }
-};
-
-// 32-bit offsets of lanes from addresses that the wave shares: no arithmetic of the lanes for a load.
-template <class V>
-__device__ __forceinline__ V at_offset(const uint8_t *base, const uint32_t offset) { return *reinterpret_cast<const V *>(base + offset); }
-
 // The scales of Q quads of one column, as they are loaded: at(i, run) belongs to block `run` of quad i.
 template <int S, int MODE, int Q>
 struct GroupedScaleSet {
     static constexpr bool WIDE = S == QM_IN_F32;
-    static constexpr int SB = WIDE ? 4 : 2, COUNT = MODE == 0 ? 4 : MODE, ALL = Q * COUNT, WORDS = WIDE || MODE == 0 ? ALL : ALL / 2;
+    static constexpr int SB = WIDE ? 4 : 2, COUNT = MODE == 0 ? 4 : MODE, ALL = Q * COUNT, WORDS = WIDE || MODE == 0 || ALL == 1 ? ALL : ALL / 2;
     uint32_t raw[WORDS];
     // scale number i of the set, whose first block is number `block` of the row
     static __device__ __forceinline__ int index(const int block, const int i, const int group)
@@ -227,7 +173,9 @@ struct GroupedScaleSet {
 #pragma unroll
             for (int w = 0; w < WORDS; w += 4) {
                 const uint32_t at = (uint32_t)(first * SB + w * 4);
-                if constexpr (WORDS == 2) {
+                if constexpr (WORDS == 1) {
+                    raw[0] = SB * ALL == 4 ? scales.load4(to, at) : scales.load2(to, at);
+                } else if constexpr (WORDS == 2) {
                     const v2i v = scales.load8(to, at);
                     raw[0] = (uint32_t)v[0], raw[1] = (uint32_t)v[1];
                 } else {
@@ -421,159 +369,133 @@ __global__ __launch_bounds__(256) void gemm_grouped_join_kernel(const GroupedArg
     }
 }
 
-// Up to 16 MT rows: a workgroup has 16 NT columns, its waves take turns at 256 elements of K (one line of every row of B) in two halves, and
-// their sums meet in the LDS. Bound by the weights' way from HBM: the next DEPTH - 1 halves of every wave are in flight. What a half needs of x
-// (from the L2, where the workgroups share it) is loaded with its weights: loads are waited for in their order, and x loaded when it is needed, in
-// 53 us instead of 31 for 13 x 8192 x 28672, would have all weights asked for before it waited for too.
-template <int T, int S, int MODE, int MT, int NT, int NW, int DEPTH>
-__global__ __launch_bounds__(NW * 64, 2) void gemm_grouped_skinny_kernel(const GroupedArgs p)
+// More rows: tiles of 16 WM MT rows and 64 NT / WM columns, a step of four blocks (128 elements of K) at a time. x goes through the LDS, two steps of it, in
+// the order of the first operand; a wave makes the second operand of its 16 NT columns itself, from 64 bytes of each. The sums over a group
+// and those over all of K are in registers of their own. Bound by the matrix cores and, nearly as much, by the instructions that make
+// floats of the weights (46 for a tile of 16 columns and a step, against 16 MT cycles of matrix instructions each).
+// A row's 16 pieces of a step are dealt to the places r ^ piece, so that neither writing 16 of one row nor reading one of 16 rows meets a bank twice.
+template <int T, int S, int MODE, int WM, int MT, int NT>
+__global__ __launch_bounds__(256, 2) void gemm_grouped_tile_kernel(const GroupedArgs p)
 {
     typedef GroupedWeights<T> W;
     typedef typename W::frag frag;
-    __shared__ v4f sums[NW][MT * NT][64];
+    typedef GroupedScaleSet<S, MODE, 1> Scales;
+    constexpr int PER = MODE == 1 ? 4 : MODE == 2 ? 2 : 1, BM = 16 * WM * MT, BN = 64 / WM * NT, PIECES = BM / 16;  // PIECES: of x, 16 bytes each, of a thread and step
+    __shared__ v4i staged[2][4 * BM * 4];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, c = lane >> 4;
-    const int blocks = p.K / 32, quads = (blocks + 3) / 4, n0 = blockIdx.x * 16 * NT;
-    typedef GroupedScales<S, MODE> Scales;
+    const int block0 = blockIdx.z * p.chunk, blocks = min(p.chunk, p.K / 32 - block0), quads = (blocks + 3) / 4;
+    const int m0 = blockIdx.x * BM, n0 = blockIdx.y * BN + wave / WM * 16 * NT;
 
-    const uint8_t *const weights = p.B + (size_t)n0 * (p.K / 2);
-    const size_t s_from = (size_t)n0 * p.groups * Scales::SB;
-    const Bytes scales(static_cast<const uint8_t *>(p.scale) + s_from, (size_t)p.N * p.groups * Scales::SB - s_from);
-    uint32_t w_at[NT], s_at[NT], x_at[MT];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        const uint32_t n = min(16 * t + r, p.N - 1 - n0);
-        w_at[t] = n * (uint32_t)(p.K / 2), s_at[t] = n * (uint32_t)(p.groups * Scales::SB);
-    }
-#pragma unroll
-    for (int t = 0; t < MT; ++t) x_at[t] = (uint32_t)(min(16 * t + r, p.M - 1) * p.x_stride * 2) + 16 * c;
-    const uint8_t *const x = reinterpret_cast<const uint8_t *>(p.x);
-
-    struct Half {
-        v4i x[MT][4];
+    const size_t w_all = (size_t)p.N * (p.K / 2), s_all = (size_t)p.N * p.groups * Scales::SB;
+    const size_t w_from = min((size_t)n0 * (p.K / 2) + (size_t)block0 * 16, w_all), s_from = min((size_t)n0 * p.groups * Scales::SB, s_all);
+    const Bytes weights(p.B + w_from, w_all - w_from), scales(static_cast<const uint8_t *>(p.scale) + s_from, s_all - s_from);
+    const uint32_t w_at = (lane >> 2) * (uint32_t)(p.K / 2) + 16 * (lane & 3), s_at = gathered_column(r) * (uint32_t)(p.groups * Scales::SB);
+    struct Step {
         v4i w[NT];
         Scales s[NT];
     };
-    // a wave's i-th half is at four blocks number ..; `quads` or more for none
-    const int turns = (quads + 1) / 2, shift = ((blockIdx.x >> 3) * 5 & 15) * turns >> 4;
-    const auto quad = [&](const int i) {
-        const int turn = wave + NW * (i >> 1), at = turn + shift;
-        return turn < turns ? (at < turns ? at : at - turns) * 2 + (i & 1) : quads;
-    };
-    const auto more = [&](const int i) { return wave + NW * (i >> 1) < turns; };
-    const auto load = [&](Half &to, const int at) {
-        const bool whole = at * 4 + 4 <= blocks;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int block = min(at * 4 + i, blocks - 1);
-#pragma unroll
-            for (int t = 0; t < MT; ++t) to.x[t][i] = at_offset<v4i_half_aligned>(x + (size_t)block * 64, x_at[t]);
-        }
-        const uint32_t mine = whole ? 16 * c : 16 * min(c, blocks - 1 - at * 4);
+    const auto load = [&](Step &to, const int quad) {
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            to.w[t] = at_offset<v4i>(weights + (size_t)at * 64, w_at[t] + mine);
-            if (whole) to.s[t].load(scales, s_at[t], at * 4, p.group);
-            else to.s[t].load_end(scales, s_at[t], at * 4, p.group, p.groups);
+            to.w[t] = weights.load16(w_at + t * 16 * (uint32_t)(p.K / 2), quad * 64);
+            to.s[t].load(scales, s_at + t * 16 * (uint32_t)(p.groups * Scales::SB), block0 + quad * 4, p.group, p.groups);
         }
     };
+    // piece `threadIdx.x % 16` of rows threadIdx.x / 16 and every sixteenth from there on
+    const int piece = threadIdx.x & 15, my_row = threadIdx.x >> 4;
+    v4i x[PIECES];
+    const auto get = [&](const int quad) {
+        const uint16_t *const at = p.x + (size_t)(block0 * 4 + min(quad * 16 + piece, blocks * 4 - 1)) * 8;
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) x[i] = *reinterpret_cast<const v4i_half_aligned *>(at + min(m0 + my_row + 16 * i, p.M - 1) * p.x_stride);
+    };
+    const auto put_in_place = [&](const int quad) {
+        const bool in = quad * 16 + piece < blocks * 4;  // past the end of K: zeros, which whatever follows the weights meets
+        v4i *const to = staged[quad & 1] + (piece >> 2) * (BM * 4) + (piece & 3) * 16 + (my_row ^ piece);
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) to[i * 64] = in ? paired(x[i]) : v4i{};
+    };
+
     v4f total[MT][NT] = {};
-    const auto use = [&](Half &in, const int at) {
-        v4i xs[MT][4];
+    const auto use = [&](Step &in, const int quad) {
         uint32_t w[NT][4];
-        // (what turns a loaded scale into a float stays here: moved up to the load, it would wait for it and everything before it)
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-#pragma unroll
-            for (int i = 0; i < Scales::WORDS; ++i) asm("" : "+v"(in.s[t].raw[i]));
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-#pragma unroll
-            for (int t = 0; t < MT; ++t) xs[t][i] = paired(in.x[t][i]);
-        }
-        if (at * 4 + 4 > blocks) {  // past the end of K: zeros of x, whatever the weights are
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-#pragma unroll
-                for (int t = 0; t < MT; ++t) xs[t][i] = at * 4 + i < blocks ? xs[t][i] : v4i{};
-            }
-        }
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
+            in.s[t].arrive();
 #pragma unroll
             for (int i = 0; i < 4; ++i) w[t][i] = (uint32_t)in.w[t][i];
-            turn_blocks(w[t]);
+            gather_blocks(w[t]);
         }
-        constexpr int PER = MODE == 1 ? 4 : MODE == 2 ? 2 : 1;  // blocks of one scale
+        const v4i *const from = staged[quad & 1] + wave % WM * MT * 64 + c * 16;
 #pragma unroll
         for (int run = 0; run < 4; run += PER) {
             v4f part[MT][NT];
 #pragma unroll
-            for (int a = 0; a < MT; ++a) {
-                v4f begin = {};
-                if constexpr (W::OFFSET) {
-#pragma unroll
-                    for (int i = run; i < run + PER; ++i) begin = W::mfma(__builtin_bit_cast(frag, xs[a][i]), W::offset(), begin);
-                }
-#pragma unroll
-                for (int t = 0; t < NT; ++t) part[a][t] = begin;
-            }
-#pragma unroll
             for (int i = run; i < run + PER; ++i) {
+                frag xs[MT], ws[NT];
 #pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    const frag four_bits = W::of(w[t][i]);
+                for (int a = 0; a < MT; ++a) xs[a] = __builtin_bit_cast(frag, from[i * (BM * 4) + a * 64 + (r ^ (4 * i + c))]);
 #pragma unroll
-                    for (int a = 0; a < MT; ++a) part[a][t] = W::mfma(__builtin_bit_cast(frag, xs[a][i]), four_bits, part[a][t]);
+                for (int t = 0; t < NT; ++t) ws[t] = W::of(w[t][i]);
+#pragma unroll
+                for (int a = 0; a < MT; ++a) {
+                    if (i == run) {
+                        v4f first = {};
+                        if constexpr (W::OFFSET) first = W::mfma(xs[a], W::offset(), first);
+#pragma unroll
+                        for (int t = 0; t < NT; ++t) part[a][t] = W::mfma(xs[a], ws[t], first);
+                    } else {
+                        // (a run's later offsets: into the first column's sum they cannot go, the others need them too)
+                        v4f first = {};
+                        if constexpr (W::OFFSET) first = W::mfma(xs[a], W::offset(), first);
+#pragma unroll
+                        for (int t = 0; t < NT; ++t) part[a][t] = W::mfma(xs[a], ws[t], W::OFFSET ? part[a][t] + first : part[a][t]);
+                    }
                 }
             }
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                const float scale = in.s[t].at(run);
+                const float scale = in.s[t].at(0, run);
 #pragma unroll
                 for (int a = 0; a < MT; ++a) total[a][t] += part[a][t] * scale;
             }
         }
     };
 
-    // (no load of the loop behind a condition: what comes out of one is widened, and so waited for, where the branches meet)
-    Half halves[DEPTH];
-    int first = 0;
-    const auto get = [&](Half &to, const int i) { load(to, min(quad(i), quads - 1)); };
-    const auto put = [&](Half &in, const int i) {
-        const int at = quad(i);
-        if (at < quads) use(in, at);
-    };
-#pragma unroll
-    for (int i = 0; i < DEPTH - 1; ++i) get(halves[i], i);
-    for (; more(first + 2 * DEPTH - 2); first += DEPTH) {
-#pragma unroll
-        for (int i = 0; i < DEPTH; ++i) {
-            get(halves[(i + DEPTH - 1) % DEPTH], first + i + DEPTH - 1);
-            put(halves[i], first + i);
-        }
-    }
-    // the last DEPTH - 1 to 2 DEPTH - 2 halves
-#pragma unroll
-    for (int i = 0; i < 2 * DEPTH - 2; ++i) {
-        if (!more(first + i)) break;
-        if (i < DEPTH - 1) get(halves[(i + DEPTH - 1) % DEPTH], first + i + DEPTH - 1);
-        put(halves[i % DEPTH], first + i);
+    Step one, two;
+    get(0);
+    load(one, 0);
+    put_in_place(0);
+    get(min(1, quads - 1));
+    for (int quad = 0; quad < quads; quad += 2) {
+        __syncthreads();
+        put_in_place(quad + 1);  // (past the last step: zeros that nobody reads)
+        get(min(quad + 2, quads - 1));
+        load(two, min(quad + 1, quads - 1));
+        use(one, quad);
+        if (quad + 1 >= quads) break;
+        __syncthreads();
+        put_in_place(quad + 2);
+        get(min(quad + 3, quads - 1));
+        load(one, min(quad + 2, quads - 1));
+        use(two, quad + 1);
     }
 
 #pragma unroll
-    for (int a = 0; a < MT; ++a) {
+    for (int t = 0; t < NT; ++t) {
+        const int n = n0 + 16 * t + gathered_column(r);
+        const float bias = p.bias != nullptr && p.part == nullptr && n < p.N ? float_of<T>(p.bias[n]) : 0.0f;
 #pragma unroll
-        for (int t = 0; t < NT; ++t) sums[wave][a * NT + t][lane] = total[a][t];
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < MT * NT * 256; i += NW * 64) {
-        const int column = i % (16 * NT), m = i / (16 * NT), n = n0 + column;
-        const int at = (m >> 4) * NT + column / 16, from = column % 16 + 16 * ((m & 15) >> 2);
-        float v = 0.0f;
+        for (int a = 0; a < MT; ++a) {
 #pragma unroll
-        for (int w = 0; w < NW; ++w) v += sums[w][at][from][m & 3];
-        if (m < p.M && n < p.N) p.D[(size_t)m * p.N + n] = round16<T>(p.bias != nullptr ? v + float_of<T>(p.bias[n]) : v);
+            for (int i = 0; i < 4; ++i) {
+                const int m = m0 + (wave % WM * MT + a) * 16 + 4 * c + i;
+                if (m < p.M && n < p.N) {
+                    if (p.part != nullptr) p.part[((size_t)blockIdx.z * p.M + m) * p.N + n] = total[a][t][i];
+                    else p.D[(size_t)m * p.N + n] = round16<T>(p.bias != nullptr ? total[a][t][i] + bias : total[a][t][i]);
+                }
+            }
+        }
     }
 }
 

@@ -55,7 +55,7 @@ QM_EXPORT int qm_kv_append_i8(const qm_kv_cache *cache, const qm_kv_new *fresh, 
     const qm_kv_new &n = *fresh;
     if (n.dtype != QM_IN_F16 && n.dtype != QM_IN_BF16) return QM_ERR_DTYPE;
     if ((st = check_tokens(cache, n.tokens)) != QM_OK) return st;
-    if (n.rotary_pairs < 0 || n.rotary_pairs > cache->head_dim / 2 || n.positions < 0 || (n.q && n.heads < 1)) return QM_ERR_SHAPE;
+    if (n.rotary_pairs < 0 || n.rotary_pairs > cache->head_dim / 2 || n.positions < 0 || (n.rotary_pairs > 0 && n.positions == 0) || (n.q && (n.heads < 1 || (long long)n.tokens * n.heads > INT_MAX))) return QM_ERR_SHAPE;
     if (n.tokens == 0) return QM_OK;
     if (!n.k || !n.v || (n.q && !n.q_out) || (n.rotary_pairs > 0 && (!n.cos || !n.sin))) return QM_ERR_NULL;
     if ((((uintptr_t)n.k | (uintptr_t)n.v | (uintptr_t)n.q | (uintptr_t)n.q_out) & 1) || (((uintptr_t)n.cos | (uintptr_t)n.sin) & 3)) return QM_ERR_ALIGN;
@@ -64,12 +64,22 @@ QM_EXPORT int qm_kv_append_i8(const qm_kv_cache *cache, const qm_kv_new *fresh, 
                       n.k_token_stride, n.k_head_stride, n.v_token_stride, n.v_head_stride, n.q_token_stride, n.q_head_stride, n.cos, n.sin, n.heads,
                       n.rotary_pairs, n.positions, n.interleaved ? 1 : 0};
     const int most = most_new(cache, n.tokens, n.max_query), slots = std::min((most + c.page - 2) / c.page + 1, 4096);
-    const long long items = n.q ? (long long)most * n.heads * (c.dim / 2) : 0;
-    const int q_slots = (int)std::min<long long>((items + 2 * c.kv_heads * 256 - 1) / (2 * c.kv_heads * 256), 4096);
-    const dim3 grid(slots + q_slots, 2 * c.kv_heads, std::min(c.sequences, 65535));
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-    const auto kernel = n.dtype == QM_IN_F16 ? &kv_append_kernel<QM_IN_F16> : &kv_append_kernel<QM_IN_BF16>;
-    const hipError_t e = enqueue(kernel, grid, dim3(256), (size_t)c.page * c.dim, s, c, f, slots);
+    hipError_t e;
+    // One token of 64 sequences and 8 heads: 17.6 us by workgroups, 7.5 by waves.
+    if (most <= 8) {
+        const int tasks = slots * 2 * c.kv_heads + (n.q ? std::min(most, 64) * n.heads : 0);
+        const auto kernel = n.dtype == QM_IN_F16 ? &kv_append_few_kernel<QM_IN_F16> : &kv_append_few_kernel<QM_IN_BF16>;
+        e = enqueue(kernel, dim3((tasks + 3) / 4, std::min(c.sequences, 65535)), dim3(256), 0, s, c, f, slots, tasks);
+    } else {
+        const bool vector = n.rotary_pairs % 8 == 0;
+        const long long items = n.q ? (long long)most * n.heads * (c.dim / (vector ? 16 : 2)) : 0;
+        const int q_slots = (int)std::min<long long>((items + 2 * c.kv_heads * 256 - 1) / (2 * c.kv_heads * 256), 4096);
+        const dim3 grid(slots + q_slots, 2 * c.kv_heads, std::min(c.sequences, 65535));
+        const auto kernel = n.dtype == QM_IN_F16 ? (vector ? &kv_append_kernel<QM_IN_F16, true> : &kv_append_kernel<QM_IN_F16, false>)
+                                                 : (vector ? &kv_append_kernel<QM_IN_BF16, true> : &kv_append_kernel<QM_IN_BF16, false>);
+        e = enqueue(kernel, grid, dim3(256), (size_t)c.page * c.dim, s, c, f, slots);
+    }
     return e == hipSuccess ? QM_OK : fail_launch(e);
 }
 
@@ -149,7 +159,7 @@ QM_EXPORT int qm_kv_read_i8(const qm_kv_cache *cache, const int *page_ids, int c
     if (cache->pages == 0) return QM_ERR_SHAPE;
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     const auto kernel = dtype == QM_IN_F16 ? &kv_read_kernel<QM_IN_F16> : &kv_read_kernel<QM_IN_BF16>;
-    const hipError_t e = enqueue(kernel, dim3(std::min(count, 1 << 20), cache->kv_heads), dim3(256), 0, s, kv_args(cache, 0), page_ids, count,
+    const hipError_t e = enqueue(kernel, dim3(std::min(count, 1 << 20), cache->kv_heads), dim3(256), (size_t)cache->head_dim * (cache->page_size + 4), s, kv_args(cache, 0), page_ids, count,
                                  static_cast<uint16_t *>(k), static_cast<uint16_t *>(v));
     return e == hipSuccess ? QM_OK : fail_launch(e);
 }

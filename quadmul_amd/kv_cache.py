@@ -84,7 +84,7 @@ def append(k: torch.Tensor, v: torch.Tensor, cache_k: torch.Tensor, cache_v: tor
     if (cos is None) != (sin is None):
         raise QuadmulError("append: cos and sin go together")
     for t in () if cos is None else (cos, sin):
-        if not (t.device == cache_k.device and t.dtype == torch.float32 and t.dim() == 2 and t.is_contiguous() and t.shape == cos.shape and 2 * t.shape[1] <= c.head_dim):
+        if not (t.device == cache_k.device and t.dtype == torch.float32 and t.dim() == 2 and t.is_contiguous() and t.shape == cos.shape and t.shape[0] >= 1 and 2 * t.shape[1] <= c.head_dim):
             raise QuadmulError(f"append: cos and sin must be contiguous float32 tensors [positions, at most {c.head_dim // 2}] on the cache's device")
     out = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
     n = KvNew(k.data_ptr(), v.data_ptr(), None if q is None else q.data_ptr(), None if q is None else out.data_ptr(), k.stride(0), k.stride(1), v.stride(0),
