@@ -26,6 +26,7 @@ struct AttendArgs {
     float scale;   // times log2(e)
     int tiles;     // of rows, side by side
     int rows;      // of a tile that are used at most
+    int wide;      // 1: tiles of 64 rows (kv_attend_rows_kernel)
     // all sequences' steps one after the other cut into as many equal parts (0: a sequence to a workgroup), for each tile and head, and what
     // is left where a sequence is cut: a part's end of one and beginning of another, 16 rows of dim values and their lse each; and the
     // first part of each sequence and their number
@@ -124,6 +125,105 @@ __device__ __forceinline__ AttendCut attend_cut(const KvArgs &c, const AttendArg
     return {-1, 1, 0};
 }
 
+// q^T of one row: float16, bf16 brought into its range by a power of two. What is left for the scores to be multiplied with.
+template <int T, int D>
+__device__ __forceinline__ float attend_query(const uint16_t *x, const float scale, h8 (&query)[D / 32])
+{
+    constexpr int J = D / 32;
+    const int g = (threadIdx.x & 63) >> 4;
+    float v[J][8], most = 0.0f;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+        const int d = j * 32 + 32 <= D / 64 * 64 ? (j / 2) * 64 + 16 * g + 8 * (j & 1) : j * 32 + 8 * g;
+        const v4i w = *reinterpret_cast<const v4i_half_aligned *>(x + d);
+        if constexpr (T == QM_IN_F16) query[j] = __builtin_bit_cast(h8, w);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            v[j][e] = float_of<T>((uint16_t)((uint32_t)w[e / 2] >> (16 * (e & 1))));
+            most = fmaxf(most, fabsf(v[j][e]));
+        }
+    }
+    if constexpr (T == QM_IN_F16) {
+        return scale;
+    } else {
+        most = across_groups_max(most);
+        const int e = max((int)(__builtin_bit_cast(uint32_t, most) >> 23) - 127 - 14, -100);  // the largest becomes 2^14 to 2^15
+        const float down = __builtin_bit_cast(float, (uint32_t)(127 - e) << 23);
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) query[j][i] = (_Float16)(v[j][i] * down);
+        }
+        return scale * __builtin_bit_cast(float, (uint32_t)(127 + e) << 23);
+    }
+}
+
+// A row of the softmax so far: the maxima of the scores and of score + log2(scale of the value), the sum.
+struct AttendRow {
+    float top = ATTEND_LOW, high = ATTEND_LOW, total = 0.0f;
+};
+// Sixteen scores of a lane (tokens token0 + 4 t + i) into weights for the values: by: what a score is multiplied with; vs: the scale of the
+// values; whole: every row sees every token.
+template <int DT>
+__device__ __forceinline__ void attend_weights(v4f (&score)[4], const float by, const float vs, const bool whole, const bool there, const int token0, const int limit,
+                                               const int below, AttendRow &row, v4f (&out)[DT], h8 (&weight)[2])
+{
+    float most = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            score[t][i] *= by;
+            most = fmaxf(most, score[t][i]);
+        }
+    }
+    if (!whole) {
+        most = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int j = token0 + 4 * t + i;
+                score[t][i] = (there & (j <= limit) & (j > below)) ? score[t][i] : -INFINITY;
+                most = fmaxf(most, score[t][i]);
+            }
+        }
+    }
+    const float size = vs == 0.0f ? -INFINITY : __builtin_amdgcn_logf(fabsf(vs));
+    if (__any(most > row.top + ATTEND_SLACK || most + size > row.high + ATTEND_SLACK)) {
+        const float t1 = fmaxf(row.top, across_groups_max(most)), h1 = fmaxf(row.high, across_groups_max(most + size));
+        row.total *= __builtin_amdgcn_exp2f(row.top - t1);
+        const float shrink = __builtin_amdgcn_exp2f(row.high - h1);
+#pragma unroll
+        for (int t = 0; t < DT; ++t) out[t] *= shrink;
+        row.top = t1, row.high = h1;
+    }
+    // vs * 2^(top - high + lift): by two factors, for the power alone may leave the float range (the product does only where the
+    // weight is below 2^-118 of the largest)
+    const float root = __builtin_amdgcn_exp2f(0.5f * fminf(row.top - row.high + ATTEND_LIFT, 126.0f - size));
+    // (sixteen tokens that a mask hides count 0 whatever the scale of their page is)
+    const float weigh = vs == 0.0f || most == -INFINITY ? 0.0f : vs * root * root;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float p = __builtin_amdgcn_exp2f(score[t][i] - row.top);
+            row.total += p;
+            weight[t / 2][(t & 1) * 4 + i] = (_Float16)(p * weigh);
+        }
+    }
+}
+// four channels of each of a lane's tiles of a row; the sum is 0 where nothing is seen
+template <int T, int DT>
+__device__ __forceinline__ void attend_store(const v4f (&out)[DT], const float sum, const float root, const float by, uint16_t *to)
+{
+#pragma unroll
+    for (int t = 0; t < DT; ++t) {
+        const v4f v = sum == 0.0f ? v4f{} : out[t] * root * by;
+        *reinterpret_cast<v2i_half_aligned *>(to + 16 * t) = v2i{(int)round16_pair<T>(v[0], v[1]), (int)round16_pair<T>(v[2], v[3])};
+    }
+}
+
 // blockIdx.x: a head of the cache, and a sequence or (CUT) a part of all sequences; blockIdx.y: a tile of rows. The waves take turns at the steps.
 // (Workgroups are dealt to the XCDs in turn: with the heads side by side each has as many long and short sequences as the others.)
 template <int T, int D, int NW, bool CUT>
@@ -171,35 +271,8 @@ __global__ __launch_bounds__(NW * 64, D > 128 ? 1 : 2) void kv_attend_kernel(con
             const int sees_from = a.window > 0 ? q.begin + last - a.window + 1 : 0;
             const int sees_to = q.begin + first < 0 ? -1 : a.causal ? q.begin + first : q.length - 1;
 
-            // q^T: float16, bf16 brought into its range by a power of two
             h8 query[J];
-            float factor = a.scale;
-            {
-                const uint16_t *const x = a.q + (q.row0 + token) * a.q_token + (long long)(head * shared + row % shared) * a.q_head;
-                float v[J][8], most = 0.0f;
-#pragma unroll
-                for (int j = 0; j < J; ++j) {
-                    const int d = j * 32 + 32 <= D / 64 * 64 ? (j / 2) * 64 + 16 * g + 8 * (j & 1) : j * 32 + 8 * g;
-                    const v4i w = *reinterpret_cast<const v4i_half_aligned *>(x + d);  // (a row past the last one repeats it)
-                    if constexpr (T == QM_IN_F16) query[j] = __builtin_bit_cast(h8, w);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        v[j][e] = float_of<T>((uint16_t)((uint32_t)w[e / 2] >> (16 * (e & 1))));
-                        most = fmaxf(most, fabsf(v[j][e]));
-                    }
-                }
-                if constexpr (T == QM_IN_BF16) {
-                    most = across_groups_max(most);
-                    const int e = max((int)(__builtin_bit_cast(uint32_t, most) >> 23) - 127 - 14, -100);  // the largest becomes 2^14 to 2^15
-                    const float down = __builtin_bit_cast(float, (uint32_t)(127 - e) << 23);
-                    factor *= __builtin_bit_cast(float, (uint32_t)(127 + e) << 23);
-#pragma unroll
-                    for (int j = 0; j < J; ++j) {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) query[j][i] = (_Float16)(v[j][i] * down);
-                    }
-                }
-            }
+            const float factor = attend_query<T, D>(a.q + (q.row0 + token) * a.q_token + (long long)(head * shared + row % shared) * a.q_head, a.scale, query);
 
             struct Pages {
                 int key, value;  // of this lane's row of the keys and of its sixteen tokens; -1: none
@@ -241,7 +314,7 @@ __global__ __launch_bounds__(NW * 64, D > 128 ? 1 : 2) void kv_attend_kernel(con
             };
 
             v4f out[DT] = {};
-            float top = ATTEND_LOW, high = ATTEND_LOW, total = 0.0f;
+            AttendRow state;
             int step = step0 + wave;
             Pages now{-1, -1}, next{-1, -1};
             if (step < step1) {
@@ -267,53 +340,9 @@ __global__ __launch_bounds__(NW * 64, D > 128 ? 1 : 2) void kv_attend_kernel(con
                 const Pages then = pages(min(step + 2 * NW, step1 - 1));  // (in front of the keys: what is waited for last is loaded last)
                 if (step + NW < step1) load_keys(step + NW, next);
 
-                const int token0 = step * ATTEND_STEP + 16 * g;
                 const bool whole = step * ATTEND_STEP >= sees_from && step * ATTEND_STEP + ATTEND_STEP - 1 <= sees_to && __all(there);
-                float most = -INFINITY;
-#pragma unroll
-                for (int t = 0; t < 4; ++t) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        score[t][i] *= by;
-                        most = fmaxf(most, score[t][i]);
-                    }
-                }
-                if (!whole) {
-                    most = -INFINITY;
-#pragma unroll
-                    for (int t = 0; t < 4; ++t) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int j = token0 + 4 * t + i;
-                            score[t][i] = (there & (j <= limit) & (j > below)) ? score[t][i] : -INFINITY;
-                            most = fmaxf(most, score[t][i]);
-                        }
-                    }
-                }
-                const float size = vs == 0.0f ? -INFINITY : __builtin_amdgcn_logf(fabsf(vs));
-                if (__any(most > top + ATTEND_SLACK || most + size > high + ATTEND_SLACK)) {
-                    const float t1 = fmaxf(top, across_groups_max(most)), h1 = fmaxf(high, across_groups_max(most + size));
-                    total *= __builtin_amdgcn_exp2f(top - t1);
-                    const float shrink = __builtin_amdgcn_exp2f(high - h1);
-#pragma unroll
-                    for (int t = 0; t < DT; ++t) out[t] *= shrink;
-                    top = t1, high = h1;
-                }
-                // vs * 2^(top - high + lift): by two factors, for the power alone may leave the float range (the product does only where the
-                // weight is below 2^-118 of the largest)
-                const float root = __builtin_amdgcn_exp2f(0.5f * fminf(top - high + ATTEND_LIFT, 126.0f - size));
-                // (sixteen tokens that a mask hides count 0 whatever the scale of their page is)
-                const float weigh = vs == 0.0f || most == -INFINITY ? 0.0f : vs * root * root;
                 h8 weight[2];
-#pragma unroll
-                for (int t = 0; t < 4; ++t) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float p = __builtin_amdgcn_exp2f(score[t][i] - top);
-                        total += p;
-                        weight[t / 2][(t & 1) * 4 + i] = (_Float16)(p * weigh);
-                    }
-                }
+                attend_weights(score, by, vs, whole, there, step * ATTEND_STEP + 16 * g, limit, below, state, out, weight);
 #pragma unroll
                 for (int t = 0; t < DT; ++t) {
 #pragma unroll
@@ -325,7 +354,7 @@ __global__ __launch_bounds__(NW * 64, D > 128 ? 1 : 2) void kv_attend_kernel(con
             }
 
             // the waves' results into one
-            total = across_groups_sum(total);
+            const float top = state.top, high = state.high, total = across_groups_sum(state.total);
             __syncthreads();
             if (g == 0) stats[wave][0][r] = top, stats[wave][1][r] = high, stats[wave][2][r] = total;
             __syncthreads();
@@ -354,12 +383,7 @@ __global__ __launch_bounds__(NW * 64, D > 128 ? 1 : 2) void kv_attend_kernel(con
                 // (the sum is 0 where nothing is seen)
                 const float root = __builtin_amdgcn_exp2f(0.5f * (h1 - t1 - ATTEND_LIFT)), by = root / sum;
                 if (whole_range) {
-                    uint16_t *const to = a.out + out_row * D + 4 * g;
-#pragma unroll
-                    for (int t = 0; t < DT; ++t) {
-                        const v4f v = sum == 0.0f ? v4f{} : out[t] * root * by;
-                        *reinterpret_cast<v2i_half_aligned *>(to + 16 * t) = v2i{(int)round16_pair<T>(v[0], v[1]), (int)round16_pair<T>(v[2], v[3])};
-                    }
+                    attend_store<T>(out, sum, root, by, a.out + out_row * D + 4 * g);
                 } else {
                     const size_t at = ((size_t)(tile * c.kv_heads + head) * (2 * a.parts) + 2 * number + (begins ? 1 : 0)) * 16 + r;
                     float *const to = a.part + at * D + 4 * g;
@@ -368,6 +392,182 @@ __global__ __launch_bounds__(NW * 64, D > 128 ? 1 : 2) void kv_attend_kernel(con
                     if (g == 0) a.lse[at] = sum == 0.0f ? -INFINITY : t1 + __builtin_amdgcn_logf(sum);
                 }
             }
+        }
+    }
+}
+
+// Many rows of a sequence: 16 to a wave, four waves to every other 64 tokens. The codes of 64 tokens become float16 once for their four waves, in
+// the LDS, in the order that the operands want them; each wave makes a fourth of them from what it loaded while the step before was computed.
+// blockIdx.x: a tile of 64 rows, the last ones, which see most, first; blockIdx.y: a head of the cache and a sequence. (The other way
+// round each of 8 heads has an XCD, whose CUs read the same lines at the same time: twice as long.) Bound by the vector
+// pipeline (what a score costs until it is a weight: nine instructions and an exponential) before the matrix cores. (With 32 rows to a wave and four waves
+// 4 prompts of up to 512 tokens took 162 us: the longest sequence had a workgroup to every other CU.)
+constexpr int ATTEND_LOTS = 2;  // of 64 tokens at a time (with four the registers of 128 channels do not fit: 138 us for 94)
+template <int T, int D>
+__global__ __launch_bounds__(256 * ATTEND_LOTS, D > 128 ? 2 : 4) void kv_attend_rows_kernel(const KvArgs c, const AttendArgs a)
+{
+    constexpr int LOTS = ATTEND_LOTS, J = D / 32, DT = D / 16, KW = D / 16, QT = 1, ROWS = 64 * QT, MINE = (DT + 3) / 4;  // MINE: tiles of the values that a wave turns into floats
+    struct Floats {
+        h8 keys[4][J][64], values[DT][2][64];
+    };
+    extern __shared__ int8_t in_lds[];
+    __shared__ float stats[LOTS][4][QT][3][16];
+    const int lane = threadIdx.x & 63, all_waves = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lot = all_waves >> 2, wave = all_waves & 3, r = lane & 15, g = lane >> 4;
+    Floats &lds = reinterpret_cast<Floats *>(in_lds)[lot];
+    auto &keys = lds.keys;
+    auto &values = lds.values;
+    const int head = blockIdx.y % c.kv_heads, shared = a.heads / c.kv_heads;
+    const int page_shift = __builtin_ctz(c.page), page_mask = c.page - 1;
+    for (int s = blockIdx.y / c.kv_heads; s < c.sequences; s += gridDim.y / c.kv_heads) {
+        const KvSequence q = kv_sequence(c, s);
+        const int rows = q.count * shared, tiles = (rows + ROWS - 1) / ROWS;
+        for (int behind = blockIdx.x; behind < tiles; behind += gridDim.x) {
+            const int row0 = (tiles - 1 - behind) * ROWS, last_row = min(row0 + ROWS, rows) - 1;
+            const AttendRange range = attend_range(c, a, q, row0 / shared, last_row / shared);
+            h8 query[QT][J];
+            float factor[QT];
+            int limit[QT], below[QT];
+            AttendRow state[QT];
+            v4f out[QT][DT] = {};
+            const int my_row0 = min(row0 + wave * 16 * QT, last_row), my_last = min(my_row0 + 16 * QT - 1, last_row);
+#pragma unroll
+            for (int t = 0; t < QT; ++t) {
+                const int row = min(my_row0 + 16 * t + r, last_row), token = row / shared, position = q.begin + token;
+                limit[t] = position < 0 ? -1 : a.causal ? position : q.length - 1, below[t] = a.window > 0 ? position - a.window : -1;
+                factor[t] = attend_query<T, D>(a.q + (q.row0 + token) * a.q_token + (long long)(head * shared + row % shared) * a.q_head, a.scale, query[t]);
+            }
+            // tokens that all rows of the wave see, and those that some row may see
+            const int first = my_row0 / shared, last = my_last / shared;
+            const int sees_from = a.window > 0 ? q.begin + last - a.window + 1 : 0;
+            const int sees_to = q.begin + first < 0 ? -1 : a.causal ? q.begin + first : q.length - 1;
+            const int may_from = a.window > 0 ? q.begin + first - a.window + 1 : 0, may_to = a.causal ? q.begin + last : q.length - 1;
+
+            // this lane's part of a step: row `wave` of four in the keys, and channels of the values
+            uint32_t key_words[KW];
+            v4i value_words[MINE];
+            const auto key_page = [&](const int step) { return kv_page(c, s, (step * ATTEND_STEP + 16 * (r >> 2)) >> page_shift); };
+            const auto value_page = [&](const int step) { return kv_page(c, s, (step * ATTEND_STEP + 16 * g) >> page_shift); };
+            float2 scales = {0.0f, 0.0f};
+            const auto load = [&](const int step, const int kp, const int vp) {
+                const int8_t *const k = c.k + (((size_t)max(kp, 0) * c.kv_heads + head) * c.page + ((step * ATTEND_STEP + 16 * (r >> 2)) & page_mask) + (r & 3) + 4 * wave) * D;
+#pragma unroll
+                for (int w = 0; w < KW; w += 4) {
+                    if (w + 4 <= KW) {
+                        const v4i x = *reinterpret_cast<const v4i *>(k + w * 16 + 16 * g);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) key_words[w + e] = x[e];
+                    } else {
+                        const v2i x = *reinterpret_cast<const v2i *>(k + w * 16 + 8 * g);
+                        key_words[w] = x[0], key_words[w + 1] = x[1];
+                    }
+                }
+                const size_t at = (size_t)max(vp, 0) * c.kv_heads + head;
+                scales = *reinterpret_cast<const float2 *>(c.scales + at * 2);
+                const int8_t *const v = c.v + (at * D + r) * c.page + ((step * ATTEND_STEP + 16 * g) & page_mask);
+#pragma unroll
+                for (int t = 0; t < MINE; ++t)
+                    if (DT % 4 == 0 || 4 * t + wave < DT) value_words[t] = *reinterpret_cast<const v4i *>(v + (size_t)(4 * t + wave) * 16 * c.page);
+            };
+            const auto put_in_place = [&]() {
+#pragma unroll
+                for (int j = 0; j < J; ++j) keys[wave][j][lane] = half8_of_codes(key_words[2 * j], key_words[2 * j + 1]);
+#pragma unroll
+                for (int t = 0; t < MINE; ++t) {
+                    if (DT % 4 == 0 || 4 * t + wave < DT) {
+                        values[4 * t + wave][0][lane] = half8_of_codes((uint32_t)value_words[t][0], (uint32_t)value_words[t][1]);
+                        values[4 * t + wave][1][lane] = half8_of_codes((uint32_t)value_words[t][2], (uint32_t)value_words[t][3]);
+                    }
+                }
+            };
+            // (all lots go round as often: past its last step one has nothing to compute)
+            const int step0 = range.begin + lot, step1 = range.begin + range.steps, turns = (range.steps + LOTS - 1) / LOTS;
+            int there_now = -1, kp = -1, vp = -1;
+            float2 scales_now = {0.0f, 0.0f};
+            if (turns > 0) {
+                const int now = min(step0, step1 - 1), next = min(step0 + LOTS, step1 - 1);
+                load(now, key_page(now), there_now = value_page(now));
+                scales_now = scales;
+                kp = key_page(next), vp = value_page(next);
+                put_in_place();
+            }
+            for (int turn = 0; turn < turns; ++turn) {
+                __syncthreads();
+                const int step = step0 + LOTS * turn;
+                const bool there = there_now >= 0;
+                const int next = min(step + LOTS, step1 - 1), after = min(step + 2 * LOTS, step1 - 1);
+                const int kp2 = key_page(after), vp2 = value_page(after);
+                load(next, kp, vp);
+                there_now = vp, kp = kp2, vp = vp2;
+                const int token0 = step * ATTEND_STEP;
+                if (step < step1 && token0 <= may_to && token0 + ATTEND_STEP > may_from) {
+                    const bool whole = token0 >= sees_from && token0 + ATTEND_STEP - 1 <= sees_to && __all(there);
+                    v4f score[QT][4] = {};
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) {
+#pragma unroll
+                        for (int j = 0; j < J; ++j) {
+                            const h8 k = keys[t][j][lane];
+#pragma unroll
+                            for (int n = 0; n < QT; ++n) score[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, query[n][j], score[n][t], 0, 0, 0);
+                        }
+                    }
+                    const float vs = fabsf(scales_now.y) < 0x1p-126f ? 0.0f : scales_now.y;
+                    h8 weight[QT][2];
+#pragma unroll
+                    for (int n = 0; n < QT; ++n)
+                        attend_weights(score[n], scales_now.x * factor[n], vs, whole, there, token0 + 16 * g, limit[n], below[n], state[n], out[n], weight[n]);
+#pragma unroll
+                    for (int t = 0; t < DT; ++t) {
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+                            const h8 v = values[t][u][lane];
+#pragma unroll
+                            for (int n = 0; n < QT; ++n) out[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, weight[n][u], out[n][t], 0, 0, 0);
+                        }
+                    }
+                }
+                __syncthreads();
+                put_in_place();
+                scales_now = scales;
+            }
+            // the other lots' results to the first
+            constexpr int PITCH = D + 4, PART = 4 * QT * 16 * PITCH;  // floats of a lot
+            static_assert((LOTS - 1) * PART * sizeof(float) <= LOTS * sizeof(Floats));
+            float *const joined = reinterpret_cast<float *>(in_lds) + (wave * QT * 16 + r) * PITCH + 4 * g;
+            __syncthreads();
+            if (lot > 0) {
+#pragma unroll
+                for (int n = 0; n < QT; ++n) {
+                    const float total = across_groups_sum(state[n].total);
+                    if (g == 0) stats[lot][wave][n][0][r] = state[n].top, stats[lot][wave][n][1][r] = state[n].high, stats[lot][wave][n][2][r] = total;
+#pragma unroll
+                    for (int t = 0; t < DT; ++t) *reinterpret_cast<v4f *>(joined + (lot - 1) * PART + n * 16 * PITCH + 16 * t) = out[n][t];
+                }
+            }
+            __syncthreads();
+            if (lot == 0) {
+#pragma unroll
+                for (int n = 0; n < QT; ++n) {
+                    const int row = row0 + (wave * QT + n) * 16 + r;
+                    float top = state[n].top, high = state[n].high;
+#pragma unroll
+                    for (int l = 1; l < LOTS; ++l) top = fmaxf(top, stats[l][wave][n][0][r]), high = fmaxf(high, stats[l][wave][n][1][r]);
+                    float sum = across_groups_sum(state[n].total) * __builtin_amdgcn_exp2f(state[n].top - top);
+                    const float mine = __builtin_amdgcn_exp2f(state[n].high - high);
+#pragma unroll
+                    for (int t = 0; t < DT; ++t) out[n][t] *= mine;
+#pragma unroll
+                    for (int l = 1; l < LOTS; ++l) {
+                        sum += stats[l][wave][n][2][r] * __builtin_amdgcn_exp2f(stats[l][wave][n][0][r] - top);
+                        const float theirs = __builtin_amdgcn_exp2f(stats[l][wave][n][1][r] - high);
+#pragma unroll
+                        for (int t = 0; t < DT; ++t) out[n][t] += *reinterpret_cast<const v4f *>(joined + (l - 1) * PART + n * 16 * PITCH + 16 * t) * theirs;
+                    }
+                    const float root = __builtin_amdgcn_exp2f(0.5f * (high - top - ATTEND_LIFT));
+                    if (row <= last_row) attend_store<T>(out[n], sum, root, root / sum, a.out + ((size_t)(q.row0 + row / shared) * a.heads + head * shared + row % shared) * D + 4 * g);
+                }
+            }
+            __syncthreads();
         }
     }
 }

@@ -15,12 +15,12 @@ namespace qm {
 enum GroupedKernel { GROUPED_ANY, GROUPED_ROWS16, GROUPED_TILE };
 struct GroupedPlan {
     GroupedKernel kernel;
-    int ways, chunk, runs;  // waves to a tile of columns; blocks of 32 of K in a run, runs
+    int waves, ways, chunk, runs;  // of a workgroup, to a tile of columns; blocks of 32 of K in a run, runs
     size_t bytes;
 };
 static GroupedPlan grouped_plan(int m, int n, int k, int align)
 {
-    GroupedPlan p{GROUPED_ANY, 1, 0, 1, 0};
+    GroupedPlan p{GROUPED_ANY, 16, 1, 0, 1, 0};
     if (k == 0 || k % 32 != 0 || align < 16) return p;
     if (m > 16 && n > 65535 * 64) return p;  // (the grid's limit)
     if (m > 16) {
@@ -41,7 +41,11 @@ static GroupedPlan grouped_plan(int m, int n, int k, int align)
     p.chunk = ((blocks + p.runs - 1) / p.runs + 3) / 4 * 4;
     p.runs = (blocks + p.chunk - 1) / p.chunk;
     if (p.runs > 1) p.bytes = (size_t)p.runs * m * n * sizeof(float);
-    while (p.ways < GROUPED_WAVES && (long long)((n + 15) / 16) * p.runs * p.ways < 3072) p.ways *= 2;
+    // Waves enough for the chip. A call that is over before they are all at work has eight to a workgroup: 1 x 4096 x 4096 5.8 us, with sixteen
+    // 7.1; 1 x 28672 x 4096 (groups of 32) 20.3 and 20.4, 13 x 8192 x 28672 42 and 39, the two layers of 8 x 4096 x 4096 and 8 x 6144 x 4096 21 and 18.
+    const long long tiles = (long long)((n + 15) / 16) * p.runs;
+    if (m <= 4 && tiles <= 512) p.waves = 8;
+    while (p.ways < p.waves && tiles * p.ways < 3072) p.ways *= 2;
     return p;
 }
 
@@ -56,12 +60,12 @@ static hipError_t launch_mode(GroupedArgs p, const GroupedPlan &plan, hipStream_
         if (p.M > 64) return go(&gemm_grouped_tile_kernel<T, S, MODE, 2, 4, 2>, 128, 64);
         return p.M > 32 ? go(&gemm_grouped_tile_kernel<T, S, MODE, 1, 4, 2>, 64, 128) : go(&gemm_grouped_tile_kernel<T, S, MODE, 1, 2, 2>, 32, 128);
     }
-    const int tiles = GROUPED_WAVES / plan.ways, groups = ((p.N + 15) / 16 + tiles - 1) / tiles;
+    const int tiles = plan.waves / plan.ways, groups = ((p.N + 15) / 16 + tiles - 1) / tiles;
     const size_t lds = (size_t)plan.chunk * (64 * (p.M | 1) + 64);
-    static std::atomic<bool> known[QM_MAX_DEVICES] = {};
-    const auto kernel = &gemm_grouped_rows_kernel<T, S, MODE>;
-    if (const hipError_t e = ensure_dynamic_lds(kernel, 128 << 10, known); e != hipSuccess) return e;
-    return enqueue(kernel, dim3(std::min(groups, std::max(1, 256 / plan.runs)), plan.runs), dim3(GROUPED_WAVES * 64), lds, s, p);
+    static std::atomic<bool> known[2][QM_MAX_DEVICES] = {};
+    const auto kernel = plan.waves == 8 ? &gemm_grouped_rows_kernel<T, S, MODE, 8> : &gemm_grouped_rows_kernel<T, S, MODE, 16>;
+    if (const hipError_t e = ensure_dynamic_lds(kernel, 128 << 10, known[plan.waves == 8]); e != hipSuccess) return e;
+    return enqueue(kernel, dim3(std::min(groups, std::max(1, 256 / plan.runs)), plan.runs), dim3(plan.waves * 64), lds, s, p);
 }
 template <int T, int S>
 static hipError_t launch_grouped(GroupedArgs p, const GroupedPlan &plan, hipStream_t s)

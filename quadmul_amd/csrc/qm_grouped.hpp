@@ -214,14 +214,13 @@ struct GroupedScaleSet {
 // and by what a quad costs of the vector pipeline: about 70 instructions a kilobyte, of which 30 make floats of the weights; 6 TB/s leave it 90.
 // (With x from the L2 by each wave for itself, 4 KiB of x for a KiB or two of weights, 13 x 8192 x 28672 took 52 us; with x put into the LDS
 // by 832 workgroups 45.)
-constexpr int GROUPED_WAVES = 16;
-template <int T, int S, int MODE>
-__global__ __launch_bounds__(GROUPED_WAVES * 64, 4) void gemm_grouped_rows_kernel(const GroupedArgs p)
+template <int T, int S, int MODE, int NW>
+__global__ __launch_bounds__(NW * 64, 4) void gemm_grouped_rows_kernel(const GroupedArgs p)
 {
     typedef GroupedWeights<T> W;
     typedef typename W::frag frag;
     // SET: quads that are loaded at a time, one set ahead; PER: blocks of one scale
-    constexpr int NW = GROUPED_WAVES, SET = MODE == 1 || MODE == 2 ? 4 : 2, RING = 2, PER = MODE == 1 ? 4 : MODE == 2 ? 2 : 1;
+    constexpr int SET = MODE == 1 || MODE == 2 ? 4 : 2, RING = 2, PER = MODE == 1 ? 4 : MODE == 2 ? 2 : 1;
     typedef GroupedScaleSet<S, MODE, SET> Scales;
     extern __shared__ v4i staged[];
     __shared__ v4f sums[NW][64];

@@ -87,13 +87,13 @@ QM_EXPORT int qm_kv_append_i8(const qm_kv_cache *cache, const qm_kv_new *fresh, 
 // steps cut into equal parts and joined by a second launch.
 namespace {
 struct AttendPlan {
-    int tiles, rows, parts;
+    int tiles, rows, wide, parts;
     size_t part_bytes, lse_bytes, bytes;
 };
 }
 static AttendPlan attend_plan(const qm_kv_cache *c, int tokens, int heads, int max_query, int max_length, int window)
 {
-    AttendPlan p{1, 16, 0, 0, 0, 0};
+    AttendPlan p{1, 16, 0, 0, 0, 0, 0};
     if (tokens == 0 || c->sequences == 0) return p;
     const long long most = std::min<long long>((long long)c->table_width * c->page_size, INT_MAX - 2 * ATTEND_STEP);
     long long length = max_length > 0 ? std::min<long long>(max_length, most) : most;
@@ -103,6 +103,12 @@ static AttendPlan attend_plan(const qm_kv_cache *c, int tokens, int heads, int m
     const long long rows = (long long)fresh * (heads / c->kv_heads);
     p.tiles = (int)std::min<long long>((rows + 15) / 16, 4096);
     p.rows = (int)std::min<long long>(rows, 16);
+    // many rows, and workgroups enough of 64
+    if (rows > 64 && (rows + 63) / 64 * c->kv_heads * c->sequences >= 128) {
+        p.wide = 1;
+        p.tiles = (int)std::min<long long>((rows + 63) / 64, 65535);
+        return p;
+    }
     const long long groups = (long long)p.tiles * c->kv_heads;
     // The second launch costs 5 us, a step of a wave 2 to 3.5, a sequence in one workgroup has its waves go through an eighth of its
     // steps one by one. 32 sequences and 8 heads (256 workgroups): 2048 tokens each 31 us in one piece, 36 cut; 6000 tokens 78 and
@@ -139,7 +145,7 @@ QM_EXPORT int qm_kv_attend_i8(const qm_kv_cache *cache, const void *q, int dtype
     if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes)) return QM_ERR_SCRATCH;
     uint8_t *const scratch = static_cast<uint8_t *>(workspace);
     const AttendArgs a{static_cast<const uint16_t *>(q), static_cast<uint16_t *>(out), q_token_stride, q_head_stride, heads, causal ? 1 : 0,
-                       window > 1 << 30 ? 0 : window, scale * 1.4426950408889634f, p.tiles, p.rows, p.parts, reinterpret_cast<float *>(scratch),
+                       window > 1 << 30 ? 0 : window, scale * 1.4426950408889634f, p.tiles, p.rows, p.wide, p.parts, reinterpret_cast<float *>(scratch),
                        reinterpret_cast<float *>(scratch + p.part_bytes), reinterpret_cast<int2 *>(scratch + p.part_bytes + p.lse_bytes)};
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     const KvArgs c = kv_args(cache, tokens);

@@ -77,6 +77,17 @@ def test_prompts(counts, heads, kv_heads, dim):
     both(q, cache, table, lengths, counts, max_query=max(counts), max_length=max(lengths))
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads,dim,page,window,causal", [(32, 16, 64, 16, 0, True), (12, 12, 96, 64, 50, True), (8, 8, 128, 32, 0, False), (28, 14, 192, 16, 100, False),
+                                                                  (16, 16, 256, 128, 0, True)])
+def test_many_rows(heads, kv_heads, dim, page, window, causal, dtype):
+    """Enough rows for tiles of 64 of them: several tiles to a sequence, the last one not full, histories of all lengths, none among them, padding."""
+    lengths, counts = [150, 400, 130, 70, 3, 0], [150, 131, 65, 1, 40, 2]
+    q, cache, table = problem(lengths, counts, heads, kv_heads, dim, page, dtype, 17)
+    table[1, 1] = -1
+    both(q, cache, table, lengths, counts, causal=causal, window=window, max_query=150, max_length=400)
+
+
 def test_rows_that_see_nothing_are_zero():
     lengths, counts = [0, 30, 3, -4, 64], [1, 1, 6, 2, 1]   # no tokens at all; three rows in front of position 0; no tokens; only missing pages
     q, cache, table = problem(lengths, counts, 4, 2, 64, 16, torch.float16, 6)
