@@ -1,4 +1,6 @@
-"""A W4A4 linear layer on top of the packed-int4 GEMM: the caller the reference's README
+"""Linear layers on packed int4 weights.
+
+:class:`W4A4Linear`, a W4A4 linear layer on top of the packed-int4 GEMM: the caller the reference's README
 (README.md:7, "easy to fuse with quantisation") has in mind and does not ship.
 
     y[t, n] = round16((sum_k xq[t, k] * wq[n, k]) * x_scale[t] * w_scale[n]) (+ bias[n])
@@ -7,6 +9,9 @@ with ``xq, x_scale = quantize_pack(x)`` (per-token symmetric int4, scale = amax 
 ``wq, w_scale`` the same quantisation of the weight rows, done once.  One or two launches out of one native
 call: quantise + pack the activations, and the GEMM with the dequantising epilogue, which adds
 the bias too; the int32 product never reaches memory.
+
+:class:`W4A16Linear`: the activations stay 16-bit floats and the weights have a scale per group of
+``in_features`` (:func:`quadmul_amd.gemm_grouped`); no counterpart in the reference.
 """
 from __future__ import annotations
 
@@ -15,7 +20,7 @@ from typing import Optional
 import torch
 from torch.autograd import forward_ad
 
-from . import QuadmulError, _native, gemm_scaled, quantize_pack
+from . import QuadmulError, _native, gemm_grouped, gemm_scaled, quantize_groups, quantize_pack
 
 
 def _fusable(bias: torch.Tensor, x: torch.Tensor, out_dtype: torch.dtype, n: int) -> bool:
@@ -100,3 +105,45 @@ class W4A4Linear(torch.nn.Module):
 
 
 _CLASS = W4A4Linear.__dict__  # (as it is at the time of a call)
+
+
+class W4A16Linear(torch.nn.Module):
+    """``forward(x)``: ``x`` [..., in_features] float16 or bfloat16 on the GPU -> [..., out_features] of its type: one to thousands of rows. Not
+    differentiable."""
+
+    def __init__(self, weight_packed: torch.Tensor, weight_scale: torch.Tensor, group_size: int, bias: Optional[torch.Tensor] = None):
+        super().__init__()
+        if weight_packed.dim() != 2 or weight_packed.dtype not in (torch.int8, torch.uint8):
+            raise QuadmulError("W4A16Linear: weight_packed must be [out_features, in_features / 2] int8 or uint8")
+        n, k = weight_packed.shape[0], weight_packed.shape[1] * 2
+        if group_size < 32 or group_size % 32:
+            raise QuadmulError("W4A16Linear: group_size must be a multiple of 32")
+        if weight_scale.shape != (n, -(-k // group_size)) or weight_scale.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+            raise QuadmulError("W4A16Linear: weight_scale must be [out_features, ceil(in_features / group_size)], float32 or the activations' type")
+        if bias is not None and bias.shape != (n,):
+            raise QuadmulError("W4A16Linear: bias must be [out_features]")
+        self.out_features, self.in_features, self.group_size = n, k, group_size
+        self.register_buffer("weight_packed", weight_packed.contiguous())
+        self.register_buffer("weight_scale", weight_scale.contiguous())
+        self.register_buffer("bias", None if bias is None else bias.contiguous())
+
+    @classmethod
+    def from_float(cls, weight: torch.Tensor, group_size: int = 128, bias: Optional[torch.Tensor] = None, scale_dtype: Optional[torch.dtype] = None):
+        """Quantise a float [out_features, in_features] weight (on the GPU) group by group; ``scale_dtype`` None: the scales in the weight's type, if that is
+        one of 16 bits, else float32. The bias is taken in the same type as a 16-bit weight's."""
+        half = weight.dtype in (torch.float16, torch.bfloat16)
+        packed, scales = quantize_groups(weight.contiguous(), group_size, scale_dtype if scale_dtype is not None else weight.dtype if half else None)
+        return cls(packed, scales, group_size, bias.to(weight.dtype) if bias is not None and half else bias)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if x.shape[-1] != self.in_features:
+            raise QuadmulError(f"W4A16Linear: last dimension of x must be {self.in_features}")
+        bias = self.bias
+        if bias is not None and bias.dtype != x.dtype:
+            bias = bias.to(x.dtype)
+        flat = x.dim() == 2
+        y = gemm_grouped(x if flat else x.reshape(-1, self.in_features), self.weight_packed, self.weight_scale, self.group_size, bias)
+        return y if flat else y.reshape(*x.shape[:-1], self.out_features)
+
+    def extra_repr(self) -> str:
+        return f"in_features={self.in_features}, out_features={self.out_features}, group_size={self.group_size}, bias={self.bias is not None}"
