@@ -36,10 +36,11 @@ extern "C" {
 #define QM_ERR_SHAPE         -2 /* m, n or k negative, k odd, a size overflows int32, or a size the call does not take */
 #define QM_ERR_CONFIG        -3 /* cfg id unknown, or that config cannot run this shape     */
 #define QM_ERR_LAUNCH        -4 /* the HIP runtime refused the launch (see qm_last_hip_error) */
-#define QM_ERR_ALIGN         -5 /* C is not 4-byte aligned (a 16-bit output: 2-byte)         */
-#define QM_ERR_DTYPE         -6 /* out_dtype is none of the QM_OUT_* values                 */
+#define QM_ERR_ALIGN         -5 /* C is not 4-byte aligned (a 16-bit output: 2-byte), or a pointer less aligned
+                                   than the call says                                        */
+#define QM_ERR_DTYPE         -6 /* out_dtype is none of the QM_OUT_* values, or a type the call does not take */
 #define QM_ERR_SCRATCH       -7 /* qm_gemm_i4_static: the call needs more scratch memory than
-                                   QM_STATIC_SCRATCH_BYTES                                   */
+                                   QM_STATIC_SCRATCH_BYTES; others: a workspace that is too small */
 
 #define QM_CFG_AUTO          -1 /* let the shape table / heuristic choose                   */
 #define QM_CFG_RECODE        -2 /* 6-bit operands whether they pay or not, on tiles of 256 x 256:
@@ -256,10 +257,12 @@ int qm_linear_i4(const void *x, int in_dtype, const void *B, void *D, int m, int
  * D [m, n] of x's type.  Sums are IEEE single precision, the weights take part as the integers they are; one rounding, at
  * the end.  k is even (k == 0: D is the bias, or zero).  D must not overlap x.
  *   workspace  16-byte aligned device memory of qm_gemm_grouped_workspace_bytes(...) bytes, used in stream order by the
- *              kernels of this call only (align: the alignment in bytes that x, its rows and B share); QM_ERR_SCRATCH
- *              with less, and nothing is enqueued
+ *              kernels of this call only (weight_align: the alignment of B in bytes; x, the scales and D may be at any address of
+ *              their types); QM_ERR_SCRATCH with less, and nothing is enqueued
+ * With bf16 activations the weights take part as 136 more than they are, and 136 times the sum of x is taken off: an |x| above 2^119, or an
+ * infinity, makes its row of D infinite or NaN whatever the weights are.
  */
-size_t qm_gemm_grouped_workspace_bytes(int m, int n, int k, int group, int align);
+size_t qm_gemm_grouped_workspace_bytes(int m, int n, int k, int group, int weight_align);
 int qm_gemm_grouped_i4(const void *x, int dtype, long long x_stride, const void *B, const void *scale, int scale_dtype, int group,
                        const void *bias, void *D, int m, int n, int k, void *stream, void *workspace, size_t workspace_bytes);
 
@@ -276,7 +279,8 @@ int qm_gemm_grouped_i4(const void *x, int dtype, long long x_stride, const void 
  *   lengths      [sequences] int32: tokens of a sequence, the new ones included (below 1: none)
  *   query_start  [sequences + 1] int32: the new tokens of sequence s are rows query_start[s] to query_start[s + 1] - 1 of the
  *                packed tensors; NULL: every sequence has tokens / sequences of them.  They are the last tokens of their
- *                sequence: the last row is at position lengths[s] - 1.  Rows in front of position 0 are padding.
+ *                sequence: the last row is at position lengths[s] - 1.  Rows in front of position 0 are padding;
+ *                rows that query_start gives to no sequence are left as they are in the outputs.
  * page_size is 16, 32, 64 or 128; head_dim 64, 96, 128, 192 or 256.  All pointers are device pointers; what the last three hold is
  * looked at by the kernels only, and no value of theirs makes one read or write outside the tensors.
  */
@@ -294,7 +298,7 @@ typedef struct qm_kv_cache {
  * ([positions, rotary_pairs] float32); (a, b) are elements i and i + rotary_pairs, or 2i and 2i + 1 with interleaved = 1; further
  * elements stay as they are; rotary_pairs = 0: no rotation, else positions is 1 or more.  A position at or past `positions` gives NaN.
  * Storing, for each page, head and side, in single precision, every operation rounded by itself:
- *   scale' = max(scale, amax * (1 / 127)), amax over the new tokens of the page; scale counts as 0 in a page
+ *   scale' = max(scale, amax * (1 / 127)), amax over the new tokens of the page; scale (never below 0) counts as 0 in a page
  *            whose first token is new, which begins anew: all its other codes become 0
  *   code   = clamp(rint(value * (1 / scale')), -127, 127); the codes that the page held become rint(code * (scale / scale')).
  *            0 where scale' is below 2^-100.  Values that are not finite make scale' infinite or NaN, and attention to the page NaN.

@@ -380,8 +380,7 @@ def gemm_grouped(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tens
         x = x.contiguous()
     stride = x.stride(0) if m > 1 else k
     y = torch.empty((m, n), dtype=x.dtype, device=x.device)
-    low = x.data_ptr() | weight.data_ptr() | (2 * stride)
-    need = library().qm_gemm_grouped_workspace_bytes(m, n, k, group_size, low & -low if low & 15 else 16)
+    need = library().qm_gemm_grouped_workspace_bytes(m, n, k, group_size, 1 if weight.data_ptr() & 15 else 16)
     scratch = torch.empty((need,), dtype=torch.uint8, device=x.device) if need else None
     with torch.cuda.device(x.device):
         st = library().qm_gemm_grouped_i4(x.data_ptr(), kinds[x.dtype], stride, weight.data_ptr(), weight_scale.data_ptr(), kinds[weight_scale.dtype], group_size,

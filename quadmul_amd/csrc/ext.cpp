@@ -255,8 +255,7 @@ torch::Tensor gemm_grouped(torch::Tensor x, torch::Tensor weight, torch::Tensor 
     if ((k > 1 && x.stride(1) != 1) || (m > 1 && x.stride(0) < k)) x = x.contiguous();
     auto y = torch::empty({m, n}, x.options());
     const int64_t stride = m > 1 ? x.stride(0) : k;
-    const uintptr_t low = reinterpret_cast<uintptr_t>(x.data_ptr()) | reinterpret_cast<uintptr_t>(weight.data_ptr()) | (uintptr_t)(2 * stride);
-    const size_t need = qm_gemm_grouped_workspace_bytes((int)m, (int)n, (int)k, (int)group, low & 15 ? (int)(low & (~low + 1)) : 16);
+    const size_t need = qm_gemm_grouped_workspace_bytes((int)m, (int)n, (int)k, (int)group, reinterpret_cast<uintptr_t>(weight.data_ptr()) & 15 ? 1 : 16);
     torch::Tensor scratch;
     if (need > 0) scratch = torch::empty({(int64_t)need}, x.options().dtype(torch::kUInt8));
     check_status(qm_gemm_grouped_i4(x.data_ptr(), type, stride, weight.data_ptr(), weight_scale.data_ptr(), weight_scale.scalar_type() == torch::kFloat32 ? QM_IN_F32 : type,

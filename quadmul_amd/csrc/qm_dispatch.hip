@@ -928,12 +928,12 @@ QM_EXPORT const char *qm_status_string(int status)
     switch (status) {
     case QM_OK: return "ok";
     case QM_ERR_NULL: return "null pointer";
-    case QM_ERR_SHAPE: return "bad shape (m, n, k must be >= 0 and k even)";
+    case QM_ERR_SHAPE: return "bad shape (m, n, k must be >= 0 and k even), or a size the call does not take";
     case QM_ERR_CONFIG: return "unknown kernel configuration, or it cannot run this shape";
     case QM_ERR_LAUNCH: return "HIP launch failed";
-    case QM_ERR_ALIGN: return "C must be 4-byte aligned (a 16-bit output 2-byte aligned)";
-    case QM_ERR_DTYPE: return "unknown output type";
-    case QM_ERR_SCRATCH: return "the call needs more scratch memory than the library's static array (QM_STATIC_SCRATCH_BYTES) holds";
+    case QM_ERR_ALIGN: return "C must be 4-byte aligned (a 16-bit output 2-byte aligned), or a pointer is less aligned than the call asks for";
+    case QM_ERR_DTYPE: return "unknown output type, or a type the call does not take";
+    case QM_ERR_SCRATCH: return "the call needs more scratch memory than the library's static array (QM_STATIC_SCRATCH_BYTES) holds, or than the workspace given";
     default: return "unknown status";
     }
 }

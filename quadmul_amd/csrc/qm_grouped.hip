@@ -18,10 +18,11 @@ struct GroupedPlan {
     int waves, ways, chunk, runs;  // of a workgroup, to a tile of columns; blocks of 32 of K in a run, runs
     size_t bytes;
 };
-static GroupedPlan grouped_plan(int m, int n, int k, int align)
+static GroupedPlan grouped_plan(int m, int n, int k, int align)  // (align: of B; x may be anywhere)
 {
     GroupedPlan p{GROUPED_ANY, 16, 1, 0, 1, 0};
-    if (k == 0 || k % 32 != 0 || align < 16) return p;
+    // (a wave reaches up to 64 rows of B with offsets of 32 bits)
+    if (k == 0 || k % 32 != 0 || align < 16 || k >= 1 << 26) return p;
     if (m > 16 && n > 65535 * 64) return p;  // (the grid's limit)
     if (m > 16) {
         p.kernel = GROUPED_TILE;
@@ -89,13 +90,6 @@ static hipError_t launch_grouped(GroupedArgs p, const GroupedPlan &plan, hipStre
 
 using namespace qm;
 
-static int grouped_align(const void *x, long long x_stride, const void *B)
-{
-    (void)x;
-    const uintptr_t low = (uintptr_t)B;
-    return x_stride >= (1ll << 31) / 512 ? 1 : low & 15 ? (int)(low & (~low + 1)) : 16;  // (32-bit offsets of rows of x)
-}
-
 QM_EXPORT size_t qm_gemm_grouped_workspace_bytes(int m, int n, int k, int group, int align)
 {
     if (m <= 0 || n <= 0 || k <= 0 || (k & 1) || group < 32 || group % 32 != 0) return 0;
@@ -111,7 +105,7 @@ QM_EXPORT int qm_gemm_grouped_i4(const void *x, int dtype, long long x_stride, c
     if (m == 0 || n == 0) return QM_OK;
     if (!D || (k > 0 && (!x || !B || !scale))) return QM_ERR_NULL;
     if ((((uintptr_t)x | (uintptr_t)D | (uintptr_t)bias) & 1) || ((uintptr_t)scale & (scale_dtype == QM_IN_F32 ? 3 : 1)) || ((uintptr_t)workspace & 15)) return QM_ERR_ALIGN;
-    const GroupedPlan plan = grouped_plan(m, n, k, grouped_align(x, m > 1 ? x_stride : 0, B));
+    const GroupedPlan plan = grouped_plan(m, n, k, ((uintptr_t)B & 15) == 0 ? 16 : 1);
     if (plan.bytes > 0 && (!workspace || workspace_bytes < plan.bytes)) return QM_ERR_SCRATCH;
     const GroupedArgs p{static_cast<const uint16_t *>(x), static_cast<const uint8_t *>(B), scale, static_cast<const uint16_t *>(bias),
                         static_cast<uint16_t *>(D), m > 1 ? x_stride : k, m, n, k, group, (int)(((long long)k + group - 1) / group), 1, 0,

@@ -115,7 +115,7 @@ __device__ __forceinline__ void turn_blocks(uint32_t (&w)[4])
 }
 
 // The same from loads in which four lanes side by side have the four blocks of a column, its 64 bytes: the memory pipeline takes 16 bytes of neighbours
-// together and of lanes 16 apart each by itself, four times as many accesses (a third of the time of 13 x 8192 x 28672). Lane 4 n + j has dwords 0..3 of block
+// together and of lanes 16 apart each by itself, four times as many accesses. Lane 4 n + j has dwords 0..3 of block
 // j of column n; afterwards lane 16 c + 4 b + a has dword c of blocks 0..3 of column 4 a + b.
 __device__ __forceinline__ void gather_blocks(uint32_t (&w)[4])
 {
@@ -210,7 +210,7 @@ struct GroupedScaleSet {
 
 // Up to 16 rows. A workgroup has a run of K (all of it where that fits) of x in its LDS, in the order that the first operand wants it, paired, and goes
 // through tiles of columns. A wave has 16 columns and an equal share of the run's quads (four blocks, 64 bytes of each column): `ways` waves share a
-// tile, and their sums meet in the LDS. Bound by the weights' way from HBM: eight quads of a wave are in flight, from the next tile too;
+// tile, and their sums meet in the LDS. Bound by the weights' way from HBM: two to eight quads of each of 16 waves are in flight, from the next tile too;
 // and by what a quad costs of the vector pipeline: about 70 instructions a kilobyte, of which 30 make floats of the weights; 6 TB/s leave it 90.
 // (With x from the L2 by each wave for itself, 4 KiB of x for a KiB or two of weights, 13 x 8192 x 28672 took 52 us; with x put into the LDS
 // by 832 workgroups 45.)

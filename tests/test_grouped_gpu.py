@@ -163,3 +163,10 @@ def test_without_the_extension_the_same(monkeypatch):
     first = qm.gemm_grouped(*args)
     monkeypatch.setattr(qm, "_ext", types.SimpleNamespace(**dict.fromkeys(qm._EXT_FUNCTIONS, lambda *a: None)))
     assert torch.equal(first, qm.gemm_grouped(*args))
+
+
+@pytest.mark.parametrize("m,n,k,x_off,w_off", [(13, 40, 16384, 1, 0), (13, 40, 16384, 0, 16), (16, 40, 16384, 3, 3), (20, 40, 16384, 1, 0), (100, 40, 16384, 5, 16), (100, 40, 16384, 1, 1)])
+def test_any_address_with_k_in_runs(m, n, k, x_off, w_off):
+    """K summed in several runs, with x and the weights at any address: whether there is a workspace goes by the weights' alignment alone."""
+    test_any_address(m, n, k, 128, x_off, w_off)
+    assert (qm.library().qm_gemm_grouped_workspace_bytes(m, n, k, 128, 16) > 0) and qm.library().qm_gemm_grouped_workspace_bytes(m, n, k, 128, 1) == 0
