@@ -16,19 +16,24 @@ enum GroupedKernel { GROUPED_ANY, GROUPED_ROWS16, GROUPED_TILE };
 struct GroupedPlan {
     GroupedKernel kernel;
     int waves, ways, chunk, runs;  // of a workgroup, to a tile of columns; blocks of 32 of K in a run, runs
+    int rows;                      // of a tile
     size_t bytes;
 };
 static GroupedPlan grouped_plan(int m, int n, int k, int align)  // (align: of B; x may be anywhere)
 {
-    GroupedPlan p{GROUPED_ANY, 16, 1, 0, 1, 0};
+    GroupedPlan p{GROUPED_ANY, 16, 1, 0, 1, 0, 0};
     // (a wave reaches up to 64 rows of B with offsets of 32 bits)
     if (k == 0 || k % 32 != 0 || align < 16 || k >= 1 << 26) return p;
     if (m > 16 && n > 65535 * 64) return p;  // (the grid's limit)
     if (m > 16) {
         p.kernel = GROUPED_TILE;
         const int quads = (k / 32 + 3) / 4;
-        // a workgroup to a CU at least, of eight steps of K or more
-        const long long tiles = (long long)((m + (m > 64 ? 127 : m > 32 ? 63 : 31)) / (m > 64 ? 128 : m > 32 ? 64 : 32)) * ((n + 127) / 128);
+        const auto tiles_of = [&](const int rows) { return (long long)((m + rows - 1) / rows) * ((n + 127) / 128); };
+        // 256 rows where that leaves a tile to a CU and no more rows without anything to do than an eighth
+        const bool few_empty = (m + 255) / 256 * 2 == (m + 127) / 128 || m >= 1024;
+        p.rows = m <= 32 ? 32 : m <= 64 ? 64 : tiles_of(256) >= 256 && few_empty ? 256 : 128;
+        // a workgroup to a CU at least, of 1024 elements of K or more
+        const long long tiles = tiles_of(p.rows);
         p.runs = (int)std::max<long long>(1, std::min<long long>(256 / tiles, quads / 8));
         p.chunk = (quads + p.runs - 1) / p.runs * 4;
         p.runs = (k / 32 + p.chunk - 1) / p.chunk;
@@ -55,11 +60,21 @@ static hipError_t launch_mode(GroupedArgs p, const GroupedPlan &plan, hipStream_
 {
     p.chunk = plan.chunk, p.ways = plan.ways;
     if (plan.kernel == GROUPED_TILE) {
-        const auto go = [&](auto kernel, int bm, int bn) { return enqueue(kernel, dim3((p.M + bm - 1) / bm, (p.N + bn - 1) / bn, plan.runs), dim3(256), 0, s, p); };
-        // (with a scale to every one or two blocks the registers of 128 columns do not fit)
-        if (p.M > 64 && MODE == 1) return go(&gemm_grouped_tile_kernel<T, S, MODE, 2, 4, 4>, 128, 128);
-        if (p.M > 64) return go(&gemm_grouped_tile_kernel<T, S, MODE, 2, 4, 2>, 128, 64);
-        return p.M > 32 ? go(&gemm_grouped_tile_kernel<T, S, MODE, 1, 4, 2>, 64, 128) : go(&gemm_grouped_tile_kernel<T, S, MODE, 1, 2, 2>, 32, 128);
+        const dim3 grid((p.M + plan.rows - 1) / plan.rows, (p.N + 127) / 128, plan.runs);
+        // (with a scale to every one or two blocks the registers of 64 columns to a wave do not fit)
+        constexpr int NT = MODE == 1 ? 4 : 2, BN = 32 * NT;
+        const auto wide = [&](auto kernel, std::atomic<bool> *known) {
+            const int lds = 2 * 8 * 16 * (plan.rows + BN) + 2 * 2 * BN * (int)sizeof(float);
+            if (const hipError_t e = ensure_dynamic_lds(kernel, lds, known); e != hipSuccess) return e;
+            return enqueue(kernel, dim3(grid.x, (p.N + BN - 1) / BN, grid.z), dim3(plan.rows * 2), lds, s, p);
+        };
+        static std::atomic<bool> known_wide[2][QM_MAX_DEVICES] = {};
+        switch (plan.rows) {
+        case 256: return wide(&gemm_grouped_wide_kernel<T, S, MODE, 4, 2, 4, NT>, known_wide[0]);
+        case 128: return wide(&gemm_grouped_wide_kernel<T, S, MODE, 2, 2, 4, NT>, known_wide[1]);
+        case 64: return enqueue(&gemm_grouped_tile_kernel<T, S, MODE, 4, 2>, grid, dim3(256), 0, s, p);
+        case 32: return enqueue(&gemm_grouped_tile_kernel<T, S, MODE, 2, 2>, grid, dim3(256), 0, s, p);
+        }
     }
     const int tiles = plan.waves / plan.ways, groups = ((p.N + 15) / 16 + tiles - 1) / tiles;
     const size_t lds = (size_t)plan.chunk * (64 * (p.M | 1) + 64);

@@ -95,13 +95,10 @@ struct GroupedWeights<QM_IN_BF16> {
     static __device__ __forceinline__ v4f mfma(const frag a, const frag b, const v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 };
 
+__device__ __forceinline__ int low_halves(const int a, const int b) { return (int)__builtin_amdgcn_perm((uint32_t)b, (uint32_t)a, 0x05040100u); }
+__device__ __forceinline__ int high_halves(const int a, const int b) { return (int)__builtin_amdgcn_perm((uint32_t)b, (uint32_t)a, 0x07060302u); }
 // eight consecutive elements of x, paired as the nibbles are
-__device__ __forceinline__ v4i paired(const v4i x)
-{
-    const auto low = [](const int a, const int b) { return (int)__builtin_amdgcn_perm((uint32_t)b, (uint32_t)a, 0x05040100u); };
-    const auto high = [](const int a, const int b) { return (int)__builtin_amdgcn_perm((uint32_t)b, (uint32_t)a, 0x07060302u); };
-    return v4i{low(x[0], x[2]), high(x[0], x[2]), low(x[1], x[3]), high(x[1], x[3])};
-}
+__device__ __forceinline__ v4i paired(const v4i x) { return v4i{low_halves(x[0], x[2]), high_halves(x[0], x[2]), low_halves(x[1], x[3]), high_halves(x[1], x[3])}; }
 
 // lane group c has dwords 0..3 of block c  ->  it has dword c of blocks 0..3
 __device__ __forceinline__ void turn_blocks(uint32_t (&w)[4])
@@ -368,22 +365,22 @@ __global__ __launch_bounds__(256) void gemm_grouped_join_kernel(const GroupedArg
     }
 }
 
-// More rows: tiles of 16 WM MT rows and 64 NT / WM columns, a step of four blocks (128 elements of K) at a time. x goes through the LDS, two steps of it, in
-// the order of the first operand; a wave makes the second operand of its 16 NT columns itself, from 64 bytes of each. The sums over a group
-// and those over all of K are in registers of their own. Bound by the matrix cores and, nearly as much, by the instructions that make
-// floats of the weights (46 for a tile of 16 columns and a step, against 16 MT cycles of matrix instructions each).
+// 17 to 64 rows: tiles of 16 MT rows and 64 NT columns, a step of four blocks (128 elements of K) at a time. x goes through the LDS, two steps of it, in
+// the order of the first operand; a wave makes the second operand of its 16 NT columns itself, from 64 bytes of each, for all rows. The sums
+// over a group and those over all of K are in registers of their own. Bound by the instructions that make floats of the weights (46
+// for 16 columns and a step) until there are 64 rows, whose matrix instructions take as long.
 // A row's 16 pieces of a step are dealt to the places r ^ piece, so that neither writing 16 of one row nor reading one of 16 rows meets a bank twice.
-template <int T, int S, int MODE, int WM, int MT, int NT>
+template <int T, int S, int MODE, int MT, int NT>
 __global__ __launch_bounds__(256, 2) void gemm_grouped_tile_kernel(const GroupedArgs p)
 {
     typedef GroupedWeights<T> W;
     typedef typename W::frag frag;
     typedef GroupedScaleSet<S, MODE, 1> Scales;
-    constexpr int PER = MODE == 1 ? 4 : MODE == 2 ? 2 : 1, BM = 16 * WM * MT, BN = 64 / WM * NT, PIECES = BM / 16;  // PIECES: of x, 16 bytes each, of a thread and step
+    constexpr int PER = MODE == 1 ? 4 : MODE == 2 ? 2 : 1, BM = 16 * MT, BN = 64 * NT, PIECES = BM / 16;  // PIECES: of x, 16 bytes each, of a thread and step
     __shared__ v4i staged[2][4 * BM * 4];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, c = lane >> 4;
     const int block0 = blockIdx.z * p.chunk, blocks = min(p.chunk, p.K / 32 - block0), quads = (blocks + 3) / 4;
-    const int m0 = blockIdx.x * BM, n0 = blockIdx.y * BN + wave / WM * 16 * NT;
+    const int m0 = blockIdx.x * BM, n0 = blockIdx.y * BN + wave * 16 * NT;
 
     const size_t w_all = (size_t)p.N * (p.K / 2), s_all = (size_t)p.N * p.groups * Scales::SB;
     const size_t w_from = min((size_t)n0 * (p.K / 2) + (size_t)block0 * 16, w_all), s_from = min((size_t)n0 * p.groups * Scales::SB, s_all);
@@ -425,7 +422,7 @@ __global__ __launch_bounds__(256, 2) void gemm_grouped_tile_kernel(const Grouped
             for (int i = 0; i < 4; ++i) w[t][i] = (uint32_t)in.w[t][i];
             gather_blocks(w[t]);
         }
-        const v4i *const from = staged[quad & 1] + wave % WM * MT * 64 + c * 16;
+        const v4i *const from = staged[quad & 1] + c * 16;
 #pragma unroll
         for (int run = 0; run < 4; run += PER) {
             v4f part[MT][NT];
@@ -488,7 +485,157 @@ __global__ __launch_bounds__(256, 2) void gemm_grouped_tile_kernel(const Grouped
         for (int a = 0; a < MT; ++a) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int m = m0 + (wave % WM * MT + a) * 16 + 4 * c + i;
+                const int m = m0 + a * 16 + 4 * c + i;
+                if (m < p.M && n < p.N) {
+                    if (p.part != nullptr) p.part[((size_t)blockIdx.z * p.M + m) * p.N + n] = total[a][t][i];
+                    else p.D[(size_t)m * p.N + n] = round16<T>(p.bias != nullptr ? total[a][t][i] + bias : total[a][t][i]);
+                }
+            }
+        }
+    }
+}
+
+// Eight weights as 16-bit floats in the order they have in memory, exactly.
+template <int T>
+__device__ __forceinline__ v4i plain_weights(const uint32_t w)
+{
+    if constexpr (T == QM_IN_F16) {
+        const v4i v = __builtin_bit_cast(v4i, GroupedWeights<T>::of(w));
+        return v4i{low_halves(v[0], v[1]), low_halves(v[2], v[3]), high_halves(v[0], v[1]), high_halves(v[2], v[3])};
+    }
+    v4i out;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const auto value = [&](const int k) { return __builtin_bit_cast(int, (float)((int)(w << (28 - 4 * k)) >> 28)); };
+        out[i] = high_halves(value(2 * i), value(2 * i + 1));  // (the float of a small integer has zeros below)
+    }
+    return out;
+}
+
+// Many rows: tiles of 16 WM MT rows and 16 WN NT columns, a step of two blocks (64 elements of K) at a time. x and the weights, as floats, go
+// through the LDS, two steps of them, each weight made a float once by one thread of the workgroup; a wave has 16 MT rows and 16 NT columns.
+// Bound by what the matrix cores (16 cycles an instruction, 41 % of the time) and the vector pipeline (33 %: the sums times their scales, and
+// making floats) do not do at the same time. 2048 x 11008 x 4096 in groups of 128: 214 us, 863 TFLOP/s; with each wave making floats of
+// its own columns 274, without one half of the waves preparing before and the other after 226, as four waves to each of two workgroups of a CU
+// 241. Groups of 64 305 us, of 32 335.
+// Piece p (eight k) of row r lies at p * rows + (r ^ p): neither eight pieces of a row, written together, nor a piece of eight rows, read
+// together, meet a bank twice.
+template <int T, int S, int MODE, int WM, int WN, int MT, int NT>
+__global__ __launch_bounds__(64 * WM * WN, 2) void gemm_grouped_wide_kernel(const GroupedArgs p)
+{
+    typedef GroupedWeights<T> W;
+    typedef typename W::frag frag;
+    constexpr int THREADS = 64 * WM * WN, BM = 16 * WM * MT, BN = 16 * WN * NT, XP = BM * 8 / THREADS, WP = (BN * 4 + THREADS - 1) / THREADS;
+    constexpr int SCALES = MODE == 1 || MODE == 2 ? 1 : 2;  // of a step; or one
+    constexpr bool TWO = MODE == 1;                         // for two steps
+    extern __shared__ v4i staged[];
+    v4i *const all_x = staged, *const all_w = staged + 2 * 8 * BM;
+    float *const all_s = reinterpret_cast<float *>(staged + 2 * 8 * (BM + BN));
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 15, c = lane >> 4;
+    const int block0 = blockIdx.z * p.chunk, blocks = min(p.chunk, p.K / 32 - block0), steps = (blocks + 1) / 2;
+    const int m0 = blockIdx.x * BM, n0 = blockIdx.y * BN;
+
+    const uint16_t *x_at[XP];
+    const uint8_t *w_at[WP];
+#pragma unroll
+    for (int i = 0; i < XP; ++i) x_at[i] = p.x + min(m0 + tid / 8 + i * (THREADS / 8), p.M - 1) * p.x_stride + (size_t)block0 * 32;
+#pragma unroll
+    for (int i = 0; i < WP; ++i) w_at[i] = p.B + (size_t)min(n0 + tid / 4 + i * (THREADS / 4), p.N - 1) * (p.K / 2) + (size_t)block0 * 16;
+    const int s_block = SCALES == 2 ? tid / BN : 0;
+    const size_t s_row = (size_t)min(n0 + tid % BN, p.N - 1) * p.groups;
+
+    struct Raw {
+        v4i x[XP];
+        v2i w[WP];
+        uint32_t s;
+    };
+    const auto get = [&](Raw &to, int step) {
+        step = min(step, steps - 1);
+        const int k = min(step * 64 + (tid & 7) * 8, blocks * 32 - 8), half = min(step * 4 + (tid & 3), blocks * 2 - 1);
+#pragma unroll
+        for (int i = 0; i < XP; ++i) to.x[i] = *reinterpret_cast<const v4i_half_aligned *>(x_at[i] + k);
+#pragma unroll
+        for (int i = 0; i < WP; ++i) to.w[i] = *reinterpret_cast<const v2i *>(w_at[i] + half * 8);
+        if (tid < BN * SCALES) {
+            const size_t at = s_row + min((block0 + step * 2 + s_block) * 32 / p.group, p.groups - 1);
+            to.s = S == QM_IN_F32 ? static_cast<const uint32_t *>(p.scale)[at] : static_cast<const uint16_t *>(p.scale)[at];
+        }
+    };
+    const auto put_in_place = [&](const Raw &from, const int step) {
+        v4i *const to_x = all_x + (step & 1) * (8 * BM), *const to_w = all_w + (step & 1) * (8 * BN);
+        const int piece = tid & 7, row = tid / 8, half = tid & 3, column = tid / 4;
+        const bool in = step * 8 + piece < blocks * 4;  // past the end of K: zeros, which whatever weights meet
+#pragma unroll
+        for (int i = 0; i < XP; ++i) to_x[piece * BM + i * (THREADS / 8) + (row ^ piece)] = in ? from.x[i] : v4i{};
+#pragma unroll
+        for (int i = 0; i < WP; ++i) {
+            if (BN * 4 < THREADS && tid >= BN * 4) break;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) to_w[(2 * half + j) * BN + i * (THREADS / 4) + (column ^ (2 * half + j))] = plain_weights<T>((uint32_t)from.w[i][j]);
+        }
+        if (tid < BN * SCALES) all_s[(step & 1) * (BN * SCALES) + tid] = S == QM_IN_F32 ? __builtin_bit_cast(float, from.s) : float_of<S == QM_IN_F32 ? QM_IN_F16 : S>((uint16_t)from.s);
+    };
+
+    v4f total[MT][NT] = {}, part[MT][NT];
+    const int wm = wave % WM, wn = wave / WM;
+    const auto use = [&](const int step, const bool first, const bool last) {
+        const v4i *const from_x = all_x + (step & 1) * (8 * BM) + wm * (16 * MT), *const from_w = all_w + (step & 1) * (8 * BN) + wn * (16 * NT);
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            frag xs[MT], ws[NT];
+            const int piece = 4 * b + c;
+#pragma unroll
+            for (int a = 0; a < MT; ++a) xs[a] = __builtin_bit_cast(frag, from_x[piece * BM + 16 * a + (r ^ piece)]);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) ws[t] = __builtin_bit_cast(frag, from_w[piece * BN + 16 * t + (r ^ piece)]);
+            const bool fresh = SCALES == 2 || (b == 0 && first), full = SCALES == 2 || (b == 1 && last);
+#pragma unroll
+            for (int a = 0; a < MT; ++a)
+#pragma unroll
+                for (int t = 0; t < NT; ++t) part[a][t] = W::mfma(xs[a], ws[t], fresh ? v4f{} : part[a][t]);
+            if (full) {
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    const float scale = all_s[(step & 1) * (BN * SCALES) + (SCALES == 2 ? b * BN : 0) + wn * (16 * NT) + 16 * t + r];
+#pragma unroll
+                    for (int a = 0; a < MT; ++a) total[a][t] += part[a][t] * scale;
+                }
+                __builtin_amdgcn_sched_barrier(0);  // (two sets of sums at a time would not fit)
+            }
+        }
+    };
+
+    // One half of the waves, one of the two of each SIMD, prepares the next step before it multiplies, the other after: the vector pipeline and the
+    // matrix cores have something to do at the same time.
+    const bool early = wave < WM * WN / 2;
+    Raw raw[2];
+    get(raw[0], 0);
+    put_in_place(raw[0], 0);
+    get(raw[1], 1);
+    for (int step = 0; step < steps; step += 2) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            __syncthreads();
+            const auto prepare = [&] {
+                if (step + i < steps) put_in_place(raw[i ^ 1], step + i + 1);
+                get(raw[i], step + i + 2);
+            };
+            if (early) prepare();
+            use(step + i, !TWO || i == 0, !TWO || i == 1);  // (the second may be past the end of K: zeros)
+            __builtin_amdgcn_sched_barrier(0);
+            if (!early) prepare();
+        }
+    }
+
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const int n = n0 + (wn * NT + t) * 16 + r;
+        const float bias = p.bias != nullptr && p.part == nullptr && n < p.N ? float_of<T>(p.bias[n]) : 0.0f;
+#pragma unroll
+        for (int a = 0; a < MT; ++a) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int m = m0 + (wm * MT + a) * 16 + 4 * c + i;
                 if (m < p.M && n < p.N) {
                     if (p.part != nullptr) p.part[((size_t)blockIdx.z * p.M + m) * p.N + n] = total[a][t][i];
                     else p.D[(size_t)m * p.N + n] = round16<T>(p.bias != nullptr ? total[a][t][i] + bias : total[a][t][i]);
