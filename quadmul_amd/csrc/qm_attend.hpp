@@ -125,7 +125,8 @@ __device__ __forceinline__ AttendCut attend_cut(const KvArgs &c, const AttendArg
     return {-1, 1, 0};
 }
 
-// q^T of one row: float16, bf16 brought into its range by a power of two. What is left for the scores to be multiplied with.
+// q^T of one row: float16, bf16 brought into its range by a power of two, with the sign of `scale`. What is left for the scores to be
+// multiplied with, 0 or more.
 template <int T, int D>
 __device__ __forceinline__ float attend_query(const uint16_t *x, const float scale, h8 (&query)[D / 32])
 {
@@ -143,9 +144,8 @@ __device__ __forceinline__ float attend_query(const uint16_t *x, const float sca
             most = fmaxf(most, fabsf(v[j][e]));
         }
     }
-    if constexpr (T == QM_IN_F16) {
-        return scale;
-    } else {
+    float by = fabsf(scale);
+    if constexpr (T != QM_IN_F16) {
         most = across_groups_max(most);
         const int e = max((int)(__builtin_bit_cast(uint32_t, most) >> 23) - 127 - 14, -100);  // the largest becomes 2^14 to 2^15
         const float down = __builtin_bit_cast(float, (uint32_t)(127 - e) << 23);
@@ -154,29 +154,32 @@ __device__ __forceinline__ float attend_query(const uint16_t *x, const float sca
 #pragma unroll
             for (int i = 0; i < 8; ++i) query[j][i] = (_Float16)(v[j][i] * down);
         }
-        return scale * __builtin_bit_cast(float, (uint32_t)(127 + e) << 23);
+        by *= __builtin_bit_cast(float, (uint32_t)(127 + e) << 23);
     }
+    if (scale < 0.0f) {
+#pragma unroll
+        for (int j = 0; j < J; ++j) query[j] = -query[j];
+    }
+    return by;
 }
 
 // A row of the softmax so far: the maxima of the scores and of score + log2(scale of the value), the sum.
 struct AttendRow {
     float top = ATTEND_LOW, high = ATTEND_LOW, total = 0.0f;
 };
-// Sixteen scores of a lane (tokens token0 + 4 t + i) into weights for the values: by: what a score is multiplied with; vs: the scale of the
-// values; whole: every row sees every token.
+// Sixteen scores of a lane (tokens token0 + 4 t + i) into weights for the values: by: what a score is multiplied with, 0 or more; vs: the scale
+// of the values; whole: every row sees every token.
 template <int DT>
-__device__ __forceinline__ void attend_weights(v4f (&score)[4], const float by, const float vs, const bool whole, const bool there, const int token0, const int limit,
+__device__ __forceinline__ void attend_weights(v4f (&score)[4], float by, const float vs, const bool whole, const bool there, const int token0, const int limit,
                                                const int below, AttendRow &row, v4f (&out)[DT], h8 (&weight)[2])
 {
     float most = -INFINITY;
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            score[t][i] *= by;
-            most = fmaxf(most, score[t][i]);
-        }
+        for (int i = 0; i < 4; ++i) most = fmaxf(most, score[t][i]);
     }
+    most *= by;
     if (!whole) {
         most = -INFINITY;
 #pragma unroll
@@ -184,10 +187,11 @@ __device__ __forceinline__ void attend_weights(v4f (&score)[4], const float by, 
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int j = token0 + 4 * t + i;
-                score[t][i] = (there & (j <= limit) & (j > below)) ? score[t][i] : -INFINITY;
+                score[t][i] = (there & (j <= limit) & (j > below)) ? score[t][i] * by : -INFINITY;
                 most = fmaxf(most, score[t][i]);
             }
         }
+        by = 1.0f;
     }
     const float size = vs == 0.0f ? -INFINITY : __builtin_amdgcn_logf(fabsf(vs));
     if (__any(most > row.top + ATTEND_SLACK || most + size > row.high + ATTEND_SLACK)) {
@@ -207,7 +211,7 @@ __device__ __forceinline__ void attend_weights(v4f (&score)[4], const float by, 
     for (int t = 0; t < 4; ++t) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float p = __builtin_amdgcn_exp2f(score[t][i] - row.top);
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(score[t][i], by, -row.top));
             row.total += p;
             weight[t / 2][(t & 1) * 4 + i] = (_Float16)(p * weigh);
         }
