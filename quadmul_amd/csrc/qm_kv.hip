@@ -73,7 +73,7 @@ QM_EXPORT int qm_kv_append_i8(const qm_kv_cache *cache, const qm_kv_new *fresh, 
         e = enqueue(kernel, dim3((tasks + 3) / 4, std::min(c.sequences, 65535)), dim3(256), 0, s, c, f, slots, tasks);
     } else {
         const bool vector = n.rotary_pairs % 8 == 0;
-        const long long items = n.q ? (long long)most * n.heads * (c.dim / (vector ? 16 : 2)) : 0;
+        const long long items = !n.q ? 0 : vector ? (long long)most * ((n.heads + 1) / 2) * (c.dim / 16) : (long long)most * n.heads * (c.dim / 2);
         const int q_slots = (int)std::min<long long>((items + 2 * c.kv_heads * 256 - 1) / (2 * c.kv_heads * 256), 4096);
         const dim3 grid(slots + q_slots, 2 * c.kv_heads, std::min(c.sequences, 65535));
         const auto kernel = n.dtype == QM_IN_F16 ? (vector ? &kv_append_kernel<QM_IN_F16, true> : &kv_append_kernel<QM_IN_F16, false>)

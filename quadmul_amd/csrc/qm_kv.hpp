@@ -80,7 +80,8 @@ __device__ __forceinline__ int code_of(const float value, const float factor)
 // Sixteen values of a head: eight pairs that turn together (VECTOR: `pairs` is a multiple of eight), or one pair.
 template <int T, bool VECTOR>
 struct Pairs {
-    static constexpr int COUNT = VECTOR ? 8 : 1;
+    // HEADS: of the queries, that a thread has at a time, with the same cosines and sines: one 42 us for 4 prompts of up to 2048 tokens, two 35; four spill
+    static constexpr int COUNT = VECTOR ? 8 : 1, HEADS = VECTOR ? 2 : 1;
     Pair v[COUNT];
     int2 at;  // elements of the first pair; with VECTOR the eight a side by side from at.x and the eight b from at.y, or a, b, a, b, .. from at.x
     bool apart;
@@ -89,28 +90,40 @@ struct Pairs {
         at = pair_at(i * COUNT, pairs, interleaved);
         apart = i * COUNT < pairs && !interleaved;
     }
-    __device__ __forceinline__ void load(const uint16_t *x)
+    struct Raw {
+        v4i p, q;
+    };
+    __device__ __forceinline__ Raw get(const uint16_t *x) const
     {
+        if constexpr (VECTOR) return {*reinterpret_cast<const v4i_half_aligned *>(x + at.x), *reinterpret_cast<const v4i_half_aligned *>(x + (apart ? at.y : at.x + 8))};
+        else return {v4i{x[at.x]}, v4i{x[at.y]}};
+    }
+    __device__ __forceinline__ void set(const Raw &raw)
+    {
+        const v4i p = raw.p, q = raw.q;
+        const auto half = [](const v4i w, const int e) { return float_of<T>((uint16_t)((uint32_t)w[e / 2] >> (16 * (e & 1)))); };
         if constexpr (VECTOR) {
-            const v4i p = *reinterpret_cast<const v4i_half_aligned *>(x + at.x), q = *reinterpret_cast<const v4i_half_aligned *>(x + (apart ? at.y : at.x + 8));
-            const auto half = [](const v4i w, const int e) { return float_of<T>((uint16_t)((uint32_t)w[e / 2] >> (16 * (e & 1)))); };
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const float low = e < 4 ? half(p, 2 * e) : half(q, 2 * e - 8), high = e < 4 ? half(p, 2 * e + 1) : half(q, 2 * e - 7);
                 v[e] = apart ? Pair{half(p, e), half(q, e)} : Pair{low, high};
             }
         } else {
-            v[0] = Pair{float_of<T>(x[at.x]), float_of<T>(x[at.y])};
+            v[0] = Pair{half(p, 0), half(q, 0)};
         }
     }
-    // The four products and two sums are rounded one by one: the codes are defined by them.
-    __device__ __forceinline__ void turn(const KvNewArgs &f, const int position, const int i, const int pairs)
+    // Cosines and sines of lot i at a position.
+    struct Angles {
+        float c[COUNT], s[COUNT];
+        bool turns;
+    };
+    static __device__ __forceinline__ Angles angles(const KvNewArgs &f, const int position, const int i, const int pairs)
     {
-#pragma clang fp contract(off)
-        if (i * COUNT >= pairs) return;
+        Angles a{};
+        a.turns = i * COUNT < pairs;
+        if (!a.turns) return a;
         const bool in = position < f.positions;
         const size_t row = (size_t)(in ? max(position, 0) : 0) * pairs + i * COUNT;
-        float c[COUNT], s[COUNT];
         if constexpr (VECTOR) {
             const auto get = [&](float (&to)[COUNT], const float *from) {
 #pragma unroll
@@ -123,15 +136,23 @@ struct Pairs {
                     }
                 }
             };
-            get(c, f.cos + row);
-            get(s, f.sin + row);
+            get(a.c, f.cos + row);
+            get(a.s, f.sin + row);
         } else {
-            c[0] = f.cos[row], s[0] = f.sin[row];
+            a.c[0] = f.cos[row], a.s[0] = f.sin[row];
         }
 #pragma unroll
+        for (int e = 0; e < COUNT; ++e) a.c[e] = in ? a.c[e] : __builtin_nanf(""), a.s[e] = in ? a.s[e] : __builtin_nanf("");
+        return a;
+    }
+    // The four products and two sums are rounded one by one: the codes are defined by them.
+    __device__ __forceinline__ void turn(const Angles &by)
+    {
+#pragma clang fp contract(off)
+        if (!by.turns) return;
+#pragma unroll
         for (int e = 0; e < COUNT; ++e) {
-            const float cosine = in ? c[e] : __builtin_nanf(""), sine = in ? s[e] : __builtin_nanf("");
-            const float ac = v[e].a * cosine, bs = v[e].b * sine, bc = v[e].b * cosine, as = v[e].a * sine;
+            const float ac = v[e].a * by.c[e], bs = v[e].b * by.s[e], bc = v[e].b * by.c[e], as = v[e].a * by.s[e];
             v[e] = Pair{ac - bs, bc + as};
         }
     }
@@ -240,22 +261,29 @@ __global__ __launch_bounds__(256, 4) void kv_append_kernel(const KvArgs c, const
     for (int s = blockIdx.z; s < c.sequences; s += gridDim.z) {
         const KvSequence q = kv_sequence(c, s);
         if ((int)blockIdx.x >= slots) {
-            // a token's lots of all heads, tokens in turn
-            const int each = f.heads * lots, across = min(each, 256), stride = (int)(gridDim.x - slots) * gridDim.y * (256 / across);
+            // a lot of HEADS heads of a token, tokens in turn
+            const int each = (f.heads + Lot::HEADS - 1) / Lot::HEADS * lots, across = min(each, 256), stride = (int)(gridDim.x - slots) * gridDim.y * (256 / across);
             if (tid >= 256 / across * across) continue;
             for (int t = ((int)(blockIdx.x - slots) * gridDim.y + blockIdx.y) * (256 / across) + tid / across; t < q.count; t += stride) {
                 const int position = q.begin + t;
                 for (int i = tid % across; i < each; i += across) {
-                    const int head = i / lots, lot = i - head * lots;
+                    const int head0 = i / lots * Lot::HEADS, lot = i % lots;
                     Lot v;
                     v.place(lot, f.pairs, f.interleaved);
-                    v.load(f.q + (q.row0 + t) * f.q_token + head * f.q_head);
-                    v.turn(f, position, lot, f.pairs);
-                    if (position < 0) {
+                    typename Lot::Raw raw[Lot::HEADS];
 #pragma unroll
-                        for (int e = 0; e < Lot::COUNT; ++e) v.v[e] = Pair{0.0f, 0.0f};
+                    for (int h = 0; h < Lot::HEADS; ++h) raw[h] = v.get(f.q + (q.row0 + t) * f.q_token + min(head0 + h, f.heads - 1) * f.q_head);
+                    const typename Lot::Angles by = Lot::angles(f, position, lot, f.pairs);
+#pragma unroll
+                    for (int h = 0; h < Lot::HEADS; ++h) {
+                        v.set(raw[h]);
+                        v.turn(by);
+                        if (position < 0) {
+#pragma unroll
+                            for (int e = 0; e < Lot::COUNT; ++e) v.v[e] = Pair{0.0f, 0.0f};
+                        }
+                        if (head0 + h < f.heads) v.store(f.q_out + ((size_t)(q.row0 + t) * f.heads + head0 + h) * c.dim);
                     }
-                    v.store(f.q_out + ((size_t)(q.row0 + t) * f.heads + head) * c.dim);
                 }
             }
             continue;
@@ -280,8 +308,8 @@ __global__ __launch_bounds__(256, 4) void kv_append_kernel(const KvArgs c, const
             const auto key = [&](Lot &v, const int i) {
                 const int t = i / lots, lot = i - t * lots;
                 v.place(lot, f.pairs, f.interleaved);
-                v.load(x + (lo + t - q.begin) * f.k_token);
-                v.turn(f, lo + t, lot, f.pairs);
+                v.set(v.get(x + (lo + t - q.begin) * f.k_token));
+                v.turn(Lot::angles(f, lo + t, lot, f.pairs));
             };
             const auto square = [&](Square<T> &v, const int i) { v.load(x + channel(i), f.v_token, base + 4 * four(i), lo, hi, q.begin); };
             const auto put_key = [&](const Lot &v, const int i, const float inverse, const bool whole) { v.store_codes(reinterpret_cast<int8_t *>(whole ? image : codes) + (lo - base + i / lots) * c.dim, inverse); };
@@ -366,8 +394,8 @@ __global__ __launch_bounds__(256) void kv_append_few_kernel(const KvArgs c, cons
                 for (int pair = lane; pair < half; pair += 64) {
                     Lot v;
                     v.place(pair, f.pairs, f.interleaved);
-                    v.load(f.q + (q.row0 + t) * f.q_token + head * f.q_head);
-                    v.turn(f, position, pair, f.pairs);
+                    v.set(v.get(f.q + (q.row0 + t) * f.q_token + head * f.q_head));
+                    v.turn(Lot::angles(f, position, pair, f.pairs));
                     if (position < 0) v.v[0] = Pair{0.0f, 0.0f};
                     v.store(f.q_out + ((size_t)(q.row0 + t) * f.heads + head) * c.dim);
                 }
@@ -388,8 +416,8 @@ __global__ __launch_bounds__(256) void kv_append_few_kernel(const KvArgs c, cons
             uint32_t amax = 0;
             const auto key = [&](Lot &v, const int position, const int pair) {
                 v.place(pair, f.pairs, f.interleaved);
-                v.load(x + (position - q.begin) * f.k_token);
-                v.turn(f, position, pair, f.pairs);
+                v.set(v.get(x + (position - q.begin) * f.k_token));
+                v.turn(Lot::angles(f, position, pair, f.pairs));
             };
             const auto value = [&](const int position, const int d) { return float_of<T>(x[(position - q.begin) * f.v_token + d]); };
             for (int p = lo; p < hi; ++p) {
