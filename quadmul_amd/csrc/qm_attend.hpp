@@ -26,7 +26,7 @@ struct AttendArgs {
     float scale;   // times log2(e)
     int tiles;     // of rows, side by side
     int rows;      // of a tile that are used at most
-    int wide;      // 1: tiles of 64 rows (kv_attend_rows_kernel)
+    int wide;      // not 0: tiles of 64 rows (kv_attend_rows_kernel), so many steps at a time
     // all sequences' steps one after the other cut into as many equal parts (0: a sequence to a workgroup), for each tile and head, and what
     // is left where a sequence is cut: a part's end of one and beginning of another, 16 rows of dim values and their lse each; and the
     // first part of each sequence and their number
@@ -400,17 +400,19 @@ __global__ __launch_bounds__(NW * 64, D > 128 ? 1 : 2) void kv_attend_kernel(con
     }
 }
 
-// Many rows of a sequence: 16 to a wave, four waves to every other 64 tokens. The codes of 64 tokens become float16 once for their four waves, in
+// Many rows of a sequence: 16 to a wave, four waves to 64 tokens. The codes of 64 tokens become float16 once for their four waves, in
 // the LDS, in the order that the operands want them; each wave makes a fourth of them from what it loaded while the step before was computed.
 // blockIdx.x: a tile of 64 rows, the last ones, which see most, first; blockIdx.y: a head of the cache and a sequence. (The other way
 // round each of 8 heads has an XCD, whose CUs read the same lines at the same time: twice as long.) Bound by the vector
 // pipeline (what a score costs until it is a weight: nine instructions and an exponential) before the matrix cores. (With 32 rows to a wave and four waves
 // 4 prompts of up to 512 tokens took 162 us: the longest sequence had a workgroup to every other CU.)
-constexpr int ATTEND_LOTS = 2;  // of 64 tokens at a time (with four the registers of 128 channels do not fit: 138 us for 94)
-template <int T, int D>
-__global__ __launch_bounds__(256 * ATTEND_LOTS, D > 128 ? 2 : 4) void kv_attend_rows_kernel(const KvArgs c, const AttendArgs a)
+// LOTS of 64 tokens at a time share the rows: with two the longest sequence's last tiles are done sooner, with one (four workgroups to a CU) fewer waves
+// wait for each other. 4 prompts of up to 512 tokens (1024 tiles and heads) 95 us with two, 119 with one; 1 of 4096 (2048) 260 and 265; 8 of 2048
+// (8192) 561 and 490. (With four the registers of 128 channels do not fit: 138 us for the first.)
+template <int T, int D, int LOTS>
+__global__ __launch_bounds__(256 * LOTS, D > 128 ? 2 : 4) void kv_attend_rows_kernel(const KvArgs c, const AttendArgs a)
 {
-    constexpr int LOTS = ATTEND_LOTS, J = D / 32, DT = D / 16, KW = D / 16, QT = 1, ROWS = 64 * QT, MINE = (DT + 3) / 4;  // MINE: tiles of the values that a wave turns into floats
+    constexpr int J = D / 32, DT = D / 16, KW = D / 16, QT = 1, ROWS = 64 * QT, MINE = (DT + 3) / 4;  // MINE: tiles of the values that a wave turns into floats
     struct Floats {
         h8 keys[4][J][64], values[DT][2][64];
     };

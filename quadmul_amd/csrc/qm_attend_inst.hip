@@ -11,11 +11,11 @@ template <int D>
 static hipError_t launch(const KvArgs &c, const AttendArgs &a, hipStream_t s)
 {
     if (a.wide) {
-        constexpr int LOTS = ATTEND_LOTS, LDS = LOTS * (4 * (D / 32) + 2 * (D / 16)) * 64 * 16;  // keys and values of as many steps
-        static std::atomic<bool> known[QM_MAX_DEVICES] = {};
-        const auto kernel = &kv_attend_rows_kernel<QM_ATTEND_TYPE, D>;
-        if (const hipError_t e = ensure_dynamic_lds(kernel, LDS, known); e != hipSuccess) return e;
-        return enqueue(kernel, dim3(a.tiles, std::max(1, std::min(c.sequences, 65535 / c.kv_heads)) * c.kv_heads), dim3(256 * LOTS), LDS, s, c, a);
+        constexpr int LDS = (4 * (D / 32) + 2 * (D / 16)) * 64 * 16;  // keys and values of a step
+        static std::atomic<bool> known[2][QM_MAX_DEVICES] = {};
+        const auto kernel = a.wide == 1 ? &kv_attend_rows_kernel<QM_ATTEND_TYPE, D, 1> : &kv_attend_rows_kernel<QM_ATTEND_TYPE, D, 2>;
+        if (const hipError_t e = ensure_dynamic_lds(kernel, a.wide * LDS, known[a.wide - 1]); e != hipSuccess) return e;
+        return enqueue(kernel, dim3(a.tiles, std::max(1, std::min(c.sequences, 65535 / c.kv_heads)) * c.kv_heads), dim3(256 * a.wide), a.wide * LDS, s, c, a);
     }
     constexpr int NW = D > 128 ? 4 : 8;  // (with eight the registers of the wider heads do not fit)
     if (a.parts == 0) return enqueue(&kv_attend_kernel<QM_ATTEND_TYPE, D, NW, false>, dim3(std::min(c.sequences, 1 << 18) * c.kv_heads, a.tiles), dim3(NW * 64), 0, s, c, a);

@@ -104,8 +104,8 @@ static AttendPlan attend_plan(const qm_kv_cache *c, int tokens, int heads, int m
     p.tiles = (int)std::min<long long>((rows + 15) / 16, 4096);
     p.rows = (int)std::min<long long>(rows, 16);
     // many rows, and workgroups enough of 64
-    if (rows > 64 && (rows + 63) / 64 * c->kv_heads * c->sequences >= 128) {
-        p.wide = 1;
+    if (const long long workgroups = (rows + 63) / 64 * c->kv_heads * c->sequences; rows > 64 && workgroups >= 128) {
+        p.wide = workgroups >= 4096 ? 1 : 2;
         p.tiles = (int)std::min<long long>((rows + 63) / 64, 65535);
         return p;
     }

@@ -88,6 +88,16 @@ def test_many_rows(heads, kv_heads, dim, page, window, causal, dtype):
     both(q, cache, table, lengths, counts, causal=causal, window=window, max_query=150, max_length=400)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("dim,page,window,causal", [(64, 16, 0, True), (96, 64, 50, True), (128, 32, 0, False), (192, 16, 100, True), (256, 128, 0, True)])
+def test_many_rows_of_many_sequences(dim, page, window, causal, dtype):
+    """Enough tiles of 64 rows for workgroups that take the steps one by one."""
+    lengths, counts = [150, 400] + [3 * i for i in range(30)], [150, 131] + [7] * 30
+    q, cache, table = problem(lengths, counts, 16, 16, dim, page, dtype, 19)
+    table[1, 1] = -1
+    both(q, cache, table, lengths, counts, causal=causal, window=window, max_query=sum(counts), max_length=400)   # 8 tiles, 16 heads, 32 sequences
+
+
 def test_rows_that_see_nothing_are_zero():
     lengths, counts = [0, 30, 3, -4, 64], [1, 1, 6, 2, 1]   # no tokens at all; three rows in front of position 0; no tokens; only missing pages
     q, cache, table = problem(lengths, counts, 4, 2, 64, 16, torch.float16, 6)
