@@ -338,8 +338,9 @@ int qm_kv_read_i8(const qm_kv_cache *cache, const int *page_ids, int count, int 
 
 /*
  * Optional: everything a first launch on the current device would otherwise do once -- the
- * LDS size attribute and the residency query of every kernel, the address of the library's
- * scratch array -- without launching anything.  No counterpart in the reference (its
+ * LDS size attribute and the residency query of every kernel of the int4 products, the address of the library's
+ * scratch array -- without launching anything (qm_gemm_grouped_i4 and qm_kv_attend_i8 set their kernels' LDS size themselves, at the first
+ * launch, under capture too).  No counterpart in the reference (its
  * launch_igemm, kernel.cu:268-289, needs no set-up: 32 KB of shared memory at most).  First
  * launches do this by themselves, under HIP graph capture too; a caller that wants no
  * runtime queries inside a capture or a latency-critical first call makes this call first,

@@ -250,7 +250,8 @@ __device__ __forceinline__ uint32_t recoded(const uint32_t w, const float ratio)
 // blockIdx.z: a sequence; blockIdx.y: a head and a side (keys, values) of it; blockIdx.x: below `slots` the pages that the
 // sequence's new tokens fall into, past it the rotation of its queries. A thread has sixteen or 32 values at a time (its first ones stay in its
 // registers between the largest value and the codes; further ones are read again, from the L2). Where a page's codes all change they are put
-// together in the LDS and go out in whole lines. Bound by memory with many tokens, and by the chain lengths -> table -> page with few.
+// together in the LDS and go out in whole lines. 4 prompts of up to 2048 tokens, 32 heads of queries and 8 of the cache, 84 MB: 35 us, 2.4 TB/s: bound
+// by what 128 registers leave in flight.
 template <int T, bool VECTOR>
 __global__ __launch_bounds__(256, 4) void kv_append_kernel(const KvArgs c, const KvNewArgs f, const int slots)
 {

@@ -170,3 +170,13 @@ def test_any_address_with_k_in_runs(m, n, k, x_off, w_off):
     """K summed in several runs, with x and the weights at any address: whether there is a workspace goes by the weights' alignment alone."""
     test_any_address(m, n, k, 128, x_off, w_off)
     assert (qm.library().qm_gemm_grouped_workspace_bytes(m, n, k, 128, 16) > 0) and qm.library().qm_gemm_grouped_workspace_bytes(m, n, k, 128, 1) == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("m,n,k,group,wide", [(1024, 8300, 160, 64, True), (1030, 8191, 288, 32, False), (1100, 8192, 416, 128, True), (1024, 8200, 224, 96, False), (500, 16500, 96, 128, False),
+                                              (1024, 8192, 32, 256, True)])
+def test_tiles_of_256_rows(m, n, k, group, wide, dtype):
+    """Enough tiles for the largest ones: edges in rows and columns, a K that ends inside a step, every kind of group."""
+    x, q, s, b = problem(m, n, k, group, dtype, torch.float32 if wide else dtype, m == 1024, m + n + k)
+    y = qm.gemm_grouped(x.cuda(), pack_cpu(q).cuda(), s.cuda(), group, None if b is None else b.cuda())
+    check(x, q, s, group, b, y)
