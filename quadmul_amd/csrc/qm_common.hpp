@@ -32,6 +32,8 @@ struct exactly { using type = T; };
 template <class... P>
 inline hipError_t enqueue(void (*const kernel)(P...), const dim3 grid, const dim3 block, const size_t lds, hipStream_t s, typename exactly<P>::type... args)
 {
+    // (a grid has less than 2^32 threads along a side: the runtime takes them modulo 2^32, and a part of the grid would run without an error)
+    if ((uint64_t)grid.x * block.x > 0xFFFFFFFFu) return hipErrorInvalidConfiguration;
     void *at[] = {const_cast<void *>(static_cast<const void *>(&args))...};
     const hipError_t e = hipLaunchKernel(reinterpret_cast<const void *>(kernel), grid, block, at, lds, s);
     if (e != hipSuccess) (void)hipGetLastError();  // (the caller reports it)

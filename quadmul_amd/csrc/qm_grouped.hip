@@ -88,7 +88,7 @@ static hipError_t launch_grouped(GroupedArgs p, const GroupedPlan &plan, hipStre
 {
     if (plan.kernel == GROUPED_ANY) {
         const int rows = (p.M + GROUPED_ROWS - 1) / GROUPED_ROWS;
-        return enqueue(&gemm_grouped_any_kernel<T, S>, dim3((p.N + 3) / 4, std::min(rows, 65535)), dim3(256), 0, s, p);
+        return enqueue(&gemm_grouped_any_kernel<T, S>, dim3(std::min((unsigned)p.N / 4 + 1, 1u << 22), std::min(rows, 65535)), dim3(256), 0, s, p);
     }
     hipError_t e;
     switch (group_mode(p.group)) {

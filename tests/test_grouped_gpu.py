@@ -180,3 +180,16 @@ def test_tiles_of_256_rows(m, n, k, group, wide, dtype):
     x, q, s, b = problem(m, n, k, group, dtype, torch.float32 if wide else dtype, m == 1024, m + n + k)
     y = qm.gemm_grouped(x.cuda(), pack_cpu(q).cuda(), s.cuda(), group, None if b is None else b.cuda())
     check(x, q, s, group, b, y)
+
+
+@pytest.mark.parametrize("m", [1, 6])
+def test_more_columns_than_a_grid_has_threads(m):
+    """2^26 columns and a few: a wave to each would be 2^32 threads and more. Every result is an integer of few bits."""
+    n = 2 ** 26 + 5
+    g = torch.Generator(device="cuda").manual_seed(13)
+    w = torch.randint(-128, 128, (n, 1), dtype=torch.int8, device="cuda", generator=g)
+    x = torch.tensor([[i + 1.0, -3.0] for i in range(m)], dtype=torch.float16, device="cuda")
+    y = qm.gemm_grouped(x, w, torch.ones(n, 1, dtype=torch.float16, device="cuda"), 32)
+    low, high = ((w[:, 0] << 4) >> 4).half(), (w[:, 0] >> 4).half()
+    for i in range(m):
+        assert torch.equal(y[i], low * (i + 1.0) - high * 3.0)
