@@ -18,7 +18,8 @@ static hipError_t launch(const KvArgs &c, const AttendArgs &a, hipStream_t s)
         return enqueue(kernel, dim3(a.tiles, std::max(1, std::min(c.sequences, 65535 / c.kv_heads)) * c.kv_heads), dim3(256 * a.wide), a.wide * LDS, s, c, a);
     }
     constexpr int NW = D > 128 ? 4 : 8;  // (with eight the registers of the wider heads do not fit)
-    if (a.parts == 0) return enqueue(&kv_attend_kernel<QM_ATTEND_TYPE, D, NW, false>, dim3(std::min(c.sequences, 1 << 18) * c.kv_heads, a.tiles), dim3(NW * 64), 0, s, c, a);
+    // (up to 2^22 workgroups along a side, of 512 threads: a grid has less than 2^32)
+    if (a.parts == 0) return enqueue(&kv_attend_kernel<QM_ATTEND_TYPE, D, NW, false>, dim3(std::min(c.sequences, (1 << 22) / c.kv_heads) * c.kv_heads, a.tiles), dim3(NW * 64), 0, s, c, a);
     const hipError_t e = enqueue(&kv_attend_kernel<QM_ATTEND_TYPE, D, 4, true>, dim3(a.parts * c.kv_heads, a.tiles), dim3(256), 0, s, c, a);
     if (e != hipSuccess) return e;
     return enqueue(&kv_join_kernel<QM_ATTEND_TYPE, D, 8>, dim3(a.rows, a.tiles * c.kv_heads, c.sequences), dim3(512), 0, s, c, a);

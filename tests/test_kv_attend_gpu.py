@@ -266,3 +266,16 @@ def test_without_the_extension_the_same(monkeypatch):
     first = attend(q, cache, table, lengths, counts, window=100, max_query=20)
     monkeypatch.setattr(qm, "_ext", types.SimpleNamespace(**dict.fromkeys(qm._EXT_FUNCTIONS, lambda *a: None)))
     assert torch.equal(first, attend(q, cache, table, lengths, counts, window=100, max_query=20))
+
+
+def test_more_workgroups_than_a_grid_has():
+    """2^15 sequences and 256 heads in a workgroup each would be 2^32 threads. Of one token each: its values come back."""
+    sequences, heads = 2 ** 15, 256
+    cache = [t.cuda() for t in make_cache(2, heads, 64, 16, 20)]
+    table = torch.arange(sequences, dtype=torch.int32, device="cuda")[:, None] % 2
+    q = torch.ones(sequences, heads, 64, dtype=torch.float16, device="cuda")
+    out = kv_cache.attend(q, *cache, table, torch.ones(sequences, dtype=torch.int32, device="cuda"))
+    for page in range(2):
+        want = cache[1][page, :, :, 0].double() * cache[2][page, :, 1, None].double()
+        off = (out[page::2].double() - want).abs()
+        assert bool((off <= want.abs() * (2.0 ** -11 + 1.25 * 2.0 ** -11) + 2.0 ** -24).all())
