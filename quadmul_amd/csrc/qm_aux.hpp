@@ -579,7 +579,14 @@ static hipError_t launch_quantize_pack(const void *x, void *dst, float *scales, 
 {
     const uint8_t *xb = static_cast<const uint8_t *>(x);
     uint8_t *db = static_cast<uint8_t *>(dst);
-    if (k < 8) return enqueue(&quantize_pack_scalar_kernel<IN>, dim3(rows), dim3(256), 0, s, xb, db, scales, k);
+    if (k < 8) {
+        constexpr int most = 1 << 23;  // a grid has less than 2^32 threads
+        for (int r0 = 0;; r0 += most) {
+            const hipError_t e = enqueue(&quantize_pack_scalar_kernel<IN>, dim3(std::min(rows - r0, most)), dim3(256), 0, s, xb + (size_t)r0 * k * QuantIn<IN>::BYTES,
+                                         db + (size_t)r0 * (k / 2), scales + r0, k);
+            if (e != hipSuccess || rows - r0 <= most) return e;
+        }
+    }
     if (k > 16384) return launch_quantize_rows<IN, 16, 0>(xb, db, scales, rows, k, s);
     if (k > 12288) return launch_quantize_rows<IN, 16, 2>(xb, db, scales, rows, k, s);
     if (rows > 1024 && k <= 512) return launch_quantize_rows<IN, 1, 1>(xb, db, scales, rows, k, s);

@@ -230,3 +230,12 @@ def test_linear_chain_through_dispatcher_ops_traced(oracle_mod):
     owq, ows = oracle_mod.quantize_pack(w.float().numpy())
     want = oracle_mod.scale_round16(oracle_mod.gemm_i4(oxq, owq), oxs, ows, oracle_mod.OUT_F16)
     assert (y.view(torch.int16).cpu().numpy().view(np.uint16) == want).all()
+
+
+def test_more_short_rows_than_a_grid_has_workgroups():
+    """Rows below eight elements have a workgroup of 256 threads each: 2^24 of them are more than a grid has."""
+    rows = 2 ** 24 + 3
+    x = torch.randn(rows, 2, device=DEV, generator=torch.Generator(DEV).manual_seed(SEED_BASE + 8200)).to(torch.bfloat16)
+    packed, scales = qm.quantize_pack(x)
+    parts = [qm.quantize_pack(p.contiguous()) for p in x.split(2 ** 23 - 1)]
+    assert torch.equal(packed, torch.cat([p for p, _ in parts])) and torch.equal(scales, torch.cat([s for _, s in parts]))
