@@ -301,7 +301,7 @@ typedef struct qm_kv_cache {
  *   scale' = max(scale, amax * (1 / 127)), amax over the new tokens of the page; scale (never below 0) counts as 0 in a page
  *            whose first token is new, which begins anew: all its other codes become 0
  *   code   = clamp(rint(value * (1 / scale')), -127, 127); the codes that the page held become rint(code * (scale / scale')).
- *            0 where scale' is below 2^-100.  Values that are not finite make scale' infinite or NaN, and attention to the page NaN.
+ *            0 where scale' is below 2^-100.  Values that are not finite make scale' NaN, and attention to the page NaN.
  * k and v are [tokens, kv_heads, head_dim] fp16 or bf16, q [tokens, heads, head_dim] or NULL, each with strides of its own (in
  * elements) between tokens and between heads; q_out is [tokens, heads, head_dim] without gaps (rows of padding: 0) and may not overlap q.
  * No two sequences may be given the same page to write to.  max_query: the most new tokens a sequence has, for the choice of the grid only: any

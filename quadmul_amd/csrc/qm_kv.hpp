@@ -68,6 +68,8 @@ __device__ __forceinline__ PageScale page_scale(const float before, const uint32
     const float mine = __builtin_bit_cast(float, amax) * (1.0f / 127.0f);
     float scale = __builtin_bit_cast(float, max(magnitude(before), magnitude(mine)));
     if (scale < 0x1p-100f) scale = 0.0f;
+    // (no code stands for an infinity: times an infinite scale one would be a score of either sign, and the weight of minus infinity is 0)
+    if (magnitude(scale) >= 0x7F800000u) scale = __builtin_nanf("");
     return {scale, scale > 0.0f ? 1.0f / scale : 0.0f, scale > 0.0f ? before / scale : 0.0f};
 }
 __device__ __forceinline__ int code_of(const float scaled) { return (int)fminf(fmaxf(rintf(scaled), -127.0f), 127.0f); }

@@ -259,3 +259,27 @@ def test_without_the_extension_the_same(monkeypatch):
     assert all(torch.equal(a, b) for a, b in zip(first, run(*inputs, lengths, counts, 4, 2, 128)))
     ids = inputs[1][:, 0].contiguous().cuda()
     assert kv_cache.read(*[t.cuda() for t in inputs[0]], ids)[0].shape == (3, 2, 16, 128)
+
+
+@pytest.mark.parametrize("new", [1, 20], ids=["few", "many"])
+@pytest.mark.parametrize("side", ["key", "value"])
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+def test_attention_to_a_page_that_is_not_finite_is_nan(bad, side, new):
+    """Whatever the signs of the queries, and although the other tokens of the page have codes of 0; pages beside it are not touched by it, and a page
+    that begins anew is as if nothing had been."""
+    lengths, counts = [17, 33], [new if new < 17 else 17, new]
+    cache, table, qkv, _, _ = case(lengths, counts, 4, 2, 64, 16, torch.float16, 17, pairs=0)
+    on = [t.cuda() for t in cache]
+    q, k, v = split(qkv.cuda(), 4, 2, 64)
+    table, n, start = table.cuda(), torch.tensor(lengths, dtype=torch.int32, device="cuda"), starts(counts).cuda()
+    (k if side == "key" else v)[counts[0] - 1, 0] = 0
+    (k if side == "key" else v)[counts[0] - 1, 0, 5] = bad     # the only token of its page, head 0
+    kv_cache.append(k, v, *on, table, n, start)
+    ask = torch.zeros(2, 4, 64, dtype=torch.float16, device="cuda")
+    ask[:, 0::2, 5], ask[:, 1::2, 5] = 2.0, -2.0
+    out = kv_cache.attend(ask, *on, table, n)
+    assert out[0, :2].isnan().all() and out[0, 2:].isfinite().all() and out[1].isfinite().all()
+    assert kv_cache.attend(ask, *on, table, n - 1)[0].isfinite().all()
+    k[counts[0] - 1], v[counts[0] - 1] = 1.0, -1.0
+    kv_cache.append(k, v, *on, table, n, start)
+    assert kv_cache.attend(ask, *on, table, n).isfinite().all()
