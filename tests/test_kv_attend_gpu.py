@@ -279,3 +279,15 @@ def test_more_workgroups_than_a_grid_has():
         want = cache[1][page, :, :, 0].double() * cache[2][page, :, 1, None].double()
         off = (out[page::2].double() - want).abs()
         assert bool((off <= want.abs() * (2.0 ** -11 + 1.25 * 2.0 ** -11) + 2.0 ** -24).all())
+
+
+@pytest.mark.parametrize("most", [34, 64, 128, 130, 512, 528])
+def test_prompts_beside_single_tokens(most):
+    """Tiles of 64 rows, from 2 to 33 of them (even and odd, many and few powers of two), in sequences that have all of them, some and one; a hint that is
+    too small."""
+    lengths = [most + 9, most // 2 + 3, 1, 70, 33, 5, most, 2]
+    counts = [most, most // 2, 1, 1, 33, 1, 1, 0]
+    q, cache, table = problem(lengths, counts, 16, 4, 64, 16, torch.bfloat16, 21)
+    want = attend_plain(q, *cache, table, lengths, counts)
+    for hint in (most, 40):
+        check_attention(attend(q, cache, table, lengths, counts, max_query=hint, max_length=max(lengths)), want, torch.bfloat16)
