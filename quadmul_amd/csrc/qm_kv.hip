@@ -113,7 +113,10 @@ static AttendPlan attend_plan(const qm_kv_cache *c, int tokens, int heads, int m
     // The second launch costs 5 us, a step of a wave 2 to 3.5, a sequence in one workgroup has its waves go through an eighth of its
     // steps one by one. 32 sequences and 8 heads (256 workgroups): 2048 tokens each 31 us in one piece, 36 cut; 6000 tokens 78 and
     // 82; lengths from 1 to 8192 62 and 41; one sequence of 2048 tokens 15 and 11, of 1024 11 and 11.
-    if (steps <= 16 || (steps <= 32 && groups * c->sequences >= 128) || c->sequences > 256) return p;
+    // However many sequences there are, for one of them may be long: one of 131072 tokens and 299 of 200 736 us in one piece, 122 cut; of 16384 150 and
+    // 66; 2000 tokens each of 300, 1024 and 2048 sequences 228 and 230, 703 and 706, 1387 and 1387, 5000 of 600 1007 and 1024. (Measured to 4000: one of 16384
+    // 944 and 669.)
+    if (steps <= 16 || (steps <= 32 && groups * c->sequences >= 128) || c->sequences > 4096) return p;
     // two workgroups of four waves to a CU; a step to a wave at least
     p.parts = (int)std::max<long long>(1, std::min<long long>(512 / groups, (long long)steps * c->sequences / 4));
     const auto up = [](size_t v) { return (v + 255) / 256 * 256; };

@@ -291,3 +291,13 @@ def test_prompts_beside_single_tokens(most):
     want = attend_plain(q, *cache, table, lengths, counts)
     for hint in (most, 40):
         check_attention(attend(q, cache, table, lengths, counts, max_query=hint, max_length=max(lengths)), want, torch.bfloat16)
+
+
+@pytest.mark.parametrize("sequences", [257, 700])
+def test_one_long_sequence_among_many(sequences):
+    lengths = [(7 * i) % 40 for i in range(sequences)]
+    lengths[sequences // 2], lengths[-1] = 5000, 1500
+    counts = [i % 3 if i % 50 == 0 else 1 for i in range(sequences)]
+    q, cache, table = problem(lengths, counts, 4, 2, 64, 16, torch.float16, 22)
+    got = both(q, cache, table, lengths, counts, max_query=2, max_length=5000)
+    assert torch.equal(got, attend(q, cache, table, lengths, counts, max_query=2, max_length=5000))

@@ -112,3 +112,10 @@ def test_traceable_forms():
     assert ops.kv_attend(q, *codes, table, lengths, None, None, True, 0, 1, 64).shape == q.shape
     written = [a.name for a in ops.kv_append.default._schema.arguments if a.alias_info is not None and a.alias_info.is_write]
     assert written == ["cache_k", "cache_v", "scales"]
+
+
+def test_sequences_are_cut_however_many_there_are():
+    size = qm.library().qm_kv_attend_workspace_bytes
+    for sequences in (2, 256, 257, 1000, 4096):
+        c = cache(table_width=8192, sequences=sequences)
+        assert size(c, sequences, 4, 0, 0, 131072) > sequences * 8, sequences
