@@ -305,7 +305,7 @@ typedef struct qm_kv_cache {
  * k and v are [tokens, kv_heads, head_dim] fp16 or bf16, q [tokens, heads, head_dim] or NULL, each with strides of its own (in
  * elements) between tokens and between heads; q_out is [tokens, heads, head_dim] without gaps (rows of padding: 0) and may not overlap q.
  * No two sequences may be given the same page to write to.  max_query: the most new tokens a sequence has, for the choice of the grid only: any
- * value gives the same results.
+ * value gives the same results (0 or less: one, if there are no more tokens than sequences, else as many as there can be).
  */
 typedef struct qm_kv_new {
     const void *k, *v, *q;
@@ -323,7 +323,7 @@ int qm_kv_append_i8(const qm_kv_cache *cache, const qm_kv_new *fresh, void *stre
  * Heads of q share those of the cache in equal runs (heads a multiple of kv_heads).  A row that attends to nothing is 0.  Sums and softmax are
  * in single precision.  q [tokens, heads, head_dim] fp16 or bf16 with strides in elements; out [tokens, heads, head_dim] of
  * its type.  max_query and max_length: the most new tokens, and the most tokens, that a sequence has: for the choice of the
- * grid only, any values give a right result.
+ * grid only, any values give a right result (0 or less: as many as there can be, but a max_query of one, if there are no more tokens than sequences).
  *   workspace  16-byte aligned device memory of qm_kv_attend_workspace_bytes(...) bytes, used in stream order by the kernels of this
  *              call only; QM_ERR_SCRATCH with less, and nothing is enqueued
  */

@@ -36,9 +36,13 @@ static KvArgs kv_args(const qm_kv_cache *c, int tokens)
     return {static_cast<int8_t *>(c->k), static_cast<int8_t *>(c->v), c->scales, c->block_table, c->lengths, c->query_start ? c->query_start : c->lengths, c->pages,
             c->kv_heads, c->page_size, c->head_dim, c->sequences, c->table_width, tokens, c->sequences > 0 ? tokens / c->sequences : 0, c->query_start ? 1 : 0};
 }
-// The most new tokens of a sequence: what the caller says, inside what is possible.
+// The most new tokens of a sequence: what the caller says, inside what is possible. Without a word, packed tokens that are no more than the sequences are
+// taken for one each, as a step of a server has them; sequences with more are gone through all the same. 32 sequences of up to 8192 tokens, one new one
+// each: attention 38 us, 151 if all of them might be one sequence's; 64 of up to 1000 21 and 34; storing for 64 6.5 and 22. Where they are one
+// sequence's: 16 of 4000 115 us and 26, storing 14 and 5.5; 64 442 and 75, 46 and 15.
 static int most_new(const qm_kv_cache *c, int tokens, int max_query)
 {
+    if (c->query_start && max_query <= 0 && tokens <= c->sequences) return 1;
     const int most = c->query_start ? tokens : tokens / std::max(c->sequences, 1);
     return std::max(1, c->query_start && max_query > 0 ? std::min(max_query, most) : most);
 }

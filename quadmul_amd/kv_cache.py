@@ -68,7 +68,7 @@ def append(k: torch.Tensor, v: torch.Tensor, cache_k: torch.Tensor, cache_v: tor
     ``cos`` and ``sin`` [positions, pairs] float32, ``2 * pairs <= head_dim``: pairs of elements ``i`` and ``i + pairs``, or with ``interleaved`` ``2i`` and
     ``2i + 1``; without them nothing is rotated. A page that new tokens begin at its start begins anew; in one that held tokens the scale grows
     with the largest value and the codes that are there are rounded again. ``max_query``: the most new tokens of a sequence, if known (only a
-    matter of speed). No two sequences may write to one page in one call."""
+    matter of speed; 0: one, if there are no more tokens than sequences, else what the shapes allow). No two sequences may write to one page in one call."""
     interleaved, max_query = bool(interleaved), int(max_query)
     if _has_extension():
         return _native("kv_append", k, v, cache_k, cache_v, scales, block_table, lengths, query_start, q, cos, sin, interleaved, max_query)
@@ -104,7 +104,7 @@ def attend(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor, scales
     ``heads`` is a multiple of the cache's; each of those serves as many in turn. ``scale``: 1 / sqrt(head_dim) by default. ``causal``: a token sees those up to its own
     position, else all of its sequence; ``window`` > 0: only the last ``window`` of them. A row that sees nothing is 0. Softmax and sums are in float32.
     ``max_query``, ``max_length``: the most new tokens, and the most tokens, of a sequence, if known (only a matter of speed; 0: what the
-    shapes allow)."""
+    shapes allow, and for ``max_query`` one, if there are no more tokens than sequences)."""
     causal, window, max_query, max_length = bool(causal), int(window), int(max_query), int(max_length)
     out = _native("kv_attend", q, cache_k, cache_v, scales, block_table, lengths, query_start, scale, causal, window, max_query, max_length)
     if out is not None:

@@ -283,3 +283,14 @@ def test_attention_to_a_page_that_is_not_finite_is_nan(bad, side, new):
     k[counts[0] - 1], v[counts[0] - 1] = 1.0, -1.0
     kv_cache.append(k, v, *on, table, n, start)
     assert kv_cache.attend(ask, *on, table, n).isfinite().all()
+
+
+@pytest.mark.parametrize("counts", [[40, 0, 0, 0] + [0] * 40, [0, 20, 0, 23] + [0] * 40, [1] * 44])
+def test_no_more_tokens_than_sequences(counts):
+    """Without a hint these are taken for one each, which they need not be."""
+    lengths = [50, 20, 3, 70] + [i + 1 for i in range(40)]
+    cache, table, qkv, cos, sin = case(lengths, counts, 4, 2, 64, 16, torch.float16, 18)
+    got = run(cache, table, qkv, cos, sin, lengths, counts, 4, 2, 64)
+    qs, ks, vs = split(qkv, 4, 2, 64)
+    want = append_plain(ks, vs, *cache, table, lengths, counts, cos, sin, False, qs)
+    assert all(torch.equal(a, b.to(a.dtype)) for a, b in zip(got, want))

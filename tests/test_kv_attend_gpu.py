@@ -301,3 +301,10 @@ def test_one_long_sequence_among_many(sequences):
     q, cache, table = problem(lengths, counts, 4, 2, 64, 16, torch.float16, 22)
     got = both(q, cache, table, lengths, counts, max_query=2, max_length=5000)
     assert torch.equal(got, attend(q, cache, table, lengths, counts, max_query=2, max_length=5000))
+
+
+@pytest.mark.parametrize("lengths,counts", [([40, 900, 3, 2500, 1, 70], [6, 0, 0, 0, 0, 0]), ([40, 900, 3, 2500, 1, 70], [0, 2, 0, 3, 0, 1]), ([5, 1200, 33, 17, 1100, 2], [1, 1, 1, 1, 1, 1])])
+def test_no_more_tokens_than_sequences(lengths, counts):
+    """Without a hint these are taken for one each, which they need not be."""
+    q, cache, table = problem(lengths, counts, 16, 2, 64, 16, torch.float16, 23)
+    both(q, cache, table, lengths, counts)

@@ -119,3 +119,13 @@ def test_sequences_are_cut_however_many_there_are():
     for sequences in (2, 256, 257, 1000, 4096):
         c = cache(table_width=8192, sequences=sequences)
         assert size(c, sequences, 4, 0, 0, 131072) > sequences * 8, sequences
+
+
+def test_a_packed_token_each_needs_no_hint():
+    """As many packed tokens as sequences, or fewer: the plan is that of max_query = 1."""
+    size = qm.library().qm_kv_attend_workspace_bytes
+    for sequences, tokens in ((32, 32), (64, 50), (300, 300), (1, 1)):
+        c = cache(table_width=8192, sequences=sequences, query_start=ONE)
+        assert size(c, tokens, 8, 0, 0, 8192) == size(c, tokens, 8, 0, 1, 8192) > 0
+    c = cache(table_width=8192, sequences=32, query_start=ONE)
+    assert size(c, 33, 8, 0, 0, 8192) == size(c, 33, 8, 0, 33, 8192) != size(c, 33, 8, 0, 1, 8192)
