@@ -29,10 +29,14 @@ static GroupedPlan grouped_plan(int m, int n, int k, int align)  // (align: of B
         p.kernel = GROUPED_TILE;
         const int quads = (k / 32 + 3) / 4;
         const auto tiles_of = [&](const int rows) { return (long long)((m + rows - 1) / rows) * ((n + 127) / 128); };
-        // 256 rows where that leaves a tile to a CU and no more rows without anything to do than an eighth
+        // 256 rows where that leaves a tile to a CU and no more rows without anything to do than an eighth. By 256 and by 128, us: 900 x 8192 x 8192 147 and
+        // 168, 4000 x 28672 x 4096 1034 and 1139, 2048 x 11008 x 4096 222 and 239; with more rows empty, in groups of 32, 300 x 28672 x 4096 223 and 178.
+        // (Least sure where an eleventh is empty: 1300 x 11008 x 4096 202 and 169, 1300 x 65536 x 2048 465 and 487.)
         const bool few_empty = (m + 255) / 256 * 2 == (m + 127) / 128 || m >= 1024;
         p.rows = m <= 32 ? 32 : m <= 64 ? 64 : tiles_of(256) >= 256 && few_empty ? 256 : 128;
-        // a workgroup to a CU at least, of 1024 elements of K or more
+        // A workgroup to a CU at least, of 1024 elements of K or more. Above 64 rows with groups below 128 tiles have 64 columns: counted as 128 all the same,
+        // for two of them to a CU pay for the partial sums: in groups of 32, so and with 64, us, 80 x 11008 x 4096 39 and 50, 256 x 4096 x 11008 53 and 73, 384 x 8192 x
+        // 8192 117 and 119, 200 x 28672 x 4096 122 and 116.
         const long long tiles = tiles_of(p.rows);
         p.runs = (int)std::max<long long>(1, std::min<long long>(256 / tiles, quads / 8));
         p.chunk = (quads + p.runs - 1) / p.runs * 4;
