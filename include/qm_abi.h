@@ -320,9 +320,10 @@ int qm_kv_append_i8(const qm_kv_cache *cache, const qm_kv_new *fresh, void *stre
  * Attention of the new tokens over the cache:
  *   out[t][h] = sum_j softmax_j( scale * q[t][h] . key_j ) value_j
  * over the tokens j of t's sequence with j <= position of t (causal = 1; else all lengths[s]) and, with window > 0, j > position - window.
- * Heads of q share those of the cache in equal runs (heads a multiple of kv_heads).  A row that attends to nothing is 0.  Sums and softmax are
- * in single precision.  q [tokens, heads, head_dim] fp16 or bf16 with strides in elements; out [tokens, heads, head_dim] of
- * its type.  max_query and max_length: the most new tokens, and the most tokens, that a sequence has: for the choice of the
+ * Heads of q share those of the cache in equal runs (heads a multiple of kv_heads).  A row that attends to nothing is 0.  Scores, softmax and
+ * sums are in single precision.  A weight, times the scale of its value's page, enters the product with the values rounded to 11 bits (float16), or, below
+ * 2^-20 of the row's largest such product, with an error of at most 2^-31 of that; the sum that weights are divided by is of unrounded
+ * ones.  q [tokens, heads, head_dim] fp16 or bf16 with strides in elements; out [tokens, heads, head_dim] of its type.  max_query and max_length: the most new tokens, and the most tokens, that a sequence has: for the choice of the
  * grid only, any values give a right result (0 or less: as many as there can be, but a max_query of one, if there are no more tokens than sequences).
  *   workspace  16-byte aligned device memory of qm_kv_attend_workspace_bytes(...) bytes, used in stream order by the kernels of this
  *              call only; QM_ERR_SCRATCH with less, and nothing is enqueued

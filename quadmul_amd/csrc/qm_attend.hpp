@@ -11,8 +11,10 @@
 // through the LDS, and every load is 16 bytes of one page (a page has a multiple of 16 tokens).
 //
 // Both running maxima are kept in units of log2: `top` of the scores, for the sum, and `high` of score + log2(scale of the value's
-// page), for the weights that are rounded to float16: these stay within 2^14 of their largest whatever the scales of other pages
-// are (11 bits down to 2^-28 of it). A maximum moves only when it is passed by 2^8, which leaves the lanes without an exchange in most steps.
+// page), for the weights, each times its value's scale, that are rounded to float16, the type of the second product's operands. A maximum moves only
+// when it is passed by 2^8, which leaves the lanes without an exchange in most steps; the largest weight so far is then 2^6 to 2^14 whatever the scales
+// of other pages are. float16 has 11 bits down to 2^-14: 2^-20 of the largest at least (2^-28 where it is 2^14), and steps of 2^-24 below: an error of
+// at most 2^-31 of the largest, a token. The sum of the weights is of unrounded ones.
 #pragma once
 #include "qm_kv.hpp"
 

@@ -102,7 +102,8 @@ def attend(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor, scales
     """Attention of the last tokens of each sequence over the cache: ``q`` [tokens, heads, head_dim] float16 or bfloat16 -> the same shape and type.
 
     ``heads`` is a multiple of the cache's; each of those serves as many in turn. ``scale``: 1 / sqrt(head_dim) by default. ``causal``: a token sees those up to its own
-    position, else all of its sequence; ``window`` > 0: only the last ``window`` of them. A row that sees nothing is 0. Softmax and sums are in float32.
+    position, else all of its sequence; ``window`` > 0: only the last ``window`` of them. A row that sees nothing is 0. Scores, softmax and sums are in
+    float32; a weight, times its value's scale, enters the product with the values as a float16 of 11 bits, or, below 2^-20 of the row's largest, to 2^-31 of that.
     ``max_query``, ``max_length``: the most new tokens, and the most tokens, of a sequence, if known (only a matter of speed; 0: what the
     shapes allow, and for ``max_query`` one, if there are no more tokens than sequences)."""
     causal, window, max_query, max_length = bool(causal), int(window), int(max_query), int(max_length)

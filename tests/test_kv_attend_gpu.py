@@ -308,3 +308,31 @@ def test_no_more_tokens_than_sequences(lengths, counts):
     """Without a hint these are taken for one each, which they need not be."""
     q, cache, table = problem(lengths, counts, 16, 2, 64, 16, torch.float16, 23)
     both(q, cache, table, lengths, counts)
+
+
+@pytest.mark.parametrize("at", [5, 290])
+@pytest.mark.parametrize("sequences,count", [(1, 1), (3, 4), (16, 40)], ids=["one", "few", "many"])
+def test_weights_far_below_the_largest(sequences, count, at):
+    """Weights 2^-20 to 2^-30 of one token's, in channels where that token's value is 0, so that they are all there is. Beside the bound of the other tests, each
+    of them may be off by 2^-31 of the largest."""
+    length, heads, kv_heads, dim, page = 700, 16, 4, 64, 16
+    lengths, counts = [length] * sequences, [count] * sequences
+    q, (k, v, scales), table = problem(lengths, counts, heads, kv_heads, dim, page, torch.bfloat16, 24)
+    g = torch.Generator().manual_seed(25)
+    q[:], k[:] = 0, 0
+    q[..., 0] = 1.0
+    k[..., 0] = torch.randint(7, 48, k.shape[:3], generator=g).to(torch.int8)
+    for s in range(sequences):
+        p = int(table[s, at // page])
+        k[p, :, at % page, 0] = 127
+        v[p, :, :dim // 2, at % page] = 0
+    scales[..., 0], scales[..., 1] = 1.0, 100.0
+    scale = 0.25 * 0.6931471805599453   # a quarter of a bit for a step of a key
+    got = attend(q, (k, v, scales), table, lengths, counts, scale=scale, max_query=count, max_length=length).double().cpu()
+    out, spread, size = attend_plain(q, k, v, scales, table, lengths, counts, scale)
+    low = 2.0 ** -31 * 100.0 * 127.0 * length
+    bound = 2.0 ** -8 * out.abs() + (1.25 * 2.0 ** -11 + 2.0 * 2.0 ** -20 * size) * spread + low
+    off = (got - out).abs()
+    assert bool((off <= bound).all()), float((off - bound).max())
+    # nothing is lost: those channels are sums of hundreds of such weights, many times what rounding may take from them
+    assert float(spread[..., :dim // 2].min()) > 10 * low and bool((got[..., :dim // 2] != 0).any())
