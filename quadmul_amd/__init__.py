@@ -368,6 +368,8 @@ def gemm_grouped(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tens
     if not (all(t.is_cuda and t.device == x.device for t in tensors) and all(t.dim() == 2 for t in tensors[:3])):
         raise QuadmulError("gemm_grouped: x, weight and weight_scale must be 2-D GPU tensors on one device")
     (m, k), n = x.shape, weight.shape[0]
+    if max(m, n, k) > 2 ** 31 - 1:
+        raise QuadmulError("gemm_grouped: m, n, k must fit in int32")
     if x.dtype not in (torch.float16, torch.bfloat16) or weight_scale.dtype not in (torch.float32, x.dtype):
         raise QuadmulError("gemm_grouped: x must be float16 or bfloat16, the scales float32 or of x's type")
     if k % 2 or not _is_byte(weight) or not weight.is_contiguous() or weight.shape[1] != k // 2:

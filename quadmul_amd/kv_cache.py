@@ -27,12 +27,15 @@ PAGE_SIZES = (16, 32, 64, 128)
 HEAD_DIMS = (64, 96, 128, 192, 256)
 
 _KINDS = {torch.float16: 1, torch.bfloat16: 2}
+_INT_MAX = 2 ** 31 - 1
 
 
 def _cache(what, k, v, scales) -> KvCache:
     if not (k.is_cuda and k.device == v.device == scales.device and k.dim() == 4 and k.dtype == v.dtype == torch.int8 and k.is_contiguous() and v.is_contiguous()):
         raise QuadmulError(f"{what}: the codes must be contiguous 4-D int8 tensors on one GPU")
     pages, heads, page, dim = k.shape
+    if not 1 <= heads <= 4096 or pages > _INT_MAX:
+        raise QuadmulError(f"{what}: 1 to 4096 heads, and less than 2^31 pages")
     if page not in PAGE_SIZES or dim not in HEAD_DIMS or v.shape != (pages, heads, dim, page):
         raise QuadmulError(f"{what}: pages of {PAGE_SIZES} tokens, heads of {HEAD_DIMS}; the values' codes are [pages, kv_heads, head_dim, page_size]")
     if scales.shape != (pages, heads, 2) or scales.dtype != torch.float32 or not scales.is_contiguous():
@@ -47,6 +50,8 @@ def _sequences(what, c, device, block_table, lengths, query_start, tokens):
     count = lengths.shape[0]
     if block_table.shape[0] != count or (query_start is not None and query_start.shape[0] != count + 1):
         raise QuadmulError(f"{what}: block_table [sequences, width], lengths [sequences], query_start [sequences + 1]")
+    if max(tokens, count, block_table.shape[1]) > _INT_MAX:
+        raise QuadmulError(f"{what}: sizes must fit in int32")
     if tokens and (not count or (query_start is None and tokens % count)):
         raise QuadmulError(f"{what}: {tokens} tokens of {count} sequences need a query_start")
     c.block_table, c.lengths = block_table.data_ptr(), lengths.data_ptr()
@@ -79,7 +84,7 @@ def append(k: torch.Tensor, v: torch.Tensor, cache_k: torch.Tensor, cache_v: tor
         _rows("append", t, c, cache_k.device, k.dtype)
     tokens = k.shape[0]
     _sequences("append", c, cache_k.device, block_table, lengths, query_start, tokens)
-    if q is not None and (q.shape[0] != tokens or q.shape[1] < 1):
+    if q is not None and (q.shape[0] != tokens or not 1 <= q.shape[1] <= _INT_MAX):
         raise QuadmulError("append: as many queries as keys")
     if (cos is None) != (sin is None):
         raise QuadmulError("append: cos and sin go together")
@@ -90,7 +95,7 @@ def append(k: torch.Tensor, v: torch.Tensor, cache_k: torch.Tensor, cache_v: tor
     n = KvNew(k.data_ptr(), v.data_ptr(), None if q is None else q.data_ptr(), None if q is None else out.data_ptr(), k.stride(0), k.stride(1), v.stride(0),
               v.stride(1), 0 if q is None else q.stride(0), 0 if q is None else q.stride(1), None if cos is None else cos.data_ptr(),
               None if sin is None else sin.data_ptr(), tokens, 0 if q is None else q.shape[1], _KINDS[k.dtype], 0 if cos is None else cos.shape[1],
-              0 if cos is None else cos.shape[0], int(interleaved), min(max(max_query, 0), 2 ** 31 - 1))
+              0 if cos is None else cos.shape[0], int(interleaved), min(max(max_query, 0), _INT_MAX))
     with torch.cuda.device(cache_k.device):
         _check(library().qm_kv_append_i8(ctypes.byref(c), ctypes.byref(n), _stream_ptr(cache_k)), "qm_kv_append_i8")
     return out
@@ -118,7 +123,7 @@ def attend(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor, scales
     _sequences("attend", c, cache_k.device, block_table, lengths, query_start, tokens)
     if heads < 1 or heads > 65535 or heads % c.kv_heads or window < 0:
         raise QuadmulError(f"attend: the heads of the queries must be a multiple of the cache's {c.kv_heads}, the window 0 or more tokens")
-    max_query, max_length, window = (min(max(i, 0), 2 ** 31 - 1) for i in (max_query, max_length, window))
+    max_query, max_length, window = (min(max(i, 0), _INT_MAX) for i in (max_query, max_length, window))
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     need = library().qm_kv_attend_workspace_bytes(ctypes.byref(c), tokens, heads, window, max_query, max_length)
     scratch = torch.empty((need,), dtype=torch.uint8, device=q.device) if need else None

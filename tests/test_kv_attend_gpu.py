@@ -336,3 +336,22 @@ def test_weights_far_below_the_largest(sequences, count, at):
     assert bool((off <= bound).all()), float((off - bound).max())
     # nothing is lost: those channels are sums of hundreds of such weights, many times what rounding may take from them
     assert float(spread[..., :dim // 2].min()) > 10 * low and bool((got[..., :dim // 2] != 0).any())
+
+
+@pytest.mark.parametrize("extension", [True, False], ids=["extension", "without"])
+def test_sizes_that_are_refused(extension, monkeypatch):
+    """The same refusals with the extension module and without: no heads, tokens past 32 bits."""
+    import types
+
+    if not extension:
+        monkeypatch.setattr(qm, "_ext", types.SimpleNamespace(**dict.fromkeys(qm._EXT_FUNCTIONS, lambda *a: None)))
+    cache = [t.cuda() for t in make_cache(4, 2, 64, 16, 15)]
+    table, n = torch.zeros(1, 3, dtype=torch.int32, device="cuda"), torch.tensor([5], dtype=torch.int32, device="cuda")
+    one = torch.zeros(1, 2, 64, dtype=torch.float16, device="cuda")
+    none, many = [t[:, :0].contiguous() for t in cache], one.expand(2 ** 31 + 1, 2, 64)
+    for call in (lambda: kv_cache.attend(one, *none, table, n), lambda: kv_cache.append(one[:, :0], one[:, :0], *none, table, n), lambda: kv_cache.read(*none, n),
+                 lambda: kv_cache.attend(many, *cache, table, n), lambda: kv_cache.append(many, many, *cache, table, n),
+                 lambda: qm.gemm_grouped(one[0, :, :64].expand(2, 64)[:1].expand(2 ** 31 + 1, 64), torch.zeros(4, 32, dtype=torch.int8, device="cuda"),
+                                         torch.ones(4, 2, dtype=torch.float16, device="cuda"), 32)):
+        with pytest.raises(qm.QuadmulError):
+            call()
