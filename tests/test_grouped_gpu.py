@@ -193,3 +193,36 @@ def test_more_columns_than_a_grid_has_threads(m):
     low, high = ((w[:, 0] << 4) >> 4).half(), (w[:, 0] >> 4).half()
     for i in range(m):
         assert torch.equal(y[i], low * (i + 1.0) - high * 3.0)
+
+
+@pytest.mark.parametrize("m", [1, 3, 16, 20, 60, 64, 65, 300])
+def test_bf16_activations_near_the_end_of_their_range(m):
+    """Up to 64 rows the weights take part as 136 more than they are and 136 times the sum of x is taken off: 2^118 is held, above 2^119 or with an infinity the
+    row is lost and no other. Above 64 rows they are integers, and a row is lost where its exact result is. The error of a term is half a unit of it in float32, with the 136
+    and what is taken off counted to its size up to 64 rows."""
+    x, q, s, _ = problem(m, 80, 512, 64, torch.bfloat16, torch.bfloat16, False, 14)
+    w = q.double() * s.double().repeat_interleave(64, dim=1)
+    extra = 272.0 * s.double().repeat_interleave(64, dim=1) if m <= 64 else torch.zeros_like(w)
+    row, keep = m // 2, torch.arange(m) != m // 2
+    for big in (2.0 ** 118, -2.0 ** 118, 2.0 ** 121, float("inf"), float("-inf"), float("nan")):
+        x[row, 100] = big
+        y = qm.gemm_grouped(x.cuda(), pack_cpu(q).cuda(), s.cuda(), 64).cpu()
+        held = abs(big) <= (2.0 ** 118 if m <= 64 else 2.0 ** 121)
+        if held:
+            want, size = x.double() @ w.T, x.double().abs() @ (w.abs() + extra).T
+            bound = UNIT[torch.bfloat16] * want.abs() + 6.0 * math.sqrt(512) * 2.0 ** -24 * size
+            assert bool(((y.double() - want).abs() <= bound)[row].all())
+        else:
+            assert not y[row].isfinite().any()
+        if keep.any():
+            check(x[keep], q, s, 64, None, y[keep])
+
+
+@pytest.mark.parametrize("m", [1, 7, 16, 33, 64, 100, 300])
+@pytest.mark.parametrize("group", [32, 64, 96, 128, 256])
+def test_scales_and_bias_at_any_address(m, group):
+    x, q, s, b = problem(m, 70, 672, group, torch.bfloat16, torch.bfloat16, True, 15)
+    at = torch.zeros(s.numel() + 1, dtype=torch.bfloat16, device="cuda")[1:].view(s.shape)
+    bias = torch.zeros(71, dtype=torch.bfloat16, device="cuda")[1:]
+    at.copy_(s), bias.copy_(b)
+    check(x, q, s, group, b, qm.gemm_grouped(x.cuda(), pack_cpu(q).cuda(), at, group, bias))
