@@ -471,8 +471,8 @@ def unpack_int4(packed: torch.Tensor) -> torch.Tensor:
 
 
 def init(device=None) -> None:
-    """Every kernel's one-off set-up on ``device`` (default: the current one) without launching
-    anything; optional -- first launches do it by themselves."""
+    """The one-off set-up of the int4 products' kernels on ``device`` (default: the current one) without launching
+    anything; optional -- first launches do it by themselves, as those of :func:`gemm_grouped` and attention always do."""
     with torch.cuda.device(device if device is not None else torch.cuda.current_device()):
         _check(library().qm_init(), "qm_init")
 

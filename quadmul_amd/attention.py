@@ -5,8 +5,8 @@ cache with the position rotation, attention over the cache, output projection (n
     cache = PagedKVCache(pages, kv_heads, head_dim)
     y = block(x, cache, block_table, lengths)      # x: the new tokens' hidden states, one row each
 
-Five launches for a decode step (six where sequences are cut into parts), all on the current stream, none that looks at a length on the
-host: a step may be captured into a HIP graph and replayed with other contents of ``x``, ``block_table`` and ``lengths``.
+Four launches for a decode step (one more where sequences are cut into parts, and for each projection whose K is summed in runs), all on the current
+stream, none that looks at a length on the host: a step may be captured into a HIP graph and replayed with other contents of ``x``, ``block_table`` and ``lengths``.
 """
 from __future__ import annotations
 

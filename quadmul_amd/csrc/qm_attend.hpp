@@ -411,12 +411,13 @@ __global__ __launch_bounds__(NW * 64, D > 128 ? 1 : 2) void kv_attend_kernel(con
 // round each of 8 heads has an XCD, whose CUs read the same lines at the same time: twice as long.) Workgroups are dealt to the 8 XCDs in turn and there
 // to 4 parts of an XCD: where the number of tiles is even, the few tiles of sequences with few rows would all be dealt to one or some of the 32. So the first
 // tiles are turned by one place from one blockIdx.y to the next, as many of them as the number has powers of two (up to 32). A prompt of 512 tokens
-// beside 63 single tokens (32 tiles) 1354 us without, 240 turned among 8, 135 among 32; 16 prompts of 128 on 2000 tokens 120 and 119. Bound by the vector
-// pipeline (what a score costs until it is a weight: nine instructions and an exponential) before the matrix cores. (With 32 rows to a wave and four waves
+// beside 63 single tokens (32 tiles) 1354 us without, 240 turned among 8, 135 among 32; 16 prompts of 128 on 2000 tokens 120 and 119. Bound by
+// what does not run at the same time: of 180 thousand cycles (4 prompts of up to 512 tokens) the vector pipeline is busy 47 %, the LDS 35, the matrix cores 22, and between two
+// barriers all waves of a lot multiply, then all make floats. (With 32 rows to a wave and four waves
 // 4 prompts of up to 512 tokens took 162 us: the longest sequence had a workgroup to every other CU.)
 // LOTS of 64 tokens at a time share the rows: with two the longest sequence's last tiles are done sooner, with one (four workgroups to a CU) fewer waves
 // wait for each other. 4 prompts of up to 512 tokens (1024 tiles and heads) 95 us with two, 119 with one; 1 of 4096 (2048) 260 and 265; 8 of 2048
-// (8192) 561 and 490. (With four the registers of 128 channels do not fit: 138 us for the first.)
+// (8192) 561 and 490 (with the tiles turned, as above, 88, 256 and 459). (With four the registers of 128 channels do not fit: 138 us for the first.)
 template <int T, int D, int LOTS>
 __global__ __launch_bounds__(256 * LOTS, D > 128 ? 2 : 4) void kv_attend_rows_kernel(const KvArgs c, const AttendArgs a)
 {

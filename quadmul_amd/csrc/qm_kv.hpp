@@ -82,7 +82,8 @@ __device__ __forceinline__ int code_of(const float value, const float factor)
 // Sixteen values of a head: eight pairs that turn together (VECTOR: `pairs` is a multiple of eight), or one pair.
 template <int T, bool VECTOR>
 struct Pairs {
-    // HEADS: of the queries, that a thread has at a time, with the same cosines and sines: one 42 us for 4 prompts of up to 2048 tokens, two 35; four spill
+    // HEADS: of the queries, that a thread has at a time, with the same cosines and sines: one 42 us for 4 prompts of up to 2048 tokens in float16 (with
+    // reading them back), two 35; four spill. In bf16 the pairs lie in scratch memory with one as with two, 72 bytes a lane: see the kernel
     static constexpr int COUNT = VECTOR ? 8 : 1, HEADS = VECTOR ? 2 : 1;
     Pair v[COUNT];
     int2 at;  // elements of the first pair; with VECTOR the eight a side by side from at.x and the eight b from at.y, or a, b, a, b, .. from at.x
@@ -252,8 +253,8 @@ __device__ __forceinline__ uint32_t recoded(const uint32_t w, const float ratio)
 // blockIdx.z: a sequence; blockIdx.y: a head and a side (keys, values) of it; blockIdx.x: below `slots` the pages that the
 // sequence's new tokens fall into, past it the rotation of its queries. A thread has sixteen or 32 values at a time (its first ones stay in its
 // registers between the largest value and the codes; further ones are read again, from the L2). Where a page's codes all change they are put
-// together in the LDS and go out in whole lines. 4 prompts of up to 2048 tokens, 32 heads of queries and 8 of the cache, 84 MB: 35 us, 2.4 TB/s: bound
-// by what 128 registers leave in flight.
+// together in the LDS and go out in whole lines. 4 prompts of up to 2048 tokens, 2847 in all, 32 heads of queries and 8 of the cache, 66 MB: float16 28 us, 2.3
+// TB/s, bound by what 128 registers leave in flight; bf16 41, bound by the scratch memory that the rotation of the queries goes through (without queries both take 21).
 template <int T, bool VECTOR>
 __global__ __launch_bounds__(256, 4) void kv_append_kernel(const KvArgs c, const KvNewArgs f, const int slots)
 {
@@ -381,7 +382,9 @@ __global__ __launch_bounds__(256, 4) void kv_append_kernel(const KvArgs c, const
 
 // The same for few new tokens to a sequence: a wave to a page, a head and a side of it, or to a token's head of the queries, a lane to a pair or a
 // channel. No barrier and no LDS: a word that has new codes is put together by the lane that stores them, every other one of a page that
-// begins anew or is rounded again by another. Values are read twice, the second time from the cache. Bound by latency: lengths, table, values.
+// begins anew or is rounded again by another. Values are read twice, the second time from the cache. Bound by latency: lengths, table, values, and
+// the rounding of a page whose scale grows, dword after dword by one wave. 64 sequences, 8 heads of 128, a token each in a graph: 4.9 us where no scale
+// grows; a token after the other from the first to the last of a page, mean 7.7 in pages of 16 tokens, 30 in pages of 128 (one head of 256: 37).
 template <int T>
 __global__ __launch_bounds__(256) void kv_append_few_kernel(const KvArgs c, const KvNewArgs f, const int slots, const int tasks)
 {
