@@ -18,3 +18,12 @@ def oracle_mod():
 
     oracle.build()
     return oracle
+
+
+@pytest.fixture
+def gives_memory_back():
+    """For tests of large tensors: what torch's allocator would keep of them is given back afterwards."""
+    yield
+    import torch
+
+    torch.cuda.empty_cache()

@@ -182,6 +182,7 @@ def test_tiles_of_256_rows(m, n, k, group, wide, dtype):
     check(x, q, s, group, b, y)
 
 
+@pytest.mark.usefixtures("gives_memory_back")
 @pytest.mark.parametrize("m", [1, 6])
 def test_more_columns_than_a_grid_has_threads(m):
     """2^26 columns and a few: a wave to each would be 2^32 threads and more. Every result is an integer of few bits."""

@@ -268,6 +268,7 @@ def test_without_the_extension_the_same(monkeypatch):
     assert torch.equal(first, attend(q, cache, table, lengths, counts, window=100, max_query=20))
 
 
+@pytest.mark.usefixtures("gives_memory_back")
 def test_more_workgroups_than_a_grid_has():
     """2^15 sequences and 256 heads in a workgroup each would be 2^32 threads. Of one token each: its values come back."""
     sequences, heads = 2 ** 15, 256

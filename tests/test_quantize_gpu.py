@@ -232,6 +232,7 @@ def test_linear_chain_through_dispatcher_ops_traced(oracle_mod):
     assert (y.view(torch.int16).cpu().numpy().view(np.uint16) == want).all()
 
 
+@pytest.mark.usefixtures("gives_memory_back")
 def test_more_short_rows_than_a_grid_has_workgroups():
     """Rows below eight elements have a workgroup of 256 threads each: 2^24 of them are more than a grid has."""
     rows = 2 ** 24 + 3
