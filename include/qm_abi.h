@@ -338,6 +338,61 @@ int qm_kv_attend_i8(const qm_kv_cache *cache, const void *q, int dtype, long lon
 int qm_kv_read_i8(const qm_kv_cache *cache, const int *page_ids, int count, int dtype, void *k, void *v, void *stream);
 
 /*
+ * A mixture of experts on packed int4 weights (no counterpart in the reference).
+ *
+ * A router's choice: for each of `tokens` rows of logits z ([tokens, experts], fp16, bf16 or fp32, rows `row_stride` elements apart) the top_k experts and
+ * their weights, chosen [tokens, top_k] int32 and weights [tokens, top_k] float32, best first. In double precision:
+ *   s = softmax(z) (QM_SCORES_SOFTMAX; a row of minus infinities: zeros) or 1 / (1 + exp(-z)) (QM_SCORES_SIGMOID);  c = s + bias ([experts] or NULL)
+ *   groups       the experts in as many equal runs; with top_groups < groups only the top_groups groups of the largest worth are chosen from: the sum of their
+ *                group_best (1 or 2) largest c
+ *   chosen       the top_k largest c; of equal ones, and of equal groups, the one of the lower number. NaN counts as minus infinity, softmax scores
+ *                without a bias go by the logits, which are in the same order
+ *   weights      s of the chosen (without the bias), divided by their sum with renormalise = 1 (a sum of 0: by 1), times scale, rounded once
+ * 1 to QM_ROUTE_EXPERTS experts, up to 64 groups, top_k up to 64 and to the experts of top_groups groups. A NaN logit, or one of plus infinity, makes the weights
+ * of a softmax NaN; the chosen are always top_k different experts.
+ */
+#define QM_ROUTE_EXPERTS 1024
+#define QM_SCORES_SOFTMAX 0
+#define QM_SCORES_SIGMOID 1
+int qm_moe_route(const void *logits, int dtype, long long row_stride, int tokens, int experts, int top_k, const float *bias, int scores, int groups, int top_groups,
+                 int group_best, int renormalise, double scale, int *chosen, float *weights, void *stream);
+
+/*
+ * One matrix of every expert: weight [experts, n, k / 2] bytes packed as everywhere in this interface, scale [experts, n, ceil(k / group)] row-major, float32
+ * (scale_dtype = QM_IN_F32) or of the activations' type, bias [experts, n] of their type or NULL; groups as for qm_gemm_grouped_i4.
+ */
+typedef struct qm_expert_weights {
+    const void *weight, *scale, *bias;
+    int scale_dtype, experts, n, k, group;
+} qm_expert_weights;
+
+/*
+ * Each token's row times the matrix of each of its experts:
+ *   y[t][j][n] = round16( sum_g scale[e][n][g] * sum_{k in g} x[t][j][k] * weight[e][n][k] + bias[e][n] ),  e = chosen[t][j]
+ * and 0 where e is none of 0 .. experts - 1 (an expert on another GPU, a token of padding). x is fp16 or bf16, token_stride elements from token to
+ * token and choice_stride from choice to choice (0: the same row for all of a token's choices); y [tokens, top_k, n] of its type, not overlapping x.
+ * Sums are IEEE single precision, the weights take part as the integers they are; one rounding, at the end. The same expert may be
+ * chosen twice by a token. tokens * top_k below 2^31.
+ *   workspace    16-byte aligned device memory of qm_gemm_experts_workspace_bytes(...) bytes, used in stream order by the kernels of this call only;
+ *                QM_ERR_SCRATCH with less, and nothing is enqueued
+ */
+size_t qm_gemm_experts_workspace_bytes(const qm_expert_weights *weights, int tokens, int top_k);
+int qm_gemm_experts_i4(const void *x, int dtype, long long token_stride, long long choice_stride, const int *chosen, const qm_expert_weights *weights, void *y,
+                       int tokens, int top_k, void *stream, void *workspace, size_t workspace_bytes);
+
+/*
+ * The gated MLP of each token's experts, their outputs added up by weight:
+ *   h[t][j][i] = round16( silu(a[i]) * a[inner + i] ),  a = x[t] * up[e]^T,  e = chosen[t][j];   y[t] = round16( sum_j weights[t][j] * h[t][j] * down[e]^T )
+ * silu(a) = a / (1 + exp(-a)); up has n = 2 inner rows of k = hidden, down n = hidden rows of k = inner, neither a bias. Choices whose expert is none of
+ * 0 .. experts - 1 add nothing, whatever their weight is. Sums, the gates and the outputs of the experts are in single precision; h is rounded to x's type, of which the second
+ * product's operands are, and y once, at the end. x [tokens, hidden] fp16 or bf16, y [tokens, hidden] of its type, not overlapping x; weights [tokens, top_k]
+ * float32. Workspace as for qm_gemm_experts_i4, of qm_moe_mlp_workspace_bytes(...) bytes.
+ */
+size_t qm_moe_mlp_workspace_bytes(const qm_expert_weights *up, const qm_expert_weights *down, int tokens, int top_k);
+int qm_moe_mlp_i4(const void *x, int dtype, long long token_stride, const int *chosen, const float *weights, const qm_expert_weights *up, const qm_expert_weights *down,
+                  void *y, int tokens, int top_k, void *stream, void *workspace, size_t workspace_bytes);
+
+/*
  * Optional: everything a first launch on the current device would otherwise do once -- the
  * LDS size attribute and the residency query of every kernel of the int4 products, the address of the library's
  * scratch array -- without launching anything (qm_gemm_grouped_i4 and qm_kv_attend_i8 set their kernels' LDS size themselves, at the first

@@ -42,6 +42,7 @@ ABI_SYMBOLS = (
     "qm_config_supports", "qm_pack_i4", "qm_unpack_i4", "qm_status_string", "qm_last_hip_error", "qm_version", "qm_init",
     "qm_debug_set_operand_limit", "qm_linear_workspace_bytes", "qm_linear_i4",
     "qm_gemm_grouped_workspace_bytes", "qm_gemm_grouped_i4", "qm_kv_append_i8", "qm_kv_attend_workspace_bytes", "qm_kv_attend_i8", "qm_kv_read_i8",
+    "qm_moe_route", "qm_gemm_experts_workspace_bytes", "qm_gemm_experts_i4", "qm_moe_mlp_workspace_bytes", "qm_moe_mlp_i4",
 )
 
 
@@ -57,6 +58,11 @@ class KvNew(ctypes.Structure):
                 + [(f, ctypes.c_longlong) for f in ("k_token_stride", "k_head_stride", "v_token_stride", "v_head_stride", "q_token_stride", "q_head_stride")]
                 + [(f, ctypes.c_void_p) for f in ("cos", "sin")]
                 + [(f, ctypes.c_int) for f in ("tokens", "heads", "dtype", "rotary_pairs", "positions", "interleaved", "max_query")])
+
+
+class ExpertWeights(ctypes.Structure):
+    """``qm_expert_weights`` of include/qm_abi.h."""
+    _fields_ = [(f, ctypes.c_void_p) for f in ("weight", "scale", "bias")] + [(f, ctypes.c_int) for f in ("scale_dtype", "experts", "n", "k", "group")]
 
 
 class QuadmulError(RuntimeError):
@@ -145,11 +151,22 @@ def library() -> ctypes.CDLL:
     lib.qm_kv_attend_i8.restype = ci
     lib.qm_kv_read_i8.argtypes = [cache, vp, ci, ci, vp, vp, vp]
     lib.qm_kv_read_i8.restype = ci
+    matrices = ctypes.POINTER(ExpertWeights)
+    lib.qm_moe_route.argtypes = [vp, ci, ll, ci, ci, ci, vp, ci, ci, ci, ci, ci, ctypes.c_double, vp, vp, vp]
+    lib.qm_moe_route.restype = ci
+    lib.qm_gemm_experts_workspace_bytes.argtypes = [matrices, ci, ci]
+    lib.qm_gemm_experts_workspace_bytes.restype = size
+    lib.qm_gemm_experts_i4.argtypes = [vp, ci, ll, ll, vp, matrices, vp, ci, ci, vp, vp, size]
+    lib.qm_gemm_experts_i4.restype = ci
+    lib.qm_moe_mlp_workspace_bytes.argtypes = [matrices, matrices, ci, ci]
+    lib.qm_moe_mlp_workspace_bytes.restype = size
+    lib.qm_moe_mlp_i4.argtypes = [vp, ci, ll, vp, vp, matrices, matrices, vp, ci, ci, vp, vp, size]
+    lib.qm_moe_mlp_i4.restype = ci
     _lib = lib
     return lib
 
 
-_EXT_FUNCTIONS = ("gemm_grouped", "kv_append", "kv_attend", "kv_read", "linear", "pack", "quantize_pack", "unpack")
+_EXT_FUNCTIONS = ("gemm_experts", "gemm_grouped", "kv_append", "kv_attend", "kv_read", "linear", "moe_mlp", "moe_route", "pack", "quantize_pack", "unpack")
 _ext = None  # the extension module, once looked for
 
 

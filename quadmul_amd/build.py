@@ -121,6 +121,7 @@ def build_lib(jobs: int = 8, verbose: bool = False) -> str:
     units = [("qm_dispatch.o", [f'-DQM_COMPILER_VERSION="{ver}"', "-mllvm", "-amdgpu-kernarg-preload-count=16", "-c", os.path.join(CSRC, "qm_dispatch.hip")]),
              ("qm_scratch.o", ["-c", os.path.join(CSRC, "qm_scratch.hip")]),
              ("qm_grouped.o", ["-c", os.path.join(CSRC, "qm_grouped.hip")]),
+             ("qm_experts.o", ["-c", os.path.join(CSRC, "qm_experts.hip")]),
              ("qm_kv.o", ["-c", os.path.join(CSRC, "qm_kv.hip")])]
     # (the units with the scaled-output kernels, 6 and up, take longest: they go first)
     units = [(f"qm_attend_inst_{t}.o", [f"-DQM_ATTEND_TYPE={t}", "-c", os.path.join(CSRC, "qm_attend_inst.hip")]) for t in (1, 2)] + units

@@ -392,6 +392,114 @@ void gemm_scaled_op(const torch::Tensor &a, const torch::Tensor &b, torch::Tenso
 }
 
 // quantize_pack returns new tensors: the Meta form only has to give their shapes and types
+// The mixture of experts (include/qm_abi.h: qm_moe_route, qm_gemm_experts_i4, qm_moe_mlp_i4).
+int check_route(const torch::Tensor &logits, int64_t top_k, const c10::optional<torch::Tensor> &bias, int64_t groups, int64_t top_groups, int64_t group_best)
+{
+    TORCH_CHECK(logits.dim() == 2, "quadmul.moe_route: the logits must be [tokens, experts]");
+    const auto type = logits.scalar_type();
+    TORCH_CHECK(type == torch::kFloat32 || type == torch::kFloat16 || type == torch::kBFloat16, "quadmul.moe_route: the logits must be float32, float16 or bfloat16");
+    const int64_t experts = logits.size(1);
+    TORCH_CHECK(logits.size(0) <= INT32_MAX && experts >= 1 && experts <= QM_ROUTE_EXPERTS, "quadmul.moe_route: 1 to ", QM_ROUTE_EXPERTS, " experts, got ", experts);
+    TORCH_CHECK(groups >= 1 && groups <= 64 && experts % groups == 0 && top_groups >= 1 && top_groups <= groups && (group_best == 1 || group_best == 2),
+                "quadmul.moe_route: groups must divide the experts and be at most 64, top_groups at most as many, group_best 1 or 2");
+    TORCH_CHECK(top_k >= 1 && top_k <= 64 && top_k <= experts / groups * top_groups, "quadmul.moe_route: top_k must be 1 to 64, and no more than the experts to choose from, got ", top_k);
+    TORCH_CHECK(!bias.has_value() || (bias->device() == logits.device() && bias->scalar_type() == torch::kFloat32 && bias->is_contiguous() && bias->dim() == 1 && bias->numel() == experts),
+                "quadmul.moe_route: the bias must be a contiguous float32 vector of ", experts, " elements on the logits' device");
+    return type == torch::kFloat32 ? QM_IN_F32 : type == torch::kFloat16 ? QM_IN_F16 : QM_IN_BF16;
+}
+std::tuple<torch::Tensor, torch::Tensor> moe_route(torch::Tensor logits, int64_t top_k, c10::optional<torch::Tensor> bias, bool sigmoid, int64_t groups, int64_t top_groups,
+                                                   int64_t group_best, bool renormalise, double scale)
+{
+    TORCH_CHECK(logits.is_cuda(), "quadmul.moe_route: expects GPU tensors");
+    const int type = check_route(logits, top_k, bias, groups, top_groups, group_best);
+    c10::OptionalDeviceGuard guard(logits.device());
+    const int64_t tokens = logits.size(0), experts = logits.size(1);
+    if ((experts > 1 && logits.stride(1) != 1) || (tokens > 1 && logits.stride(0) < experts)) logits = logits.contiguous();
+    auto chosen = torch::empty({tokens, top_k}, logits.options().dtype(torch::kInt32)), weights = torch::empty({tokens, top_k}, logits.options().dtype(torch::kFloat32));
+    check_status(qm_moe_route(logits.data_ptr(), type, tokens > 1 ? logits.stride(0) : experts, (int)tokens, (int)experts, (int)top_k, bias.has_value() ? bias->data_ptr<float>() : nullptr,
+                              sigmoid ? QM_SCORES_SIGMOID : QM_SCORES_SOFTMAX, (int)groups, (int)top_groups, (int)group_best, renormalise, scale, chosen.data_ptr<int>(),
+                              weights.data_ptr<float>(), stream_of(logits)),
+                 "quadmul.moe_route");
+    return {chosen, weights};
+}
+
+// One matrix of every expert, checked against the activations and put together for the C interface.
+qm_expert_weights expert_weights(const char *what, const torch::Tensor &x, const torch::Tensor &weight, const torch::Tensor &scale, int64_t group, const c10::optional<torch::Tensor> &bias)
+{
+    TORCH_CHECK(weight.dim() == 3 && is_byte(weight) && weight.is_contiguous(), what, ": the weights must be contiguous [experts, n, k / 2] int8 or uint8 tensors (packed int4)");
+    TORCH_CHECK(group >= 32 && group <= INT32_MAX && group % 32 == 0, what, ": the group size must be a multiple of 32, got ", group);
+    const int64_t experts = weight.size(0), n = weight.size(1), k = weight.size(2) * 2;
+    TORCH_CHECK(experts <= INT32_MAX && n <= INT32_MAX && k <= INT32_MAX, what, ": sizes must fit in int32");
+    TORCH_CHECK(scale.dim() == 3 && scale.is_contiguous() && scale.size(0) == experts && scale.size(1) == n && scale.size(2) == (k + group - 1) / group &&
+                    (scale.scalar_type() == torch::kFloat32 || scale.scalar_type() == x.scalar_type()),
+                what, ": the scales must be contiguous [experts, n, ceil(k / group)] tensors of float32 or of x's type");
+    TORCH_CHECK(weight.device() == x.device() && scale.device() == x.device(), what, ": all tensors must be on the same device");
+    TORCH_CHECK(!bias.has_value() || (bias->device() == x.device() && bias->scalar_type() == x.scalar_type() && bias->is_contiguous() && bias->dim() == 2 && bias->size(0) == experts && bias->size(1) == n),
+                what, ": the bias must be a contiguous [experts, n] tensor of x's type on x's device");
+    return {weight.data_ptr(), scale.data_ptr(), bias.has_value() ? bias->data_ptr() : nullptr, scale.scalar_type() == torch::kFloat32 ? QM_IN_F32 : scale.scalar_type() == torch::kFloat16 ? QM_IN_F16 : QM_IN_BF16,
+            (int)experts, (int)n, (int)k, (int)group};
+}
+void check_chosen(const char *what, const torch::Tensor &x, const torch::Tensor &chosen)
+{
+    TORCH_CHECK(chosen.device() == x.device() && chosen.scalar_type() == torch::kInt32 && chosen.dim() == 2 && chosen.is_contiguous() && chosen.size(0) == x.size(0), what,
+                ": the chosen experts must be a contiguous int32 tensor [tokens, top_k] on x's device");
+    TORCH_CHECK(chosen.size(0) <= INT32_MAX && chosen.size(1) <= INT32_MAX && chosen.numel() <= INT32_MAX, what, ": tokens times top_k must fit in int32");
+}
+void check_experts(const torch::Tensor &x, const torch::Tensor &chosen, const torch::Tensor &weight)
+{
+    TORCH_CHECK(x.dim() == 2 || x.dim() == 3, "quadmul.gemm_experts: x must be [tokens, k] or [tokens, top_k, k]");
+    check_chosen("quadmul.gemm_experts", x, chosen);
+    TORCH_CHECK(x.dim() == 2 || x.size(1) == chosen.size(1), "quadmul.gemm_experts: x must have a row for each choice, or one for each token");
+    TORCH_CHECK(x.size(-1) % 2 == 0 && weight.dim() == 3 && weight.size(2) * 2 == x.size(-1), "quadmul.gemm_experts: the weights must be [experts, n, k / 2], k even and x's last dimension");
+}
+
+torch::Tensor gemm_experts(torch::Tensor x, torch::Tensor chosen, torch::Tensor weight, torch::Tensor weight_scale, int64_t group, c10::optional<torch::Tensor> bias)
+{
+    TORCH_CHECK(x.is_cuda(), "quadmul.gemm_experts: expects GPU tensors");
+    const int type = float16_type(x, "quadmul.gemm_experts: x");
+    check_experts(x, chosen, weight);
+    const qm_expert_weights w = expert_weights("quadmul.gemm_experts", x, weight, weight_scale, group, bias);
+    c10::OptionalDeviceGuard guard(x.device());
+    if (w.k > 1 && x.stride(-1) != 1) x = x.contiguous();
+    const int tokens = (int)chosen.size(0), top_k = (int)chosen.size(1);
+    auto y = torch::empty({tokens, top_k, w.n}, x.options());
+    const size_t need = qm_gemm_experts_workspace_bytes(&w, tokens, top_k);
+    torch::Tensor scratch;
+    if (need > 0) scratch = torch::empty({(int64_t)need}, x.options().dtype(torch::kUInt8));
+    check_status(qm_gemm_experts_i4(x.data_ptr(), type, x.stride(0), x.dim() == 3 ? x.stride(1) : 0, chosen.data_ptr<int>(), &w, y.data_ptr(), tokens, top_k, stream_of(x),
+                                    need > 0 ? scratch.data_ptr() : nullptr, need),
+                 "quadmul.gemm_experts");
+    return y;
+}
+
+void check_mlp(const torch::Tensor &x, const torch::Tensor &chosen, const torch::Tensor &weights, const torch::Tensor &up, const torch::Tensor &down)
+{
+    TORCH_CHECK(x.dim() == 2, "quadmul.moe_mlp: x must be [tokens, hidden]");
+    check_chosen("quadmul.moe_mlp", x, chosen);
+    TORCH_CHECK(weights.device() == x.device() && weights.scalar_type() == torch::kFloat32 && weights.is_contiguous() && weights.sizes() == chosen.sizes(),
+                "quadmul.moe_mlp: the weights of the chosen must be a contiguous float32 tensor [tokens, top_k] on x's device");
+    TORCH_CHECK(up.dim() == 3 && down.dim() == 3 && x.size(1) % 2 == 0 && up.size(2) * 2 == x.size(1) && down.size(1) == x.size(1) && up.size(0) == down.size(0) && up.size(1) == 4 * down.size(2),
+                "quadmul.moe_mlp: up must be [experts, 2 inner, hidden / 2], down [experts, hidden, inner / 2]");
+}
+torch::Tensor moe_mlp(torch::Tensor x, torch::Tensor chosen, torch::Tensor weights, torch::Tensor up, torch::Tensor up_scale, torch::Tensor down, torch::Tensor down_scale, int64_t group)
+{
+    TORCH_CHECK(x.is_cuda(), "quadmul.moe_mlp: expects GPU tensors");
+    const int type = float16_type(x, "quadmul.moe_mlp: x");
+    check_mlp(x, chosen, weights, up, down);
+    const qm_expert_weights u = expert_weights("quadmul.moe_mlp", x, up, up_scale, group, c10::nullopt), d = expert_weights("quadmul.moe_mlp", x, down, down_scale, group, c10::nullopt);
+    c10::OptionalDeviceGuard guard(x.device());
+    if (u.k > 1 && x.stride(1) != 1) x = x.contiguous();
+    const int tokens = (int)chosen.size(0), top_k = (int)chosen.size(1);
+    auto y = torch::empty({x.size(0), x.size(1)}, x.options());
+    const size_t need = qm_moe_mlp_workspace_bytes(&u, &d, tokens, top_k);
+    torch::Tensor scratch;
+    if (need > 0) scratch = torch::empty({(int64_t)need}, x.options().dtype(torch::kUInt8));
+    check_status(qm_moe_mlp_i4(x.data_ptr(), type, x.stride(0), chosen.data_ptr<int>(), weights.data_ptr<float>(), &u, &d, y.data_ptr(), tokens, top_k, stream_of(x),
+                               need > 0 ? scratch.data_ptr() : nullptr, need),
+                 "quadmul.moe_mlp");
+    return y;
+}
+
 std::tuple<torch::Tensor, torch::Tensor> quantize_pack_meta(const torch::Tensor &x)
 {
     TORCH_CHECK(x.dim() == 2 && x.size(1) % 2 == 0, "quadmul.quantize_pack: expects a 2-D tensor with even K");
@@ -442,6 +550,44 @@ torch::Tensor kv_attend_meta(const torch::Tensor &q, const torch::Tensor &, cons
     return torch::empty(q.sizes(), q.options());
 }
 
+std::tuple<torch::Tensor, torch::Tensor> moe_route_op(const torch::Tensor &logits, int64_t top_k, const c10::optional<torch::Tensor> &bias, bool sigmoid, int64_t groups, int64_t top_groups,
+                                                      int64_t group_best, bool renormalise, double scale)
+{
+    return moe_route(logits, top_k, bias, sigmoid, groups, top_groups, group_best, renormalise, scale);
+}
+std::tuple<torch::Tensor, torch::Tensor> moe_route_meta(const torch::Tensor &logits, int64_t top_k, const c10::optional<torch::Tensor> &bias, bool, int64_t groups, int64_t top_groups,
+                                                        int64_t group_best, bool, double)
+{
+    check_route(logits, top_k, bias, groups, top_groups, group_best);
+    return {torch::empty({logits.size(0), top_k}, logits.options().dtype(torch::kInt32)), torch::empty({logits.size(0), top_k}, logits.options().dtype(torch::kFloat32))};
+}
+torch::Tensor gemm_experts_op(const torch::Tensor &x, const torch::Tensor &chosen, const torch::Tensor &weight, const torch::Tensor &weight_scale, int64_t group,
+                              const c10::optional<torch::Tensor> &bias)
+{
+    return gemm_experts(x, chosen, weight, weight_scale, group, bias);
+}
+torch::Tensor gemm_experts_meta(const torch::Tensor &x, const torch::Tensor &chosen, const torch::Tensor &weight, const torch::Tensor &weight_scale, int64_t group,
+                                const c10::optional<torch::Tensor> &bias)
+{
+    float16_type(x, "quadmul.gemm_experts: x");
+    check_experts(x, chosen, weight);
+    TORCH_CHECK(weight_scale.dim() == 3 && group >= 32 && group % 32 == 0 && weight_scale.size(2) == (x.size(-1) + group - 1) / group, "quadmul.gemm_experts: the scales must be [experts, n, ceil(k / group)]");
+    (void)bias;
+    return torch::empty({chosen.size(0), chosen.size(1), weight.size(1)}, x.options());
+}
+torch::Tensor moe_mlp_op(const torch::Tensor &x, const torch::Tensor &chosen, const torch::Tensor &weights, const torch::Tensor &up, const torch::Tensor &up_scale, const torch::Tensor &down,
+                         const torch::Tensor &down_scale, int64_t group)
+{
+    return moe_mlp(x, chosen, weights, up, up_scale, down, down_scale, group);
+}
+torch::Tensor moe_mlp_meta(const torch::Tensor &x, const torch::Tensor &chosen, const torch::Tensor &weights, const torch::Tensor &up, const torch::Tensor &, const torch::Tensor &down,
+                           const torch::Tensor &, int64_t)
+{
+    float16_type(x, "quadmul.moe_mlp: x");
+    check_mlp(x, chosen, weights, up, down);
+    return torch::empty({x.size(0), x.size(1)}, x.options());
+}
+
 }  // namespace
 
 TORCH_LIBRARY(quadmul, m)
@@ -456,6 +602,9 @@ TORCH_LIBRARY(quadmul, m)
           "Tensor? query_start, Tensor? cos, Tensor? sin, bool interleaved, int max_query) -> Tensor");
     m.def("kv_attend(Tensor q, Tensor cache_k, Tensor cache_v, Tensor scales, Tensor block_table, Tensor lengths, Tensor? query_start, float? scale, bool causal, "
           "int window, int max_query, int max_length) -> Tensor");
+    m.def("moe_route(Tensor logits, int top_k, Tensor? bias, bool sigmoid, int groups, int top_groups, int group_best, bool renormalise, float scale) -> (Tensor, Tensor)");
+    m.def("gemm_experts(Tensor x, Tensor chosen, Tensor weight, Tensor weight_scale, int group_size, Tensor? bias) -> Tensor");
+    m.def("moe_mlp(Tensor x, Tensor chosen, Tensor weights, Tensor up, Tensor up_scale, Tensor down, Tensor down_scale, int group_size) -> Tensor");
 }
 TORCH_LIBRARY_IMPL(quadmul, CUDA, m)
 {
@@ -466,6 +615,9 @@ TORCH_LIBRARY_IMPL(quadmul, CUDA, m)
     m.impl("kv_append", &kv_append_op);
     m.impl("kv_append_rotate", &kv_append_rotate_op);
     m.impl("kv_attend", &kv_attend_op);
+    m.impl("moe_route", &moe_route_op);
+    m.impl("gemm_experts", &gemm_experts_op);
+    m.impl("moe_mlp", &moe_mlp_op);
 }
 TORCH_LIBRARY_IMPL(quadmul, Meta, m)
 {
@@ -476,6 +628,9 @@ TORCH_LIBRARY_IMPL(quadmul, Meta, m)
     m.impl("kv_append", &kv_append_meta);
     m.impl("kv_append_rotate", &kv_append_rotate_meta);
     m.impl("kv_attend", &kv_attend_meta);
+    m.impl("moe_route", &moe_route_meta);
+    m.impl("gemm_experts", &gemm_experts_meta);
+    m.impl("moe_mlp", &moe_mlp_meta);
 }
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
@@ -497,6 +652,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
           py::arg("lengths"), py::arg("query_start") = py::none(), py::arg("scale") = py::none(), py::arg("causal") = true, py::arg("window") = 0, py::arg("max_query") = 0,
           py::arg("max_length") = 0, nogil());
     m.def("kv_read", &kv_read, "Pages of the 8-bit cache as 16-bit floats", py::arg("cache_k"), py::arg("cache_v"), py::arg("scales"), py::arg("pages"), py::arg("bf16"), nogil());
+    m.def("moe_route", &moe_route, "A router's choice of experts and their weights", py::arg("logits"), py::arg("top_k"), py::arg("bias") = py::none(), py::arg("sigmoid") = false,
+          py::arg("groups") = 1, py::arg("top_groups") = 1, py::arg("group_best") = 2, py::arg("renormalise") = false, py::arg("scale") = 1.0, nogil());
+    m.def("gemm_experts", &gemm_experts, "Each token's row times the packed int4 weights of each of its experts", py::arg("x"), py::arg("chosen"), py::arg("weight"),
+          py::arg("weight_scale"), py::arg("group_size"), py::arg("bias") = py::none(), nogil());
+    m.def("moe_mlp", &moe_mlp, "The gated MLP of each token's experts, added up by weight", py::arg("x"), py::arg("chosen"), py::arg("weights"), py::arg("up"), py::arg("up_scale"),
+          py::arg("down"), py::arg("down_scale"), py::arg("group_size"), nogil());
     m.def("pack", &pack, nogil(), "Pack a [rows, K] int8 tensor of int4 values into [rows, K/2] bytes on the GPU");
     m.def("quantize_pack", &quantize_pack, nogil(), "Per-row symmetric int4 quantisation of a [rows, K] float tensor, packed; returns (packed, scales)");
     m.def("unpack", &unpack, nogil(), "Unpack [rows, K/2] bytes into a [rows, K] int8 tensor on the GPU");

@@ -1,0 +1,166 @@
+// C entries of the mixture of experts (include/qm_abi.h): argument checks, choice of kernels, launches.
+#include <algorithm>
+#include <climits>
+
+#include "../../include/qm_abi.h"
+#include "qm_launch.hpp"
+#include "qm_experts.hpp"
+#include "qm_route.hpp"
+
+#define QM_EXPORT extern "C" __attribute__((visibility("default")))
+
+namespace qm {
+
+static int check_weights(const qm_expert_weights *w, const int dtype)
+{
+    if (!w) return QM_ERR_NULL;
+    if (w->scale_dtype != QM_IN_F32 && w->scale_dtype != dtype) return QM_ERR_DTYPE;
+    if (w->experts < 0 || w->n < 0 || w->k < 0 || (w->k & 1) || w->group < 32 || w->group % 32 != 0) return QM_ERR_SHAPE;
+    if (w->experts > 0 && w->n > 0 && w->k > 0 && (!w->weight || !w->scale)) return QM_ERR_NULL;
+    return ((uintptr_t)w->scale & (w->scale_dtype == QM_IN_F32 ? 3 : 1)) || ((uintptr_t)w->bias & 1) ? QM_ERR_ALIGN : QM_OK;
+}
+
+struct ExpertsPlan {
+    size_t hidden, part, bytes;  // where in the workspace the gated products and the outputs of experts are
+};
+static size_t up256(const size_t n) { return (n + 255) / 256 * 256; }
+
+static hipError_t launch_product(const ExpertsArgs &p, const int dtype, const int scale_dtype, const ExpertsOut out, hipStream_t s)
+{
+    const int columns = out == EXPERTS_GATED ? p.N / 2 : p.N;
+    const dim3 grid(std::min(columns / 4 + 1, 1 << 20), std::min(p.slots, 65535));
+    const auto by_type = [&](auto t, auto st) {
+        constexpr int T = decltype(t)::value, S = decltype(st)::value;
+        switch (out) {
+        case EXPERTS_PLAIN: return enqueue(&experts_any_kernel<T, S, EXPERTS_PLAIN>, grid, dim3(256), 0, s, p);
+        case EXPERTS_GATED: return enqueue(&experts_any_kernel<T, S, EXPERTS_GATED>, grid, dim3(256), 0, s, p);
+        default: return enqueue(&experts_any_kernel<T, S, EXPERTS_PART>, grid, dim3(256), 0, s, p);
+        }
+    };
+    typedef std::integral_constant<int, QM_IN_F16> F16;
+    typedef std::integral_constant<int, QM_IN_BF16> BF16;
+    typedef std::integral_constant<int, QM_IN_F32> F32;
+    if (dtype == QM_IN_F16) return scale_dtype == QM_IN_F32 ? by_type(F16{}, F32{}) : by_type(F16{}, F16{});
+    return scale_dtype == QM_IN_F32 ? by_type(BF16{}, F32{}) : by_type(BF16{}, BF16{});
+}
+static ExpertsArgs args_of(const qm_expert_weights *w, const void *x, const long long x_token, const long long x_choice, const int *chosen, void *out, const int tokens, const int top_k)
+{
+    return {static_cast<const uint16_t *>(x), x_token, x_choice, chosen, static_cast<const uint8_t *>(w->weight), w->scale, static_cast<const uint16_t *>(w->bias), out,
+            tokens * top_k, top_k, w->experts, w->n, w->k, w->group, (int)(((long long)w->k + w->group - 1) / w->group)};
+}
+
+static ExpertsPlan mlp_plan(const int tokens, const int top_k, const int inner, const int hidden)
+{
+    ExpertsPlan p{};
+    p.part = up256((size_t)tokens * top_k * inner * 2);
+    p.bytes = p.part + up256((size_t)tokens * top_k * hidden * 4);
+    return p;
+}
+
+}  // namespace qm
+
+using namespace qm;
+
+QM_EXPORT int qm_moe_route(const void *logits, int dtype, long long row_stride, int tokens, int experts, int top_k, const float *bias, int scores, int groups, int top_groups,
+                           int group_best, int renormalise, double scale, int *chosen, float *weights, void *stream)
+{
+    if (dtype != QM_IN_F16 && dtype != QM_IN_BF16 && dtype != QM_IN_F32) return QM_ERR_DTYPE;
+    if (tokens < 0 || experts < 1 || experts > QM_ROUTE_EXPERTS || groups < 1 || groups > 64 || experts % groups != 0 || top_groups < 1 || top_groups > groups) return QM_ERR_SHAPE;
+    if (top_k < 1 || top_k > 64 || top_k > experts / groups * top_groups || (tokens > 1 && row_stride < experts)) return QM_ERR_SHAPE;
+    if ((scores != QM_SCORES_SOFTMAX && scores != QM_SCORES_SIGMOID) || (group_best != 1 && group_best != 2)) return QM_ERR_SHAPE;
+    if (tokens == 0) return QM_OK;
+    if (!logits || !chosen || !weights) return QM_ERR_NULL;
+    if (((uintptr_t)logits & (dtype == QM_IN_F32 ? 3 : 1)) || (((uintptr_t)bias | (uintptr_t)chosen | (uintptr_t)weights) & 3)) return QM_ERR_ALIGN;
+    // 16 lanes to a token where that many tokens are enough for the chip, else 64
+    const bool narrow = tokens > 1024 && experts <= 256 && top_k <= 16 && groups <= 16;
+    int parts = 1;
+    while (parts * 2 * groups <= (narrow ? 16 : 64)) parts *= 2;
+    const RouteArgs p{logits, bias, chosen, weights, tokens > 1 ? row_stride : experts, tokens, experts, top_k, groups, top_groups, scores == QM_SCORES_SIGMOID, group_best == 2,
+                      renormalise != 0, parts, (uint32_t)(((1 << 20) + experts / groups - 1) / (experts / groups)), scale};
+    const bool by_logits = scores == QM_SCORES_SOFTMAX && !bias && top_groups == groups;
+    const auto run = [&](auto t, auto l) {
+        constexpr int T = decltype(t)::value;
+        constexpr bool LOGITS = decltype(l)::value;
+        const auto kernel = narrow ? experts <= 64    ? &route_kernel<T, 4, 16, LOGITS>
+                                     : experts <= 128 ? &route_kernel<T, 8, 16, LOGITS>
+                                                      : &route_kernel<T, 16, 16, LOGITS>
+                            : experts <= 64    ? &route_kernel<T, 1, 64, LOGITS>
+                            : experts <= 128   ? &route_kernel<T, 2, 64, LOGITS>
+                            : experts <= 256   ? &route_kernel<T, 4, 64, LOGITS>
+                                               : &route_kernel<T, 16, 64, LOGITS>;
+        const int each = narrow ? 16 : 4;
+        return enqueue(kernel, dim3(std::min((tokens + each - 1) / each, 1 << 20)), dim3(256), 0, reinterpret_cast<hipStream_t>(stream), p);
+    };
+    const auto by_type = [&](auto t) { return by_logits ? run(t, std::true_type{}) : run(t, std::false_type{}); };
+    const hipError_t e = dtype == QM_IN_F16    ? by_type(std::integral_constant<int, QM_IN_F16>{})
+                         : dtype == QM_IN_BF16 ? by_type(std::integral_constant<int, QM_IN_BF16>{})
+                                               : by_type(std::integral_constant<int, QM_IN_F32>{});
+    return e == hipSuccess ? QM_OK : fail_launch(e);
+}
+
+// what both products check of tokens and choices
+static int check_choices(const int tokens, const int top_k, const int dtype)
+{
+    if (dtype != QM_IN_F16 && dtype != QM_IN_BF16) return QM_ERR_DTYPE;
+    return tokens < 0 || top_k < 0 || (long long)tokens * top_k > INT_MAX ? QM_ERR_SHAPE : QM_OK;
+}
+
+QM_EXPORT size_t qm_gemm_experts_workspace_bytes(const qm_expert_weights *weights, int tokens, int top_k)
+{
+    if (check_weights(weights, weights ? weights->scale_dtype : 0) != QM_OK || check_choices(tokens, top_k, QM_IN_F16) != QM_OK) return 0;
+    return 0;
+}
+
+QM_EXPORT int qm_gemm_experts_i4(const void *x, int dtype, long long token_stride, long long choice_stride, const int *chosen, const qm_expert_weights *weights, void *y,
+                                 int tokens, int top_k, void *stream, void *workspace, size_t workspace_bytes)
+{
+    if (const int e = check_choices(tokens, top_k, dtype); e != QM_OK) return e;
+    if (const int e = check_weights(weights, dtype); e != QM_OK) return e;
+    if (token_stride < 0 || choice_stride < 0) return QM_ERR_SHAPE;
+    if (tokens == 0 || top_k == 0 || weights->n == 0) return QM_OK;
+    if (!chosen || !y || (!x && weights->k > 0)) return QM_ERR_NULL;
+    if ((((uintptr_t)x | (uintptr_t)y) & 1) || ((uintptr_t)chosen & 3) || ((uintptr_t)workspace & 15)) return QM_ERR_ALIGN;
+    if (workspace_bytes < qm_gemm_experts_workspace_bytes(weights, tokens, top_k)) return QM_ERR_SCRATCH;
+    const hipError_t e = launch_product(args_of(weights, x, token_stride, choice_stride, chosen, y, tokens, top_k), dtype, weights->scale_dtype, EXPERTS_PLAIN, reinterpret_cast<hipStream_t>(stream));
+    return e == hipSuccess ? QM_OK : fail_launch(e);
+}
+
+static int check_mlp(const qm_expert_weights *up, const qm_expert_weights *down, const int dtype)
+{
+    if (const int e = check_weights(up, dtype); e != QM_OK) return e;
+    if (const int e = check_weights(down, dtype); e != QM_OK) return e;
+    return (long long)down->k * 2 != up->n || down->n != up->k || up->experts != down->experts || up->bias || down->bias ? QM_ERR_SHAPE : QM_OK;
+}
+
+QM_EXPORT size_t qm_moe_mlp_workspace_bytes(const qm_expert_weights *up, const qm_expert_weights *down, int tokens, int top_k)
+{
+    if (!up || !down || check_mlp(up, down, up->scale_dtype == QM_IN_F32 ? down->scale_dtype : up->scale_dtype) != QM_OK || check_choices(tokens, top_k, QM_IN_F16) != QM_OK) return 0;
+    return mlp_plan(tokens, top_k, down->k, down->n).bytes;
+}
+
+QM_EXPORT int qm_moe_mlp_i4(const void *x, int dtype, long long token_stride, const int *chosen, const float *weights, const qm_expert_weights *up, const qm_expert_weights *down,
+                            void *y, int tokens, int top_k, void *stream, void *workspace, size_t workspace_bytes)
+{
+    if (const int e = check_choices(tokens, top_k, dtype); e != QM_OK) return e;
+    if (const int e = check_mlp(up, down, dtype); e != QM_OK) return e;
+    if (token_stride < 0) return QM_ERR_SHAPE;
+    if (tokens == 0 || down->n == 0) return QM_OK;
+    if (!y || !x || (top_k > 0 && (!chosen || !weights))) return QM_ERR_NULL;
+    if ((((uintptr_t)x | (uintptr_t)y) & 1) || (((uintptr_t)chosen | (uintptr_t)weights) & 3) || ((uintptr_t)workspace & 15)) return QM_ERR_ALIGN;
+    const ExpertsPlan plan = mlp_plan(tokens, top_k, down->k, down->n);
+    if (plan.bytes > 0 && (!workspace || workspace_bytes < plan.bytes)) return QM_ERR_SCRATCH;
+    char *const at = static_cast<char *>(workspace);
+    const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    hipError_t e = hipSuccess;
+    if (top_k > 0) {
+        if (down->k > 0) e = launch_product(args_of(up, x, token_stride, 0, chosen, at + plan.hidden, tokens, top_k), dtype, up->scale_dtype, EXPERTS_GATED, s);
+        if (e == hipSuccess) e = launch_product(args_of(down, at + plan.hidden, (long long)top_k * down->k, down->k, chosen, at + plan.part, tokens, top_k), dtype, down->scale_dtype, EXPERTS_PART, s);
+    }
+    if (e == hipSuccess) {
+        const unsigned grid = (unsigned)std::min<size_t>(((size_t)tokens * down->n + 255) / 256, 1 << 20);
+        const float *const part = reinterpret_cast<const float *>(at + plan.part);
+        const auto sum = dtype == QM_IN_F16 ? &experts_sum_kernel<QM_IN_F16> : &experts_sum_kernel<QM_IN_BF16>;
+        e = enqueue(sum, dim3(grid), dim3(256), 0, s, part, chosen, weights, static_cast<uint16_t *>(y), tokens, top_k, up->experts, down->n);
+    }
+    return e == hipSuccess ? QM_OK : fail_launch(e);
+}
