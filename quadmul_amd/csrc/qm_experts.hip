@@ -20,40 +20,117 @@ static int check_weights(const qm_expert_weights *w, const int dtype)
     return ((uintptr_t)w->scale & (w->scale_dtype == QM_IN_F32 ? 3 : 1)) || ((uintptr_t)w->bias & 1) ? QM_ERR_ALIGN : QM_OK;
 }
 
-struct ExpertsPlan {
-    size_t hidden, part, bytes;  // where in the workspace the gated products and the outputs of experts are
-};
 static size_t up256(const size_t n) { return (n + 255) / 256 * 256; }
 
-static hipError_t launch_product(const ExpertsArgs &p, const int dtype, const int scale_dtype, const ExpertsOut out, hipStream_t s)
-{
-    const int columns = out == EXPERTS_GATED ? p.N / 2 : p.N;
-    const dim3 grid(std::min(columns / 4 + 1, 1 << 20), std::min(p.slots, 65535));
-    const auto by_type = [&](auto t, auto st) {
-        constexpr int T = decltype(t)::value, S = decltype(st)::value;
-        switch (out) {
-        case EXPERTS_PLAIN: return enqueue(&experts_any_kernel<T, S, EXPERTS_PLAIN>, grid, dim3(256), 0, s, p);
-        case EXPERTS_GATED: return enqueue(&experts_any_kernel<T, S, EXPERTS_GATED>, grid, dim3(256), 0, s, p);
-        default: return enqueue(&experts_any_kernel<T, S, EXPERTS_PART>, grid, dim3(256), 0, s, p);
-        }
-    };
-    typedef std::integral_constant<int, QM_IN_F16> F16;
-    typedef std::integral_constant<int, QM_IN_BF16> BF16;
-    typedef std::integral_constant<int, QM_IN_F32> F32;
-    if (dtype == QM_IN_F16) return scale_dtype == QM_IN_F32 ? by_type(F16{}, F32{}) : by_type(F16{}, F16{});
-    return scale_dtype == QM_IN_F32 ? by_type(BF16{}, F32{}) : by_type(BF16{}, BF16{});
-}
-static ExpertsArgs args_of(const qm_expert_weights *w, const void *x, const long long x_token, const long long x_choice, const int *chosen, void *out, const int tokens, const int top_k)
-{
-    return {static_cast<const uint16_t *>(x), x_token, x_choice, chosen, static_cast<const uint8_t *>(w->weight), w->scale, static_cast<const uint16_t *>(w->bias), out,
-            tokens * top_k, top_k, w->experts, w->n, w->k, w->group, (int)(((long long)w->k + w->group - 1) / w->group)};
-}
-
-static ExpertsPlan mlp_plan(const int tokens, const int top_k, const int inner, const int hidden)
+// How the slots of a call are cut into tiles, and where in the workspace the lists are.
+struct ExpertsPlan {
+    int rows;       // of a tile; 0: no tiles
+    int tiles;      // at most
+    size_t order, list, count, bytes;
+};
+static ExpertsPlan experts_plan(const int slots, const int experts, size_t at)
 {
     ExpertsPlan p{};
+    p.bytes = at;
+    if (slots == 0 || experts == 0 || experts > EXPERTS_SORTED) return p;
+    const int mean = slots / experts;
+    p.rows = mean >= 256 ? 256 : mean >= 96 ? 128 : mean >= 24 ? 64 : 32;
+    p.tiles = slots / p.rows + std::min(experts + 1, slots);
+    p.order = at;
+    p.list = p.order + up256((size_t)slots * 4);
+    p.count = p.list + up256((size_t)p.tiles * 16);
+    p.bytes = p.count + 256;
+    return p;
+}
+static hipError_t sort_slots(const ExpertsPlan &plan, const int *chosen, const int slots, const int experts, char *at, hipStream_t s)
+{
+    return enqueue(&experts_sort_kernel, dim3(1), dim3(1024), (size_t)(experts + 1) * 4, s, chosen, slots, experts, plan.rows, reinterpret_cast<int *>(at + plan.order),
+                   reinterpret_cast<int *>(at + plan.list), reinterpret_cast<int *>(at + plan.count));
+}
+
+// Whether the kernels on the matrix cores take these weights (the others: experts_any_kernel).
+static bool tiles_take(const qm_expert_weights *w) { return w->k > 0 && w->k % 32 == 0 && w->n <= 65535 * 32 && ((uintptr_t)w->weight & 15) == 0 && w->experts > 0 && w->experts <= EXPERTS_SORTED; }
+
+static ExpertsArgs args_of(const qm_expert_weights *w, const void *x, const long long x_token, const long long x_choice, const int *chosen, void *out, const int tokens, const int top_k,
+                           const ExpertsPlan &plan, const char *at)
+{
+    return {static_cast<const uint16_t *>(x), x_token, x_choice, chosen, static_cast<const uint8_t *>(w->weight), w->scale, static_cast<const uint16_t *>(w->bias), out,
+            tokens * top_k, top_k, w->experts, w->n, w->k, w->group, (int)(((long long)w->k + w->group - 1) / w->group), w->k / 32, reinterpret_cast<const int *>(at + plan.order),
+            reinterpret_cast<const int *>(at + plan.list), reinterpret_cast<const int *>(at + plan.count)};
+}
+
+template <int T, int S, ExpertsOut OUT>
+static hipError_t launch_any(const ExpertsArgs &p, hipStream_t s)
+{
+    const int columns = OUT == EXPERTS_GATED ? p.N / 2 : p.N;
+    return enqueue(&experts_any_kernel<T, S, OUT>, dim3(std::min(columns / 4 + 1, 1 << 20), std::min(p.slots, 65535)), dim3(256), 0, s, p);
+}
+template <int T, int S, int MODE, ExpertsOut OUT>
+static hipError_t launch_tiles(const ExpertsArgs &p, const ExpertsPlan &plan, hipStream_t s)
+{
+    // (with a scale to every one or two blocks the registers of 64 columns to a wave do not fit)
+    constexpr int NT = MODE == 1 ? 4 : 2;
+    const int columns = OUT == EXPERTS_GATED ? p.N / 2 : p.N;
+    const auto wide = [&](auto wm, auto wn, auto mt, auto nt) {
+        constexpr int WM = decltype(wm)::value, WN = decltype(wn)::value, MT = decltype(mt)::value, N = decltype(nt)::value, BM = 16 * WM * MT, BN = 16 * WN * N, OF = OUT == EXPERTS_GATED ? BN / 2 : BN;
+        static std::atomic<bool> known[QM_MAX_DEVICES] = {};
+        const auto kernel = [] {
+            if constexpr (OUT == EXPERTS_PLAIN) return &gemm_grouped_wide_kernel<T, S, MODE, WM, WN, MT, N, ExpertsArgs, ExpertsPlainTile>;
+            else if constexpr (OUT == EXPERTS_GATED) return &gemm_grouped_wide_kernel<T, S, MODE, WM, WN, MT, N, ExpertsArgs, ExpertsGatedTile>;
+            else return &gemm_grouped_wide_kernel<T, S, MODE, WM, WN, MT, N, ExpertsArgs, ExpertsPartTile>;
+        }();
+        constexpr int lds = 2 * 8 * 16 * (BM + BN) + 2 * 2 * BN * (int)sizeof(float);
+        if (const hipError_t e = ensure_dynamic_lds(kernel, lds, known); e != hipSuccess) return e;
+        return enqueue(kernel, dim3(plan.tiles, (columns + OF - 1) / OF), dim3(64 * WM * WN), lds, s, p);
+    };
+    const std::integral_constant<int, 1> one{};
+    const std::integral_constant<int, 2> two{};
+    const std::integral_constant<int, 4> four{};
+    const std::integral_constant<int, NT> nt{};
+    switch (plan.rows) {
+    case 256: return wide(four, two, four, nt);
+    case 128: return wide(two, two, four, nt);
+    case 64: return wide(one, four, four, two);
+    default: return wide(one, four, two, two);
+    }
+}
+static hipError_t launch_product(const ExpertsArgs &p, const bool tiled, const ExpertsPlan &plan, const int dtype, const int scale_dtype, const ExpertsOut out, hipStream_t s)
+{
+    const auto by_out = [&](auto t, auto st, auto o) {
+        constexpr int T = decltype(t)::value, S = decltype(st)::value;
+        constexpr ExpertsOut OUT = (ExpertsOut)decltype(o)::value;
+        if (!tiled) return launch_any<T, S, OUT>(p, s);
+        switch (group_mode(p.group)) {
+        case 1: return launch_tiles<T, S, 1, OUT>(p, plan, s);
+        case 2: return launch_tiles<T, S, 2, OUT>(p, plan, s);
+        case 4: return launch_tiles<T, S, 4, OUT>(p, plan, s);
+        default: return launch_tiles<T, S, 0, OUT>(p, plan, s);
+        }
+    };
+    const auto by_type = [&](auto t, auto st) {
+        switch (out) {
+        case EXPERTS_PLAIN: return by_out(t, st, std::integral_constant<int, EXPERTS_PLAIN>{});
+        case EXPERTS_GATED: return by_out(t, st, std::integral_constant<int, EXPERTS_GATED>{});
+        default: return by_out(t, st, std::integral_constant<int, EXPERTS_PART>{});
+        }
+    };
+    const std::integral_constant<int, QM_IN_F16> f16{};
+    const std::integral_constant<int, QM_IN_BF16> bf16{};
+    const std::integral_constant<int, QM_IN_F32> f32{};
+    if (dtype == QM_IN_F16) return scale_dtype == QM_IN_F32 ? by_type(f16, f32) : by_type(f16, f16);
+    return scale_dtype == QM_IN_F32 ? by_type(bf16, f32) : by_type(bf16, bf16);
+}
+
+// The workspace of the gated MLP: the gated products and the outputs of the experts in front of the lists.
+struct MlpPlan {
+    size_t part;
+    ExpertsPlan sorted;
+};
+static MlpPlan mlp_plan(const int tokens, const int top_k, const int experts, const int inner, const int hidden)
+{
+    MlpPlan p{};
     p.part = up256((size_t)tokens * top_k * inner * 2);
-    p.bytes = p.part + up256((size_t)tokens * top_k * hidden * 4);
+    p.sorted = experts_plan(tokens * top_k, experts, p.part + up256((size_t)tokens * top_k * hidden * 4));
     return p;
 }
 
@@ -108,7 +185,7 @@ static int check_choices(const int tokens, const int top_k, const int dtype)
 QM_EXPORT size_t qm_gemm_experts_workspace_bytes(const qm_expert_weights *weights, int tokens, int top_k)
 {
     if (check_weights(weights, weights ? weights->scale_dtype : 0) != QM_OK || check_choices(tokens, top_k, QM_IN_F16) != QM_OK) return 0;
-    return 0;
+    return experts_plan(tokens * top_k, weights->experts, 0).bytes;
 }
 
 QM_EXPORT int qm_gemm_experts_i4(const void *x, int dtype, long long token_stride, long long choice_stride, const int *chosen, const qm_expert_weights *weights, void *y,
@@ -120,8 +197,13 @@ QM_EXPORT int qm_gemm_experts_i4(const void *x, int dtype, long long token_strid
     if (tokens == 0 || top_k == 0 || weights->n == 0) return QM_OK;
     if (!chosen || !y || (!x && weights->k > 0)) return QM_ERR_NULL;
     if ((((uintptr_t)x | (uintptr_t)y) & 1) || ((uintptr_t)chosen & 3) || ((uintptr_t)workspace & 15)) return QM_ERR_ALIGN;
-    if (workspace_bytes < qm_gemm_experts_workspace_bytes(weights, tokens, top_k)) return QM_ERR_SCRATCH;
-    const hipError_t e = launch_product(args_of(weights, x, token_stride, choice_stride, chosen, y, tokens, top_k), dtype, weights->scale_dtype, EXPERTS_PLAIN, reinterpret_cast<hipStream_t>(stream));
+    const ExpertsPlan plan = experts_plan(tokens * top_k, weights->experts, 0);
+    if (plan.bytes > 0 && (!workspace || workspace_bytes < plan.bytes)) return QM_ERR_SCRATCH;
+    char *const at = static_cast<char *>(workspace);
+    const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    const bool tiled = tiles_take(weights);
+    hipError_t e = tiled ? sort_slots(plan, chosen, tokens * top_k, weights->experts, at, s) : hipSuccess;
+    if (e == hipSuccess) e = launch_product(args_of(weights, x, token_stride, choice_stride, chosen, y, tokens, top_k, plan, at), tiled, plan, dtype, weights->scale_dtype, EXPERTS_PLAIN, s);
     return e == hipSuccess ? QM_OK : fail_launch(e);
 }
 
@@ -135,7 +217,7 @@ static int check_mlp(const qm_expert_weights *up, const qm_expert_weights *down,
 QM_EXPORT size_t qm_moe_mlp_workspace_bytes(const qm_expert_weights *up, const qm_expert_weights *down, int tokens, int top_k)
 {
     if (!up || !down || check_mlp(up, down, up->scale_dtype == QM_IN_F32 ? down->scale_dtype : up->scale_dtype) != QM_OK || check_choices(tokens, top_k, QM_IN_F16) != QM_OK) return 0;
-    return mlp_plan(tokens, top_k, down->k, down->n).bytes;
+    return mlp_plan(tokens, top_k, up->experts, down->k, down->n).sorted.bytes;
 }
 
 QM_EXPORT int qm_moe_mlp_i4(const void *x, int dtype, long long token_stride, const int *chosen, const float *weights, const qm_expert_weights *up, const qm_expert_weights *down,
@@ -147,14 +229,18 @@ QM_EXPORT int qm_moe_mlp_i4(const void *x, int dtype, long long token_stride, co
     if (tokens == 0 || down->n == 0) return QM_OK;
     if (!y || !x || (top_k > 0 && (!chosen || !weights))) return QM_ERR_NULL;
     if ((((uintptr_t)x | (uintptr_t)y) & 1) || (((uintptr_t)chosen | (uintptr_t)weights) & 3) || ((uintptr_t)workspace & 15)) return QM_ERR_ALIGN;
-    const ExpertsPlan plan = mlp_plan(tokens, top_k, down->k, down->n);
-    if (plan.bytes > 0 && (!workspace || workspace_bytes < plan.bytes)) return QM_ERR_SCRATCH;
+    const MlpPlan plan = mlp_plan(tokens, top_k, up->experts, down->k, down->n);
+    if (plan.sorted.bytes > 0 && (!workspace || workspace_bytes < plan.sorted.bytes)) return QM_ERR_SCRATCH;
     char *const at = static_cast<char *>(workspace);
     const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     hipError_t e = hipSuccess;
     if (top_k > 0) {
-        if (down->k > 0) e = launch_product(args_of(up, x, token_stride, 0, chosen, at + plan.hidden, tokens, top_k), dtype, up->scale_dtype, EXPERTS_GATED, s);
-        if (e == hipSuccess) e = launch_product(args_of(down, at + plan.hidden, (long long)top_k * down->k, down->k, chosen, at + plan.part, tokens, top_k), dtype, down->scale_dtype, EXPERTS_PART, s);
+        const bool up_tiled = tiles_take(up), down_tiled = tiles_take(down);
+        const ExpertsArgs first = args_of(up, x, token_stride, 0, chosen, at, tokens, top_k, plan.sorted, at);
+        const ExpertsArgs second = args_of(down, at, (long long)top_k * down->k, down->k, chosen, at + plan.part, tokens, top_k, plan.sorted, at);
+        if (up_tiled || down_tiled) e = sort_slots(plan.sorted, chosen, tokens * top_k, up->experts, at, s);
+        if (e == hipSuccess && down->k > 0) e = launch_product(first, up_tiled, plan.sorted, dtype, up->scale_dtype, EXPERTS_GATED, s);
+        if (e == hipSuccess) e = launch_product(second, down_tiled, plan.sorted, dtype, down->scale_dtype, EXPERTS_PART, s);
     }
     if (e == hipSuccess) {
         const unsigned grid = (unsigned)std::min<size_t>(((size_t)tokens * down->n + 255) / 256, 1 << 20);

@@ -1,4 +1,4 @@
-// 16-bit floats in and out of registers, by the QM_IN_* type they are stored in.
+// 16-bit floats in and out of registers, by the QM_IN_* type they are stored in; integers that are the same for a whole wave.
 #pragma once
 #include "qm_common.hpp"
 #include "../../include/qm_abi.h"
@@ -25,5 +25,9 @@ __device__ __forceinline__ float element(const void *p, size_t i)
     if constexpr (T == QM_IN_F32) return static_cast<const float *>(p)[i];
     else return float_of<T>(static_cast<const uint16_t *>(p)[i]);
 }
+
+// Integers that are the same for a whole wave, through the scalar cache.
+typedef const __attribute__((address_space(4))) int *scalar_ints;
+__device__ __forceinline__ scalar_ints scalars(const int *p) { return (scalar_ints)(uintptr_t)p; }
 
 }  // namespace qm

@@ -19,10 +19,7 @@ struct KvArgs {
 struct KvSequence {
     int row0, count, begin, length;
 };
-// Integers that are the same for a whole wave come through the scalar cache: one round trip for the three of them, where vector loads behind
-// the test for `start` made three.
-typedef const __attribute__((address_space(4))) int *scalar_ints;
-__device__ __forceinline__ scalar_ints scalars(const int *p) { return (scalar_ints)(uintptr_t)p; }
+// (through the scalar cache: one round trip for the three of them, where vector loads behind the test for `start` made three)
 __device__ __forceinline__ KvSequence kv_sequence(const KvArgs &c, const int s)
 {
     const int n = scalars(c.lengths)[s], from = scalars(c.start)[s], to = scalars(c.start)[s + c.packed];
