@@ -125,6 +125,7 @@ def build_lib(jobs: int = 8, verbose: bool = False) -> str:
              ("qm_kv.o", ["-c", os.path.join(CSRC, "qm_kv.hip")])]
     # (the units with the scaled-output kernels, 6 and up, take longest: they go first)
     units = [(f"qm_attend_inst_{t}.o", [f"-DQM_ATTEND_TYPE={t}", "-c", os.path.join(CSRC, "qm_attend_inst.hip")]) for t in (1, 2)] + units
+    units = [(f"qm_experts_inst_{t}.o", [f"-DQM_EXPERTS_TYPE={t}", "-c", os.path.join(CSRC, "qm_experts_inst.hip")]) for t in (1, 2)] + units
     units = [(f"qm_tile6_inst_{out}.o", [f"-DQM_TILE6_OUT={out}", "-c", os.path.join(CSRC, "qm_tile6_inst.hip")]) for out in (0, 1, 2)] + units
     units = [(f"qm_tile_inst_{tu}.o", [f"-DQM_TU={tu}", "-c", os.path.join(CSRC, "qm_tile_inst.hip")])
              for tu in sorted(range(N_TILE_TUS), key=lambda t: (t < 6, t))] + units

@@ -453,6 +453,17 @@ void check_experts(const torch::Tensor &x, const torch::Tensor &chosen, const to
     TORCH_CHECK(x.size(-1) % 2 == 0 && weight.dim() == 3 && weight.size(2) * 2 == x.size(-1), "quadmul.gemm_experts: the weights must be [experts, n, k / 2], k even and x's last dimension");
 }
 
+// Rows that the kernels for few rows to an expert can load, sixteen aligned bytes at a time; others are copied first: a pass over x, where the kernels that take
+// rows at any address are up to three times as slow, and results are the same wherever x lies.
+torch::Tensor aligned_rows(torch::Tensor x)
+{
+    const int64_t k = x.size(-1);
+    bool apart = (reinterpret_cast<uintptr_t>(x.data_ptr()) & 15) != 0;
+    for (int64_t d = 0; d + 1 < x.dim(); ++d) apart |= x.size(d) > 1 && x.stride(d) % 8 != 0;
+    if ((k > 1 && x.stride(-1) != 1) || (apart && k % 32 == 0)) return x.clone(at::MemoryFormat::Contiguous);
+    return x;
+}
+
 torch::Tensor gemm_experts(torch::Tensor x, torch::Tensor chosen, torch::Tensor weight, torch::Tensor weight_scale, int64_t group, c10::optional<torch::Tensor> bias)
 {
     TORCH_CHECK(x.is_cuda(), "quadmul.gemm_experts: expects GPU tensors");
@@ -460,7 +471,7 @@ torch::Tensor gemm_experts(torch::Tensor x, torch::Tensor chosen, torch::Tensor 
     check_experts(x, chosen, weight);
     const qm_expert_weights w = expert_weights("quadmul.gemm_experts", x, weight, weight_scale, group, bias);
     c10::OptionalDeviceGuard guard(x.device());
-    if (w.k > 1 && x.stride(-1) != 1) x = x.contiguous();
+    x = aligned_rows(x);
     const int tokens = (int)chosen.size(0), top_k = (int)chosen.size(1);
     auto y = torch::empty({tokens, top_k, w.n}, x.options());
     const size_t need = qm_gemm_experts_workspace_bytes(&w, tokens, top_k);
@@ -488,7 +499,7 @@ torch::Tensor moe_mlp(torch::Tensor x, torch::Tensor chosen, torch::Tensor weigh
     check_mlp(x, chosen, weights, up, down);
     const qm_expert_weights u = expert_weights("quadmul.moe_mlp", x, up, up_scale, group, c10::nullopt), d = expert_weights("quadmul.moe_mlp", x, down, down_scale, group, c10::nullopt);
     c10::OptionalDeviceGuard guard(x.device());
-    if (u.k > 1 && x.stride(1) != 1) x = x.contiguous();
+    x = aligned_rows(x);
     const int tokens = (int)chosen.size(0), top_k = (int)chosen.size(1);
     auto y = torch::empty({x.size(0), x.size(1)}, x.options());
     const size_t need = qm_moe_mlp_workspace_bytes(&u, &d, tokens, top_k);

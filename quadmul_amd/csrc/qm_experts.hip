@@ -5,6 +5,7 @@
 #include "../../include/qm_abi.h"
 #include "qm_launch.hpp"
 #include "qm_experts.hpp"
+#include "qm_experts_sort.hpp"
 #include "qm_route.hpp"
 
 #define QM_EXPORT extern "C" __attribute__((visibility("default")))
@@ -22,19 +23,14 @@ static int check_weights(const qm_expert_weights *w, const int dtype)
 
 static size_t up256(const size_t n) { return (n + 255) / 256 * 256; }
 
-// How the slots of a call are cut into tiles, and where in the workspace the lists are.
-struct ExpertsPlan {
-    int rows;       // of a tile; 0: no tiles
-    int tiles;      // at most
-    size_t order, list, count, bytes;
-};
-static ExpertsPlan experts_plan(const int slots, const int experts, size_t at)
+static ExpertsPlan experts_plan(const int tokens, const int top_k, const int experts, size_t at)
 {
+    const int slots = tokens * top_k;
     ExpertsPlan p{};
     p.bytes = at;
     if (slots == 0 || experts == 0 || experts > EXPERTS_SORTED) return p;
     const int mean = slots / experts;
-    p.rows = mean >= 256 ? 256 : mean >= 96 ? 128 : mean >= 24 ? 64 : 32;
+    p.rows = mean >= 256 ? 256 : mean >= 96 ? 128 : mean >= 24 ? 64 : mean >= 16 ? 32 : mean >= 6 ? 16 : slots >= 2 * experts ? 8 : tokens > 2 ? 4 : 2;
     p.tiles = slots / p.rows + std::min(experts + 1, slots);
     p.order = at;
     p.list = p.order + up256((size_t)slots * 4);
@@ -55,70 +51,19 @@ static ExpertsArgs args_of(const qm_expert_weights *w, const void *x, const long
                            const ExpertsPlan &plan, const char *at)
 {
     return {static_cast<const uint16_t *>(x), x_token, x_choice, chosen, static_cast<const uint8_t *>(w->weight), w->scale, static_cast<const uint16_t *>(w->bias), out,
-            tokens * top_k, top_k, w->experts, w->n, w->k, w->group, (int)(((long long)w->k + w->group - 1) / w->group), w->k / 32, reinterpret_cast<const int *>(at + plan.order),
+            tokens * top_k, top_k, w->experts, w->n, w->k, w->group, (int)(((long long)w->k + w->group - 1) / w->group), w->k / 32, w->group == 32 ? 0u : (uint32_t)(((1ull << 32) + w->group / 32 - 1) / (w->group / 32)), ((1ull << 32) + top_k - 1) / top_k, reinterpret_cast<const int *>(at + plan.order),
             reinterpret_cast<const int *>(at + plan.list), reinterpret_cast<const int *>(at + plan.count)};
 }
 
-template <int T, int S, ExpertsOut OUT>
-static hipError_t launch_any(const ExpertsArgs &p, hipStream_t s)
+// Whether x's rows can be loaded sixteen aligned bytes at a time, at 32-bit offsets.
+static bool aligned_rows(const ExpertsArgs &p)
 {
-    const int columns = OUT == EXPERTS_GATED ? p.N / 2 : p.N;
-    return enqueue(&experts_any_kernel<T, S, OUT>, dim3(std::min(columns / 4 + 1, 1 << 20), std::min(p.slots, 65535)), dim3(256), 0, s, p);
-}
-template <int T, int S, int MODE, ExpertsOut OUT>
-static hipError_t launch_tiles(const ExpertsArgs &p, const ExpertsPlan &plan, hipStream_t s)
-{
-    // (with a scale to every one or two blocks the registers of 64 columns to a wave do not fit)
-    constexpr int NT = MODE == 1 ? 4 : 2;
-    const int columns = OUT == EXPERTS_GATED ? p.N / 2 : p.N;
-    const auto wide = [&](auto wm, auto wn, auto mt, auto nt) {
-        constexpr int WM = decltype(wm)::value, WN = decltype(wn)::value, MT = decltype(mt)::value, N = decltype(nt)::value, BM = 16 * WM * MT, BN = 16 * WN * N, OF = OUT == EXPERTS_GATED ? BN / 2 : BN;
-        static std::atomic<bool> known[QM_MAX_DEVICES] = {};
-        const auto kernel = [] {
-            if constexpr (OUT == EXPERTS_PLAIN) return &gemm_grouped_wide_kernel<T, S, MODE, WM, WN, MT, N, ExpertsArgs, ExpertsPlainTile>;
-            else if constexpr (OUT == EXPERTS_GATED) return &gemm_grouped_wide_kernel<T, S, MODE, WM, WN, MT, N, ExpertsArgs, ExpertsGatedTile>;
-            else return &gemm_grouped_wide_kernel<T, S, MODE, WM, WN, MT, N, ExpertsArgs, ExpertsPartTile>;
-        }();
-        constexpr int lds = 2 * 8 * 16 * (BM + BN) + 2 * 2 * BN * (int)sizeof(float);
-        if (const hipError_t e = ensure_dynamic_lds(kernel, lds, known); e != hipSuccess) return e;
-        return enqueue(kernel, dim3(plan.tiles, (columns + OF - 1) / OF), dim3(64 * WM * WN), lds, s, p);
-    };
-    const std::integral_constant<int, 1> one{};
-    const std::integral_constant<int, 2> two{};
-    const std::integral_constant<int, 4> four{};
-    const std::integral_constant<int, NT> nt{};
-    switch (plan.rows) {
-    case 256: return wide(four, two, four, nt);
-    case 128: return wide(two, two, four, nt);
-    case 64: return wide(one, four, four, two);
-    default: return wide(one, four, two, two);
-    }
+    const long long last = (p.slots / p.top_k - 1) * p.x_token + (p.top_k - 1) * p.x_choice + p.K;
+    return ((uintptr_t)p.x & 15) == 0 && p.x_token % 8 == 0 && p.x_choice % 8 == 0 && last < 1ll << 31 && (long long)p.slots * p.top_k < 1ll << 32;
 }
 static hipError_t launch_product(const ExpertsArgs &p, const bool tiled, const ExpertsPlan &plan, const int dtype, const int scale_dtype, const ExpertsOut out, hipStream_t s)
 {
-    const auto by_out = [&](auto t, auto st, auto o) {
-        constexpr int T = decltype(t)::value, S = decltype(st)::value;
-        constexpr ExpertsOut OUT = (ExpertsOut)decltype(o)::value;
-        if (!tiled) return launch_any<T, S, OUT>(p, s);
-        switch (group_mode(p.group)) {
-        case 1: return launch_tiles<T, S, 1, OUT>(p, plan, s);
-        case 2: return launch_tiles<T, S, 2, OUT>(p, plan, s);
-        case 4: return launch_tiles<T, S, 4, OUT>(p, plan, s);
-        default: return launch_tiles<T, S, 0, OUT>(p, plan, s);
-        }
-    };
-    const auto by_type = [&](auto t, auto st) {
-        switch (out) {
-        case EXPERTS_PLAIN: return by_out(t, st, std::integral_constant<int, EXPERTS_PLAIN>{});
-        case EXPERTS_GATED: return by_out(t, st, std::integral_constant<int, EXPERTS_GATED>{});
-        default: return by_out(t, st, std::integral_constant<int, EXPERTS_PART>{});
-        }
-    };
-    const std::integral_constant<int, QM_IN_F16> f16{};
-    const std::integral_constant<int, QM_IN_BF16> bf16{};
-    const std::integral_constant<int, QM_IN_F32> f32{};
-    if (dtype == QM_IN_F16) return scale_dtype == QM_IN_F32 ? by_type(f16, f32) : by_type(f16, f16);
-    return scale_dtype == QM_IN_F32 ? by_type(bf16, f32) : by_type(bf16, bf16);
+    return (dtype == QM_IN_F16 ? launch_experts_f16 : launch_experts_bf16)(p, plan, scale_dtype, out, tiled, aligned_rows(p), s);
 }
 
 // The workspace of the gated MLP: the gated products and the outputs of the experts in front of the lists.
@@ -130,7 +75,7 @@ static MlpPlan mlp_plan(const int tokens, const int top_k, const int experts, co
 {
     MlpPlan p{};
     p.part = up256((size_t)tokens * top_k * inner * 2);
-    p.sorted = experts_plan(tokens * top_k, experts, p.part + up256((size_t)tokens * top_k * hidden * 4));
+    p.sorted = experts_plan(tokens, top_k, experts, p.part + up256((size_t)tokens * top_k * hidden * 4));
     return p;
 }
 
@@ -185,7 +130,7 @@ static int check_choices(const int tokens, const int top_k, const int dtype)
 QM_EXPORT size_t qm_gemm_experts_workspace_bytes(const qm_expert_weights *weights, int tokens, int top_k)
 {
     if (check_weights(weights, weights ? weights->scale_dtype : 0) != QM_OK || check_choices(tokens, top_k, QM_IN_F16) != QM_OK) return 0;
-    return experts_plan(tokens * top_k, weights->experts, 0).bytes;
+    return experts_plan(tokens, top_k, weights->experts, 0).bytes;
 }
 
 QM_EXPORT int qm_gemm_experts_i4(const void *x, int dtype, long long token_stride, long long choice_stride, const int *chosen, const qm_expert_weights *weights, void *y,
@@ -197,7 +142,7 @@ QM_EXPORT int qm_gemm_experts_i4(const void *x, int dtype, long long token_strid
     if (tokens == 0 || top_k == 0 || weights->n == 0) return QM_OK;
     if (!chosen || !y || (!x && weights->k > 0)) return QM_ERR_NULL;
     if ((((uintptr_t)x | (uintptr_t)y) & 1) || ((uintptr_t)chosen & 3) || ((uintptr_t)workspace & 15)) return QM_ERR_ALIGN;
-    const ExpertsPlan plan = experts_plan(tokens * top_k, weights->experts, 0);
+    const ExpertsPlan plan = experts_plan(tokens, top_k, weights->experts, 0);
     if (plan.bytes > 0 && (!workspace || workspace_bytes < plan.bytes)) return QM_ERR_SCRATCH;
     char *const at = static_cast<char *>(workspace);
     const hipStream_t s = reinterpret_cast<hipStream_t>(stream);

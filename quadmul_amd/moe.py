@@ -90,6 +90,14 @@ def _activations(what, x, chosen, dims):
         raise QuadmulError(f"{what}: tokens times top_k must fit in int32")
 
 
+def _aligned(x):
+    """Rows that the kernels for few rows to an expert can load, sixteen aligned bytes at a time; others are copied."""
+    apart = x.data_ptr() % 16 != 0 or any(n > 1 and by % 8 for n, by in zip(x.shape[:-1], x.stride()[:-1]))
+    if (x.shape[-1] > 1 and x.stride(-1) != 1) or (apart and x.shape[-1] % 32 == 0):
+        return x.clone(memory_format=torch.contiguous_format)
+    return x
+
+
 def gemm_experts(x: torch.Tensor, chosen: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, group_size: int, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``y[t, j] = x[t] @ weight[e].T + bias[e]`` with ``e = chosen[t, j]``, as :func:`quadmul_amd.gemm_grouped` gives it, ``[tokens, top_k, n]``; zeros where ``e`` is
     no expert.
@@ -105,8 +113,7 @@ def gemm_experts(x: torch.Tensor, chosen: torch.Tensor, weight: torch.Tensor, we
     w = _weights("gemm_experts", x, weight, weight_scale, group_size, bias)
     if w.k != x.shape[-1]:
         raise QuadmulError("gemm_experts: the weights must be [experts, n, k / 2], k x's last dimension")
-    if w.k > 1 and x.stride(-1) != 1:
-        x = x.contiguous()
+    x = _aligned(x)
     tokens, top_k = chosen.shape
     y = torch.empty((tokens, top_k, w.n), dtype=x.dtype, device=x.device)
     need = library().qm_gemm_experts_workspace_bytes(ctypes.byref(w), tokens, top_k)
@@ -134,8 +141,7 @@ def mlp(x: torch.Tensor, chosen: torch.Tensor, weights: torch.Tensor, up: torch.
     tokens, hidden = x.shape
     if not (u.k == d.n == hidden and u.n == 2 * d.k and u.experts == d.experts):
         raise QuadmulError("mlp: up must be [experts, 2 inner, hidden / 2], down [experts, hidden, inner / 2]")
-    if hidden > 1 and x.stride(1) != 1:
-        x = x.contiguous()
+    x = _aligned(x)
     y = torch.empty((tokens, hidden), dtype=x.dtype, device=x.device)
     need = library().qm_moe_mlp_workspace_bytes(ctypes.byref(u), ctypes.byref(d), tokens, chosen.shape[1])
     scratch = torch.empty((need,), dtype=torch.uint8, device=x.device) if need else None
