@@ -44,26 +44,36 @@ static hipError_t sort_slots(const ExpertsPlan &plan, const int *chosen, const i
                    reinterpret_cast<int *>(at + plan.list), reinterpret_cast<int *>(at + plan.count));
 }
 
-// Whether the kernels on the matrix cores take these weights (the others: experts_any_kernel).
-static bool tiles_take(const qm_expert_weights *w) { return w->k > 0 && w->k % 32 == 0 && w->n <= 65535 * 32 && ((uintptr_t)w->weight & 15) == 0 && w->experts > 0 && w->experts <= EXPERTS_SORTED; }
-
 static ExpertsArgs args_of(const qm_expert_weights *w, const void *x, const long long x_token, const long long x_choice, const int *chosen, void *out, const int tokens, const int top_k,
                            const ExpertsPlan &plan, const char *at)
 {
-    return {static_cast<const uint16_t *>(x), x_token, x_choice, chosen, static_cast<const uint8_t *>(w->weight), w->scale, static_cast<const uint16_t *>(w->bias), out,
-            tokens * top_k, top_k, w->experts, w->n, w->k, w->group, (int)(((long long)w->k + w->group - 1) / w->group), w->k / 32, w->group == 32 ? 0u : (uint32_t)(((1ull << 32) + w->group / 32 - 1) / (w->group / 32)), ((1ull << 32) + top_k - 1) / top_k, reinterpret_cast<const int *>(at + plan.order),
-            reinterpret_cast<const int *>(at + plan.list), reinterpret_cast<const int *>(at + plan.count)};
+    ExpertsArgs p{};
+    p.x = static_cast<const uint16_t *>(x), p.x_token = x_token, p.x_choice = x_choice, p.chosen = chosen;
+    p.B = static_cast<const uint8_t *>(w->weight), p.scale = w->scale, p.bias = static_cast<const uint16_t *>(w->bias), p.out = out;
+    p.slots = tokens * top_k, p.top_k = top_k, p.experts = w->experts, p.N = w->n, p.K = w->k, p.group = w->group;
+    p.groups = (int)(((long long)w->k + w->group - 1) / w->group), p.chunk = w->k / 32;
+    p.magic = w->group == 32 ? 0u : (uint32_t)(((1ull << 32) + w->group / 32 - 1) / (w->group / 32));
+    p.top_k_magic = ((1ull << 32) + top_k - 1) / top_k;
+    p.order = reinterpret_cast<const int *>(at + plan.order), p.tiles = reinterpret_cast<const int *>(at + plan.list), p.count = reinterpret_cast<const int *>(at + plan.count);
+    return p;
 }
 
-// Whether x's rows can be loaded sixteen aligned bytes at a time, at 32-bit offsets.
-static bool aligned_rows(const ExpertsArgs &p)
+// Which kernel runs a product. The matrix cores want a K of whole blocks and weights at sixteen bytes; the kernel for few rows, rows of x at sixteen bytes too, offsets of
+// 32 bits from its first one and from an expert's first weight and scale, and block numbers below 2^15 for the division by the size of a group.
+static ExpertsKernel kernel_of(const ExpertsArgs &p, const ExpertsPlan &plan)
 {
+    if (p.K == 0 || p.K % 32 != 0 || ((uintptr_t)p.B & 15) != 0 || plan.rows == 0 || p.N > 65535 * 32) return EXPERTS_ANY;
     const long long last = (p.slots / p.top_k - 1) * p.x_token + (p.top_k - 1) * p.x_choice + p.K;
-    return ((uintptr_t)p.x & 15) == 0 && p.x_token % 8 == 0 && p.x_choice % 8 == 0 && last < 1ll << 31 && (long long)p.slots * p.top_k < 1ll << 32;
+    const bool rows = ((uintptr_t)p.x & 15) == 0 && p.x_token % 8 == 0 && p.x_choice % 8 == 0 && last < 1ll << 31;
+    const bool fits = p.K < 1 << 20 && (unsigned long long)p.N * std::max(p.K / 2, p.groups * 4) < 1ull << 32;
+    return plan.rows <= 16 && rows && fits && (long long)p.slots * p.top_k < 1ll << 32 && (long long)plan.tiles * ((p.N + 15) / 16) < 1ll << 31 ? EXPERTS_ROWS : EXPERTS_TILES;
 }
-static hipError_t launch_product(const ExpertsArgs &p, const bool tiled, const ExpertsPlan &plan, const int dtype, const int scale_dtype, const ExpertsOut out, hipStream_t s)
+// Up to 64 slots the kernel for few rows finds its tiles by itself.
+static bool sorts(const ExpertsKernel kernel, const int slots) { return kernel == EXPERTS_TILES || (kernel == EXPERTS_ROWS && slots > 64); }
+static hipError_t launch_product(ExpertsArgs p, const ExpertsKernel kernel, const ExpertsPlan &plan, const int dtype, const int scale_dtype, const ExpertsOut out, hipStream_t s)
 {
-    return (dtype == QM_IN_F16 ? launch_experts_f16 : launch_experts_bf16)(p, plan, scale_dtype, out, tiled, aligned_rows(p), s);
+    if (!sorts(kernel, p.slots)) p.order = nullptr;
+    return (dtype == QM_IN_F16 ? launch_experts_f16 : launch_experts_bf16)(p, plan, scale_dtype, out, kernel, s);
 }
 
 // The workspace of the gated MLP: the gated products and the outputs of the experts in front of the lists.
@@ -146,9 +156,10 @@ QM_EXPORT int qm_gemm_experts_i4(const void *x, int dtype, long long token_strid
     if (plan.bytes > 0 && (!workspace || workspace_bytes < plan.bytes)) return QM_ERR_SCRATCH;
     char *const at = static_cast<char *>(workspace);
     const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-    const bool tiled = tiles_take(weights);
-    hipError_t e = tiled ? sort_slots(plan, chosen, tokens * top_k, weights->experts, at, s) : hipSuccess;
-    if (e == hipSuccess) e = launch_product(args_of(weights, x, token_stride, choice_stride, chosen, y, tokens, top_k, plan, at), tiled, plan, dtype, weights->scale_dtype, EXPERTS_PLAIN, s);
+    const ExpertsArgs p = args_of(weights, x, token_stride, choice_stride, chosen, y, tokens, top_k, plan, at);
+    const ExpertsKernel kernel = kernel_of(p, plan);
+    hipError_t e = sorts(kernel, p.slots) ? sort_slots(plan, chosen, p.slots, p.experts, at, s) : hipSuccess;
+    if (e == hipSuccess) e = launch_product(p, kernel, plan, dtype, weights->scale_dtype, EXPERTS_PLAIN, s);
     return e == hipSuccess ? QM_OK : fail_launch(e);
 }
 
@@ -180,12 +191,19 @@ QM_EXPORT int qm_moe_mlp_i4(const void *x, int dtype, long long token_stride, co
     const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     hipError_t e = hipSuccess;
     if (top_k > 0) {
-        const bool up_tiled = tiles_take(up), down_tiled = tiles_take(down);
         const ExpertsArgs first = args_of(up, x, token_stride, 0, chosen, at, tokens, top_k, plan.sorted, at);
-        const ExpertsArgs second = args_of(down, at, (long long)top_k * down->k, down->k, chosen, at + plan.part, tokens, top_k, plan.sorted, at);
-        if (up_tiled || down_tiled) e = sort_slots(plan.sorted, chosen, tokens * top_k, up->experts, at, s);
-        if (e == hipSuccess && down->k > 0) e = launch_product(first, up_tiled, plan.sorted, dtype, up->scale_dtype, EXPERTS_GATED, s);
-        if (e == hipSuccess) e = launch_product(second, down_tiled, plan.sorted, dtype, down->scale_dtype, EXPERTS_PART, s);
+        ExpertsArgs second = args_of(down, at, (long long)top_k * down->k, down->k, chosen, at + plan.part, tokens, top_k, plan.sorted, at);
+        const ExpertsKernel one = kernel_of(first, plan.sorted), two = kernel_of(second, plan.sorted);
+        // A token's choices one after the other, added up on the way, where hardly any expert has two tokens (whose weights would be read twice).
+        const bool apart = two == EXPERTS_ROWS && (tokens == 1 || (first.slots <= 64 && first.slots * 4 <= up->experts));
+        if (sorts(one, first.slots) || (!apart && sorts(two, first.slots))) e = sort_slots(plan.sorted, chosen, first.slots, up->experts, at, s);
+        if (e == hipSuccess && down->k > 0) e = launch_product(first, one, plan.sorted, dtype, up->scale_dtype, EXPERTS_GATED, s);
+        if (apart) {
+            second.out = y, second.shares = weights;
+            if (e == hipSuccess) e = launch_product(second, two, plan.sorted, dtype, down->scale_dtype, EXPERTS_SUM, s);
+            return e == hipSuccess ? QM_OK : fail_launch(e);
+        }
+        if (e == hipSuccess) e = launch_product(second, two, plan.sorted, dtype, down->scale_dtype, EXPERTS_PART, s);
     }
     if (e == hipSuccess) {
         const unsigned grid = (unsigned)std::min<size_t>(((size_t)tokens * down->n + 255) / 256, 1 << 20);

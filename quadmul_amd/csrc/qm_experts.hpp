@@ -8,8 +8,8 @@ namespace qm {
 constexpr int EXPERTS_SORTED = 4096;  // experts at most that the slots are sorted by
 
 // What becomes of a slot's products: rounded, with the bias (and zeros where the expert is none of these); the first half of the columns as gates of
-// the second, rounded; as they are, to be added up by weight.
-enum ExpertsOut { EXPERTS_PLAIN, EXPERTS_GATED, EXPERTS_PART };
+// the second, rounded; as they are, to be added up by weight; a token's added up by weight, rounded.
+enum ExpertsOut { EXPERTS_PLAIN, EXPERTS_GATED, EXPERTS_PART, EXPERTS_SUM };
 
 struct ExpertsArgs {
     const uint16_t *x;
@@ -18,12 +18,13 @@ struct ExpertsArgs {
     const uint8_t *B;             // [experts, N, K/2]
     const void *scale;            // [experts, N, groups]
     const uint16_t *bias;         // [experts, N] or null
-    void *out;                    // [slots, N], [slots, N/2] 16-bit, or [slots, N] float
+    void *out;                    // [slots, N], [slots, N/2] 16-bit, [slots, N] float, or [tokens, N] 16-bit
+    const float *shares;          // EXPERTS_SUM: [slots], the weights of the choices
     int slots, top_k, experts, N, K, group, groups;
     int chunk;                // blocks of 32 of K
     uint32_t magic;           // 2^32 / (blocks of a group), rounded up: block * magic >> 32 is the block's group, for a K up to 2^20; 0 for one block
     unsigned long long top_k_magic;  // 2^32 / top_k, rounded up, for less than 2^32 / top_k slots
-    // The slots sorted by expert, cut into tiles of rows: their expert, where they begin in `order` and how many they are. After
+    // (null where there are no more than 64 slots, and experts_rows_kernel finds its tiles by itself:) the slots sorted by expert, cut into tiles of rows: their expert, where they begin in `order` and how many they are. After
     // those of the last expert, as number `experts`, slots that have none.
     const int *order, *tiles, *count;  // [slots], [tiles][4]; how many tiles, how many of them of an expert, where the slots without one begin in `order`
 };
@@ -33,9 +34,11 @@ struct ExpertsPlan {
     int tiles;  // at most
     size_t order, list, count, bytes;
 };
-// qm_experts_inst.hip, by the type of x; `few`: x's rows can be loaded sixteen aligned bytes at a time.
-hipError_t launch_experts_f16(const ExpertsArgs &p, const ExpertsPlan &plan, int scale_dtype, ExpertsOut out, bool tiled, bool few, hipStream_t s);
-hipError_t launch_experts_bf16(const ExpertsArgs &p, const ExpertsPlan &plan, int scale_dtype, ExpertsOut out, bool tiled, bool few, hipStream_t s);
+// The kernel for a product: that for any address, the tiles, or that for few rows.
+enum ExpertsKernel { EXPERTS_ANY, EXPERTS_TILES, EXPERTS_ROWS };
+// qm_experts_inst.hip, by the type of x.
+hipError_t launch_experts_f16(const ExpertsArgs &p, const ExpertsPlan &plan, int scale_dtype, ExpertsOut out, ExpertsKernel kernel, hipStream_t s);
+hipError_t launch_experts_bf16(const ExpertsArgs &p, const ExpertsPlan &plan, int scale_dtype, ExpertsOut out, ExpertsKernel kernel, hipStream_t s);
 
 __device__ __forceinline__ const uint16_t *row_of(const ExpertsArgs &p, const int slot)
 {
@@ -102,41 +105,86 @@ using ExpertsPartTile = ExpertsTile<T, BM, BN, EXPERTS_PART>;
 // waves of a CU have 80 to 130 KB on the way (two runs of fewer waves were slower: their registers and their LDS cost more waves than that). The waves' sums meet in the LDS, one barrier an item. In the
 // LDS the 16 bytes of a line, or of a row of x, are turned round by the number of the line or row, so that no read of sixteen lanes meets a bank twice.
 //
-// WHOLE: 128 of K have one scale, so a matrix instruction may take its 32 of K from anywhere in them: a lane's sixteen bytes of a column, read as they
-// are, are its dwords for four instructions. Else every 32 of K go into sums of their own, and a lane reads its dword of each.
-template <bool WHOLE, int R, int NW, ExpertsOut OUT>
+// G: 32 G of K have one scale (G 4, 2 or 1), so a matrix instruction may take its 32 of K from anywhere in them: a lane's 4 G bytes of a column, read as they
+// are, are its dwords for G instructions into the same sums.
+template <int G, int R, int C, int NW, ExpertsOut OUT>
 struct ExpertsRowsShape {
-    static constexpr int C = 2, QUARTERS = (R + 3) / 4;                           // tiles of columns; of 16 rows that have sums
-    static constexpr int WEIGHTS = C * 2048, X = R * 512, SCALES = WHOLE ? 1 : 4;  // bytes of a run; instructions
-    static constexpr int BIAS = OUT == EXPERTS_PLAIN ? 1 : 0;
-    static constexpr int STAGE = WEIGHTS + X + (SCALES + BIAS) * 256;
+    static constexpr int QUARTERS = (R + 3) / 4;                                   // of 16 rows that have sums
+    static constexpr int GROUPS = 8 / G, SCALES = GROUPS * C > 4 ? GROUPS * C / 4 : 1;  // of a run: scales of a column, instructions that load them
+    static constexpr int WEIGHTS = C * 2048, X = R * 512, BIAS = OUT == EXPERTS_PLAIN ? 1 : 0;
+    static constexpr int STAGE = WEIGHTS + X + (SCALES + BIAS) * 256;               // bytes of a run
     static constexpr int RING = NW * STAGE, SUMS = NW * C * QUARTERS * 256, BYTES = RING + 2 * SUMS;
-    static constexpr int COLUMNS = OUT == EXPERTS_GATED ? 16 : 32;                  // of the output
-    static constexpr int WAVES = NW > 4 || !WHOLE || R > 8 ? 4 : 5;                 // to a SIMD, by the registers
+    static constexpr int COLUMNS = OUT == EXPERTS_GATED ? C * 8 : C * 16;           // of the output
+    static constexpr int WAVES = NW == 16 ? 4 : G == 1 ? (R > 8 ? 3 : 4) : R > 2 * G ? 4 : 5;  // to a SIMD, by the registers
     static constexpr int PER_CU = 163840 / BYTES < WAVES * 4 / NW ? 163840 / BYTES : WAVES * 4 / NW;  // workgroups, by the LDS too
 };
-template <int T, int S, bool WHOLE, int R, int NW, ExpertsOut OUT>
-__global__ __launch_bounds__(64 * NW, (ExpertsRowsShape<WHOLE, R, NW, OUT>::WAVES)) void experts_rows_kernel(const ExpertsArgs p)
+template <int T, int S, int G, int R, int C, int NW, ExpertsOut OUT>
+__global__ __launch_bounds__(64 * NW, (ExpertsRowsShape<G, R, C, NW, OUT>::WAVES)) void experts_rows_kernel(const ExpertsArgs p)
 {
     typedef GroupedWeights<T> W;
     typedef typename W::frag frag;
-    typedef ExpertsRowsShape<WHOLE, R, NW, OUT> Shape;
-    constexpr bool PAIRS = OUT == EXPERTS_GATED;
-    constexpr int C = Shape::C, COLUMNS = Shape::COLUMNS, SB = S == QM_IN_F32 ? 4 : 2;
+    typedef ExpertsRowsShape<G, R, C, NW, OUT> Shape;
+    constexpr bool PAIRS = OUT == EXPERTS_GATED, SUM = OUT == EXPERTS_SUM;
+    constexpr int COLUMNS = Shape::COLUMNS, SB = S == QM_IN_F32 ? 4 : 2;
     extern __shared__ __align__(16) uint8_t smem[];
     v4f *const sums = reinterpret_cast<v4f *>(smem + Shape::RING);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 15, c = lane >> 4;
     const int columns = PAIRS ? p.N / 2 : p.N, across = (columns + COLUMNS - 1) / COLUMNS, line = p.K / 2, runs = (line + 127) / 128;
 
+    // ---- the tiles: of the lists, or, of up to 64 slots, from their experts, a slot to a lane; a token each, with its choices one after the other in K ----
+    const bool listed = SUM || p.order != nullptr;
+    const int chosen = listed ? 0 : p.chosen[min(lane, p.slots - 1)];
+    const uint64_t valid = __ballot(!listed && lane < p.slots && (unsigned)chosen < (unsigned)p.experts);
+    // the slots of tile t, and how many tiles there are in front of it or in all
+    const auto find = [&](int t, int &expert, uint64_t &of) {
+        int before = 0;
+        of = 0;
+        for (uint64_t left = valid; left != 0;) {
+            expert = __builtin_amdgcn_readlane(chosen, __builtin_ctzll(left));
+            uint64_t same = __ballot(chosen == expert) & valid;
+            left &= ~same;
+            const int more = (__builtin_popcountll(same) + R - 1) / R;
+            if (t < before + more) {
+                for (int i = (t - before) * R; i > 0; --i) same &= same - 1;
+                of = same;
+                break;
+            }
+            before += more;
+        }
+        return before;
+    };
+    // its expert, how many rows it has and their slots (past the last one: that again)
+    const auto get_tile = [&](const int t, int &expert, int &rows, int (&slot)[R]) {
+        if (p.order != nullptr) {
+            const scalar_ints tile = scalars(p.tiles + 4 * (size_t)t);
+            const int first = tile[1];
+            expert = tile[0], rows = tile[2];
+#pragma unroll
+            for (int i = 0; i < R; ++i) slot[i] = scalars(p.order)[first + min(i, rows - 1)];
+        } else {
+            uint64_t of;
+            find(t, expert, of);
+            rows = min((int)__builtin_popcountll(of), R);
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                slot[i] = __builtin_ctzll(of);
+                if ((of & (of - 1)) != 0) of &= of - 1;
+            }
+        }
+    };
+    int none;
+    uint64_t nobody;
+    const int tiles = SUM ? p.slots / p.top_k : listed ? scalars(p.count)[1] : find(INT32_MAX, none, nobody), choices = SUM ? p.top_k : 1;
+
     // ---- this workgroup's items: an equal share of tiles times columns, side by side ----
-    const int tiles = scalars(p.count)[1], all = tiles * across, each = all / (int)gridDim.x, rest = all - each * (int)gridDim.x, me = blockIdx.x;
+    const int all = tiles * across, each = all / (int)gridDim.x, rest = all - each * (int)gridDim.x, me = blockIdx.x;
     const int item0 = each * me + min(me, rest), item1 = item0 + each + (me < rest ? 1 : 0);
 
     // ---- the loading side: where a lane loads from, eight lanes to a line of a column, 32 to a row of x, 32 to the scales of a quad or block ----
     const int line_column = lane >> 3;
     uint32_t w_at[C][2], s_at, b_at, x_at[R / 2];
     const uint8_t *weights, *scales;
-    int load_tile = item0 / max(across, 1), load_block = item0 - load_tile * across, load_left = item1 - item0, load_run = wave;
+    int load_tile = item0 / across, load_block = item0 - load_tile * across, load_left = item1 - item0, load_run = 0, load_choice = 0, load_expert = 0;
     const auto load_columns = [&] {
         const int n0 = load_block * COLUMNS, last = columns - 1;
         // the row of the weights of column i of tile t
@@ -145,28 +193,32 @@ __global__ __launch_bounds__(64 * NW, (ExpertsRowsShape<WHOLE, R, NW, OUT>::WAVE
         for (int t = 0; t < C; ++t)
 #pragma unroll
             for (int h = 0; h < 2; ++h) w_at[t][h] = (uint32_t)row(t, 8 * h + line_column) * (uint32_t)line;
-        const uint32_t mine = (uint32_t)((lane & 16) ? row(1, r) : row(0, r));
+        const uint32_t mine = (uint32_t)(C == 2 && (lane & 16) ? row(1, r) : row(0, r));
         s_at = mine * (uint32_t)(p.groups * SB);
         b_at = mine * 2;
     };
     const auto load_rows = [&] {
-        const scalar_ints tile = scalars(p.tiles + 4 * (size_t)load_tile);
-        const int expert = tile[0], first = tile[1], rows = tile[2];
-        weights = p.B + (size_t)expert * p.N * line;
-        scales = static_cast<const uint8_t *>(p.scale) + (size_t)expert * p.N * (p.groups * SB);
+        int slot[R], rows = 1;
+        if constexpr (SUM) {
+#pragma unroll
+            for (int i = 0; i < R; ++i) slot[i] = load_tile * p.top_k + load_choice;
+            load_expert = scalars(p.chosen)[slot[0]];
+            if ((unsigned)load_expert >= (unsigned)p.experts) load_expert = 0;  // (loaded all the same, and not used)
+        } else {
+            get_tile(load_tile, load_expert, rows, slot);
+        }
+        weights = p.B + (size_t)load_expert * p.N * line;
+        scales = static_cast<const uint8_t *>(p.scale) + (size_t)load_expert * p.N * (p.groups * SB);
         uint32_t at[R];
 #pragma unroll
         for (int i = 0; i < R; ++i) {
-            const uint32_t slot = (uint32_t)scalars(p.order)[first + min(i, rows - 1)], t = (uint32_t)(slot * p.top_k_magic >> 32);
-            at[i] = (t * (uint32_t)p.x_token + (slot - t * (uint32_t)p.top_k) * (uint32_t)p.x_choice) * 2;
+            const uint32_t t = (uint32_t)((uint32_t)slot[i] * p.top_k_magic >> 32);
+            at[i] = (t * (uint32_t)p.x_token + ((uint32_t)slot[i] - t * (uint32_t)p.top_k) * (uint32_t)p.x_choice) * 2;
         }
 #pragma unroll
         for (int j = 0; j < R / 2; ++j) x_at[j] = at[2 * j] ^ ((at[2 * j] ^ at[2 * j + 1]) & (lane & 32 ? ~0u : 0u));
-        load_columns();
-        return expert;
     };
     const uint32_t ring = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)smem + wave * Shape::STAGE);
-    int load_expert = 0;
     const auto load_stage = [&]() __attribute__((always_inline)) {
         const uint32_t to = ring;
 #pragma unroll
@@ -183,8 +235,8 @@ __global__ __launch_bounds__(64 * NW, (ExpertsRowsShape<WHOLE, R, NW, OUT>::WAVE
         }
 #pragma unroll
         for (int j = 0; j < Shape::SCALES; ++j) {
-            // quad lane / 32 of the run, or block 2 j + lane / 32
-            const uint32_t block = (uint32_t)load_run * 8 + (WHOLE ? 4 : 1) * (lane >> 5) + 2 * j, group = p.magic == 0 ? block : __umulhi(block, p.magic);
+            // group number `sub` of the run
+            const uint32_t sub = (lane / (16 * C) + j * (4 / C)) % Shape::GROUPS, block = (uint32_t)load_run * 8 + sub * G, group = p.magic == 0 ? block : __umulhi(block, p.magic);
             const uint32_t from = s_at + min(group, (uint32_t)p.groups - 1) * SB;
             if constexpr (SB == 4) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(to + Shape::WEIGHTS + Shape::X + j * 256), "v"(from), "s"(scales) : "memory", "m0");
             else asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_ushort %1, %2" ::"s"(to + Shape::WEIGHTS + Shape::X + j * 256), "v"(from), "s"(scales) : "memory", "m0");
@@ -196,51 +248,64 @@ __global__ __launch_bounds__(64 * NW, (ExpertsRowsShape<WHOLE, R, NW, OUT>::WAVE
             asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_ushort %1, %2" ::"s"(to + Shape::WEIGHTS + Shape::X + Shape::SCALES * 256), "v"(at), "s"(from) : "memory", "m0");
         }
     };
-    // to this wave's next run
-    const auto advance = [&] {
-        load_run += NW;
+    // to this wave's next run: `by` further on
+    const auto advance = [&](const int by) {
+        load_run += by;
         if (load_run < runs) return;
-        load_run = wave;
-        if (--load_left == 0) return;
-        if (++load_block == across) {
-            load_block = 0, ++load_tile;
-            load_expert = load_rows();
-        } else {
+        while (load_run >= runs) load_run -= runs, ++load_choice;
+        if (load_choice >= choices) {
+            if (--load_left == 0) return;
+            load_run = wave, load_choice = 0;
+            while (load_run >= runs) load_run -= runs, ++load_choice;
+            if (++load_block == across) load_block = 0, ++load_tile;
+            if (SUM || load_block == 0) load_rows();
             load_columns();
+        } else {
+            load_rows();
         }
     };
-    const bool works = wave < runs;
+    const bool works = wave < runs * choices;
     if (item0 < item1 && works) {
-        load_expert = load_rows();
-        load_stage(), advance();
+        load_run = wave;
+        while (load_run >= runs) load_run -= runs, ++load_choice;
+        load_rows(), load_columns();
+        load_stage(), advance(NW);
     }
 
     // ---- the multiplying side ----
     // (numbers of pieces come into an address by exclusive or: its bits for them are those of the turn)
     const int x_row = min(r, R - 1);
-    const uint32_t w_from = (r >> 3) * 1024 + (r & 7) * 128 + (((r >> 1) & 7) ^ (WHOLE ? c : 0)) * 16 + (WHOLE ? 0 : 4 * c);
-    const uint32_t x_from = Shape::WEIGHTS + x_row * 512 + (x_row ^ (WHOLE ? 4 * c : c)) * 16;
-    int tile = item0 / max(across, 1), block0 = item0 - tile * across, parity = 0;
-    int rows = 0, my_slot[(R * COLUMNS + 64 * NW - 1) / (64 * NW)];
+    const uint32_t w_from = (r >> 3) * 1024 + (r & 7) * 128 + (((r >> 1) & 7) ^ (c * G / 4)) * 16 + c * G % 4 * 4;
+    const uint32_t x_from = Shape::WEIGHTS + x_row * 512 + (x_row ^ (c * G)) * 16;
+    int tile = item0 / across, block0 = item0 - tile * across, parity = 0, rows = 1;
+    size_t to[(R * COLUMNS + 64 * NW - 1) / (64 * NW)];  // where in the output the rows are whose sums a thread puts together
     for (int item = item0; item < item1; ++item) {
         if (item == item0 || block0 == across) {
             if (block0 == across) block0 = 0, ++tile;
-            const scalar_ints of = scalars(p.tiles + 4 * (size_t)tile);
-            const int first = of[1];
-            rows = of[2];
-            // the slot of the row whose sums a thread puts together
+            int expert, slot[R];
+            if constexpr (!SUM) get_tile(tile, expert, rows, slot);
 #pragma unroll
-            for (int i = 0; i < (int)(sizeof(my_slot) / sizeof(int)); ++i) {
+            for (int i = 0; i < (int)(sizeof(to) / sizeof(size_t)); ++i) {
                 const int m = ((tid + i * 64 * NW) >> 4) % R;
+                int mine = tile;
+                if constexpr (!SUM) {
 #pragma unroll
-                for (int row = 0; row < R; ++row) {
-                    const int slot = scalars(p.order)[first + min(row, rows - 1)];
-                    my_slot[i] = m == row ? slot : my_slot[i];
+                    for (int row = 0; row < R; ++row) mine = m == row ? slot[row] : mine;
                 }
+                to[i] = (size_t)mine * columns;
             }
         }
         v4f total[C] = {};
-        for (int run = wave; run < runs; run += NW) {
+        for (int run = wave, choice = 0; works; run += NW) {
+            while (run >= runs) run -= runs, ++choice;
+            if (choice >= choices) break;
+            float share = 1.0f;
+            bool counts = true;
+            if constexpr (SUM) {
+                const int slot = tile * p.top_k + choice;
+                counts = (unsigned)scalars(p.chosen)[slot] < (unsigned)p.experts;
+                share = __builtin_bit_cast(float, (int)scalars(reinterpret_cast<const int *>(p.shares))[slot]);
+            }
             const uint8_t *const at = smem + wave * Shape::STAGE;
             uint32_t w_here = w_from, x_here = x_from;
             asm("" : "+v"(w_here), "+v"(x_here));  // (sixteen addresses that do not change would take as many registers)
@@ -257,58 +322,54 @@ __global__ __launch_bounds__(64 * NW, (ExpertsRowsShape<WHOLE, R, NW, OUT>::WAVE
             // 128 of K at a time (all 256 would not leave registers for five waves)
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
+                __builtin_amdgcn_sched_barrier(0);
                 v4i x[4];
-                uint32_t w[C][4], scale[C][WHOLE ? 1 : 4];
+                uint32_t w[C][4], scale[C][4 / G];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const v4i *>(at + (x_here ^ (WHOLE ? i : 4 * i) * 16) + q * 256);
+                for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const v4i *>(at + (x_here ^ (i / G * 4 * G + i % G) * 16) + q * 256);
 #pragma unroll
                 for (int t = 0; t < C; ++t) {
-                    if constexpr (WHOLE) {
-                        const v4i whole = *reinterpret_cast<const v4i *>(at + (w_here ^ q * 64) + t * 2048);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) w[t][i] = (uint32_t)whole[i];
-                    } else {
+                    for (int g = 0; g < 4 / G; ++g) {
+                        typedef uint32_t Words __attribute__((ext_vector_type(G)));
+                        const Words some = *reinterpret_cast<const Words *>(at + (w_here ^ (4 * q + g * G) * 16) + t * 2048);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) w[t][i] = *reinterpret_cast<const uint32_t *>(at + (w_here ^ (4 * q + i) * 16) + t * 2048);
+                        for (int i = 0; i < G; ++i) w[t][g * G + i] = some[i];
+                        scale[t][g] = *reinterpret_cast<const uint32_t *>(at + Shape::WEIGHTS + Shape::X + ((q * (4 / G) + g) * 16 * C + t * 16 + r) * 4);
                     }
-#pragma unroll
-                    for (int i = 0; i < (WHOLE ? 1 : 4); ++i) scale[t][i] = *reinterpret_cast<const uint32_t *>(at + Shape::WEIGHTS + Shape::X + ((WHOLE ? q : 4 * q + i) * 32 + t * 16 + r) * 4);
                 }
                 // (a 16-bit one is in the lower half of its dword)
-                const auto scale_of = [&](const int t, const int i) { return S == QM_IN_F32 ? __builtin_bit_cast(float, scale[t][i]) : float_of<S == QM_IN_F32 ? QM_IN_F16 : S>((uint16_t)scale[t][i]); };
+                const auto scale_of = [&](const int t, const int i) {
+                    const float own = S == QM_IN_F32 ? __builtin_bit_cast(float, scale[t][i]) : float_of<S == QM_IN_F32 ? QM_IN_F16 : S>((uint16_t)scale[t][i]);
+                    return SUM ? own * share : own;
+                };
                 if (q == 1) {
                     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (all of the run is in registers: its place is free)
-                    if (load_left > 0) load_stage(), advance();
+                    if (load_left > 0) load_stage(), advance(NW);
                 }
+                if (!counts) continue;
                 const int block = run * 8 + q * 4;  // of 32 of K
                 if ((block + 4) * 32 > p.K) {
                     // past the end of K: zeros, which whatever weights and scales meet
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) x[i] = (block + (WHOLE ? c : i)) * 32 < p.K ? x[i] : v4i{};
+                    for (int i = 0; i < 4; ++i) x[i] = block * 32 + (i / G * 4 * G + c * G + i % G) * 8 < p.K ? x[i] : v4i{};
                 }
                 frag xs[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) xs[i] = __builtin_bit_cast(frag, paired(x[i]));
-                if constexpr (WHOLE) {
+#pragma unroll
+                for (int g = 0; g < 4 / G; ++g) {
                     v4f start = {}, part[C];
                     if constexpr (W::OFFSET) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) start = W::mfma(xs[i], W::offset(), start);
+                        for (int i = 0; i < G; ++i) start = W::mfma(xs[g * G + i], W::offset(), start);
                     }
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
+                    for (int i = 0; i < G; ++i)
 #pragma unroll
-                        for (int t = 0; t < C; ++t) part[t] = W::mfma(xs[i], W::of(w[t][i]), i == 0 ? start : part[t]);
+                        for (int t = 0; t < C; ++t) part[t] = W::mfma(xs[g * G + i], W::of(w[t][g * G + i]), i == 0 ? start : part[t]);
 #pragma unroll
-                    for (int t = 0; t < C; ++t) total[t] += part[t] * scale_of(t, 0);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        v4f start = {};
-                        if constexpr (W::OFFSET) start = W::mfma(xs[i], W::offset(), start);
-#pragma unroll
-                        for (int t = 0; t < C; ++t) total[t] += W::mfma(xs[i], W::of(w[t][i]), start) * scale_of(t, i);
-                    }
+                    for (int t = 0; t < C; ++t) total[t] += part[t] * scale_of(t, g);
                 }
             }
         }
@@ -321,7 +382,7 @@ __global__ __launch_bounds__(64 * NW, (ExpertsRowsShape<WHOLE, R, NW, OUT>::WAVE
             if (c < Shape::QUARTERS) here[(wave * C + t) * (Shape::QUARTERS * 16) + lane] = total[t];
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
-        for (int i = 0; i < (int)(sizeof(my_slot) / sizeof(int)); ++i) {
+        for (int i = 0; i < (int)(sizeof(to) / sizeof(size_t)); ++i) {
             const int at = tid + i * 64 * NW, column = at & 15, m = (at >> 4) % R, t = (at >> 4) / R, n = block0 * COLUMNS + t * 16 + column;
             const auto sum = [&](const int of) {
                 float v = 0.0f;
@@ -330,20 +391,21 @@ __global__ __launch_bounds__(64 * NW, (ExpertsRowsShape<WHOLE, R, NW, OUT>::WAVE
                 return v;
             };
             if (at >= R * COLUMNS || m >= rows || n >= columns) continue;
-            const size_t to = (size_t)my_slot[i] * columns + n;
-            if constexpr (OUT == EXPERTS_PART) static_cast<float *>(p.out)[to] = sum(t);
-            else if constexpr (OUT == EXPERTS_GATED) static_cast<uint16_t *>(p.out)[to] = round16<T>(gated(sum(0), sum(1)));
-            else static_cast<uint16_t *>(p.out)[to] = round16<T>(sum(t));
+            if constexpr (OUT == EXPERTS_PART) static_cast<float *>(p.out)[to[i] + n] = sum(t);
+            else if constexpr (OUT == EXPERTS_GATED) static_cast<uint16_t *>(p.out)[to[i] + n] = round16<T>(gated(sum(0), sum(1)));
+            else static_cast<uint16_t *>(p.out)[to[i] + n] = round16<T>(sum(t));
         }
         ++block0;
     }
 
     if constexpr (OUT == EXPERTS_PLAIN) {
-        // the slots without an expert: those behind the others
-        const int from = scalars(p.count)[2];
-        const size_t none = (size_t)(p.slots - from) * p.N;
-        for (size_t i = (size_t)blockIdx.x * (64 * NW) + tid; i < none; i += (size_t)gridDim.x * (64 * NW))
-            static_cast<uint16_t *>(p.out)[(size_t)p.order[from + i / p.N] * p.N + i % p.N] = 0;
+        // zeros for the slots without an expert: those behind the others
+        const int from = listed ? scalars(p.count)[2] : 0;
+        const size_t empty = (size_t)(p.slots - from) * p.N;
+        for (size_t i = (size_t)blockIdx.x * (64 * NW) + tid; i < empty; i += (size_t)gridDim.x * (64 * NW)) {
+            const size_t slot = listed ? p.order[from + i / p.N] : i / p.N;
+            if (listed || !(valid >> slot & 1)) static_cast<uint16_t *>(p.out)[slot * p.N + i % p.N] = 0;
+        }
     }
 }
 

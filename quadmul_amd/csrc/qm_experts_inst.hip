@@ -14,34 +14,40 @@ static hipError_t launch_any(const ExpertsArgs &p, hipStream_t s)
     const int columns = OUT == EXPERTS_GATED ? p.N / 2 : p.N;
     return enqueue(&experts_any_kernel<T, S, OUT>, dim3(std::min(columns / 4 + 1, 1 << 20), std::min(p.slots, 65535)), dim3(256), 0, s, p);
 }
-template <int T, int S, int MODE, ExpertsOut OUT>
-static hipError_t launch_tiles(const ExpertsArgs &p, const ExpertsPlan &plan, const bool few, hipStream_t s)
+template <int T, int S, int G, ExpertsOut OUT>
+static hipError_t launch_rows(const ExpertsArgs &p, const ExpertsPlan &plan, hipStream_t s)
 {
     const int columns = OUT == EXPERTS_GATED ? p.N / 2 : p.N;
-    if (plan.rows <= 16 && few && p.K < 1 << 20 && (unsigned long long)p.N * std::max(p.K / 2, p.groups * 4) < 1ull << 32 && (long long)plan.tiles * ((columns + 15) / 16) < 1ll << 31) {
-        const auto rows = [&](auto r, auto nw) {
-            constexpr int R = decltype(r)::value, NW = decltype(nw)::value;
-            typedef ExpertsRowsShape<MODE == 1, R, NW, OUT> Shape;
-            static std::atomic<bool> known[QM_MAX_DEVICES] = {};
-            const auto kernel = &experts_rows_kernel<T, S, MODE == 1, R, NW, OUT>;
-            if (const hipError_t e = ensure_dynamic_lds(kernel, Shape::BYTES, known); e != hipSuccess) return e;
-            const long long items = (long long)plan.tiles * ((columns + Shape::COLUMNS - 1) / Shape::COLUMNS);
-            return enqueue(kernel, dim3((unsigned)std::min<long long>(items, 256 * Shape::PER_CU)), dim3(64 * NW), Shape::BYTES, s, p);
-        };
-        // Eight waves to an item where there are few items and each is long: one token's second product with 2 of 8 experts, K 14336 on 4096 columns, 18.6 us with
-        // four and 13.8 with eight; with more items fewer waves to each have less to put together: 32 tokens, 8 of 128 of 2048 x 1024, 77 and 83 us.
-        const std::integral_constant<int, 2> i2{};
-        const std::integral_constant<int, 4> i4{};
-        const std::integral_constant<int, 8> i8{};
-        const std::integral_constant<int, 16> i16{};
-        bool eight = (long long)std::min(p.slots, p.experts) * ((columns + 31) / 32) <= 512 && p.K >= 4096;
-        switch (plan.rows) {
-        case 2: return eight ? rows(i2, i8) : rows(i2, i4);
-        case 4: return eight ? rows(i4, i8) : rows(i4, i4);
-        case 8: return eight ? rows(i8, i8) : rows(i8, i4);
-        default: return eight ? rows(i16, i8) : rows(i16, i4);
-        }
+    const auto rows = [&](auto r, auto c, auto nw) {
+        constexpr int R = decltype(r)::value, C = decltype(c)::value, NW = decltype(nw)::value;
+        typedef ExpertsRowsShape<G, R, C, NW, OUT> Shape;
+        static std::atomic<bool> known[QM_MAX_DEVICES] = {};
+        const auto kernel = &experts_rows_kernel<T, S, G, R, C, NW, OUT>;
+        if (const hipError_t e = ensure_dynamic_lds(kernel, Shape::BYTES, known); e != hipSuccess) return e;
+        const long long items = (long long)(OUT == EXPERTS_SUM ? p.slots / p.top_k : plan.tiles) * ((columns + Shape::COLUMNS - 1) / Shape::COLUMNS);
+        return enqueue(kernel, dim3((unsigned)std::min<long long>(items, 256 * Shape::PER_CU)), dim3(64 * NW), Shape::BYTES, s, p);
+    };
+    // Eight waves to an item where there are few items and each is long: one token's second product with 2 of 8 experts, K 14336 on 4096 columns, 18.6 us with
+    // four and 13.8 with eight; with more items fewer waves to each have less to put together: 32 tokens, 8 of 128 of 2048 x 1024, 77 and 83 us.
+    const std::integral_constant<int, 1> i1{};
+    const std::integral_constant<int, 2> i2{};
+    const std::integral_constant<int, 4> i4{};
+    const std::integral_constant<int, 8> i8{};
+    const std::integral_constant<int, 16> i16{};
+    bool eight = (long long)std::min(p.slots, p.experts) * ((columns + 31) / 32) <= 512 && p.K >= 4096;
+    // (a token's choices one after the other: as many waves as a workgroup can have)
+    if constexpr (OUT == EXPERTS_SUM) return (long long)(p.slots / p.top_k) * ((columns + 31) / 32) <= 256 ? rows(i2, i1, i16) : rows(i2, i2, i16);
+    else switch (plan.rows) {
+    case 2: return eight ? rows(i2, i2, i8) : rows(i2, i2, i4);
+    case 4: return eight ? rows(i4, i2, i8) : rows(i4, i2, i4);
+    case 8: return eight ? rows(i8, i2, i8) : rows(i8, i2, i4);
+    default: return eight ? rows(i16, i2, i8) : rows(i16, i2, i4);
     }
+}
+template <int T, int S, int MODE, ExpertsOut OUT>
+static hipError_t launch_tiles(const ExpertsArgs &p, const ExpertsPlan &plan, hipStream_t s)
+{
+    const int columns = OUT == EXPERTS_GATED ? p.N / 2 : p.N;
     // (with a scale to every one or two blocks the registers of 64 columns to a wave do not fit)
     constexpr int NT = MODE == 1 ? 4 : 2;
     const auto wide = [&](auto wm, auto wn, auto mt, auto nt) {
@@ -73,25 +79,28 @@ static hipError_t launch_tiles(const ExpertsArgs &p, const ExpertsPlan &plan, co
 #else
 #define QM_LAUNCH_EXPERTS launch_experts_bf16
 #endif
-hipError_t QM_LAUNCH_EXPERTS(const ExpertsArgs &p, const ExpertsPlan &plan, const int scale_dtype, const ExpertsOut out, const bool tiled, const bool few, hipStream_t s)
+hipError_t QM_LAUNCH_EXPERTS(const ExpertsArgs &p, const ExpertsPlan &plan, const int scale_dtype, const ExpertsOut out, const ExpertsKernel kernel, hipStream_t s)
 {
     constexpr int T = QM_EXPERTS_TYPE;
     const auto by_out = [&](auto st, auto o) {
         constexpr int S = decltype(st)::value;
         constexpr ExpertsOut OUT = (ExpertsOut)decltype(o)::value;
-        if (!tiled) return launch_any<T, S, OUT>(p, s);
-        switch (group_mode(p.group)) {
-        case 1: return launch_tiles<T, S, 1, OUT>(p, plan, few, s);
-        case 2: return launch_tiles<T, S, 2, OUT>(p, plan, few, s);
-        case 4: return launch_tiles<T, S, 4, OUT>(p, plan, few, s);
-        default: return launch_tiles<T, S, 0, OUT>(p, plan, few, s);
-        }
+        if (kernel == EXPERTS_ROWS) return p.group % 128 == 0 ? launch_rows<T, S, 4, OUT>(p, plan, s) : p.group % 64 == 0 ? launch_rows<T, S, 2, OUT>(p, plan, s) : launch_rows<T, S, 1, OUT>(p, plan, s);
+        if constexpr (OUT == EXPERTS_SUM) return hipErrorInvalidValue;  // (no other kernel adds up)
+        else if (kernel == EXPERTS_ANY) return launch_any<T, S, OUT>(p, s);
+        else switch (group_mode(p.group)) {
+            case 1: return launch_tiles<T, S, 1, OUT>(p, plan, s);
+            case 2: return launch_tiles<T, S, 2, OUT>(p, plan, s);
+            case 4: return launch_tiles<T, S, 4, OUT>(p, plan, s);
+            default: return launch_tiles<T, S, 0, OUT>(p, plan, s);
+            }
     };
     const auto by_type = [&](auto st) {
         switch (out) {
         case EXPERTS_PLAIN: return by_out(st, std::integral_constant<int, EXPERTS_PLAIN>{});
         case EXPERTS_GATED: return by_out(st, std::integral_constant<int, EXPERTS_GATED>{});
-        default: return by_out(st, std::integral_constant<int, EXPERTS_PART>{});
+        case EXPERTS_PART: return by_out(st, std::integral_constant<int, EXPERTS_PART>{});
+        default: return by_out(st, std::integral_constant<int, EXPERTS_SUM>{});
         }
     };
     return scale_dtype == QM_IN_F32 ? by_type(std::integral_constant<int, QM_IN_F32>{}) : by_type(std::integral_constant<int, T>{});
