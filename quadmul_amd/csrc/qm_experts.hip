@@ -29,8 +29,11 @@ static ExpertsPlan experts_plan(const int tokens, const int top_k, const int exp
     ExpertsPlan p{};
     p.bytes = at;
     if (slots == 0 || experts == 0 || experts > EXPERTS_SORTED) return p;
-    const int mean = slots / experts;
-    p.rows = mean >= 256 ? 256 : mean >= 96 ? 128 : mean >= 24 ? 64 : mean >= 16 ? 32 : mean >= 6 ? 16 : slots >= 2 * experts ? 8 : tokens > 2 ? 4 : 2;
+    // By the mean number of an expert's rows (where there are many experts some have several times the mean). us, rows of a tile in front; 128 experts of 2048 x 1024, bf16:
+    // mean 6 8: 119, 32: 120; 8 16: 132, 32: 117; 64 32: 245, 64: 249; 256 32: 786, 64: 712. 8 experts of 4096 x 14336, float16: 2 4: 104, 8: 113; 4 4: 178, 8: 158; 6 8: 184, 16: 182;
+    // 12 16: 237, 32: 265; 16 16: 285, 32: 262; 48 32: 313, 64: 315; 64 32: 426, 64: 373.
+    const auto mean = [&](const int rows) { return slots >= (long long)rows * experts; };
+    p.rows = mean(64) ? 64 : mean(experts > 16 ? 7 : 14) ? 32 : mean(6) ? 16 : mean(3) ? 8 : tokens > 2 ? 4 : 2;
     p.tiles = slots / p.rows + std::min(experts + 1, slots);
     p.order = at;
     p.list = p.order + up256((size_t)slots * 4);
@@ -38,10 +41,12 @@ static ExpertsPlan experts_plan(const int tokens, const int top_k, const int exp
     p.bytes = p.count + 256;
     return p;
 }
-static hipError_t sort_slots(const ExpertsPlan &plan, const int *chosen, const int slots, const int experts, char *at, hipStream_t s)
+// The slots sorted (where `slots` is not 0) and x made ready (where it has rows).
+static hipError_t sort_slots(const ExpertsPlan &plan, const int *chosen, const int slots, const int experts, const ExpertsReady &ready, const int dtype, char *at, hipStream_t s)
 {
-    return enqueue(&experts_sort_kernel, dim3(1), dim3(1024), (size_t)(experts + 1) * 4, s, chosen, slots, experts, plan.rows, reinterpret_cast<int *>(at + plan.order),
-                   reinterpret_cast<int *>(at + plan.list), reinterpret_cast<int *>(at + plan.count));
+    const int grid = (slots > 0 ? 1 : 0) + std::min((ready.rows + 15) / 16, 4096);
+    return enqueue(dtype == QM_IN_F16 ? &experts_sort_kernel<QM_IN_F16> : &experts_sort_kernel<QM_IN_BF16>, dim3(grid), dim3(1024), (size_t)(experts + 1) * 4, s, chosen, slots, experts, plan.rows,
+                   reinterpret_cast<int *>(at + plan.order), reinterpret_cast<int *>(at + plan.list), reinterpret_cast<int *>(at + plan.count), ready);
 }
 
 static ExpertsArgs args_of(const qm_expert_weights *w, const void *x, const long long x_token, const long long x_choice, const int *chosen, void *out, const int tokens, const int top_k,
@@ -51,22 +56,32 @@ static ExpertsArgs args_of(const qm_expert_weights *w, const void *x, const long
     p.x = static_cast<const uint16_t *>(x), p.x_token = x_token, p.x_choice = x_choice, p.chosen = chosen;
     p.B = static_cast<const uint8_t *>(w->weight), p.scale = w->scale, p.bias = static_cast<const uint16_t *>(w->bias), p.out = out;
     p.slots = tokens * top_k, p.top_k = top_k, p.experts = w->experts, p.N = w->n, p.K = w->k, p.group = w->group;
-    p.groups = (int)(((long long)w->k + w->group - 1) / w->group), p.chunk = w->k / 32;
+    p.groups = (int)(((long long)w->k + w->group - 1) / w->group);
     p.magic = w->group == 32 ? 0u : (uint32_t)(((1ull << 32) + w->group / 32 - 1) / (w->group / 32));
     p.top_k_magic = ((1ull << 32) + top_k - 1) / top_k;
     p.order = reinterpret_cast<const int *>(at + plan.order), p.tiles = reinterpret_cast<const int *>(at + plan.list), p.count = reinterpret_cast<const int *>(at + plan.count);
     return p;
 }
 
-// Which kernel runs a product. The matrix cores want a K of whole blocks and weights at sixteen bytes; the kernel for few rows, rows of x at sixteen bytes too, offsets of
-// 32 bits from its first one and from an expert's first weight and scale, and block numbers below 2^15 for the division by the size of a group.
+// Which kernel runs a product. The matrix cores want a K of whole blocks, weights at sixteen bytes, offsets of 32 bits from an expert's first weight and scale, and block
+// numbers below 2^15 for the division by the size of a group; the kernel for few rows, rows of x at sixteen bytes too and offsets of 32 bits from the first one.
 static ExpertsKernel kernel_of(const ExpertsArgs &p, const ExpertsPlan &plan)
 {
-    if (p.K == 0 || p.K % 32 != 0 || ((uintptr_t)p.B & 15) != 0 || plan.rows == 0 || p.N > 65535 * 32) return EXPERTS_ANY;
+    if (p.K == 0 || p.K % 32 != 0 || p.K >= 1 << 20 || ((uintptr_t)p.B & 15) != 0 || plan.rows == 0 || p.N > 65535 * 32) return EXPERTS_ANY;
+    if ((unsigned long long)p.N * std::max(p.K / 2, p.groups * 4) >= 1ull << 32) return EXPERTS_ANY;
     const long long last = (p.slots / p.top_k - 1) * p.x_token + (p.top_k - 1) * p.x_choice + p.K;
     const bool rows = ((uintptr_t)p.x & 15) == 0 && p.x_token % 8 == 0 && p.x_choice % 8 == 0 && last < 1ll << 31;
-    const bool fits = p.K < 1 << 20 && (unsigned long long)p.N * std::max(p.K / 2, p.groups * 4) < 1ull << 32;
-    return plan.rows <= 16 && rows && fits && (long long)p.slots * p.top_k < 1ll << 32 && (long long)plan.tiles * ((p.N + 15) / 16) < 1ll << 31 ? EXPERTS_ROWS : EXPERTS_TILES;
+    return plan.rows <= 16 && rows && (long long)p.slots * p.top_k < 1ll << 32 && (long long)plan.tiles * ((p.N + 15) / 16) < 1ll << 31 ? EXPERTS_ROWS : EXPERTS_TILES;
+}
+// Room for x made ready: its rows and a float for each.
+static size_t ready_bytes(const size_t rows, const int k) { return up256(rows * ready_stride(k) * 2) + up256(rows * 4); }
+static ExpertsReady make_ready(ExpertsArgs &p, const int dtype, void *to)
+{
+    p.shared = p.x_choice == 0;
+    const int rows = p.shared ? p.slots / p.top_k : p.slots;
+    float *const back = reinterpret_cast<float *>(static_cast<char *>(to) + up256((size_t)rows * ready_stride(p.K) * 2));
+    p.ready = static_cast<const uint16_t *>(to), p.back = dtype == QM_IN_BF16 ? back : nullptr;
+    return {p.x, p.x_token, p.x_choice, p.shared ? 1 : p.top_k, rows, p.K, static_cast<uint16_t *>(to), back};
 }
 // Up to 64 slots the kernel for few rows finds its tiles by itself.
 static bool sorts(const ExpertsKernel kernel, const int slots) { return kernel == EXPERTS_TILES || (kernel == EXPERTS_ROWS && slots > 64); }
@@ -76,16 +91,19 @@ static hipError_t launch_product(ExpertsArgs p, const ExpertsKernel kernel, cons
     return (dtype == QM_IN_F16 ? launch_experts_f16 : launch_experts_bf16)(p, plan, scale_dtype, out, kernel, s);
 }
 
-// The workspace of the gated MLP: the gated products and the outputs of the experts in front of the lists.
+// The workspace of the gated MLP: the gated products, x and they made ready, the outputs of the experts, in front of the lists.
 struct MlpPlan {
-    size_t part;
+    size_t x_ready, hidden_ready, part;
     ExpertsPlan sorted;
 };
 static MlpPlan mlp_plan(const int tokens, const int top_k, const int experts, const int inner, const int hidden)
 {
+    const size_t slots = (size_t)tokens * top_k;
     MlpPlan p{};
-    p.part = up256((size_t)tokens * top_k * inner * 2);
-    p.sorted = experts_plan(tokens, top_k, experts, p.part + up256((size_t)tokens * top_k * hidden * 4));
+    p.x_ready = up256(slots * ready_stride(inner) * 2);
+    p.hidden_ready = p.x_ready + ready_bytes(tokens, hidden);
+    p.part = p.hidden_ready + ready_bytes(slots, inner);
+    p.sorted = experts_plan(tokens, top_k, experts, p.part + up256(slots * hidden * 4));
     return p;
 }
 
@@ -140,7 +158,7 @@ static int check_choices(const int tokens, const int top_k, const int dtype)
 QM_EXPORT size_t qm_gemm_experts_workspace_bytes(const qm_expert_weights *weights, int tokens, int top_k)
 {
     if (check_weights(weights, weights ? weights->scale_dtype : 0) != QM_OK || check_choices(tokens, top_k, QM_IN_F16) != QM_OK) return 0;
-    return experts_plan(tokens, top_k, weights->experts, 0).bytes;
+    return experts_plan(tokens, top_k, weights->experts, ready_bytes((size_t)tokens * top_k, weights->k)).bytes;
 }
 
 QM_EXPORT int qm_gemm_experts_i4(const void *x, int dtype, long long token_stride, long long choice_stride, const int *chosen, const qm_expert_weights *weights, void *y,
@@ -152,13 +170,14 @@ QM_EXPORT int qm_gemm_experts_i4(const void *x, int dtype, long long token_strid
     if (tokens == 0 || top_k == 0 || weights->n == 0) return QM_OK;
     if (!chosen || !y || (!x && weights->k > 0)) return QM_ERR_NULL;
     if ((((uintptr_t)x | (uintptr_t)y) & 1) || ((uintptr_t)chosen & 3) || ((uintptr_t)workspace & 15)) return QM_ERR_ALIGN;
-    const ExpertsPlan plan = experts_plan(tokens, top_k, weights->experts, 0);
+    const ExpertsPlan plan = experts_plan(tokens, top_k, weights->experts, ready_bytes((size_t)tokens * top_k, weights->k));
     if (plan.bytes > 0 && (!workspace || workspace_bytes < plan.bytes)) return QM_ERR_SCRATCH;
     char *const at = static_cast<char *>(workspace);
     const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-    const ExpertsArgs p = args_of(weights, x, token_stride, choice_stride, chosen, y, tokens, top_k, plan, at);
+    ExpertsArgs p = args_of(weights, x, token_stride, choice_stride, chosen, y, tokens, top_k, plan, at);
     const ExpertsKernel kernel = kernel_of(p, plan);
-    hipError_t e = sorts(kernel, p.slots) ? sort_slots(plan, chosen, p.slots, p.experts, at, s) : hipSuccess;
+    const ExpertsReady ready = kernel == EXPERTS_TILES ? make_ready(p, dtype, at) : ExpertsReady{};
+    hipError_t e = sorts(kernel, p.slots) ? sort_slots(plan, chosen, p.slots, p.experts, ready, dtype, at, s) : hipSuccess;
     if (e == hipSuccess) e = launch_product(p, kernel, plan, dtype, weights->scale_dtype, EXPERTS_PLAIN, s);
     return e == hipSuccess ? QM_OK : fail_launch(e);
 }
@@ -191,13 +210,22 @@ QM_EXPORT int qm_moe_mlp_i4(const void *x, int dtype, long long token_stride, co
     const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     hipError_t e = hipSuccess;
     if (top_k > 0) {
-        const ExpertsArgs first = args_of(up, x, token_stride, 0, chosen, at, tokens, top_k, plan.sorted, at);
+        ExpertsArgs first = args_of(up, x, token_stride, 0, chosen, at, tokens, top_k, plan.sorted, at);
         ExpertsArgs second = args_of(down, at, (long long)top_k * down->k, down->k, chosen, at + plan.part, tokens, top_k, plan.sorted, at);
         const ExpertsKernel one = kernel_of(first, plan.sorted), two = kernel_of(second, plan.sorted);
         // A token's choices one after the other, added up on the way, where hardly any expert has two tokens (whose weights would be read twice).
         const bool apart = two == EXPERTS_ROWS && (tokens == 1 || (first.slots <= 64 && first.slots * 4 <= up->experts));
-        if (sorts(one, first.slots) || (!apart && sorts(two, first.slots))) e = sort_slots(plan.sorted, chosen, first.slots, up->experts, at, s);
+        const ExpertsReady ready = one == EXPERTS_TILES ? make_ready(first, dtype, at + plan.x_ready) : ExpertsReady{};
+        if (sorts(one, first.slots) || (!apart && sorts(two, first.slots))) e = sort_slots(plan.sorted, chosen, first.slots, up->experts, ready, dtype, at, s);
+        // (float16 products are left as the second one's tiles want them; others they make ready first)
+        first.pairs_out = one == EXPERTS_TILES && two == EXPERTS_TILES && dtype == QM_IN_F16;
         if (e == hipSuccess && down->k > 0) e = launch_product(first, one, plan.sorted, dtype, up->scale_dtype, EXPERTS_GATED, s);
+        if (first.pairs_out) {
+            second.ready = reinterpret_cast<const uint16_t *>(at), second.shared = 0;
+        } else if (two == EXPERTS_TILES && e == hipSuccess) {
+            const ExpertsReady again = make_ready(second, dtype, at + plan.hidden_ready);
+            e = sort_slots(plan.sorted, chosen, 0, 0, again, dtype, at, s);
+        }
         if (apart) {
             second.out = y, second.shares = weights;
             if (e == hipSuccess) e = launch_product(second, two, plan.sorted, dtype, down->scale_dtype, EXPERTS_SUM, s);
@@ -206,10 +234,10 @@ QM_EXPORT int qm_moe_mlp_i4(const void *x, int dtype, long long token_stride, co
         if (e == hipSuccess) e = launch_product(second, two, plan.sorted, dtype, down->scale_dtype, EXPERTS_PART, s);
     }
     if (e == hipSuccess) {
-        const unsigned grid = (unsigned)std::min<size_t>(((size_t)tokens * down->n + 255) / 256, 1 << 20);
         const float *const part = reinterpret_cast<const float *>(at + plan.part);
-        const auto sum = dtype == QM_IN_F16 ? &experts_sum_kernel<QM_IN_F16> : &experts_sum_kernel<QM_IN_BF16>;
-        e = enqueue(sum, dim3(grid), dim3(256), 0, s, part, chosen, weights, static_cast<uint16_t *>(y), tokens, top_k, up->experts, down->n);
+        const bool fours = down->n % 4 == 0;
+        const auto sum = dtype == QM_IN_F16 ? fours ? &experts_sum_kernel<QM_IN_F16, 4> : &experts_sum_kernel<QM_IN_F16, 1> : fours ? &experts_sum_kernel<QM_IN_BF16, 4> : &experts_sum_kernel<QM_IN_BF16, 1>;
+        e = enqueue(sum, dim3((down->n / (fours ? 4 : 1) + 255) / 256, std::min(tokens, 65535)), dim3(256), 0, s, part, chosen, weights, static_cast<uint16_t *>(y), tokens, top_k, up->experts, down->n);
     }
     return e == hipSuccess ? QM_OK : fail_launch(e);
 }

@@ -21,7 +21,11 @@ struct ExpertsArgs {
     void *out;                    // [slots, N], [slots, N/2] 16-bit, [slots, N] float, or [tokens, N] 16-bit
     const float *shares;          // EXPERTS_SUM: [slots], the weights of the choices
     int slots, top_k, experts, N, K, group, groups;
-    int chunk;                // blocks of 32 of K
+    // For experts_tile_kernel: x made ready, a row to a token (`shared`) or to a slot, and what a row's sums are multiplied with or null; whether gated products
+    // are left ready for the next one.
+    const uint16_t *ready;
+    const float *back;
+    int shared, pairs_out;
     uint32_t magic;           // 2^32 / (blocks of a group), rounded up: block * magic >> 32 is the block's group, for a K up to 2^20; 0 for one block
     unsigned long long top_k_magic;  // 2^32 / top_k, rounded up, for less than 2^32 / top_k slots
     // (null where there are no more than 64 slots, and experts_rows_kernel finds its tiles by itself:) the slots sorted by expert, cut into tiles of rows: their expert, where they begin in `order` and how many they are. After
@@ -47,57 +51,6 @@ __device__ __forceinline__ const uint16_t *row_of(const ExpertsArgs &p, const in
 }
 // silu(gate) * value
 __device__ __forceinline__ float gated(const float gate, const float value) { return gate / (1.0f + __expf(-gate)) * value; }
-
-// The tile of a workgroup of gemm_grouped_wide_kernel: rows of one expert.
-template <int T, int BM, int BN, ExpertsOut OUT>
-struct ExpertsTile {
-    static constexpr bool PAIRS = OUT == EXPERTS_GATED;
-    const ExpertsArgs &p;
-    int expert, first, rows, n0;  // n0: in columns of the output
-    __device__ __forceinline__ ExpertsTile(const ExpertsArgs &args) : p(args), expert(-1), n0(blockIdx.y * (PAIRS ? BN / 2 : BN))
-    {
-        if ((int)blockIdx.x >= scalars(p.count)[0]) return;
-        const scalar_ints tile = scalars(p.tiles + 4 * (size_t)blockIdx.x);
-        expert = tile[0], first = tile[1], rows = tile[2];
-    }
-    __device__ __forceinline__ bool none() const
-    {
-        if (expert < 0) return true;
-        if (expert < p.experts) return false;
-        if constexpr (OUT == EXPERTS_PLAIN) {
-            const int columns = min(BN, p.N - n0);
-            for (int i = threadIdx.x; i < rows * columns; i += blockDim.x) static_cast<uint16_t *>(p.out)[(size_t)p.order[first + i / columns] * p.N + n0 + i % columns] = 0;
-        }
-        return true;
-    }
-    __device__ __forceinline__ const uint16_t *row(const int i) const { return row_of(p, p.order[first + min(i, rows - 1)]); }
-    // column j's row of the weights: of 32 columns sixteen gates, then what they gate
-    __device__ __forceinline__ size_t weight(const int j) const
-    {
-        if constexpr (PAIRS) return (size_t)expert * p.N + min(n0 + j / 32 * 16 + j % 16, p.N / 2 - 1) + (j & 16 ? p.N / 2 : 0);
-        return (size_t)expert * p.N + min(n0 + j, p.N - 1);
-    }
-    __device__ __forceinline__ void put(const int i, const int j, const v4f v, const v4f value = {}) const
-    {
-        const int n = n0 + (PAIRS ? j / 32 * 16 + j % 16 : j), columns = PAIRS ? p.N / 2 : p.N;
-        if (n >= columns) return;
-        const float bias = OUT == EXPERTS_PLAIN && p.bias != nullptr ? float_of<T>(p.bias[(size_t)expert * p.N + n]) : 0.0f;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            if (i + e >= rows) return;
-            const size_t at = (size_t)p.order[first + i + e] * columns + n;
-            if constexpr (OUT == EXPERTS_PART) static_cast<float *>(p.out)[at] = v[e];
-            else if constexpr (OUT == EXPERTS_GATED) static_cast<uint16_t *>(p.out)[at] = round16<T>(gated(v[e], value[e]));
-            else static_cast<uint16_t *>(p.out)[at] = round16<T>(p.bias != nullptr ? v[e] + bias : v[e]);
-        }
-    }
-};
-template <int T, int BM, int BN>
-using ExpertsPlainTile = ExpertsTile<T, BM, BN, EXPERTS_PLAIN>;
-template <int T, int BM, int BN>
-using ExpertsGatedTile = ExpertsTile<T, BM, BN, EXPERTS_GATED>;
-template <int T, int BM, int BN>
-using ExpertsPartTile = ExpertsTile<T, BM, BN, EXPERTS_PART>;
 
 // Few rows to an expert. An item is up to R rows of one expert and two tiles of 16 columns (a gate's and its value's where one gates the other); a workgroup goes through a
 // run of items, its NW waves each through every NW-th run of 256 of K. A wave loads its runs of the weights (whole lines of 128 bytes), of x and
@@ -446,19 +399,37 @@ __global__ __launch_bounds__(256) void experts_any_kernel(const ExpertsArgs p)
     }
 }
 
-// y[t] = sum over a token's choices, in their order, of weight times product.
-template <int T>
+// y[t] = sum over a token's choices, in their order, of weight times product; four columns to a thread where N has whole fours. Bound by memory: 4096 tokens, 2 choices of 4096
+// columns, 168 MB, 34 us.
+template <int T, int V>
 __global__ __launch_bounds__(256) void experts_sum_kernel(const float *part, const int *chosen, const float *weights, uint16_t *y, const int tokens, const int top_k, const int experts, const int N)
 {
-    const size_t all = (size_t)tokens * N;
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (size_t)gridDim.x * 256) {
-        const size_t t = i / N, n = i - t * N;
-        float v = 0.0f;
-        for (int j = 0; j < top_k; ++j) {
-            const size_t slot = t * top_k + j;
-            if ((unsigned)chosen[slot] < (unsigned)experts) v = __builtin_fmaf(weights[slot], part[slot * N + n], v);
+    typedef float Values __attribute__((ext_vector_type(V)));
+    const int across = N / V;
+    for (long long t = blockIdx.y; t < tokens; t += gridDim.y) {
+        for (int n = blockIdx.x * 256 + threadIdx.x; n < across; n += gridDim.x * 256) {
+            Values v = {};
+            // (the loads of eight choices before the first is used)
+            for (int j0 = 0; j0 < top_k; j0 += 8) {
+                Values each[8];
+                float share[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const size_t slot = (size_t)t * top_k + min(j0 + j, top_k - 1);
+                    each[j] = *reinterpret_cast<const Values *>(part + slot * N + (size_t)n * V);
+                    share[j] = weights[slot];
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const bool counts = j0 + j < top_k && (unsigned)chosen[(size_t)t * top_k + min(j0 + j, top_k - 1)] < (unsigned)experts;
+#pragma unroll
+                    for (int e = 0; e < V; ++e) v[e] = counts ? __builtin_fmaf(share[j], each[j][e], v[e]) : v[e];
+                }
+            }
+            uint16_t *const to = y + (size_t)t * N + (size_t)n * V;
+            if constexpr (V == 4) *reinterpret_cast<v2i_half_aligned *>(to) = v2i{(int)round16_pair<T>(v[0], v[1]), (int)round16_pair<T>(v[2], v[3])};
+            else to[0] = round16<T>(v[0]);
         }
-        y[i] = round16<T>(v);
     }
 }
 

@@ -4,7 +4,7 @@
 #include <cstdlib>
 
 #include "qm_launch.hpp"
-#include "qm_experts.hpp"
+#include "qm_experts_tile.hpp"
 
 namespace qm {
 
@@ -44,34 +44,18 @@ static hipError_t launch_rows(const ExpertsArgs &p, const ExpertsPlan &plan, hip
     default: return eight ? rows(i16, i2, i8) : rows(i16, i2, i4);
     }
 }
-template <int T, int S, int MODE, ExpertsOut OUT>
+template <int T, int S, int G, ExpertsOut OUT>
 static hipError_t launch_tiles(const ExpertsArgs &p, const ExpertsPlan &plan, hipStream_t s)
 {
     const int columns = OUT == EXPERTS_GATED ? p.N / 2 : p.N;
-    // (with a scale to every one or two blocks the registers of 64 columns to a wave do not fit)
-    constexpr int NT = MODE == 1 ? 4 : 2;
-    const auto wide = [&](auto wm, auto wn, auto mt, auto nt) {
-        constexpr int WM = decltype(wm)::value, WN = decltype(wn)::value, MT = decltype(mt)::value, N = decltype(nt)::value, BM = 16 * WM * MT, BN = 16 * WN * N, OF = OUT == EXPERTS_GATED ? BN / 2 : BN;
+    const auto tiles = [&](auto mt) {
+        typedef ExpertsTileShape<G, decltype(mt)::value, OUT> Shape;
         static std::atomic<bool> known[QM_MAX_DEVICES] = {};
-        const auto kernel = [] {
-            if constexpr (OUT == EXPERTS_PLAIN) return &gemm_grouped_wide_kernel<T, S, MODE, WM, WN, MT, N, ExpertsArgs, ExpertsPlainTile>;
-            else if constexpr (OUT == EXPERTS_GATED) return &gemm_grouped_wide_kernel<T, S, MODE, WM, WN, MT, N, ExpertsArgs, ExpertsGatedTile>;
-            else return &gemm_grouped_wide_kernel<T, S, MODE, WM, WN, MT, N, ExpertsArgs, ExpertsPartTile>;
-        }();
-        constexpr int lds = 2 * 8 * 16 * (BM + BN) + 2 * 2 * BN * (int)sizeof(float);
-        if (const hipError_t e = ensure_dynamic_lds(kernel, lds, known); e != hipSuccess) return e;
-        return enqueue(kernel, dim3(plan.tiles, (columns + OF - 1) / OF), dim3(64 * WM * WN), lds, s, p);
+        const auto kernel = &experts_tile_kernel<T, S, G, decltype(mt)::value, OUT>;
+        if (const hipError_t e = ensure_dynamic_lds(kernel, Shape::BYTES, known); e != hipSuccess) return e;
+        return enqueue(kernel, dim3(plan.tiles * Shape::across(columns)), dim3(Shape::THREADS), Shape::BYTES, s, p);
     };
-    const std::integral_constant<int, 1> one{};
-    const std::integral_constant<int, 2> two{};
-    const std::integral_constant<int, 4> four{};
-    const std::integral_constant<int, NT> nt{};
-    switch (plan.rows) {
-    case 256: return wide(four, two, four, nt);
-    case 128: return wide(two, two, four, nt);
-    case 64: return wide(one, four, four, two);
-    default: return wide(one, four, two, two);
-    }
+    return plan.rows == 64 ? tiles(std::integral_constant<int, 2>{}) : tiles(std::integral_constant<int, 1>{});
 }
 
 #if QM_EXPERTS_TYPE == QM_IN_F16
@@ -88,12 +72,7 @@ hipError_t QM_LAUNCH_EXPERTS(const ExpertsArgs &p, const ExpertsPlan &plan, cons
         if (kernel == EXPERTS_ROWS) return p.group % 128 == 0 ? launch_rows<T, S, 4, OUT>(p, plan, s) : p.group % 64 == 0 ? launch_rows<T, S, 2, OUT>(p, plan, s) : launch_rows<T, S, 1, OUT>(p, plan, s);
         if constexpr (OUT == EXPERTS_SUM) return hipErrorInvalidValue;  // (no other kernel adds up)
         else if (kernel == EXPERTS_ANY) return launch_any<T, S, OUT>(p, s);
-        else switch (group_mode(p.group)) {
-            case 1: return launch_tiles<T, S, 1, OUT>(p, plan, s);
-            case 2: return launch_tiles<T, S, 2, OUT>(p, plan, s);
-            case 4: return launch_tiles<T, S, 4, OUT>(p, plan, s);
-            default: return launch_tiles<T, S, 0, OUT>(p, plan, s);
-            }
+        else return p.group % 128 == 0 ? launch_tiles<T, S, 4, OUT>(p, plan, s) : p.group % 64 == 0 ? launch_tiles<T, S, 2, OUT>(p, plan, s) : launch_tiles<T, S, 1, OUT>(p, plan, s);
     };
     const auto by_type = [&](auto st) {
         switch (out) {

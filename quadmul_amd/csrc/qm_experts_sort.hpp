@@ -1,13 +1,20 @@
 // Slots sorted by their expert, for the products of qm_experts.hpp.
 #pragma once
-#include "qm_experts.hpp"
+#include "qm_experts_tile.hpp"
 
 namespace qm {
 
 // The slots by expert, and tiles of up to `rows` of each expert's. One workgroup: counts, their sums, places, all in the LDS. Which place of its expert's a slot gets is
 // chance, and no result depends on it: every row of a tile is summed by itself.
-__global__ __launch_bounds__(1024) void experts_sort_kernel(const int *chosen, const int slots, const int experts, const int rows, int *order, int *tiles, int *count)
+// With it the rows of x made ready, by the workgroups after that one (all of them where there are no slots).
+template <int T>
+__global__ __launch_bounds__(1024) void experts_sort_kernel(const int *chosen, const int slots, const int experts, const int rows, int *order, int *tiles, int *count, const ExpertsReady ready)
 {
+    const int sorting = slots > 0 ? 1 : 0;
+    if ((int)blockIdx.x >= sorting) {
+        experts_ready_rows<T>(ready, ((long long)blockIdx.x - sorting) * 16 + (threadIdx.x >> 6), ((long long)gridDim.x - sorting) * 16);
+        return;
+    }
     extern __shared__ int bins[];  // [experts + 1]
     __shared__ int sums[2][16];
     constexpr int AHEAD = 8;

@@ -74,8 +74,8 @@ static hipError_t launch_mode(GroupedArgs p, const GroupedPlan &plan, hipStream_
         };
         static std::atomic<bool> known_wide[2][QM_MAX_DEVICES] = {};
         switch (plan.rows) {
-        case 256: return wide(&gemm_grouped_wide_kernel<T, S, MODE, 4, 2, 4, NT, GroupedArgs, GroupedTile>, known_wide[0]);
-        case 128: return wide(&gemm_grouped_wide_kernel<T, S, MODE, 2, 2, 4, NT, GroupedArgs, GroupedTile>, known_wide[1]);
+        case 256: return wide(&gemm_grouped_wide_kernel<T, S, MODE, 4, 2, 4, NT>, known_wide[0]);
+        case 128: return wide(&gemm_grouped_wide_kernel<T, S, MODE, 2, 2, 4, NT>, known_wide[1]);
         case 64: return enqueue(&gemm_grouped_tile_kernel<T, S, MODE, 4, 2>, grid, dim3(256), 0, s, p);
         case 32: return enqueue(&gemm_grouped_tile_kernel<T, S, MODE, 2, 2>, grid, dim3(256), 0, s, p);
         }

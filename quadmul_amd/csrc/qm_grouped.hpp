@@ -513,32 +513,6 @@ __device__ __forceinline__ v4i plain_weights(const uint32_t w)
     return out;
 }
 
-// The tile of a workgroup: where its rows of x and of the weights are, and what becomes of its sums. BM rows, BN columns.
-template <int T, int BM, int BN>
-struct GroupedTile {
-    static constexpr bool PAIRS = false;
-    const GroupedArgs &p;
-    const int m0, n0;
-    __device__ __forceinline__ GroupedTile(const GroupedArgs &args) : p(args), m0(blockIdx.x * BM), n0(blockIdx.y * BN) {}
-    __device__ __forceinline__ bool none() const { return false; }
-    __device__ __forceinline__ const uint16_t *row(const int i) const { return p.x + min(m0 + i, p.M - 1) * p.x_stride; }
-    __device__ __forceinline__ size_t weight(const int i) const { return (size_t)min(n0 + i, p.N - 1); }
-    // four sums of column j, of rows i and up
-    __device__ __forceinline__ void put(const int i, const int j, const v4f v) const
-    {
-        const int n = n0 + j;
-        const float bias = p.bias != nullptr && p.part == nullptr && n < p.N ? float_of<T>(p.bias[n]) : 0.0f;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int m = m0 + i + e;
-            if (m < p.M && n < p.N) {
-                if (p.part != nullptr) p.part[((size_t)blockIdx.z * p.M + m) * p.N + n] = v[e];
-                else p.D[(size_t)m * p.N + n] = round16<T>(p.bias != nullptr ? v[e] + bias : v[e]);
-            }
-        }
-    }
-};
-
 // Many rows: tiles of 16 WM MT rows and 16 WN NT columns, a step of two blocks (64 elements of K) at a time. x and the weights, as floats, go
 // through the LDS, two steps of them, each weight made a float once by one thread of the workgroup; a wave has 16 MT rows and 16 NT columns.
 // Bound by what the matrix cores (16 cycles an instruction, 41 % of the time) and the vector pipeline (33 %: the sums times their scales, and
@@ -547,8 +521,8 @@ struct GroupedTile {
 // 241. Groups of 64 305 us, of 32 335.
 // Piece p (eight k) of row r lies at p * rows + (r ^ p): neither eight pieces of a row, written together, nor a piece of eight rows, read
 // together, meet a bank twice.
-template <int T, int S, int MODE, int WM, int WN, int MT, int NT, class Args, template <int, int, int> class Tile>
-__global__ __launch_bounds__(64 * WM * WN, 2) void gemm_grouped_wide_kernel(const Args p)
+template <int T, int S, int MODE, int WM, int WN, int MT, int NT>
+__global__ __launch_bounds__(64 * WM * WN, 2) void gemm_grouped_wide_kernel(const GroupedArgs p)
 {
     typedef GroupedWeights<T> W;
     typedef typename W::frag frag;
@@ -560,17 +534,16 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_grouped_wide_kernel(cons
     float *const all_s = reinterpret_cast<float *>(staged + 2 * 8 * (BM + BN));
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 15, c = lane >> 4;
     const int block0 = blockIdx.z * p.chunk, blocks = min(p.chunk, p.K / 32 - block0), steps = (blocks + 1) / 2;
-    const Tile<T, BM, BN> tile(p);
-    if (tile.none()) return;
+    const int m0 = blockIdx.x * BM, n0 = blockIdx.y * BN;
 
     const uint16_t *x_at[XP];
     const uint8_t *w_at[WP];
 #pragma unroll
-    for (int i = 0; i < XP; ++i) x_at[i] = tile.row(tid / 8 + i * (THREADS / 8)) + (size_t)block0 * 32;
+    for (int i = 0; i < XP; ++i) x_at[i] = p.x + min(m0 + tid / 8 + i * (THREADS / 8), p.M - 1) * p.x_stride + (size_t)block0 * 32;
 #pragma unroll
-    for (int i = 0; i < WP; ++i) w_at[i] = p.B + tile.weight(tid / 4 + i * (THREADS / 4)) * (p.K / 2) + (size_t)block0 * 16;
+    for (int i = 0; i < WP; ++i) w_at[i] = p.B + (size_t)min(n0 + tid / 4 + i * (THREADS / 4), p.N - 1) * (p.K / 2) + (size_t)block0 * 16;
     const int s_block = SCALES == 2 ? tid / BN : 0;
-    const size_t s_row = tile.weight(tid % BN) * p.groups;
+    const size_t s_row = (size_t)min(n0 + tid % BN, p.N - 1) * p.groups;
 
     struct Raw {
         v4i x[XP];
@@ -655,15 +628,20 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_grouped_wide_kernel(cons
         }
     }
 
-    // (PAIRS: the tiles of columns by twos, the second multiplied by the gate of the first)
-    constexpr int STEP = Tile<T, BM, BN>::PAIRS ? 2 : 1;
 #pragma unroll
-    for (int t = 0; t < NT; t += STEP) {
+    for (int t = 0; t < NT; ++t) {
+        const int n = n0 + (wn * NT + t) * 16 + r;
+        const float bias = p.bias != nullptr && p.part == nullptr && n < p.N ? float_of<T>(p.bias[n]) : 0.0f;
 #pragma unroll
         for (int a = 0; a < MT; ++a) {
-            const int i = (wm * MT + a) * 16 + 4 * c, j = (wn * NT + t) * 16 + r;
-            if constexpr (STEP == 2) tile.put(i, j, total[a][t], total[a][t + 1]);
-            else tile.put(i, j, total[a][t]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int m = m0 + (wm * MT + a) * 16 + 4 * c + i;
+                if (m < p.M && n < p.N) {
+                    if (p.part != nullptr) p.part[((size_t)blockIdx.z * p.M + m) * p.N + n] = total[a][t][i];
+                    else p.D[(size_t)m * p.N + n] = round16<T>(p.bias != nullptr ? total[a][t][i] + bias : total[a][t][i]);
+                }
+            }
         }
     }
 }
