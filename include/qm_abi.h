@@ -372,7 +372,8 @@ typedef struct qm_expert_weights {
  * and 0 where e is none of 0 .. experts - 1 (an expert on another GPU, a token of padding). x is fp16 or bf16, token_stride elements from token to
  * token and choice_stride from choice to choice (0: the same row for all of a token's choices); y [tokens, top_k, n] of its type, not overlapping x.
  * Sums are IEEE single precision, the weights take part as the integers they are; one rounding, at the end. The same expert may be
- * chosen twice by a token. tokens * top_k below 2^31.
+ * chosen twice by a token. tokens * top_k below 2^31. A row of x with an infinity or a NaN has infinities or NaN in all its columns, other rows none of them; a finite element
+ * of bf16 above 2^112 may make infinities or NaN of its row's sums.
  *   workspace    16-byte aligned device memory of qm_gemm_experts_workspace_bytes(...) bytes, used in stream order by the kernels of this call only;
  *                QM_ERR_SCRATCH with less, and nothing is enqueued
  */
@@ -395,8 +396,8 @@ int qm_moe_mlp_i4(const void *x, int dtype, long long token_stride, const int *c
 /*
  * Optional: everything a first launch on the current device would otherwise do once -- the
  * LDS size attribute and the residency query of every kernel of the int4 products, the address of the library's
- * scratch array -- without launching anything (qm_gemm_grouped_i4 and qm_kv_attend_i8 set their kernels' LDS size themselves, at the first
- * launch, under capture too).  No counterpart in the reference (its
+ * scratch array -- without launching anything (qm_gemm_grouped_i4, qm_gemm_experts_i4, qm_moe_mlp_i4 and qm_kv_attend_i8 set their kernels' LDS size
+ * themselves, at the first launch, under capture too).  No counterpart in the reference (its
  * launch_igemm, kernel.cu:268-289, needs no set-up: 32 KB of shared memory at most).  First
  * launches do this by themselves, under HIP graph capture too; a caller that wants no
  * runtime queries inside a capture or a latency-critical first call makes this call first,

@@ -453,8 +453,8 @@ void check_experts(const torch::Tensor &x, const torch::Tensor &chosen, const to
     TORCH_CHECK(x.size(-1) % 2 == 0 && weight.dim() == 3 && weight.size(2) * 2 == x.size(-1), "quadmul.gemm_experts: the weights must be [experts, n, k / 2], k even and x's last dimension");
 }
 
-// Rows that the kernels for few rows to an expert can load, sixteen aligned bytes at a time; others are copied first: a pass over x, where the kernels that take
-// rows at any address are up to three times as slow, and results are the same wherever x lies.
+// Rows that the kernels for few rows to an expert can load, sixteen aligned bytes at a time; others are copied first: a pass over x. The kernels that take rows at
+// any address cost more: a token, 8 of 128 of 2048 x 2048, 21 us where a copy and the product are 8.8; 16 tokens 44.5, 37.5; results are the same wherever x lies.
 torch::Tensor aligned_rows(torch::Tensor x)
 {
     const int64_t k = x.size(-1);

@@ -44,7 +44,7 @@ static ExpertsPlan experts_plan(const int tokens, const int top_k, const int exp
 // The slots sorted (where `slots` is not 0) and x made ready (where it has rows).
 static hipError_t sort_slots(const ExpertsPlan &plan, const int *chosen, const int slots, const int experts, const ExpertsReady &ready, const int dtype, char *at, hipStream_t s)
 {
-    const int grid = (slots > 0 ? 1 : 0) + std::min((ready.rows + 15) / 16, 4096);
+    const int grid = (slots > 0 ? 1 : 0) + (int)std::min((ready.rows + 15ll) / 16, 4096ll);
     return enqueue(dtype == QM_IN_F16 ? &experts_sort_kernel<QM_IN_F16> : &experts_sort_kernel<QM_IN_BF16>, dim3(grid), dim3(1024), (size_t)(experts + 1) * 4, s, chosen, slots, experts, plan.rows,
                    reinterpret_cast<int *>(at + plan.order), reinterpret_cast<int *>(at + plan.list), reinterpret_cast<int *>(at + plan.count), ready);
 }
@@ -53,7 +53,8 @@ static ExpertsArgs args_of(const qm_expert_weights *w, const void *x, const long
                            const ExpertsPlan &plan, const char *at)
 {
     ExpertsArgs p{};
-    p.x = static_cast<const uint16_t *>(x), p.x_token = x_token, p.x_choice = x_choice, p.chosen = chosen;
+    // (the distance of rows of which there is only one says nothing)
+    p.x = static_cast<const uint16_t *>(x), p.x_token = tokens > 1 ? x_token : 0, p.x_choice = top_k > 1 ? x_choice : 0, p.chosen = chosen;
     p.B = static_cast<const uint8_t *>(w->weight), p.scale = w->scale, p.bias = static_cast<const uint16_t *>(w->bias), p.out = out;
     p.slots = tokens * top_k, p.top_k = top_k, p.experts = w->experts, p.N = w->n, p.K = w->k, p.group = w->group;
     p.groups = (int)(((long long)w->k + w->group - 1) / w->group);
@@ -63,18 +64,21 @@ static ExpertsArgs args_of(const qm_expert_weights *w, const void *x, const long
     return p;
 }
 
+static bool tiles_take(const int k) { return k > 0 && k % 32 == 0 && k < 1 << 20; }
 // Which kernel runs a product. The matrix cores want a K of whole blocks, weights at sixteen bytes, offsets of 32 bits from an expert's first weight and scale, and block
 // numbers below 2^15 for the division by the size of a group; the kernel for few rows, rows of x at sixteen bytes too and offsets of 32 bits from the first one.
 static ExpertsKernel kernel_of(const ExpertsArgs &p, const ExpertsPlan &plan)
 {
-    if (p.K == 0 || p.K % 32 != 0 || p.K >= 1 << 20 || ((uintptr_t)p.B & 15) != 0 || plan.rows == 0 || p.N > 65535 * 32) return EXPERTS_ANY;
+    if (!tiles_take(p.K) || ((uintptr_t)p.B & 15) != 0 || plan.rows == 0 || p.N > 65535 * 32) return EXPERTS_ANY;
     if ((unsigned long long)p.N * std::max(p.K / 2, p.groups * 4) >= 1ull << 32) return EXPERTS_ANY;
     const long long last = (p.slots / p.top_k - 1) * p.x_token + (p.top_k - 1) * p.x_choice + p.K;
     const bool rows = ((uintptr_t)p.x & 15) == 0 && p.x_token % 8 == 0 && p.x_choice % 8 == 0 && last < 1ll << 31;
-    return plan.rows <= 16 && rows && (long long)p.slots * p.top_k < 1ll << 32 && (long long)plan.tiles * ((p.N + 15) / 16) < 1ll << 31 ? EXPERTS_ROWS : EXPERTS_TILES;
+    if (plan.rows <= 16 && rows && (long long)p.slots * p.top_k < 1ll << 32 && (long long)plan.tiles * ((p.N + 15) / 16) < 1ll << 31) return EXPERTS_ROWS;
+    // (a launch has less than 2^32 threads: more than 100 GB of products)
+    return (long long)plan.tiles * ((p.N + 127) / 128) < 1ll << 24 ? EXPERTS_TILES : EXPERTS_ANY;
 }
-// Room for x made ready: its rows and a float for each.
-static size_t ready_bytes(const size_t rows, const int k) { return up256(rows * ready_stride(k) * 2) + up256(rows * 4); }
+// Room for x made ready: its rows and a float for each; none where K is not for the tiles.
+static size_t ready_bytes(const size_t rows, const int k) { return tiles_take(k) ? up256(rows * ready_stride(k) * 2) + up256(rows * 4) : 0; }
 static ExpertsReady make_ready(ExpertsArgs &p, const int dtype, void *to)
 {
     p.shared = p.x_choice == 0;
@@ -83,8 +87,9 @@ static ExpertsReady make_ready(ExpertsArgs &p, const int dtype, void *to)
     p.ready = static_cast<const uint16_t *>(to), p.back = dtype == QM_IN_BF16 ? back : nullptr;
     return {p.x, p.x_token, p.x_choice, p.shared ? 1 : p.top_k, rows, p.K, static_cast<uint16_t *>(to), back};
 }
-// Up to 64 slots the kernel for few rows finds its tiles by itself.
-static bool sorts(const ExpertsKernel kernel, const int slots) { return kernel == EXPERTS_TILES || (kernel == EXPERTS_ROWS && slots > 64); }
+// Up to 64 slots the kernel for few rows finds its tiles by itself: 8 tokens, 8 of 128 of 2048 x 1024, 34.8 us, 36.8 with the slots sorted first; 1 token 13.3, 15.9.
+static bool sorts(const ExpertsKernel kernel, const int slots) {
+    return kernel == EXPERTS_TILES || (kernel == EXPERTS_ROWS && slots > 64); }
 static hipError_t launch_product(ExpertsArgs p, const ExpertsKernel kernel, const ExpertsPlan &plan, const int dtype, const int scale_dtype, const ExpertsOut out, hipStream_t s)
 {
     if (!sorts(kernel, p.slots)) p.order = nullptr;
@@ -100,7 +105,7 @@ static MlpPlan mlp_plan(const int tokens, const int top_k, const int experts, co
 {
     const size_t slots = (size_t)tokens * top_k;
     MlpPlan p{};
-    p.x_ready = up256(slots * ready_stride(inner) * 2);
+    p.x_ready = up256(slots * (tiles_take(inner) ? ready_stride(inner) : inner) * 2);
     p.hidden_ready = p.x_ready + ready_bytes(tokens, hidden);
     p.part = p.hidden_ready + ready_bytes(slots, inner);
     p.sorted = experts_plan(tokens, top_k, experts, p.part + up256(slots * hidden * 4));
@@ -121,13 +126,14 @@ QM_EXPORT int qm_moe_route(const void *logits, int dtype, long long row_stride, 
     if (tokens == 0) return QM_OK;
     if (!logits || !chosen || !weights) return QM_ERR_NULL;
     if (((uintptr_t)logits & (dtype == QM_IN_F32 ? 3 : 1)) || (((uintptr_t)bias | (uintptr_t)chosen | (uintptr_t)weights) & 3)) return QM_ERR_ALIGN;
-    // 16 lanes to a token where that many tokens are enough for the chip, else 64
-    const bool narrow = tokens > 1024 && experts <= 256 && top_k <= 16 && groups <= 16;
+    // 16 lanes to a token where so many tokens keep the chip busy all the same, else 64. us with 64 and 16 lanes, bf16: softmax, 8 of 128: 1024 tokens 4.9, 4.8; 2048 5.0, 4.8;
+    // 16384 14.1, 7.3; of 256: 1024 5.3, 6.1; 4096 6.8, 6.1; 16384 16.8, 10.6. Sigmoid, 8 of 256 in 4 of 8 groups: 4096 12.3, 14.8; 8192 20.1, 17.5; 65536 131, 119.
+    const bool by_logits = scores == QM_SCORES_SOFTMAX && !bias && top_groups == groups;
+    bool narrow = tokens > (by_logits && experts <= 128 ? 1024 : 4096) && experts <= 256 && top_k <= 16 && groups <= 16;
     int parts = 1;
     while (parts * 2 * groups <= (narrow ? 16 : 64)) parts *= 2;
     const RouteArgs p{logits, bias, chosen, weights, tokens > 1 ? row_stride : experts, tokens, experts, top_k, groups, top_groups, scores == QM_SCORES_SIGMOID, group_best == 2,
                       renormalise != 0, parts, (uint32_t)(((1 << 20) + experts / groups - 1) / (experts / groups)), scale};
-    const bool by_logits = scores == QM_SCORES_SOFTMAX && !bias && top_groups == groups;
     const auto run = [&](auto t, auto l) {
         constexpr int T = decltype(t)::value;
         constexpr bool LOGITS = decltype(l)::value;
@@ -213,8 +219,10 @@ QM_EXPORT int qm_moe_mlp_i4(const void *x, int dtype, long long token_stride, co
         ExpertsArgs first = args_of(up, x, token_stride, 0, chosen, at, tokens, top_k, plan.sorted, at);
         ExpertsArgs second = args_of(down, at, (long long)top_k * down->k, down->k, chosen, at + plan.part, tokens, top_k, plan.sorted, at);
         const ExpertsKernel one = kernel_of(first, plan.sorted), two = kernel_of(second, plan.sorted);
-        // A token's choices one after the other, added up on the way, where hardly any expert has two tokens (whose weights would be read twice).
-        const bool apart = two == EXPERTS_ROWS && (tokens == 1 || (first.slots <= 64 && first.slots * 4 <= up->experts));
+        // A token's choices one after the other, added up on the way: one launch less, but weights that two tokens share are read twice. us, experts by themselves and added up
+        // on the way, 8 of 128 of 2048 x 1024: 4 tokens 28.6, 25.9; 8 35.1, 33.6; 9 40.2, 43.5; of 256: 8 38.6, 36.0; 9 45.6, 46.6; 16 60.2, 63.9; 2 of 8 of 4096 x 14336: 1 token
+        // 36.2, 34.4; 3 71.6, 85.0; 6 of 64 of 2048 x 1408: 4 29.8, 28.3; 6 36.3, 37.5.
+        bool apart = two == EXPERTS_ROWS && (tokens == 1 || (first.slots <= 64 && first.slots * 2 <= up->experts));
         const ExpertsReady ready = one == EXPERTS_TILES ? make_ready(first, dtype, at + plan.x_ready) : ExpertsReady{};
         if (sorts(one, first.slots) || (!apart && sorts(two, first.slots))) e = sort_slots(plan.sorted, chosen, first.slots, up->experts, ready, dtype, at, s);
         // (float16 products are left as the second one's tiles want them; others they make ready first)

@@ -55,7 +55,7 @@ __device__ __forceinline__ float gated(const float gate, const float value) { re
 // Few rows to an expert. An item is up to R rows of one expert and two tiles of 16 columns (a gate's and its value's where one gates the other); a workgroup goes through a
 // run of items, its NW waves each through every NW-th run of 256 of K. A wave loads its runs of the weights (whole lines of 128 bytes), of x and
 // of the scales straight into the LDS, the next one as soon as the one before is in registers, on into the next item, and waits for nothing but its own loads: twelve to twenty
-// waves of a CU have 80 to 130 KB on the way (two runs of fewer waves were slower: their registers and their LDS cost more waves than that). The waves' sums meet in the LDS, one barrier an item. In the
+// waves of a CU have 100 to 150 KB on the way (two runs of fewer waves were slower: their registers and their LDS cost more waves than that). The waves' sums meet in the LDS, one barrier an item. In the
 // LDS the 16 bytes of a line, or of a row of x, are turned round by the number of the line or row, so that no read of sixteen lanes meets a bank twice.
 //
 // G: 32 G of K have one scale (G 4, 2 or 1), so a matrix instruction may take its 32 of K from anywhere in them: a lane's 4 G bytes of a column, read as they
@@ -68,7 +68,7 @@ struct ExpertsRowsShape {
     static constexpr int STAGE = WEIGHTS + X + (SCALES + BIAS) * 256;               // bytes of a run
     static constexpr int RING = NW * STAGE, SUMS = NW * C * QUARTERS * 256, BYTES = RING + 2 * SUMS;
     static constexpr int COLUMNS = OUT == EXPERTS_GATED ? C * 8 : C * 16;           // of the output
-    static constexpr int WAVES = NW == 16 ? 4 : G == 1 ? (R > 8 ? 3 : 4) : R > 2 * G ? 4 : 5;  // to a SIMD, by the registers
+    static constexpr int WAVES = NW == 16 ? 4 : G == 1 ? (R > 8 ? 3 : 4) : R > 2 * G || NW == 8 ? 4 : 5;  // to a SIMD, by the registers
     static constexpr int PER_CU = 163840 / BYTES < WAVES * 4 / NW ? 163840 / BYTES : WAVES * 4 / NW;  // workgroups, by the LDS too
 };
 template <int T, int S, int G, int R, int C, int NW, ExpertsOut OUT>
@@ -88,23 +88,22 @@ __global__ __launch_bounds__(64 * NW, (ExpertsRowsShape<G, R, C, NW, OUT>::WAVES
     const bool listed = SUM || p.order != nullptr;
     const int chosen = listed ? 0 : p.chosen[min(lane, p.slots - 1)];
     const uint64_t valid = __ballot(!listed && lane < p.slots && (unsigned)chosen < (unsigned)p.experts);
-    // the slots of tile t, and how many tiles there are in front of it or in all
-    const auto find = [&](int t, int &expert, uint64_t &of) {
-        int before = 0;
-        of = 0;
-        for (uint64_t left = valid; left != 0;) {
-            expert = __builtin_amdgcn_readlane(chosen, __builtin_ctzll(left));
-            uint64_t same = __ballot(chosen == expert) & valid;
-            left &= ~same;
-            const int more = (__builtin_popcountll(same) + R - 1) / R;
-            if (t < before + more) {
-                for (int i = (t - before) * R; i > 0; --i) same &= same - 1;
-                of = same;
-                break;
-            }
-            before += more;
+    // A tile begins with every R-th slot of an expert; its number is that of the tiles that begin in slots before that one. The slots of tile t (and of its expert's tiles
+    // behind it), and how many tiles there are in all. A lane finds the slots of its expert bit by bit of the expert's number, whatever experts there are.
+    const auto find = [&](const int t, int &expert, uint64_t &of) {
+        uint32_t low = (uint32_t)valid, high = (uint32_t)(valid >> 32);
+        for (int bits = p.experts - 1, bit = 0; bits >> bit; ++bit) {
+            const uint64_t set = __ballot(chosen >> bit & 1);
+            const uint32_t flip = (uint32_t)(chosen >> bit & 1) - 1;  // all ones where this lane's bit is not set
+            low &= (uint32_t)set ^ flip, high &= (uint32_t)(set >> 32) ^ flip;
         }
-        return before;
+        const uint32_t rank = __builtin_amdgcn_mbcnt_hi(high, __builtin_amdgcn_mbcnt_lo(low, 0));
+        const uint64_t begins = __ballot((rank & (R - 1)) == 0) & valid;
+        const uint64_t here = __ballot(__builtin_amdgcn_mbcnt_hi((uint32_t)(begins >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)begins, 0)) == (uint32_t)t) & begins;
+        const int first = __builtin_ctzll(here | 1ull << 63);
+        expert = __builtin_amdgcn_readlane(chosen, first);
+        of = ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)high, first) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)low, first)) >> first << first;
+        return (int)__builtin_popcountll(begins);
     };
     // its expert, how many rows it has and their slots (past the last one: that again)
     const auto get_tile = [&](const int t, int &expert, int &rows, int (&slot)[R]) {
@@ -303,9 +302,13 @@ __global__ __launch_bounds__(64 * NW, (ExpertsRowsShape<G, R, C, NW, OUT>::WAVES
                 if (!counts) continue;
                 const int block = run * 8 + q * 4;  // of 32 of K
                 if ((block + 4) * 32 > p.K) {
-                    // past the end of K: zeros, which whatever weights and scales meet
+                    // past the end of K: zeros, whatever weights they meet, and scales of zero, whatever the last one is
 #pragma unroll
                     for (int i = 0; i < 4; ++i) x[i] = block * 32 + (i / G * 4 * G + c * G + i % G) * 8 < p.K ? x[i] : v4i{};
+#pragma unroll
+                    for (int t = 0; t < C; ++t)
+#pragma unroll
+                        for (int g = 0; g < 4 / G; ++g) scale[t][g] = (block + g * G) * 32 < p.K ? scale[t][g] : 0;
                 }
                 frag xs[4];
 #pragma unroll

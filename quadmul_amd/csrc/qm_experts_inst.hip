@@ -27,16 +27,17 @@ static hipError_t launch_rows(const ExpertsArgs &p, const ExpertsPlan &plan, hip
         const long long items = (long long)(OUT == EXPERTS_SUM ? p.slots / p.top_k : plan.tiles) * ((columns + Shape::COLUMNS - 1) / Shape::COLUMNS);
         return enqueue(kernel, dim3((unsigned)std::min<long long>(items, 256 * Shape::PER_CU)), dim3(64 * NW), Shape::BYTES, s, p);
     };
-    // Eight waves to an item where there are few items and each is long: one token's second product with 2 of 8 experts, K 14336 on 4096 columns, 18.6 us with
-    // four and 13.8 with eight; with more items fewer waves to each have less to put together: 32 tokens, 8 of 128 of 2048 x 1024, 77 and 83 us.
+    // Eight waves to an item where there are no more items than CUs and each is long: us with four and eight, a token's product with 2 of 8 experts, N 4096 (256 items): K 2048
+    // 5.2, 5.2; 4096 6.8, 6.4; 14336 16.2, 13.0; with 3 of them (384 items): 14336 19.9, 20.2.
     const std::integral_constant<int, 1> i1{};
     const std::integral_constant<int, 2> i2{};
     const std::integral_constant<int, 4> i4{};
     const std::integral_constant<int, 8> i8{};
     const std::integral_constant<int, 16> i16{};
-    bool eight = (long long)std::min(p.slots, p.experts) * ((columns + 31) / 32) <= 512 && p.K >= 4096;
-    // (a token's choices one after the other: as many waves as a workgroup can have)
-    if constexpr (OUT == EXPERTS_SUM) return (long long)(p.slots / p.top_k) * ((columns + 31) / 32) <= 256 ? rows(i2, i1, i16) : rows(i2, i2, i16);
+    bool eight = (long long)std::min(p.slots, p.experts) * ((columns + 31) / 32) <= 256 && p.K >= 4096;
+    // (a token's choices one after the other: as many waves as a workgroup can have, and items of 16 columns where those of 32 are for half of the CUs: us of the MLP with 32
+    // and 16, 2 tokens, 8 of 128 of 2048 x 1024 (128 items of 32): 17.7, 16.6; 3 (192): 22.5, 24.2; 1 of 2 of 8 of 4096 x 14336 (128): 38.7, 34.3; 2 (256): 68.8, 72.0)
+    if constexpr (OUT == EXPERTS_SUM) return (long long)(p.slots / p.top_k) * ((columns + 31) / 32) <= 128 ? rows(i2, i1, i16) : rows(i2, i2, i16);
     else switch (plan.rows) {
     case 2: return eight ? rows(i2, i2, i8) : rows(i2, i2, i4);
     case 4: return eight ? rows(i4, i2, i8) : rows(i4, i2, i4);

@@ -205,7 +205,7 @@ __global__ __launch_bounds__(256, 2) void experts_tile_kernel(const ExpertsArgs 
             for (int m = 0; m < MT; ++m)
 #pragma unroll
                 for (int t = 0; t < 2; ++t) part[m][t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[m], f[t], fresh ? v16f{} : part[m][t], 0, 0, 0);
-            if (G == 1 && i % 2 == 1) apply(quad, 2 * ODD + i / 2);
+            if (G == 1 && i % 2 == 1 && (i == 1 || step * 64 + 32 < p.K)) apply(quad, 2 * ODD + i / 2);
         }
         if (G == 2) apply(quad, ODD);
         if (G == 4 && (ODD || step + 1 == steps)) apply(quad, 0);

@@ -174,8 +174,8 @@ class W4A16Experts(torch.nn.Module):
         ``scale_dtype`` None: the scales in the weights' type, if that is one of 16 bits, else float32."""
         parts = []
         for w in (up, down):
-            if w.dim() != 3:
-                raise QuadmulError("W4A16Experts: expects up [experts, 2 inner, hidden] and down [experts, hidden, inner]")
+            if w.dim() != 3 or w.shape[0] == 0:
+                raise QuadmulError("W4A16Experts: expects up [experts, 2 inner, hidden] and down [experts, hidden, inner], an expert or more")
             kind = scale_dtype if scale_dtype is not None else w.dtype if w.dtype in (torch.float16, torch.bfloat16) else None
             each = [quantize_groups(e.contiguous(), group_size, kind) for e in w]
             parts += [torch.stack([p for p, _ in each]), torch.stack([s for _, s in each])]

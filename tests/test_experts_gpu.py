@@ -145,6 +145,19 @@ def test_infinities_and_nans_stay_with_their_token(tokens):
             assert torch.equal(was[keep], now[keep]) and not now[~keep].isfinite().all()
 
 
+@pytest.mark.parametrize("tokens", [1, 40, 300])
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("k,group", [(96, 32), (160, 64), (320, 128), (352, 32)])
+def test_an_infinite_scale_meets_no_element_past_the_end(k, group, dtype, tokens):
+    # ones times ones: the sum of the last group is positive, so its scale makes infinity of every product, and NaN would come from places behind K
+    x, chosen = torch.ones((tokens, k), dtype=dtype, device="cuda"), torch.zeros((tokens, 1), dtype=torch.int32, device="cuda")
+    scale = torch.ones((2, 40, -(-k // group)), device="cuda")
+    scale[..., -1] = float("inf")
+    packed = torch.full((2, 40, k // 2), 0x11, dtype=torch.uint8, device="cuda")
+    y = moe.gemm_experts(x, chosen, packed, scale, group)
+    assert bool((y == float("inf")).all())
+
+
 @pytest.mark.parametrize("tokens", [1, 5, 70])
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
 def test_gates_at_both_ends(tokens, dtype):

@@ -88,3 +88,14 @@ def test_traceable_forms():
                 lambda: ops.moe_mlp(meta(5, 128), chosen, weights, w, s, meta(8, 64, 64, dtype=torch.int8), meta(8, 64, 2), 64)):
         with pytest.raises(RuntimeError):
             bad()
+
+
+def test_workspaces_of_the_longest_rows():
+    lib, longest = qm.library(), 2 ** 31 - 2
+    # (one row: what lists there are, and no copy of a row that no tiles take)
+    assert 0 < lib.qm_gemm_experts_workspace_bytes(matrices(experts=1, n=1, k=longest), 1, 1) < 4096
+    # (a row of gated products in 16 bits, a row of sums in 32)
+    need = lib.qm_moe_mlp_workspace_bytes(matrices(experts=1, n=4, k=longest), matrices(experts=1, n=longest, k=2), 1, 1)
+    assert 0 <= need - 4 * longest < 4096
+    need = lib.qm_moe_mlp_workspace_bytes(matrices(experts=1, n=2 ** 31 - 4, k=2), matrices(experts=1, n=2, k=2 ** 30 - 2), 1, 1)
+    assert 0 <= need - 2 * (2 ** 30 - 2) < 4096
