@@ -129,7 +129,7 @@ QM_EXPORT int qm_moe_route(const void *logits, int dtype, long long row_stride, 
     // 16 lanes to a token where so many tokens keep the chip busy all the same, else 64. us with 64 and 16 lanes, bf16: softmax, 8 of 128: 1024 tokens 4.9, 4.8; 2048 5.0, 4.8;
     // 16384 14.1, 7.3; of 256: 1024 5.3, 6.1; 4096 6.8, 6.1; 16384 16.8, 10.6. Sigmoid, 8 of 256 in 4 of 8 groups: 4096 12.3, 14.8; 8192 20.1, 17.5; 65536 131, 119.
     const bool by_logits = scores == QM_SCORES_SOFTMAX && !bias && top_groups == groups;
-    bool narrow = tokens > (by_logits && experts <= 128 ? 1024 : 4096) && experts <= 256 && top_k <= 16 && groups <= 16;
+    const bool narrow = tokens > (by_logits && experts <= 128 ? 1024 : 4096) && experts <= 256 && top_k <= 16 && groups <= 16;
     int parts = 1;
     while (parts * 2 * groups <= (narrow ? 16 : 64)) parts *= 2;
     const RouteArgs p{logits, bias, chosen, weights, tokens > 1 ? row_stride : experts, tokens, experts, top_k, groups, top_groups, scores == QM_SCORES_SIGMOID, group_best == 2,
@@ -222,7 +222,7 @@ QM_EXPORT int qm_moe_mlp_i4(const void *x, int dtype, long long token_stride, co
         // A token's choices one after the other, added up on the way: one launch less, but weights that two tokens share are read twice. us, experts by themselves and added up
         // on the way, 8 of 128 of 2048 x 1024: 4 tokens 28.6, 25.9; 8 35.1, 33.6; 9 40.2, 43.5; of 256: 8 38.6, 36.0; 9 45.6, 46.6; 16 60.2, 63.9; 2 of 8 of 4096 x 14336: 1 token
         // 36.2, 34.4; 3 71.6, 85.0; 6 of 64 of 2048 x 1408: 4 29.8, 28.3; 6 36.3, 37.5.
-        bool apart = two == EXPERTS_ROWS && (tokens == 1 || (first.slots <= 64 && first.slots * 2 <= up->experts));
+        const bool apart = two == EXPERTS_ROWS && (tokens == 1 || (first.slots <= 64 && first.slots * 2 <= up->experts));
         const ExpertsReady ready = one == EXPERTS_TILES ? make_ready(first, dtype, at + plan.x_ready) : ExpertsReady{};
         if (sorts(one, first.slots) || (!apart && sorts(two, first.slots))) e = sort_slots(plan.sorted, chosen, first.slots, up->experts, ready, dtype, at, s);
         // (float16 products are left as the second one's tiles want them; others they make ready first)

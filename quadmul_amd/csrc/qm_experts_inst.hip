@@ -34,7 +34,7 @@ static hipError_t launch_rows(const ExpertsArgs &p, const ExpertsPlan &plan, hip
     const std::integral_constant<int, 4> i4{};
     const std::integral_constant<int, 8> i8{};
     const std::integral_constant<int, 16> i16{};
-    bool eight = (long long)std::min(p.slots, p.experts) * ((columns + 31) / 32) <= 256 && p.K >= 4096;
+    const bool eight = (long long)std::min(p.slots, p.experts) * ((columns + 31) / 32) <= 256 && p.K >= 4096;
     // (a token's choices one after the other: as many waves as a workgroup can have, and items of 16 columns where those of 32 are for half of the CUs: us of the MLP with 32
     // and 16, 2 tokens, 8 of 128 of 2048 x 1024 (128 items of 32): 17.7, 16.6; 3 (192): 22.5, 24.2; 1 of 2 of 8 of 4096 x 14336 (128): 38.7, 34.3; 2 (256): 68.8, 72.0)
     if constexpr (OUT == EXPERTS_SUM) return (long long)(p.slots / p.top_k) * ((columns + 31) / 32) <= 128 ? rows(i2, i1, i16) : rows(i2, i2, i16);

@@ -271,3 +271,68 @@ def test_without_the_extension_the_same(monkeypatch):
     assert all(torch.equal(a, call()) for a, call in zip(first, calls))
     test_refusals()
     test_nothing_to_do()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("tokens,top_k,experts", [(1, 70, 80), (2, 33, 40), (8, 8, 128), (16, 4, 129), (1, 130, 64), (9, 8, 128), (1, 2, 4200), (30, 3, 4097)])
+def test_numbers_of_choices_and_of_experts(tokens, top_k, experts, dtype):
+    """One token of more choices than a wave has lanes, 64 slots and one or two more, more experts than slots are sorted by."""
+    product(tokens, top_k, experts, 34, 96, 32, dtype, dtype, experts, distinct=top_k <= experts, with_bias=True)
+    gated(tokens, top_k, experts, 96, 32, 32, dtype, dtype, experts, distinct=top_k <= experts, absent=0.1)
+
+
+@pytest.mark.parametrize("tokens", [2, 70, 300])
+def test_two_streams_at_once(tokens):
+    g = torch.Generator().manual_seed(16)
+    layer = moe.SparseMLP(torch.randn(16, 512, generator=g).half().cuda(), moe.W4A16Experts.from_float(torch.randn(16, 512, 512, generator=g).half().cuda() * 0.04,
+                          torch.randn(16, 512, 256, generator=g).half().cuda() * 0.06, 128), 4)
+    xs = [torch.randn(tokens, 512, generator=g).half().cuda() for _ in range(2)]
+    want, streams, got = [layer(x) for x in xs], [torch.cuda.Stream() for _ in xs], [[], []]
+    torch.cuda.synchronize()
+    for _ in range(8):
+        for x, s, y in zip(xs, streams, got):
+            with torch.cuda.stream(s):
+                y.append(layer(x))
+    torch.cuda.synchronize()
+    for w, ys in zip(want, got):
+        assert all(torch.equal(w, y) for y in ys)
+
+
+def test_weights_behind_four_gigabytes():
+    """Ten experts of half a gigabyte; and all of it as one expert, whose offsets have more than 32 bits."""
+    experts, n, k, group = 10, 65536, 16384, 128
+    g = torch.Generator(device="cuda").manual_seed(17)
+    flat = torch.empty(experts * n * (k // 2) + 16, dtype=torch.uint8, device="cuda").random_(0, 256, generator=g)
+    scale = (torch.rand(experts, n, k // group, generator=g, device="cuda") * 0.02 + 0.001).half()
+    x = torch.randn(200, k, generator=g, device="cuda").half()
+    for tokens, off in ((2, 0), (200, 0), (2, 1)):
+        packed = flat[off:off + experts * n * (k // 2)].view(experts, n, k // 2)
+        chosen = (torch.arange(tokens, device="cuda") % 2 * -3 + 9).to(torch.int32)[:, None].contiguous()  # the last expert and one in the middle
+        y = moe.gemm_experts(x[:tokens], chosen, packed, scale, group)
+        for first in (0, n - 40):
+            some = slice(first, first + 40)
+            q = torch.stack([qm.unpack_int4(packed[e, some].contiguous()) for e in range(experts)])
+            moe_util.check_product(x[:tokens], chosen, q, scale[:, some].contiguous(), group, None, y[:, :, some])
+    one, zero = flat[:-16].view(1, experts * n, k // 2), torch.zeros(2, 1, dtype=torch.int32, device="cuda")
+    y = moe.gemm_experts(x[:2], zero, one, scale.view(1, experts * n, -1), group)
+    q = qm.unpack_int4(one[0, -40:].contiguous())[None]
+    moe_util.check_product(x[:2], zero, q, scale.view(1, experts * n, -1)[:, -40:].contiguous(), group, None, y[:, :, -40:])
+
+
+def test_rows_behind_four_gigabytes():
+    """Activations a gigabyte apart; products and sums of more elements than 32 bits count."""
+    _, chosen, q, s = moe_util.problem(3, 2, 4, 64, 256, 64, torch.float16, torch.float16, 18)
+    far = torch.zeros((1 << 31) + 256, dtype=torch.float16, device="cuda").as_strided((3, 256), (1 << 30, 1))
+    far.copy_(torch.randn(3, 256, generator=torch.Generator().manual_seed(18)))
+    moe_util.check_product(far, chosen, q, s, 64, None, moe.gemm_experts(far, chosen, moe_util.pack(q), s, 64))
+    del far
+    tokens, hidden, inner = 70000, 65536, 32
+    g = torch.Generator(device="cuda").manual_seed(19)
+    x = torch.randn(tokens, hidden, generator=g, device="cuda", dtype=torch.bfloat16)
+    _, _, q_up, s_up = moe_util.problem(1, 1, 2, 2 * inner, hidden, 128, torch.bfloat16, torch.bfloat16, 20)
+    _, _, q_down, s_down = moe_util.problem(1, 1, 2, hidden, inner, 128, torch.bfloat16, torch.bfloat16, 21)
+    chosen = (torch.arange(tokens, device="cuda") % 2).to(torch.int32)[:, None].contiguous()
+    weights = torch.rand(tokens, 1, generator=g, device="cuda")
+    y = moe.mlp(x, chosen, weights, moe_util.pack(q_up), s_up, moe_util.pack(q_down), s_down, 128)
+    for some in (slice(0, 2), slice(32767, 32770), slice(65535, 65538), slice(tokens - 3, tokens)):
+        moe_util.check_mlp(x[some], chosen[some], weights[some], q_up, s_up, q_down, s_down, 128, y[some])

@@ -172,3 +172,18 @@ def test_without_the_extension_the_same(monkeypatch):
     again = moe.route(z, 5, **rule)
     assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
     test_refusals()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("experts,top_k,groups,top_groups", [(8, 2, 1, 1), (60, 6, 3, 2), (128, 8, 16, 3), (200, 16, 1, 1), (256, 8, 8, 4)])
+@pytest.mark.parametrize("scores", moe.SCORES)
+def test_so_many_tokens_that_16_lanes_are_enough(scores, experts, top_k, groups, top_groups, dtype):
+    """More than 4096 tokens, a workgroup's last ones missing; rows of equal logits, masked ones and NaN among them."""
+    z = (torch.randn(4099, experts, generator=torch.Generator().manual_seed(experts)) * 2.0).to(dtype)
+    z[5], z[4098], z[77, ::2], z[78, 1:] = 0.5, -float("inf"), -float("inf"), torch.finfo(dtype).min
+    z[79, 3] = float("nan")
+    z = z.cuda()
+    bias = torch.randn(experts, generator=torch.Generator().manual_seed(1)).cuda() * 0.1
+    check(z, top_k, scores=scores, renormalise=True)
+    check(z, top_k, bias, scores=scores, scale=1.5)
+    check(z, top_k, scores=scores, groups=groups, top_groups=top_groups, renormalise=True)
