@@ -55,21 +55,29 @@ __device__ __forceinline__ float gated(const float gate, const float value) { re
 // Few rows to an expert. An item is up to R rows of one expert and two tiles of 16 columns (a gate's and its value's where one gates the other); a workgroup goes through a
 // run of items, its NW waves each through every NW-th run of 256 of K. A wave loads its runs of the weights (whole lines of 128 bytes), of x and
 // of the scales straight into the LDS, the next one as soon as the one before is in registers, on into the next item, and waits for nothing but its own loads: twelve to twenty
-// waves of a CU have 100 to 150 KB on the way (two runs of fewer waves were slower: their registers and their LDS cost more waves than that). The waves' sums meet in the LDS, one barrier an item. In the
-// LDS the 16 bytes of a line, or of a row of x, are turned round by the number of the line or row, so that no read of sixteen lanes meets a bank twice.
+// waves of a CU have 100 to 150 KB on the way (two runs of fewer waves were slower: their registers and their LDS cost more waves than that). The waves' sums meet in the LDS. There
+// the 16 bytes of a line, or of a row of x, are turned round by the number of the line or row, so that no read of sixteen lanes meets a bank twice.
 //
 // G: 32 G of K have one scale (G 4, 2 or 1), so a matrix instruction may take its 32 of K from anywhere in them: a lane's 4 G bytes of a column, read as they
 // are, are its dwords for G instructions into the same sums.
+//
+// Bound by memory, and by what lies between a load and the next: 32 tokens, 8 of 128 of 2048 x 1024, bf16: 191 MB in 42 us, 4.5 TB/s, the vector pipeline busy for 67 % of them (it makes floats of
+// nibbles), the matrix cores for 26; one token, 2 of 8 of 4096 x 14336: 121 MB in 24 us and 60 in 15. The few wide experts of one token come at 4.9 TB/s, 25 MB of many narrow ones at 2: a wave
+// has two to four runs, one after the other's latency.
 template <int G, int R, int C, int NW, ExpertsOut OUT>
 struct ExpertsRowsShape {
     static constexpr int QUARTERS = (R + 3) / 4;                                   // of 16 rows that have sums
     static constexpr int GROUPS = 8 / G, SCALES = GROUPS * C > 4 ? GROUPS * C / 4 : 1;  // of a run: scales of a column, instructions that load them
     static constexpr int WEIGHTS = C * 2048, X = R * 512, BIAS = OUT == EXPERTS_PLAIN ? 1 : 0;
     static constexpr int STAGE = WEIGHTS + X + (SCALES + BIAS) * 256;               // bytes of a run
-    static constexpr int RING = NW * STAGE, SUMS = NW * C * QUARTERS * 256, BYTES = RING + 2 * SUMS;
+    static constexpr int RING = NW * STAGE, SUMS = NW * C * QUARTERS * 256;
     static constexpr int COLUMNS = OUT == EXPERTS_GATED ? C * 8 : C * 16;           // of the output
     static constexpr int WAVES = NW == 16 ? 4 : G == 1 ? (R > 8 ? 3 : 4) : R > 2 * G || NW == 8 ? 4 : 5;  // to a SIMD, by the registers
-    static constexpr int PER_CU = 163840 / BYTES < WAVES * 4 / NW ? 163840 / BYTES : WAVES * 4 / NW;  // workgroups, by the LDS too
+    static constexpr int of_lds(const int bytes) { return 163840 / bytes < WAVES * 4 / NW ? 163840 / bytes : WAVES * 4 / NW; }
+    // Places for the waves' sums: two, for one barrier an item, or one and two barriers where a CU has room for one workgroup more with it: 48 tokens, 6 of 64 of 2048 x 1408 in groups
+    // of 64 (R 8), 91.5 us with two, 88.7 with one
+    static constexpr int PLACES = of_lds(RING + 2 * SUMS) < of_lds(RING + SUMS) ? 1 : 2;
+    static constexpr int BYTES = RING + PLACES * SUMS, PER_CU = of_lds(BYTES);  // workgroups of a CU
 };
 template <int T, int S, int G, int R, int C, int NW, ExpertsOut OUT>
 __global__ __launch_bounds__(64 * NW, (ExpertsRowsShape<G, R, C, NW, OUT>::WAVES)) void experts_rows_kernel(const ExpertsArgs p)
@@ -330,9 +338,10 @@ __global__ __launch_bounds__(64 * NW, (ExpertsRowsShape<G, R, C, NW, OUT>::WAVES
             }
         }
 
-        // ---- the waves' sums, always in the same order; two places for them, so that one barrier is enough ----
+        // ---- the waves' sums, always in the same order ----
         v4f *const here = sums + parity * (Shape::SUMS / 16);
-        parity ^= 1;
+        if constexpr (Shape::PLACES == 2) parity ^= 1;
+        else if (item > item0) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // (those of the item before are read)
 #pragma unroll
         for (int t = 0; t < C; ++t)
             if (c < Shape::QUARTERS) here[(wave * C + t) * (Shape::QUARTERS * 16) + lane] = total[t];
