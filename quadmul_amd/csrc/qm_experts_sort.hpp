@@ -6,6 +6,7 @@ namespace qm {
 
 // The slots by expert, and tiles of up to `rows` of each expert's. One workgroup: counts, their sums, places, all in the LDS. Which place of its expert's a slot gets is
 // chance, and no result depends on it: every row of a tile is summed by itself.
+// A chain of latencies, 4.5 us for 256 slots, 13 for 8192 with the rows of x (67 MB moved): the tiles are known on the device only, and nothing waits for the host.
 // With it the rows of x made ready, by the workgroups after that one (all of them where there are no slots).
 template <int T>
 __global__ __launch_bounds__(1024) void experts_sort_kernel(const int *chosen, const int slots, const int experts, const int rows, int *order, int *tiles, int *count, const ExpertsReady ready)

@@ -10,6 +10,11 @@
 //
 // In the LDS a row of x is eight units of sixteen bytes, turned by half the row's number, a quad of a column four, turned by a quarter of the column's: sixteen lanes meet
 // every bank once.
+//
+// Bound by nothing alone: 4096 tokens, 2 of 8 experts of 4096 x 11008, float16: the first product 1.67 ms (885 TFLOP/s), the second 0.90 (818); matrix cores busy 50 %, vector
+// pipeline 59, and the clock falls to 1.85 GHz; 2.54 ms in all are 1.99 without matrix instructions, 1.83 without loads, 2.39 without the making of floats. 600 tokens,
+// 8 of 128 of 2048 x 1024, bf16: 98 and 54 us; vector pipeline busy 60 %, as floats made of a nibble serve 32 rows only, matrix cores 30, memory 2.9 TB/s. us of all of the first with
+// other tiles: 128 x 128 2545 to 2611, 128 x 256 of eight waves 2499 (the second product of the 600 tokens slower), 64 x 512 2660, 256 x 128 2680.
 #pragma once
 #include "qm_experts.hpp"
 

@@ -54,6 +54,9 @@ __device__ __forceinline__ V over_lanes(V v, const Join &join)
     return v;
 }
 
+// Bound by its chain of steps for few tokens: one, 6 of 64 experts, 3.5 us, 1.6 of them the launch; 64 tokens, 8 of 256 in 4 of 8 groups, 7.7, most of it exponentials of 64 bits and top_k
+// joins over the lanes one after the other; 16384 tokens, 8 of 128, 8.4 MB in 7.6 us (6.8 with the launches overlapped): the same joins, four tokens to a wave.
+//
 // L lanes to a token, expert number lane + L i in register i of a lane. What is chosen lies next to a border, where 32 bits would decide by
 // their rounding: scores are in 64 bits. Without a bias a softmax has the order of its logits (LOGITS): no score is worked out for the choice, and
 // with renormalised weights only those of the chosen.
