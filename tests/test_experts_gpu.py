@@ -336,3 +336,26 @@ def test_rows_behind_four_gigabytes():
     y = moe.mlp(x, chosen, weights, moe_util.pack(q_up), s_up, moe_util.pack(q_down), s_down, 128)
     for some in (slice(0, 2), slice(32767, 32770), slice(65535, 65538), slice(tokens - 3, tokens)):
         moe_util.check_mlp(x[some], chosen[some], weights[some], q_up, s_up, q_down, s_down, 128, y[some])
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("tokens", [1, 5, 70, 300])
+def test_a_row_that_is_not_finite_is_so_in_all_columns(tokens, dtype):
+    x, chosen, q, s = moe_util.problem(tokens, 2, 3, 64, 256, 64, dtype, dtype, 22)
+    first = moe.gemm_experts(x, chosen, moe_util.pack(q), s, 64)
+    for bad in (float("inf"), -float("inf"), float("nan")):
+        lost = x.clone()
+        lost[tokens // 2, 100] = bad
+        y, others = moe.gemm_experts(lost, chosen, moe_util.pack(q), s, 64), torch.arange(tokens, device="cuda") != tokens // 2
+        assert not y[tokens // 2].isfinite().any() and torch.equal(y[others], first[others])
+
+
+@pytest.mark.parametrize("tokens", [1, 5, 70, 300])
+@pytest.mark.parametrize("power", [-126, -110, 100])
+def test_rows_of_any_size(power, tokens):
+    """bf16 rows far from float16's range, each of another size; elements from there down to nothing in one row."""
+    x, chosen, q, s = moe_util.problem(tokens, 2, 3, 64, 256, 64, torch.bfloat16, torch.float32, 23)
+    x = torch.ldexp(x.float(), torch.full((tokens, 1), power, device="cuda") + torch.arange(tokens, device="cuda")[:, None] % 7)
+    x[tokens - 1] = torch.ldexp(x[tokens - 1], -(torch.arange(256, device="cuda") % 60))
+    x = x.to(torch.bfloat16)
+    moe_util.check_product(x, chosen, q, s, 64, None, moe.gemm_experts(x, chosen, moe_util.pack(q), s, 64))
