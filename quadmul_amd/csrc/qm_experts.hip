@@ -23,17 +23,27 @@ static int check_weights(const qm_expert_weights *w, const int dtype)
 
 static size_t up256(const size_t n) { return (n + 255) / 256 * 256; }
 
-static ExpertsPlan experts_plan(const int tokens, const int top_k, const int experts, size_t at)
+// `across`: tiles that the columns of the (first) product with experts_tile_kernel are; k, group: that product's.
+static ExpertsPlan experts_plan(const int tokens, const int top_k, const int experts, const int across, const int k, const int group, size_t at)
 {
     const int slots = tokens * top_k;
     ExpertsPlan p{};
     p.bytes = at;
     if (slots == 0 || experts == 0 || experts > EXPERTS_SORTED) return p;
-    // By the mean number of an expert's rows (where there are many experts some have several times the mean). us, rows of a tile in front; 128 experts of 2048 x 1024, bf16:
-    // mean 6 8: 119, 32: 120; 8 16: 132, 32: 117; 64 32: 245, 64: 249; 256 32: 786, 64: 712. 8 experts of 4096 x 14336, float16: 2 4: 104, 8: 113; 4 4: 178, 8: 158; 6 8: 184, 16: 182;
-    // 12 16: 237, 32: 265; 16 16: 285, 32: 262; 48 32: 313, 64: 315; 64 32: 426, 64: 373.
     const auto mean = [&](const int rows) { return slots >= (long long)rows * experts; };
-    p.rows = mean(64) ? 64 : mean(experts > 16 ? 7 : 14) ? 32 : mean(6) ? 16 : mean(3) ? 8 : tokens > 2 ? 4 : 2;
+    // Up to 16 rows, by the mean number of an expert's rows (some have several times the mean), are for experts_rows_kernel; tiles of 32 and 64 want work for the chip too. us of the MLP:
+    // rows of a tile in front (a slash: parts of K in the second product), "wide" 8 experts, 2 of them, 4096 x 14336, float16, groups of 128; "odd" the same of 4096 x 11008, bf16, groups of 32;
+    // "narrow" 128, 8, 2048 x 1024, bf16, 128; "64" 6 of 64, 2048 x 1408, float16, 32; "short" 4 of 16, 4096 x 1024, bf16, 64.
+    //   mean 4    wide   8: 159, 16: 175, 32/2: 220;   narrow  8: 98, 16: 114, 32: 110
+    //   mean 6    narrow  16: 131, 32: 117              mean 8    wide  16: 203, 32/2: 223;   narrow  16: 132, 32: 115;   64 (mean 9)  16: 134, 32: 143
+    //   mean 12   wide  16: 241, 32/2: 226, 64/2: 239;   odd  16: 228, 32/2: 286;   64  16: 148, 32: 144
+    //   mean 16   wide  16: 283, 32/2: 259, 64/2: 241;   odd  16: 302, 32/8: 344, 64/2: 302;   narrow  16: 183, 32: 133, 64: 148;   short  16: 52, 32: 73, 64: 89
+    //   mean 32   wide  32/4: 281, 64/2: 249;   odd  16: 475, 32/4: 379, 64/2: 313;   narrow  32: 164, 64: 176;   short  16: 79, 32: 80, 64: 93
+    //   mean 48   64  32: 239, 64: 206;   narrow  32: 198, 64: 209;   short  32: 82, 64: 100      mean 64   wide  32/4: 407, 64/4: 353;   short  32: 104, 64: 103
+    const long long work = (long long)slots * across, filled = (long long)std::min(experts, slots) * across;
+    const bool tiles = mean(32) || (mean(6) && (filled >= 1024 || work >= (group % 64 == 0 ? 8192 : 10240)));
+    const bool high = mean(64) || (filled >= 512 && mean(k >= 4096 ? 16 : 48));
+    p.rows = tiles ? high ? 64 : 32 : mean(6) ? 16 : mean(3) ? 8 : tokens > 2 ? 4 : 2;
     p.tiles = slots / p.rows + std::min(experts + 1, slots);
     p.order = at;
     p.list = p.order + up256((size_t)slots * 4);
@@ -96,19 +106,38 @@ static hipError_t launch_product(ExpertsArgs p, const ExpertsKernel kernel, cons
     return (dtype == QM_IN_F16 ? launch_experts_f16 : launch_experts_bf16)(p, plan, scale_dtype, out, kernel, s);
 }
 
+// The workspace of one product: x made ready in front of the lists.
+static ExpertsPlan plan_of(const qm_expert_weights *w, const int tokens, const int top_k)
+{
+    return experts_plan(tokens, top_k, w->experts, (int)((w->n + 255ll) / 256), w->k, w->group, ready_bytes((size_t)tokens * top_k, w->k));
+}
+
+// Into how many parts K is cut for a second product whose tiles are not enough for the chip, at least 1024 of K to each: for a workgroup to a CU, or two where tiles of 64 rows are filled. us of
+// "wide" as above with 1, 2, 4, 8 parts: mean 16 295, 241, 252, 260; 32 303, 249, 266, 273; 48 327, 317, 292, 290; 64 385, 374, 353, 372; 128 585, 537, 548, 590.
+static int splits_of(const int rows, const int slots, const int experts, const int k, const int n)
+{
+    if (rows < 32 || !tiles_take(k) || n == 0) return 1;
+    const long long there = (long long)std::max(slots / rows, std::min(slots, experts)) * ((n + 255ll) / 256), room = rows == 64 && slots >= 48ll * experts ? 512 : 256;
+    return (int)std::max(1ll, std::min({room / there, (long long)(k / 1024), 8ll}));
+}
+
 // The workspace of the gated MLP: the gated products, x and they made ready, the outputs of the experts, in front of the lists.
 struct MlpPlan {
     size_t x_ready, hidden_ready, part;
+    int splits;  // of K, where the second product is in tiles
     ExpertsPlan sorted;
 };
-static MlpPlan mlp_plan(const int tokens, const int top_k, const int experts, const int inner, const int hidden)
+static MlpPlan mlp_plan(const int tokens, const int top_k, const qm_expert_weights *up, const qm_expert_weights *down)
 {
+    const int experts = up->experts, inner = down->k, hidden = down->n;
+    const auto lists = [&](const size_t at) { return experts_plan(tokens, top_k, experts, (int)((inner + 127ll) / 128), hidden, up->group, at); };
     const size_t slots = (size_t)tokens * top_k;
     MlpPlan p{};
     p.x_ready = up256(slots * (tiles_take(inner) ? ready_stride(inner) : inner) * 2);
     p.hidden_ready = p.x_ready + ready_bytes(tokens, hidden);
     p.part = p.hidden_ready + ready_bytes(slots, inner);
-    p.sorted = experts_plan(tokens, top_k, experts, p.part + up256(slots * hidden * 4));
+    p.splits = splits_of(lists(0).rows, tokens * top_k, experts, inner, hidden);
+    p.sorted = lists(p.part + up256(p.splits * slots * hidden * 4));
     return p;
 }
 
@@ -164,7 +193,7 @@ static int check_choices(const int tokens, const int top_k, const int dtype)
 QM_EXPORT size_t qm_gemm_experts_workspace_bytes(const qm_expert_weights *weights, int tokens, int top_k)
 {
     if (check_weights(weights, weights ? weights->scale_dtype : 0) != QM_OK || check_choices(tokens, top_k, QM_IN_F16) != QM_OK) return 0;
-    return experts_plan(tokens, top_k, weights->experts, ready_bytes((size_t)tokens * top_k, weights->k)).bytes;
+    return plan_of(weights, tokens, top_k).bytes;
 }
 
 QM_EXPORT int qm_gemm_experts_i4(const void *x, int dtype, long long token_stride, long long choice_stride, const int *chosen, const qm_expert_weights *weights, void *y,
@@ -176,7 +205,7 @@ QM_EXPORT int qm_gemm_experts_i4(const void *x, int dtype, long long token_strid
     if (tokens == 0 || top_k == 0 || weights->n == 0) return QM_OK;
     if (!chosen || !y || (!x && weights->k > 0)) return QM_ERR_NULL;
     if ((((uintptr_t)x | (uintptr_t)y) & 1) || ((uintptr_t)chosen & 3) || ((uintptr_t)workspace & 15)) return QM_ERR_ALIGN;
-    const ExpertsPlan plan = experts_plan(tokens, top_k, weights->experts, ready_bytes((size_t)tokens * top_k, weights->k));
+    const ExpertsPlan plan = plan_of(weights, tokens, top_k);
     if (plan.bytes > 0 && (!workspace || workspace_bytes < plan.bytes)) return QM_ERR_SCRATCH;
     char *const at = static_cast<char *>(workspace);
     const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
@@ -198,7 +227,7 @@ static int check_mlp(const qm_expert_weights *up, const qm_expert_weights *down,
 QM_EXPORT size_t qm_moe_mlp_workspace_bytes(const qm_expert_weights *up, const qm_expert_weights *down, int tokens, int top_k)
 {
     if (!up || !down || check_mlp(up, down, up->scale_dtype == QM_IN_F32 ? down->scale_dtype : up->scale_dtype) != QM_OK || check_choices(tokens, top_k, QM_IN_F16) != QM_OK) return 0;
-    return mlp_plan(tokens, top_k, up->experts, down->k, down->n).sorted.bytes;
+    return mlp_plan(tokens, top_k, up, down).sorted.bytes;
 }
 
 QM_EXPORT int qm_moe_mlp_i4(const void *x, int dtype, long long token_stride, const int *chosen, const float *weights, const qm_expert_weights *up, const qm_expert_weights *down,
@@ -210,15 +239,18 @@ QM_EXPORT int qm_moe_mlp_i4(const void *x, int dtype, long long token_stride, co
     if (tokens == 0 || down->n == 0) return QM_OK;
     if (!y || !x || (top_k > 0 && (!chosen || !weights))) return QM_ERR_NULL;
     if ((((uintptr_t)x | (uintptr_t)y) & 1) || (((uintptr_t)chosen | (uintptr_t)weights) & 3) || ((uintptr_t)workspace & 15)) return QM_ERR_ALIGN;
-    const MlpPlan plan = mlp_plan(tokens, top_k, up->experts, down->k, down->n);
+    const MlpPlan plan = mlp_plan(tokens, top_k, up, down);
     if (plan.sorted.bytes > 0 && (!workspace || workspace_bytes < plan.sorted.bytes)) return QM_ERR_SCRATCH;
     char *const at = static_cast<char *>(workspace);
     const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     hipError_t e = hipSuccess;
+    int splits = 1;
     if (top_k > 0) {
         ExpertsArgs first = args_of(up, x, token_stride, 0, chosen, at, tokens, top_k, plan.sorted, at);
         ExpertsArgs second = args_of(down, at, (long long)top_k * down->k, down->k, chosen, at + plan.part, tokens, top_k, plan.sorted, at);
         const ExpertsKernel one = kernel_of(first, plan.sorted), two = kernel_of(second, plan.sorted);
+        const int quads = (second.K + 127) / 128, quads_each = (quads + plan.splits - 1) / plan.splits;
+        second.splits = splits = two == EXPERTS_TILES ? (quads + quads_each - 1) / quads_each : 1, second.steps_each = 2 * quads_each;
         // A token's choices one after the other, added up on the way: one launch less, but weights that two tokens share are read twice. us, experts by themselves and added up
         // on the way, 8 of 128 of 2048 x 1024: 4 tokens 28.6, 25.9; 8 35.1, 33.6; 9 40.2, 43.5; of 256: 8 38.6, 36.0; 9 45.6, 46.6; 16 60.2, 63.9; 2 of 8 of 4096 x 14336: 1 token
         // 36.2, 34.4; 3 71.6, 85.0; 6 of 64 of 2048 x 1408: 4 29.8, 28.3; 6 36.3, 37.5.
@@ -245,7 +277,7 @@ QM_EXPORT int qm_moe_mlp_i4(const void *x, int dtype, long long token_stride, co
         const float *const part = reinterpret_cast<const float *>(at + plan.part);
         const bool fours = down->n % 4 == 0;
         const auto sum = dtype == QM_IN_F16 ? fours ? &experts_sum_kernel<QM_IN_F16, 4> : &experts_sum_kernel<QM_IN_F16, 1> : fours ? &experts_sum_kernel<QM_IN_BF16, 4> : &experts_sum_kernel<QM_IN_BF16, 1>;
-        e = enqueue(sum, dim3((down->n / (fours ? 4 : 1) + 255) / 256, std::min(tokens, 65535)), dim3(256), 0, s, part, chosen, weights, static_cast<uint16_t *>(y), tokens, top_k, up->experts, down->n);
+        e = enqueue(sum, dim3((down->n / (fours ? 4 : 1) + 255) / 256, std::min(tokens, 65535)), dim3(256), 0, s, part, splits, chosen, weights, static_cast<uint16_t *>(y), tokens, top_k, up->experts, down->n);
     }
     return e == hipSuccess ? QM_OK : fail_launch(e);
 }

@@ -26,6 +26,7 @@ struct ExpertsArgs {
     const uint16_t *ready;
     const float *back;
     int shared, pairs_out;
+    int splits, steps_each;   // EXPERTS_PART: parts of K, each with sums of its own one after the other in `out`, and steps of 64 in each but the last, an even number
     uint32_t magic;           // 2^32 / (blocks of a group), rounded up: block * magic >> 32 is the block's group, for a K up to 2^20; 0 for one block
     unsigned long long top_k_magic;  // 2^32 / top_k, rounded up, for less than 2^32 / top_k slots
     // (null where there are no more than 64 slots, and experts_rows_kernel finds its tiles by itself:) the slots sorted by expert, cut into tiles of rows: their expert, where they begin in `order` and how many they are. After
@@ -414,7 +415,7 @@ __global__ __launch_bounds__(256) void experts_any_kernel(const ExpertsArgs p)
 // y[t] = sum over a token's choices, in their order, of weight times product; four columns to a thread where N has whole fours. Bound by memory: 4096 tokens, 2 choices of 4096
 // columns, 168 MB, 34 us.
 template <int T, int V>
-__global__ __launch_bounds__(256) void experts_sum_kernel(const float *part, const int *chosen, const float *weights, uint16_t *y, const int tokens, const int top_k, const int experts, const int N)
+__global__ __launch_bounds__(256) void experts_sum_kernel(const float *part, const int splits, const int *chosen, const float *weights, uint16_t *y, const int tokens, const int top_k, const int experts, const int N)
 {
     typedef float Values __attribute__((ext_vector_type(V)));
     const int across = N / V;
@@ -431,6 +432,9 @@ __global__ __launch_bounds__(256) void experts_sum_kernel(const float *part, con
                     each[j] = *reinterpret_cast<const Values *>(part + slot * N + (size_t)n * V);
                     share[j] = weights[slot];
                 }
+                for (int s = 1; s < splits; ++s)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) each[j] += *reinterpret_cast<const Values *>(part + (((size_t)s * tokens + t) * top_k + min(j0 + j, top_k - 1)) * N + (size_t)n * V);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const bool counts = j0 + j < top_k && (unsigned)chosen[(size_t)t * top_k + min(j0 + j, top_k - 1)] < (unsigned)experts;

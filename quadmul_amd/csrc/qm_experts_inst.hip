@@ -54,7 +54,7 @@ static hipError_t launch_tiles(const ExpertsArgs &p, const ExpertsPlan &plan, hi
         static std::atomic<bool> known[QM_MAX_DEVICES] = {};
         const auto kernel = &experts_tile_kernel<T, S, G, decltype(mt)::value, OUT>;
         if (const hipError_t e = ensure_dynamic_lds(kernel, Shape::BYTES, known); e != hipSuccess) return e;
-        return enqueue(kernel, dim3(plan.tiles * Shape::across(columns)), dim3(Shape::THREADS), Shape::BYTES, s, p);
+        return enqueue(kernel, dim3(plan.tiles * Shape::across(columns) * (OUT == EXPERTS_PART ? p.splits : 1)), dim3(Shape::THREADS), Shape::BYTES, s, p);
     };
     return plan.rows == 64 ? tiles(std::integral_constant<int, 2>{}) : tiles(std::integral_constant<int, 1>{});
 }

@@ -96,9 +96,9 @@ __global__ __launch_bounds__(256, 2) void experts_tile_kernel(const ExpertsArgs 
     int *const slots = reinterpret_cast<int *>(smem + Shape::ROWS_AT);
     float *const backs = reinterpret_cast<float *>(slots + Shape::BM);
     // An XCD has tiles side by side in an order that goes through the columns with EXPERTS_BAND tiles of rows at a time
-    const int columns = PAIRS ? p.N / 2 : p.N, across = Shape::across(columns), there = scalars(p.count)[0];
-    if ((int)blockIdx.x >= there * across) return;
-    const int place_in = xcd_contiguous_id(blockIdx.x, there * across), band0 = place_in / (EXPERTS_BAND * across) * EXPERTS_BAND, band = min(EXPERTS_BAND, there - band0), inside = place_in - band0 * across;
+    const int columns = PAIRS ? p.N / 2 : p.N, across = Shape::across(columns), there = scalars(p.count)[0], splits = OUT == EXPERTS_PART ? p.splits : 1;
+    if ((int)blockIdx.x >= there * across * splits) return;
+    const int at = xcd_contiguous_id(blockIdx.x, there * across * splits), split = OUT == EXPERTS_PART ? at / (there * across) : 0, place_in = at - split * there * across, band0 = place_in / (EXPERTS_BAND * across) * EXPERTS_BAND, band = min(EXPERTS_BAND, there - band0), inside = place_in - band0 * across;
     const int block = __builtin_amdgcn_readfirstlane(inside / band), number = __builtin_amdgcn_readfirstlane(band0 + inside - block * band);
     const scalar_ints tile = scalars(p.tiles + 4 * (size_t)number);
     const int expert = tile[0], first = tile[1], rows = tile[2], n0 = block * Shape::COLUMNS;
@@ -111,7 +111,7 @@ __global__ __launch_bounds__(256, 2) void experts_tile_kernel(const ExpertsArgs 
         return;
     }
     const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, h = lane >> 5;
-    const int line = p.K / 2, steps = (p.K + 63) / 64;
+    const int line = p.K / 2, step0 = OUT == EXPERTS_PART ? __builtin_amdgcn_readfirstlane(split) * p.steps_each : 0, steps = OUT == EXPERTS_PART ? min((p.K + 63) / 64, step0 + p.steps_each) : (p.K + 63) / 64;
 
     for (int i = tid; i < Shape::BM; i += Shape::THREADS) {
         const int slot = p.order[first + min(i, rows - 1)];
@@ -216,11 +216,11 @@ __global__ __launch_bounds__(256, 2) void experts_tile_kernel(const ExpertsArgs 
         if (G == 4 && (ODD || step + 1 == steps)) apply(quad, 0);
     };
 
-    load_x(0, 0);
-    load_w(0);
-    if (steps > 1) load_x(1, 1);
+    load_x(step0, 0);
+    load_w(step0 >> 1);
+    if (step0 + 1 < steps) load_x(step0 + 1, 1);
     int place = 0;
-    for (int step = 0; step < steps; step += 2) {
+    for (int step = step0; step < steps; step += 2) {
         // the step's x, and its quad, have come when no more are on the way than the step before has asked for
         if (step + 2 < steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(Shape::X_LOADS) : "memory");
         else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -255,7 +255,7 @@ __global__ __launch_bounds__(256, 2) void experts_tile_kernel(const ExpertsArgs 
                     if (n + 32 * t >= columns) continue;
                     const float v = total[m][t][i] * back;
                     const size_t to = (size_t)slots[row] * columns + n + 32 * t;
-                    if constexpr (OUT == EXPERTS_PART) static_cast<float *>(p.out)[to] = v;
+                    if constexpr (OUT == EXPERTS_PART) static_cast<float *>(p.out)[(size_t)split * p.slots * columns + to] = v;
                     else static_cast<uint16_t *>(p.out)[to] = round16<T>(p.bias != nullptr ? v + float_of<T>(p.bias[(size_t)expert * p.N + n + 32 * t]) : v);
                 }
             }

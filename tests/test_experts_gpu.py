@@ -359,3 +359,10 @@ def test_rows_of_any_size(power, tokens):
     x[tokens - 1] = torch.ldexp(x[tokens - 1], -(torch.arange(256, device="cuda") % 60))
     x = x.to(torch.bfloat16)
     moe_util.check_product(x, chosen, q, s, 64, None, moe.gemm_experts(x, chosen, moe_util.pack(q), s, 64))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("tokens,top_k,experts,hidden,inner,group", [(70, 2, 4, 256, 2112, 64), (40, 1, 1, 384, 4096, 128), (150, 2, 3, 288, 3104, 32), (300, 1, 4, 640, 9600, 128), (500, 2, 2, 4096, 2048, 256)])
+def test_second_products_cut_along_k(tokens, top_k, experts, hidden, inner, group, dtype):
+    gated(tokens, top_k, experts, hidden, inner, group, dtype, dtype, inner)
+    gated(tokens, top_k, experts, hidden, inner, group, dtype, torch.float32, inner + 1, absent=0.3)
