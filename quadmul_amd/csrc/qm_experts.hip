@@ -23,8 +23,8 @@ static int check_weights(const qm_expert_weights *w, const int dtype)
 
 static size_t up256(const size_t n) { return (n + 255) / 256 * 256; }
 
-// `across`: tiles that the columns of the (first) product with experts_tile_kernel are; k, group: that product's.
-static ExpertsPlan experts_plan(const int tokens, const int top_k, const int experts, const int across, const int k, const int group, size_t at)
+// `across`: tiles that the columns of the (an MLP's first) product with experts_tile_kernel are; k, group: that product's.
+static ExpertsPlan experts_plan(const bool mlp, const int tokens, const int top_k, const int experts, const int across, const int k, const int group, size_t at)
 {
     const int slots = tokens * top_k;
     ExpertsPlan p{};
@@ -41,8 +41,13 @@ static ExpertsPlan experts_plan(const int tokens, const int top_k, const int exp
     //   mean 32   wide  32/4: 281, 64/2: 249;   odd  16: 475, 32/4: 379, 64/2: 313;   narrow  32: 164, 64: 176;   short  16: 79, 32: 80, 64: 93
     //   mean 48   64  32: 239, 64: 206;   narrow  32: 198, 64: 209;   short  32: 82, 64: 100      mean 64   wide  32/4: 407, 64/4: 353;   short  32: 104, 64: 103
     const long long work = (long long)slots * across, filled = (long long)std::min(experts, slots) * across;
-    const bool tiles = mean(32) || (mean(6) && (filled >= 1024 || work >= (group % 64 == 0 ? 8192 : 10240)));
-    const bool high = mean(64) || (filled >= 512 && mean(k >= 4096 ? 16 : 48));
+    // One product, "down" 8 experts, 2 of them, 4096 x 11008 (K), bf16, "up" 11008 x 4096, "short" 4 of 16, 4096 x 1024, "64" 6 of 64, 2048 x 1408, groups of 32:
+    //   mean 8    down  16: 54, 32/2: 88;   up  16: 55, 32: 70;   short  16: 19, 32: 21        mean 12   64  16: 55, 32: 42, 64: 52
+    //   mean 16   down  16: 80, 32/2: 114, 64/2: 98;   up  16: 79, 32: 73, 64/2: 78            mean 32   down  16: 132, 32/2: 116, 64/2: 99;   short  16: 34, 32: 27, 64: 31
+    //   mean 64   down  32/4: 146, 64/4: 131;   up  32: 117, 64/2: 117;   short  32: 31, 64: 37      mean 128   up  32: 169, 64/2: 163;   short  32: 47, 64: 61
+    //   mean 512  up  32: 517, 64: 458;   short  32: 127, 64: 138
+    const bool tiles = mean(32) || (mean(6) && (mlp ? filled >= 1024 || work >= (group % 64 == 0 ? 8192 : 10240) : work >= 4096));
+    const bool high = mlp ? mean(64) || (filled >= 512 && mean(k >= 4096 ? 16 : 48)) : mean(k >= 8192 ? 16 : k >= 4096 ? 64 : 1024);
     p.rows = tiles ? high ? 64 : 32 : mean(6) ? 16 : mean(3) ? 8 : tokens > 2 ? 4 : 2;
     p.tiles = slots / p.rows + std::min(experts + 1, slots);
     p.order = at;
@@ -106,19 +111,38 @@ static hipError_t launch_product(ExpertsArgs p, const ExpertsKernel kernel, cons
     return (dtype == QM_IN_F16 ? launch_experts_f16 : launch_experts_bf16)(p, plan, scale_dtype, out, kernel, s);
 }
 
-// The workspace of one product: x made ready in front of the lists.
-static ExpertsPlan plan_of(const qm_expert_weights *w, const int tokens, const int top_k)
-{
-    return experts_plan(tokens, top_k, w->experts, (int)((w->n + 255ll) / 256), w->k, w->group, ready_bytes((size_t)tokens * top_k, w->k));
-}
-
-// Into how many parts K is cut for a second product whose tiles are not enough for the chip, at least 1024 of K to each: for a workgroup to a CU, or two where tiles of 64 rows are filled. us of
+// Into how many parts K is cut for a product (of an MLP the second) whose tiles are not enough for the chip, at least 1024 of K to each: for a workgroup to a CU, or two where tiles of 64 rows are filled. us of
 // "wide" as above with 1, 2, 4, 8 parts: mean 16 295, 241, 252, 260; 32 303, 249, 266, 273; 48 327, 317, 292, 290; 64 385, 374, 353, 372; 128 585, 537, 548, 590.
 static int splits_of(const int rows, const int slots, const int experts, const int k, const int n)
 {
     if (rows < 32 || !tiles_take(k) || n == 0) return 1;
     const long long there = (long long)std::max(slots / rows, std::min(slots, experts)) * ((n + 255ll) / 256), room = rows == 64 && slots >= 48ll * experts ? 512 : 256;
     return (int)std::max(1ll, std::min({room / there, (long long)(k / 1024), 8ll}));
+}
+
+// K in so many parts, of whole quads of steps.
+static int cut(ExpertsArgs &p, const int splits)
+{
+    const int quads = (p.K + 127) / 128, each = (quads + splits - 1) / splits;
+    p.steps_each = 2 * each;
+    return p.splits = (quads + each - 1) / each;
+}
+
+// The workspace of one product: x made ready, the sums of parts of K, in front of the lists.
+struct ProductPlan {
+    size_t part;
+    int splits;
+    ExpertsPlan sorted;
+};
+static ProductPlan product_plan(const qm_expert_weights *w, const int tokens, const int top_k)
+{
+    const size_t slots = (size_t)tokens * top_k;
+    const auto lists = [&](const size_t at) { return experts_plan(false, tokens, top_k, w->experts, (int)((w->n + 255ll) / 256), w->k, w->group, at); };
+    ProductPlan p{};
+    p.part = ready_bytes(slots, w->k);
+    p.splits = splits_of(lists(0).rows, tokens * top_k, w->experts, w->k, w->n);
+    p.sorted = lists(p.part + (p.splits > 1 ? up256(p.splits * slots * w->n * 4) : 0));
+    return p;
 }
 
 // The workspace of the gated MLP: the gated products, x and they made ready, the outputs of the experts, in front of the lists.
@@ -130,7 +154,7 @@ struct MlpPlan {
 static MlpPlan mlp_plan(const int tokens, const int top_k, const qm_expert_weights *up, const qm_expert_weights *down)
 {
     const int experts = up->experts, inner = down->k, hidden = down->n;
-    const auto lists = [&](const size_t at) { return experts_plan(tokens, top_k, experts, (int)((inner + 127ll) / 128), hidden, up->group, at); };
+    const auto lists = [&](const size_t at) { return experts_plan(true, tokens, top_k, experts, (int)((inner + 127ll) / 128), hidden, up->group, at); };
     const size_t slots = (size_t)tokens * top_k;
     MlpPlan p{};
     p.x_ready = up256(slots * (tiles_take(inner) ? ready_stride(inner) : inner) * 2);
@@ -193,7 +217,7 @@ static int check_choices(const int tokens, const int top_k, const int dtype)
 QM_EXPORT size_t qm_gemm_experts_workspace_bytes(const qm_expert_weights *weights, int tokens, int top_k)
 {
     if (check_weights(weights, weights ? weights->scale_dtype : 0) != QM_OK || check_choices(tokens, top_k, QM_IN_F16) != QM_OK) return 0;
-    return plan_of(weights, tokens, top_k).bytes;
+    return product_plan(weights, tokens, top_k).sorted.bytes;
 }
 
 QM_EXPORT int qm_gemm_experts_i4(const void *x, int dtype, long long token_stride, long long choice_stride, const int *chosen, const qm_expert_weights *weights, void *y,
@@ -205,7 +229,8 @@ QM_EXPORT int qm_gemm_experts_i4(const void *x, int dtype, long long token_strid
     if (tokens == 0 || top_k == 0 || weights->n == 0) return QM_OK;
     if (!chosen || !y || (!x && weights->k > 0)) return QM_ERR_NULL;
     if ((((uintptr_t)x | (uintptr_t)y) & 1) || ((uintptr_t)chosen & 3) || ((uintptr_t)workspace & 15)) return QM_ERR_ALIGN;
-    const ExpertsPlan plan = plan_of(weights, tokens, top_k);
+    const ProductPlan product = product_plan(weights, tokens, top_k);
+    const ExpertsPlan &plan = product.sorted;
     if (plan.bytes > 0 && (!workspace || workspace_bytes < plan.bytes)) return QM_ERR_SCRATCH;
     char *const at = static_cast<char *>(workspace);
     const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
@@ -213,7 +238,19 @@ QM_EXPORT int qm_gemm_experts_i4(const void *x, int dtype, long long token_strid
     const ExpertsKernel kernel = kernel_of(p, plan);
     const ExpertsReady ready = kernel == EXPERTS_TILES ? make_ready(p, dtype, at) : ExpertsReady{};
     hipError_t e = sorts(kernel, p.slots) ? sort_slots(plan, chosen, p.slots, p.experts, ready, dtype, at, s) : hipSuccess;
-    if (e == hipSuccess) e = launch_product(p, kernel, plan, dtype, weights->scale_dtype, EXPERTS_PLAIN, s);
+    if (kernel != EXPERTS_TILES || product.splits == 1) {
+        if (e == hipSuccess) e = launch_product(p, kernel, plan, dtype, weights->scale_dtype, EXPERTS_PLAIN, s);
+        return e == hipSuccess ? QM_OK : fail_launch(e);
+    }
+    const int splits = cut(p, product.splits);
+    float *const part = reinterpret_cast<float *>(at + product.part);
+    p.out = part;
+    if (e == hipSuccess) e = launch_product(p, kernel, plan, dtype, weights->scale_dtype, EXPERTS_PART, s);
+    if (e == hipSuccess) {
+        const bool fours = p.N % 4 == 0;
+        const auto join = dtype == QM_IN_F16 ? fours ? &experts_join_kernel<QM_IN_F16, 4> : &experts_join_kernel<QM_IN_F16, 1> : fours ? &experts_join_kernel<QM_IN_BF16, 4> : &experts_join_kernel<QM_IN_BF16, 1>;
+        e = enqueue(join, dim3((p.N / (fours ? 4 : 1) + 255) / 256, std::min(p.slots, 65535)), dim3(256), 0, s, part, splits, chosen, p.bias, static_cast<uint16_t *>(y), p.slots, p.experts, p.N);
+    }
     return e == hipSuccess ? QM_OK : fail_launch(e);
 }
 
@@ -249,8 +286,7 @@ QM_EXPORT int qm_moe_mlp_i4(const void *x, int dtype, long long token_stride, co
         ExpertsArgs first = args_of(up, x, token_stride, 0, chosen, at, tokens, top_k, plan.sorted, at);
         ExpertsArgs second = args_of(down, at, (long long)top_k * down->k, down->k, chosen, at + plan.part, tokens, top_k, plan.sorted, at);
         const ExpertsKernel one = kernel_of(first, plan.sorted), two = kernel_of(second, plan.sorted);
-        const int quads = (second.K + 127) / 128, quads_each = (quads + plan.splits - 1) / plan.splits;
-        second.splits = splits = two == EXPERTS_TILES ? (quads + quads_each - 1) / quads_each : 1, second.steps_each = 2 * quads_each;
+        splits = two == EXPERTS_TILES ? cut(second, plan.splits) : 1;
         // A token's choices one after the other, added up on the way: one launch less, but weights that two tokens share are read twice. us, experts by themselves and added up
         // on the way, 8 of 128 of 2048 x 1024: 4 tokens 28.6, 25.9; 8 35.1, 33.6; 9 40.2, 43.5; of 256: 8 38.6, 36.0; 9 45.6, 46.6; 16 60.2, 63.9; 2 of 8 of 4096 x 14336: 1 token
         // 36.2, 34.4; 3 71.6, 85.0; 6 of 64 of 2048 x 1408: 4 29.8, 28.3; 6 36.3, 37.5.

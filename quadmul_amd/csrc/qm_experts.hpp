@@ -449,4 +449,27 @@ __global__ __launch_bounds__(256) void experts_sum_kernel(const float *part, con
     }
 }
 
+// A product whose K was cut: y[slot] = the parts' sums in their order, and the bias; zeros where there is no expert.
+template <int T, int V>
+__global__ __launch_bounds__(256) void experts_join_kernel(const float *part, const int splits, const int *chosen, const uint16_t *bias, uint16_t *y, const int slots, const int experts, const int N)
+{
+    typedef float Values __attribute__((ext_vector_type(V)));
+    for (long long slot = blockIdx.y; slot < slots; slot += gridDim.y) {
+        const int expert = chosen[slot];
+        const bool none = (unsigned)expert >= (unsigned)experts;
+        for (int n = blockIdx.x * 256 + threadIdx.x; n < N / V; n += gridDim.x * 256) {
+            Values v = {};
+            if (!none) {
+                for (int s = 0; s < splits; ++s) v += *reinterpret_cast<const Values *>(part + ((size_t)s * slots + slot) * N + (size_t)n * V);
+                if (bias != nullptr)
+#pragma unroll
+                    for (int e = 0; e < V; ++e) v[e] += float_of<T>(bias[(size_t)expert * N + (size_t)n * V + e]);
+            }
+            uint16_t *const to = y + (size_t)slot * N + (size_t)n * V;
+            if constexpr (V == 4) *reinterpret_cast<v2i_half_aligned *>(to) = v2i{(int)round16_pair<T>(v[0], v[1]), (int)round16_pair<T>(v[2], v[3])};
+            else to[0] = round16<T>(v[0]);
+        }
+    }
+}
+
 }  // namespace qm

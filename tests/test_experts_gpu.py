@@ -366,3 +366,10 @@ def test_rows_of_any_size(power, tokens):
 def test_second_products_cut_along_k(tokens, top_k, experts, hidden, inner, group, dtype):
     gated(tokens, top_k, experts, hidden, inner, group, dtype, dtype, inner)
     gated(tokens, top_k, experts, hidden, inner, group, dtype, torch.float32, inner + 1, absent=0.3)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("tokens,top_k,experts,n,k,group", [(140, 2, 4, 259, 2112, 64), (200, 1, 5, 36, 9312, 32), (64, 2, 2, 260, 8192, 128), (33, 1, 1, 7, 2304, 256)])
+def test_products_cut_along_k(tokens, top_k, experts, n, k, group, dtype):
+    product(tokens, top_k, experts, n, k, group, dtype, dtype, k, with_bias=True)
+    product(tokens, top_k, experts, n, k, group, dtype, torch.float32, k + 1, per_choice=True, with_bias=n % 2 == 0, absent=0.3)
