@@ -9,7 +9,7 @@
 // what floats would take, and each float is used for 32 MT rows. One barrier a step.
 //
 // In the LDS a row of x is eight units of sixteen bytes, turned by half the row's number, a quad of a column four, turned by a quarter of the column's: sixteen lanes meet
-// every bank once.
+// every bank once. A product whose tiles are fewer than the CUs has its K in parts, each with sums of its own (EXPERTS_PART), which the kernel that reads them adds in their order.
 //
 // Bound by nothing alone: 4096 tokens, 2 of 8 experts of 4096 x 11008, float16: the first product 1.67 ms (885 TFLOP/s), the second 0.90 (818); matrix cores busy 50 %, vector
 // pipeline 59, and the clock falls to 1.85 GHz; 2.54 ms in all are 1.99 without matrix instructions, 1.83 without loads, 2.39 without the making of floats. 600 tokens,
