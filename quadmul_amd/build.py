@@ -76,9 +76,9 @@ def _run(cmd):
 # A memory instruction must not read a scalar register within five wait states of a vector
 # instruction that wrote it (v_readlane, v_readfirstlane, a comparison into a register pair).
 # The compiler inserts the wait states for its own memory instructions and cannot for the
-# ones inside asm statements -- the ring's loads and the stores of tiles that stick out of C
-# take a base pointer in scalar registers -- so the generated code is scanned for it.
-_ASM_VMEM = re.compile(r"global_(?:store_dwordx[24]|load_lds_dwordx4)\s.*\bs\[(\d+):(\d+)\]")
+# ones inside asm statements -- the loads into the LDS, of four bytes and two too, and the stores
+# of tiles that stick out of C take a base pointer in scalar registers -- so the generated code is scanned for it.
+_ASM_VMEM = re.compile(r"global_(?:store_dwordx[24]|load_lds_(?:dwordx4|dword|ushort))\s.*\bs\[(\d+):(\d+)\]")
 
 
 def scalar_operand_hazards(isa_path: str):

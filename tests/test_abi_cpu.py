@@ -400,6 +400,19 @@ def test_the_build_scans_for_scalar_operands_written_just_before_an_asm_load_or_
     assert "v_readlane_b32 s11" in found[0][1] and "v_readfirstlane_b32 s20" in found[1][1]
 
 
+def test_the_scan_covers_every_load_into_the_lds(tmp_path):
+    """Scales and biases come into the LDS by loads of four and of two bytes, from a base in scalar registers like the others."""
+    from quadmul_amd.build import scalar_operand_hazards
+
+    isa = tmp_path / "unit.s"
+    lines = []
+    for width in ("dwordx4", "dword", "ushort"):
+        lines += ["\tv_readfirstlane_b32 s9, v7", "\ts_mov_b32 m0, s3", "\ts_nop 0", f"\tglobal_load_lds_{width} v1, s[8:9]",
+                  "\tv_readfirstlane_b32 s9, v7", "\ts_nop 4", f"\tglobal_load_lds_{width} v1, s[8:9]"]
+    isa.write_text("\n".join(lines))
+    assert [f[0] for f in scalar_operand_hazards(str(isa))] == [4, 11, 18]
+
+
 def test_bias_that_the_kernel_cannot_read_as_it_is_is_added_apart():
     from quadmul_amd.linear import _fusable
 
