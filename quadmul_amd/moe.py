@@ -152,8 +152,23 @@ def mlp(x: torch.Tensor, chosen: torch.Tensor, weights: torch.Tensor, up: torch.
     return y
 
 
-class W4A16Experts(torch.nn.Module):
-    """The gated MLPs of a layer's experts: ``forward(x, chosen, weights)`` is :func:`mlp`, for ``x`` [..., hidden] with as many rows as ``chosen`` has."""
+class _Float32Kept(torch.nn.Module):
+    """A module whose float32 buffers stay float32 where it is cast (``to(dtype)``, ``half``, ``bfloat16``, ``double``): a router that is rounded chooses other experts,
+    :func:`route` takes its bias in float32 only, and the products take float32 scales beside activations of either type. Buffers of 16 bits follow the cast."""
+
+    def _apply(self, fn, recurse=True):
+        kept = {name: t for name, t in self._buffers.items() if t is not None and t.dtype == torch.float32}
+        super()._apply(fn, recurse)
+        for name, t in kept.items():
+            now = self._buffers[name]
+            if now.dtype != torch.float32:
+                self._buffers[name] = t.to(now.device)
+        return self
+
+
+class W4A16Experts(_Float32Kept):
+    """The gated MLPs of a layer's experts: ``forward(x, chosen, weights)`` is :func:`mlp`, for ``x`` [..., hidden] with as many rows as ``chosen`` has. A cast of the
+    module leaves float32 scales as they are."""
 
     def __init__(self, up_packed: torch.Tensor, up_scale: torch.Tensor, down_packed: torch.Tensor, down_scale: torch.Tensor, group_size: int):
         super().__init__()
@@ -192,8 +207,9 @@ class W4A16Experts(torch.nn.Module):
         return f"experts={self.experts}, hidden={self.hidden}, inner={self.inner}, group_size={self.group_size}"
 
 
-class SparseMLP(torch.nn.Module):
-    """``forward(x)``, ``x`` [..., hidden]: the router's logits (``router`` [experts, hidden], in its own type), :func:`route` with ``rule``'s options, the experts' MLPs."""
+class SparseMLP(_Float32Kept):
+    """``forward(x)``, ``x`` [..., hidden]: the router's logits (``router`` [experts, hidden], in its own type), :func:`route` with ``rule``'s options, the experts' MLPs. A cast
+    of the module leaves a float32 router, the bias and float32 scales as they are."""
 
     def __init__(self, router: torch.Tensor, experts: W4A16Experts, top_k: int, bias: Optional[torch.Tensor] = None, **rule):
         super().__init__()

@@ -373,3 +373,20 @@ def test_second_products_cut_along_k(tokens, top_k, experts, hidden, inner, grou
 def test_products_cut_along_k(tokens, top_k, experts, n, k, group, dtype):
     product(tokens, top_k, experts, n, k, group, dtype, dtype, k, with_bias=True)
     product(tokens, top_k, experts, n, k, group, dtype, torch.float32, k + 1, per_choice=True, with_bias=n % 2 == 0, absent=0.3)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_a_cast_module_chooses_the_same_experts(dtype):
+    """The usual cast of a model to its activations' type: float32 router, bias and scales stay, and so do the choices and every bit of the result."""
+    g = torch.Generator().manual_seed(24)
+    experts, hidden, inner, top_k = 16, 256, 64, 4
+    _, _, q_up, s_up = moe_util.problem(1, 1, experts, 2 * inner, hidden, 64, dtype, torch.float32, 25)
+    _, _, q_down, s_down = moe_util.problem(1, 1, experts, hidden, inner, 64, dtype, torch.float32, 26)
+    router, bias = (torch.randn(experts, hidden, generator=g) / 16).cuda(), torch.randn(experts, generator=g).cuda() * 0.05
+    layer = moe.SparseMLP(router, moe.W4A16Experts(moe_util.pack(q_up), s_up, moe_util.pack(q_down), s_down, 64), top_k, bias, scores="sigmoid")
+    x = torch.randn(50, hidden, generator=g).to(dtype).cuda()
+    first, chosen = layer(x), moe.route(x.float() @ router.t(), top_k, bias=bias, scores="sigmoid")[0]
+    for cast in (layer.half, layer.bfloat16, lambda: layer.to("cuda", torch.float16)):
+        assert cast() is layer
+        assert torch.equal(layer(x), first)
+        assert torch.equal(moe.route(x.to(layer.router.dtype) @ layer.router.t(), top_k, bias=layer.bias, scores="sigmoid")[0], chosen)

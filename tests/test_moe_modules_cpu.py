@@ -1,0 +1,41 @@
+"""The modules of the mixture of experts without a GPU: what a cast does to their tensors, and what their constructors refuse."""
+import pytest
+import torch
+
+from quadmul_amd import moe
+
+
+def experts(scales=torch.float32, count=6, hidden=64, inner=32):
+    g = torch.Generator().manual_seed(count)
+    packed = lambda *shape: torch.randint(-128, 128, shape, dtype=torch.int8, generator=g)  # noqa: E731
+    return moe.W4A16Experts(packed(count, 2 * inner, hidden // 2), torch.rand(count, 2 * inner, hidden // 32, generator=g).to(scales), packed(count, hidden, inner // 2),
+                            torch.rand(count, hidden, inner // 32, generator=g).to(scales), 32)
+
+
+def layer(scales=torch.float32, **rule):
+    g = torch.Generator().manual_seed(1)
+    return moe.SparseMLP(torch.randn(6, 64, generator=g), experts(scales), 2, torch.randn(6, generator=g), **rule)
+
+
+@pytest.mark.parametrize("cast", [lambda m: m.half(), lambda m: m.bfloat16(), lambda m: m.double(), lambda m: m.to(torch.bfloat16), lambda m: m.to("cpu", torch.float16)],
+                         ids=["half", "bfloat16", "double", "to", "to_device"])
+def test_a_cast_leaves_float32_as_it_is(cast):
+    m = layer()
+    before = {name: t.clone() for name, t in m.state_dict().items()}
+    assert cast(m) is m
+    after = m.state_dict()
+    assert set(after) == set(before) == {"router", "bias", "experts.up_packed", "experts.up_scale", "experts.down_packed", "experts.down_scale"}
+    assert all(after[name].dtype == t.dtype and torch.equal(after[name], t) for name, t in before.items())
+
+
+def test_a_cast_of_sixteen_bits_is_one():
+    m = layer(torch.float16)
+    assert m.bfloat16().experts.up_scale.dtype == torch.bfloat16 and m.router.dtype == m.bias.dtype == torch.float32
+    assert m.float().experts.down_scale.dtype == torch.float32
+
+
+def test_a_cast_with_a_move():
+    m = layer().to("meta", torch.bfloat16)
+    assert all(t.is_meta for t in m.state_dict().values()) and m.bias.dtype == m.router.dtype == m.experts.up_scale.dtype == torch.float32
+    m = moe.SparseMLP(torch.randn(6, 64), experts(), 2).half()  # no bias
+    assert m.bias is None and m.router.dtype == torch.float32
