@@ -27,6 +27,16 @@ MAX_EXPERTS, MAX_TOP_K, MAX_GROUPS = 1024, 64, 64
 
 _KINDS = {torch.float16: 1, torch.bfloat16: 2, torch.float32: 3}
 _INT_MAX = 2 ** 31 - 1
+_RULE = {"scores": "softmax", "groups": 1, "top_groups": 1, "group_best": 2, "renormalise": False, "scale": 1.0}  # route's options and what they are without a word
+
+
+def _check_rule(what: str, experts: int, top_k: int, scores: str, groups: int, top_groups: int, group_best: int) -> None:
+    if scores not in SCORES:
+        raise QuadmulError(f"{what}: scores must be one of {SCORES}")
+    if not (1 <= groups <= MAX_GROUPS and experts % groups == 0 and 1 <= top_groups <= groups and group_best in (1, 2)):
+        raise QuadmulError(f"{what}: groups must divide the experts and be at most {MAX_GROUPS}, top_groups at most as many, group_best 1 or 2")
+    if not 1 <= top_k <= min(MAX_TOP_K, experts // groups * top_groups):
+        raise QuadmulError(f"{what}: top_k must be 1 to {MAX_TOP_K}, and no more than the experts to choose from")
 
 
 def route(logits: torch.Tensor, top_k: int, *, bias: Optional[torch.Tensor] = None, scores: str = "softmax", groups: int = 1, top_groups: int = 1, group_best: int = 2,
@@ -46,10 +56,7 @@ def route(logits: torch.Tensor, top_k: int, *, bias: Optional[torch.Tensor] = No
     if not (logits.is_cuda and logits.dim() == 2 and logits.dtype in _KINDS and logits.shape[0] <= _INT_MAX and 1 <= logits.shape[1] <= MAX_EXPERTS):
         raise QuadmulError(f"route: the logits must be a GPU tensor [tokens, 1 to {MAX_EXPERTS} experts], float32, float16 or bfloat16")
     tokens, experts = logits.shape
-    if not (1 <= groups <= MAX_GROUPS and experts % groups == 0 and 1 <= top_groups <= groups and group_best in (1, 2)):
-        raise QuadmulError(f"route: groups must divide the experts and be at most {MAX_GROUPS}, top_groups at most as many, group_best 1 or 2")
-    if not 1 <= top_k <= min(MAX_TOP_K, experts // groups * top_groups):
-        raise QuadmulError(f"route: top_k must be 1 to {MAX_TOP_K}, and no more than the experts to choose from")
+    _check_rule("route", experts, top_k, scores, groups, top_groups, group_best)
     if bias is not None and not (bias.device == logits.device and bias.dtype == torch.float32 and bias.is_contiguous() and bias.shape == (experts,)):
         raise QuadmulError(f"route: the bias must be a contiguous float32 vector of {experts} elements on the logits' device")
     if (experts > 1 and logits.stride(1) != 1) or (tokens > 1 and logits.stride(0) < experts):
@@ -215,11 +222,24 @@ class SparseMLP(_Float32Kept):
         super().__init__()
         if router.shape != (experts.experts, experts.hidden):
             raise QuadmulError(f"SparseMLP: the router must be [{experts.experts}, {experts.hidden}]")
+        if router.dtype not in _KINDS:
+            raise QuadmulError("SparseMLP: the router must be float32, float16 or bfloat16")
+        if bias is not None and (bias.shape != (experts.experts,) or bias.dtype not in _KINDS):
+            raise QuadmulError(f"SparseMLP: the bias must be float32 [{experts.experts}]")
+        wrong = set(rule) - set(_RULE)
+        if wrong:
+            raise QuadmulError(f"SparseMLP: route has no option {', '.join(sorted(wrong))}")
+        if not 1 <= experts.experts <= MAX_EXPERTS:
+            raise QuadmulError(f"SparseMLP: 1 to {MAX_EXPERTS} experts")
+        full = _RULE | rule
+        _check_rule("SparseMLP", experts.experts, int(top_k), full["scores"], int(full["groups"]), int(full["top_groups"]), int(full["group_best"]))
         self.experts, self.top_k, self.rule = experts, top_k, rule
         self.register_buffer("router", router)
-        self.register_buffer("bias", bias)
+        self.register_buffer("bias", None if bias is None else bias.float().contiguous())
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if x.shape[-1] != self.experts.hidden:
+            raise QuadmulError(f"SparseMLP: last dimension of x must be {self.experts.hidden}")
         flat = x.reshape(-1, x.shape[-1])
         chosen, weights = route(flat.to(self.router.dtype) @ self.router.t(), self.top_k, bias=self.bias, **self.rule)
         return self.experts(flat, chosen, weights).reshape(x.shape)

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from quadmul_amd import moe
+from quadmul_amd import QuadmulError, moe
 
 
 def experts(scales=torch.float32, count=6, hidden=64, inner=32):
@@ -39,3 +39,23 @@ def test_a_cast_with_a_move():
     assert all(t.is_meta for t in m.state_dict().values()) and m.bias.dtype == m.router.dtype == m.experts.up_scale.dtype == torch.float32
     m = moe.SparseMLP(torch.randn(6, 64), experts(), 2).half()  # no bias
     assert m.bias is None and m.router.dtype == torch.float32
+
+
+@pytest.mark.parametrize("rule", [{"score": "sigmoid"}, {"renormalize": True}, {"scores": "tanh"}, {"groups": 4}, {"groups": 0}, {"groups": 3, "top_groups": 4}, {"groups": 6, "top_groups": 1},
+                                  {"group_best": 3}], ids=str)
+def test_options_that_route_would_refuse(rule):
+    with pytest.raises(QuadmulError):
+        layer(**rule)
+
+
+def test_what_the_layer_refuses():
+    router, e = torch.randn(6, 64), experts()
+    for args in [(router, e, 0), (router, e, 7), (router[:5], e, 2), (router.double(), e, 2), (router.int(), e, 2), (router, e, 2, torch.zeros(5)), (router, e, 2, torch.zeros(6, 1)),
+                 (router, e, 2, torch.zeros(6, dtype=torch.int32))]:
+        with pytest.raises(QuadmulError):
+            moe.SparseMLP(*args)
+    for x in (torch.randn(3, 32), torch.randn(2, 3, 128)):
+        with pytest.raises(QuadmulError):
+            moe.SparseMLP(router, e, 2)(x)
+    m = moe.SparseMLP(router, e, 2, torch.ones(6, dtype=torch.bfloat16), scores="sigmoid", groups=3, top_groups=1, group_best=1, renormalise=True, scale=2.5)
+    assert m.bias.dtype == torch.float32 and m.bias.tolist() == [1.0] * 6
