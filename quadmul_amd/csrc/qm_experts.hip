@@ -120,6 +120,9 @@ static int splits_of(const int rows, const int slots, const int experts, const i
     return (int)std::max(1ll, std::min({room / there, (long long)(k / 1024), 8ll}));
 }
 
+// Workgroups of 256 threads for n columns, `each` to a thread.
+static unsigned blocks_across(const int n, const int each) { return (unsigned)((n / each + 255ll) / 256); }
+
 // K in so many parts, of whole quads of steps.
 static int cut(ExpertsArgs &p, const int splits)
 {
@@ -249,7 +252,7 @@ QM_EXPORT int qm_gemm_experts_i4(const void *x, int dtype, long long token_strid
     if (e == hipSuccess) {
         const bool fours = p.N % 4 == 0;
         const auto join = dtype == QM_IN_F16 ? fours ? &experts_join_kernel<QM_IN_F16, 4> : &experts_join_kernel<QM_IN_F16, 1> : fours ? &experts_join_kernel<QM_IN_BF16, 4> : &experts_join_kernel<QM_IN_BF16, 1>;
-        e = enqueue(join, dim3((p.N / (fours ? 4 : 1) + 255) / 256, std::min(p.slots, 65535)), dim3(256), 0, s, part, splits, chosen, p.bias, static_cast<uint16_t *>(y), p.slots, p.experts, p.N);
+        e = enqueue(join, dim3(blocks_across(p.N, fours ? 4 : 1), std::min(p.slots, 65535)), dim3(256), 0, s, part, splits, chosen, p.bias, static_cast<uint16_t *>(y), p.slots, p.experts, p.N);
     }
     return e == hipSuccess ? QM_OK : fail_launch(e);
 }
@@ -313,7 +316,7 @@ QM_EXPORT int qm_moe_mlp_i4(const void *x, int dtype, long long token_stride, co
         const float *const part = reinterpret_cast<const float *>(at + plan.part);
         const bool fours = down->n % 4 == 0;
         const auto sum = dtype == QM_IN_F16 ? fours ? &experts_sum_kernel<QM_IN_F16, 4> : &experts_sum_kernel<QM_IN_F16, 1> : fours ? &experts_sum_kernel<QM_IN_BF16, 4> : &experts_sum_kernel<QM_IN_BF16, 1>;
-        e = enqueue(sum, dim3((down->n / (fours ? 4 : 1) + 255) / 256, std::min(tokens, 65535)), dim3(256), 0, s, part, splits, chosen, weights, static_cast<uint16_t *>(y), tokens, top_k, up->experts, down->n);
+        e = enqueue(sum, dim3(blocks_across(down->n, fours ? 4 : 1), std::min(tokens, 65535)), dim3(256), 0, s, part, splits, chosen, weights, static_cast<uint16_t *>(y), tokens, top_k, up->experts, down->n);
     }
     return e == hipSuccess ? QM_OK : fail_launch(e);
 }

@@ -418,34 +418,34 @@ template <int T, int V>
 __global__ __launch_bounds__(256) void experts_sum_kernel(const float *part, const int splits, const int *chosen, const float *weights, uint16_t *y, const int tokens, const int top_k, const int experts, const int N)
 {
     typedef float Values __attribute__((ext_vector_type(V)));
-    const int across = N / V;
+    // (the grid covers the columns; there may be nearly 2^31, and an int does not hold the one behind a grid of them)
+    const uint32_t n = blockIdx.x * 256 + threadIdx.x;
+    if (n >= (uint32_t)N / V) return;
     for (long long t = blockIdx.y; t < tokens; t += gridDim.y) {
-        for (int n = blockIdx.x * 256 + threadIdx.x; n < across; n += gridDim.x * 256) {
-            Values v = {};
-            // (the loads of eight choices before the first is used)
-            for (int j0 = 0; j0 < top_k; j0 += 8) {
-                Values each[8];
-                float share[8];
+        Values v = {};
+        // (the loads of eight choices before the first is used)
+        for (int j0 = 0; j0 < top_k; j0 += 8) {
+            Values each[8];
+            float share[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const size_t slot = (size_t)t * top_k + min(j0 + j, top_k - 1);
-                    each[j] = *reinterpret_cast<const Values *>(part + slot * N + (size_t)n * V);
-                    share[j] = weights[slot];
-                }
-                for (int s = 1; s < splits; ++s)
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) each[j] += *reinterpret_cast<const Values *>(part + (((size_t)s * tokens + t) * top_k + min(j0 + j, top_k - 1)) * N + (size_t)n * V);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const bool counts = j0 + j < top_k && (unsigned)chosen[(size_t)t * top_k + min(j0 + j, top_k - 1)] < (unsigned)experts;
-#pragma unroll
-                    for (int e = 0; e < V; ++e) v[e] = counts ? __builtin_fmaf(share[j], each[j][e], v[e]) : v[e];
-                }
+            for (int j = 0; j < 8; ++j) {
+                const size_t slot = (size_t)t * top_k + min(j0 + j, top_k - 1);
+                each[j] = *reinterpret_cast<const Values *>(part + slot * N + (size_t)n * V);
+                share[j] = weights[slot];
             }
-            uint16_t *const to = y + (size_t)t * N + (size_t)n * V;
-            if constexpr (V == 4) *reinterpret_cast<v2i_half_aligned *>(to) = v2i{(int)round16_pair<T>(v[0], v[1]), (int)round16_pair<T>(v[2], v[3])};
-            else to[0] = round16<T>(v[0]);
+            for (int s = 1; s < splits; ++s)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) each[j] += *reinterpret_cast<const Values *>(part + (((size_t)s * tokens + t) * top_k + min(j0 + j, top_k - 1)) * N + (size_t)n * V);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const bool counts = j0 + j < top_k && (unsigned)chosen[(size_t)t * top_k + min(j0 + j, top_k - 1)] < (unsigned)experts;
+#pragma unroll
+                for (int e = 0; e < V; ++e) v[e] = counts ? __builtin_fmaf(share[j], each[j][e], v[e]) : v[e];
+            }
         }
+        uint16_t *const to = y + (size_t)t * N + (size_t)n * V;
+        if constexpr (V == 4) *reinterpret_cast<v2i_half_aligned *>(to) = v2i{(int)round16_pair<T>(v[0], v[1]), (int)round16_pair<T>(v[2], v[3])};
+        else to[0] = round16<T>(v[0]);
     }
 }
 
@@ -454,21 +454,21 @@ template <int T, int V>
 __global__ __launch_bounds__(256) void experts_join_kernel(const float *part, const int splits, const int *chosen, const uint16_t *bias, uint16_t *y, const int slots, const int experts, const int N)
 {
     typedef float Values __attribute__((ext_vector_type(V)));
+    const uint32_t n = blockIdx.x * 256 + threadIdx.x;
+    if (n >= (uint32_t)N / V) return;
     for (long long slot = blockIdx.y; slot < slots; slot += gridDim.y) {
         const int expert = chosen[slot];
         const bool none = (unsigned)expert >= (unsigned)experts;
-        for (int n = blockIdx.x * 256 + threadIdx.x; n < N / V; n += gridDim.x * 256) {
-            Values v = {};
-            if (!none) {
-                for (int s = 0; s < splits; ++s) v += *reinterpret_cast<const Values *>(part + ((size_t)s * slots + slot) * N + (size_t)n * V);
-                if (bias != nullptr)
+        Values v = {};
+        if (!none) {
+            for (int s = 0; s < splits; ++s) v += *reinterpret_cast<const Values *>(part + ((size_t)s * slots + slot) * N + (size_t)n * V);
+            if (bias != nullptr)
 #pragma unroll
-                    for (int e = 0; e < V; ++e) v[e] += float_of<T>(bias[(size_t)expert * N + (size_t)n * V + e]);
-            }
-            uint16_t *const to = y + (size_t)slot * N + (size_t)n * V;
-            if constexpr (V == 4) *reinterpret_cast<v2i_half_aligned *>(to) = v2i{(int)round16_pair<T>(v[0], v[1]), (int)round16_pair<T>(v[2], v[3])};
-            else to[0] = round16<T>(v[0]);
+                for (int e = 0; e < V; ++e) v[e] += float_of<T>(bias[(size_t)expert * N + (size_t)n * V + e]);
         }
+        uint16_t *const to = y + (size_t)slot * N + (size_t)n * V;
+        if constexpr (V == 4) *reinterpret_cast<v2i_half_aligned *>(to) = v2i{(int)round16_pair<T>(v[0], v[1]), (int)round16_pair<T>(v[2], v[3])};
+        else to[0] = round16<T>(v[0]);
     }
 }
 
