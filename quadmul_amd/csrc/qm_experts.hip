@@ -201,7 +201,7 @@ QM_EXPORT int qm_moe_route(const void *logits, int dtype, long long row_stride, 
                             : experts <= 256   ? &route_kernel<T, 4, 64, LOGITS>
                                                : &route_kernel<T, 16, 64, LOGITS>;
         const int each = narrow ? 16 : 4;
-        return enqueue(kernel, dim3(std::min((tokens + each - 1) / each, 1 << 20)), dim3(256), 0, reinterpret_cast<hipStream_t>(stream), p);
+        return enqueue(kernel, dim3((unsigned)std::min(((long long)tokens + each - 1) / each, 1ll << 20)), dim3(256), 0, reinterpret_cast<hipStream_t>(stream), p);
     };
     const auto by_type = [&](auto t) { return by_logits ? run(t, std::true_type{}) : run(t, std::false_type{}); };
     const hipError_t e = dtype == QM_IN_F16    ? by_type(std::integral_constant<int, QM_IN_F16>{})

@@ -26,3 +26,16 @@ def test_sums_of_the_most_columns(hidden, top_k):
     assert st == 0
     torch.cuda.synchronize()
     assert not at[:hidden].any() and bool((y[:256] == 7.0).all()) and bool((at[hidden:] == 7.0).all())
+
+
+@pytest.mark.parametrize("tokens", [2 ** 31 - 1, 2 ** 31 - 15])
+def test_choices_of_the_most_tokens(tokens):
+    """One expert: it is chosen, with a weight of one, by every token up to the last."""
+    logits = torch.zeros(tokens, 1, dtype=torch.float16, device="cuda")
+    chosen = torch.full((tokens + 64,), 9, dtype=torch.int32, device="cuda")
+    weights = torch.full((tokens + 64,), 9.0, device="cuda")
+    st = qm.library().qm_moe_route(logits.data_ptr(), 1, 1, tokens, 1, 1, None, 0, 1, 1, 1, 0, 1.0, chosen.data_ptr(), weights.data_ptr(), torch.cuda.current_stream().cuda_stream)
+    assert st == 0
+    torch.cuda.synchronize()
+    assert not chosen[:tokens].any() and bool((weights[:tokens] == 1.0).all())
+    assert bool((chosen[tokens:] == 9).all()) and bool((weights[tokens:] == 9.0).all())
