@@ -372,7 +372,7 @@ typedef struct qm_expert_weights {
  * and 0 where e is none of 0 .. experts - 1 (an expert on another GPU, a token of padding). x is fp16 or bf16, token_stride elements from token to
  * token and choice_stride from choice to choice (0: the same row for all of a token's choices); y [tokens, top_k, n] of its type, not overlapping x.
  * Sums are IEEE single precision, the weights take part as the integers they are; one rounding, at the end. The same expert may be
- * chosen twice by a token. tokens * top_k below 2^31. A row of x with an infinity or a NaN has infinities or NaN in all its columns, other rows none of them; a finite element
+ * chosen twice by a token. tokens * top_k up to 2^31 - 64. A row of x with an infinity or a NaN has infinities or NaN in all its columns, other rows none of them; a finite element
  * of bf16 above 2^112 may make infinities or NaN of its row's sums.
  *   workspace    16-byte aligned device memory of qm_gemm_experts_workspace_bytes(...) bytes, used in stream order by the kernels of this call only;
  *                QM_ERR_SCRATCH with less, and nothing is enqueued

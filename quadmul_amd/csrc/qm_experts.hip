@@ -210,11 +210,11 @@ QM_EXPORT int qm_moe_route(const void *logits, int dtype, long long row_stride, 
     return e == hipSuccess ? QM_OK : fail_launch(e);
 }
 
-// what both products check of tokens and choices
+// what both products check of tokens and choices; their kernels go through these by eights and sixty-fours in an int
 static int check_choices(const int tokens, const int top_k, const int dtype)
 {
     if (dtype != QM_IN_F16 && dtype != QM_IN_BF16) return QM_ERR_DTYPE;
-    return tokens < 0 || top_k < 0 || (long long)tokens * top_k > INT_MAX ? QM_ERR_SHAPE : QM_OK;
+    return tokens < 0 || top_k < 0 || (long long)tokens * top_k > INT_MAX - 63 ? QM_ERR_SHAPE : QM_OK;
 }
 
 QM_EXPORT size_t qm_gemm_experts_workspace_bytes(const qm_expert_weights *weights, int tokens, int top_k)

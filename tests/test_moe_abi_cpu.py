@@ -99,3 +99,12 @@ def test_workspaces_of_the_longest_rows():
     assert 0 <= need - 4 * longest < 4096
     need = lib.qm_moe_mlp_workspace_bytes(matrices(experts=1, n=2 ** 31 - 4, k=2), matrices(experts=1, n=2, k=2 ** 30 - 2), 1, 1)
     assert 0 <= need - 2 * (2 ** 30 - 2) < 4096
+
+
+def test_the_most_choices():
+    """The kernels step through a token's choices, and through the slots of an expert, by up to 64: so many below 2^31 are refused."""
+    lib, w, down, most = qm.library(), matrices(), matrices(n=128, k=128), 2 ** 31 - 64
+    for tokens, top_k, code in ((1, most, -7), (1, most + 1, -2), (1, 2 ** 31 - 1, -2), (most, 1, -7), (2 ** 31 - 1, 1, -2), (2, 2 ** 30 - 32, -7), (2, 2 ** 30 - 31, -2)):
+        assert lib.qm_gemm_experts_i4(ONE, 1, 128, 0, ONE, w, ONE, tokens, top_k, None, None, 0) == code
+        assert lib.qm_moe_mlp_i4(ONE, 1, 128, ONE, ONE, w, down, ONE, tokens, top_k, None, None, 0) == code
+        assert (lib.qm_gemm_experts_workspace_bytes(w, tokens, top_k) > 0) == (lib.qm_moe_mlp_workspace_bytes(w, down, tokens, top_k) > 0) == (code == -7)
