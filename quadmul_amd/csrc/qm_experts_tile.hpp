@@ -235,6 +235,71 @@ __global__ __launch_bounds__(256, 2) void experts_tile_kernel(const ExpertsArgs 
         place = place2;
     }
 
+    // A bf16 row's power of two comes off its sums after the scales: rows far below 2^14 times scales far above 1 can leave float32's range on the way to a result that does not. Where a
+    // wave's sums have, it makes them once more, the power of two in front of the scales: by the same instructions, so what was finite keeps its bits, and straight from memory, as it takes
+    // scales above 2^88 (or a row that is not finite). us without and with this: the MLP of 600 tokens, 8 of 128 of 2048 x 1024, 178.9 and 179.4; a product of 300 tokens, 4 of 32, 2048 x 1024,
+    // 25.7 and 26.2; the whole loop over K a second time, which the workgroup's waves would have to agree on, 181.5 and 26.2.
+    bool back_done = T == QM_IN_F16;
+    if constexpr (T != QM_IN_F16) {
+        v16f all = total[0][0] + total[0][1];  // (not finite where one of them is not, and where the next step would not be)
+#pragma unroll
+        for (int m = 1; m < MT; ++m) all += total[m][0] + total[m][1];
+        float any = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) any += (all[i] + all[i + 1]) + (all[i + 2] + all[i + 3]);
+        const bool over = !(__builtin_fabsf(any) < __builtin_inff());
+        if (__builtin_expect(__ballot(over) != 0, 0)) {
+            back_done = true;
+            const uint16_t *x_row[MT];
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                total[m][0] = total[m][1] = v16f{};
+                x_row[m] = p.ready + (size_t)(p.shared ? slots[m * 32 + r] / p.top_k : slots[m * 32 + r]) * ready_stride(p.K);
+            }
+            for (int step = step0; step < steps; ++step) {
+                const int quad = step >> 1, odd = step & 1;
+                const auto add = [&](const int i) __attribute__((always_inline)) {
+                    const int block = quad * 4 + i * G, group = min(p.magic == 0 ? block : (int)((unsigned long long)block * p.magic >> 32), p.groups - 1);
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        const float scale = element<S>(scales, (size_t)weight(wave * 64 + 32 * t + r) * p.groups + group);
+#pragma unroll
+                        for (int m = 0; m < MT; ++m)
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) total[m][t][j] += part[m][t][j] * backs[m * 32 + 8 * (j / 4) + 4 * h + j % 4] * scale;
+                    }
+                };
+                // (pieces of a quad and units of a step as `use` has them; the last quad may end with the line)
+                uint32_t w[2][4];
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t piece = G == 1 ? 2 * odd + i / 2 : h + 2 * odd, dword = G == 1 ? 2 * h + i % 2 : i;
+                        const uint32_t from = min((uint32_t)quad * 64 + piece * 16, (uint32_t)line - 16) + dword * 4;
+                        w[t][i] = *reinterpret_cast<const uint32_t *>(weights + (size_t)weight(wave * 64 + 32 * t + r) * line + from);
+                    }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int unit = G == 1 ? 2 * h + i / 2 * 4 + i % 2 : 4 * h + i;
+                    const bool fresh = G == 1 ? i % 2 == 0 : i == 0 && (G == 2 || !odd);
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) {
+                        const h8 x = *reinterpret_cast<const h8 *>(x_row[m] + (size_t)step * 64 + unit * 8);
+#pragma unroll
+                        for (int t = 0; t < 2; ++t) {
+                            if (fresh) part[m][t] = v16f{};
+                            part[m][t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, Weights::of(w[t][i]), part[m][t], 0, 0, 0);
+                        }
+                    }
+                    if (G == 1 && i % 2 == 1 && (i == 1 || step * 64 + 32 < p.K)) add(2 * odd + i / 2);
+                }
+                if (G == 2) add(odd);
+                if (G == 4 && (odd || step + 1 == steps)) add(0);
+            }
+        }
+    }
+
     // ---- out ----
     const int n = n0 + (PAIRS ? wave * 32 + r : wave * 64 + r);
 #pragma unroll
@@ -243,7 +308,7 @@ __global__ __launch_bounds__(256, 2) void experts_tile_kernel(const ExpertsArgs 
         for (int i = 0; i < 16; ++i) {
             const int row = m * 32 + 8 * (i / 4) + 4 * h + i % 4;
             if (row >= rows) continue;
-            const float back = T == QM_IN_F16 ? 1.0f : backs[row];
+            const float back = back_done ? 1.0f : backs[row];
             if constexpr (PAIRS) {
                 // (ready for the second product, with zeros to the end of its last step)
                 const int stride = p.pairs_out ? ready_stride(columns) : columns;

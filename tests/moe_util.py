@@ -73,8 +73,33 @@ def spread(s, group, k, dtype):
     return 272.0 * s.double().repeat_interleave(group, dim=-1)[..., :k] if dtype == torch.bfloat16 else 0.0 * s.double().repeat_interleave(group, dim=-1)[..., :k]
 
 
-def check_product(x, chosen, q, s, group, bias, y):
-    """y [tokens, top_k, n] of gemm_experts against 64 bits; x [tokens, k] or [tokens, top_k, k]."""
+def near_product(x, q, s, group, dtype, tiles):
+    """x [rows, k] float64 times w = q * s of one expert, and how far the kernels' sums may be off, for checks that would see one wrong scale among hundreds.
+
+    A product of 16 bits and four is exact in float32. The sum over a part of a group (the largest common divisor of its size and 128) has a rounding of half a unit to each
+    product, of a partial sum that is no larger than the sum of sizes; such errors of all parts are independent: 6 standard deviations. Parts times their scales are added up one
+    after the other, over waves and runs of K: a rounding to each. Few rows of bf16 use 136 + q, and take 136 sum(x) off: as many roundings again, of sums that are that much larger. Many
+    rows of bf16 (``tiles``) are float16 numbers under a power of two of their row: each element off by 2^-39 of the row's largest at most."""
+    s = s.double()
+    k, part = x.shape[1], math.gcd(group, 128)
+    shift = 136.0 if dtype == torch.bfloat16 and not tiles else 0.0
+    want, size = torch.zeros(x.shape[0], q.shape[0], dtype=torch.float64, device=x.device), 0.0
+    variance = torch.zeros_like(want)
+    for c in range(0, k, part):
+        a, w = x[:, c:c + part], q[:, c:c + part].double()
+        scale = s[:, c // group].abs()
+        part_size = a.abs() @ w.abs().T * scale
+        want += a @ w.T * s[:, c // group]
+        size = size + part_size
+        variance += 2.0 * part * (part_size + shift * a.abs().sum(dim=1)[:, None] * scale) ** 2
+    off = 6.0 * 2.0 ** -24 * (variance.sqrt() + math.sqrt(k // part + 32) * size)
+    if dtype == torch.bfloat16 and tiles:
+        off = off + 2.0 ** -39 * x.abs().amax(dim=1)[:, None] * (q.double().abs() * s.repeat_interleave(group, dim=-1)[:, :k].abs()).sum(dim=1) if k else off
+    return want, off
+
+
+def check_product(x, chosen, q, s, group, bias, y, near=False):
+    """y [tokens, top_k, n] of gemm_experts against 64 bits; x [tokens, k] or [tokens, top_k, k]. ``near``: within near_product's bounds."""
     rows = (x if x.dim() == 3 else x[:, None].expand(-1, chosen.shape[1], -1)).flatten(0, 1).double()
     which, got = chosen.flatten(), y.flatten(0, 1).double()
     assert y.dtype == x.dtype and y.shape == (*chosen.shape, q.shape[1])
@@ -82,7 +107,10 @@ def check_product(x, chosen, q, s, group, bias, y):
     assert not got[none].any()
     for e in torch.unique(which[~none]).tolist():
         mine = which == e
-        want, off = product(rows[mine], values(q[e], s[e], group), spread(s[e], group, q.shape[2], x.dtype))
+        if near:  # (a mean of 32 rows and more is always in tiles)
+            want, off = near_product(rows[mine], q[e], s[e], group, x.dtype, which.numel() >= 32 * q.shape[0])
+        else:
+            want, off = product(rows[mine], values(q[e], s[e], group), spread(s[e], group, q.shape[2], x.dtype))
         if bias is not None:
             want, off = want + bias[e].double(), off + 2.0 ** -24 * bias[e].double().abs()
         bound = off + UNIT[x.dtype] * (want.abs() + off) + TINY[x.dtype]
@@ -90,7 +118,7 @@ def check_product(x, chosen, q, s, group, bias, y):
         assert bool((bad <= 0).all()), (e, float(bad.max()))
 
 
-def check_mlp(x, chosen, weights, q_up, s_up, q_down, s_down, group, y):
+def check_mlp(x, chosen, weights, q_up, s_up, q_down, s_down, group, y, near=False):
     """y of mlp against 64 bits. What the gates are off by, the rounding of h (independent errors of at most half a step, 6 standard deviations), the sums in
     float32, one rounding at the end."""
     unit, tiny, xs, inner = UNIT[x.dtype], TINY[x.dtype], x.double(), q_down.shape[2]
@@ -104,14 +132,21 @@ def check_mlp(x, chosen, weights, q_up, s_up, q_down, s_down, group, y):
             if not who.any():
                 continue
             share = weights[who, j].double()[:, None]
-            a, da = product(xs[who], values(q_up[e], s_up[e], group), spread(s_up[e], group, q_up.shape[2], x.dtype))
+            tiles = chosen.numel() >= 32 * q_up.shape[0]
+            if near:
+                a, da = near_product(xs[who], q_up[e], s_up[e], group, x.dtype, tiles)
+            else:
+                a, da = product(xs[who], values(q_up[e], s_up[e], group), spread(s_up[e], group, q_up.shape[2], x.dtype))
             gate, value, dg, dv = a[:, :inner], a[:, inner:], da[:, :inner], da[:, inner:]
             silu = gate * torch.sigmoid(gate)
             h = silu * value
             # (|silu'| is below 1.1; exp and the division in float32: (|gate| + 8) units)
             dh = 1.1 * value.abs() * dg + silu.abs() * dv + 1.1 * dg * dv + (gate.abs() + 8.0) * 2.0 ** -23 * h.abs()
             w = values(q_down[e], s_down[e], group)
-            part, dpart = product(h, w, spread(s_down[e], group, inner, x.dtype))
+            if near:
+                part, dpart = near_product(h, q_down[e], s_down[e], group, x.dtype, tiles)
+            else:
+                part, dpart = product(h, w, spread(s_down[e], group, inner, x.dtype))
             want[who] += share * part
             off[who] += share.abs() * (dpart + (dh + tiny) @ w.abs().T) + chosen.shape[1] * 2.0 ** -24 * (share * part).abs()
             variance[who] += share ** 2 * (((unit * (h.abs() + dh)) ** 2) @ (w ** 2).T)

@@ -1,0 +1,58 @@
+"""Products with experts' weights and their gated MLP at sizes far from one: activations, scales and weights of the choices of which some step on the way could leave float32's range
+though the result does not, for few rows to an expert and for many."""
+import math
+
+import pytest
+import torch
+
+import moe_util
+from quadmul_amd import moe
+
+pytestmark = pytest.mark.gpu
+
+TOKENS = [1, 5, 70, 300]
+
+
+@pytest.mark.parametrize("tokens", TOKENS)
+@pytest.mark.parametrize("k,group", [(96, 32), (256, 64), (416, 128), (2304, 128), (66, 64)])
+@pytest.mark.parametrize("down,up", [(-100, 115), (-126, 120), (-60, 126), (100, -120)])
+def test_small_rows_and_large_scales(down, up, k, group, tokens):
+    """bf16 rows of about 2^down (every third one no larger than ordinary ones), float32 scales of about 2^(up - 4)."""
+    x, chosen, q, s = moe_util.problem(tokens, 2, 3, 40, k, group, torch.bfloat16, torch.float32, 31)
+    x = torch.ldexp(x.float(), torch.where(torch.arange(tokens, device="cuda") % 3 == 2, min(down, 0), down)[:, None]).to(torch.bfloat16)
+    s = (s.double() * 2.0 ** (up - 4 + math.floor(math.log2(math.sqrt(k) * 4.0)))).float()
+    y = moe.gemm_experts(x, chosen, moe_util.pack(q), s, group)
+    assert bool(y.isfinite().all())
+    moe_util.check_product(x, chosen, q, s, group, None, y, near=True)
+
+
+@pytest.mark.parametrize("tokens", [70, 300])
+def test_a_row_keeps_its_bits_beside_one_that_is_summed_again(tokens):
+    """Rows of a tile in which another one's sums pass float32's range before the row's power of two comes off."""
+    x, chosen, q, s = moe_util.problem(tokens, 1, 2, 300, 640, 64, torch.bfloat16, torch.float32, 32)
+    s[:, :, 3] *= 2.0 ** 115
+    q[:, :, 192:256] = torch.where(q[:, :, 192:256] == 0, 1, q[:, :, 192:256])
+    x[:, 192:256] = 0.0
+    first = moe.gemm_experts(x, chosen, moe_util.pack(q), s, 64)
+    small = torch.arange(tokens, device="cuda") % 5 == 1
+    other = x.clone()
+    other[small, 192:256] = 2.0 ** -100
+    other[small, :192] *= 2.0 ** -90
+    other[small, 256:] *= 2.0 ** -90
+    again = moe.gemm_experts(other, chosen, moe_util.pack(q), s, 64)
+    assert torch.equal(first[~small], again[~small]) and bool(again.isfinite().all())
+    moe_util.check_product(other, chosen, q, s, 64, None, again, near=True)
+
+
+@pytest.mark.parametrize("tokens", TOKENS)
+@pytest.mark.parametrize("hidden,inner,group", [(256, 96, 32), (384, 128, 128), (384, 2176, 64), (34, 6, 32)])
+@pytest.mark.parametrize("rows,up,down", [(-100, 100, 0), (0, -30, 115), (0, 0, -40)])
+def test_an_mlp_of_small_values_and_large_scales(rows, up, down, hidden, inner, group, tokens):
+    """bf16 rows of about 2^rows, float32 scales of the first matrix 2^up and of the second 2^down times the usual ones."""
+    x, chosen, q_up, s_up = moe_util.problem(tokens, 2, 3, 2 * inner, hidden, group, torch.bfloat16, torch.float32, 33)
+    _, _, q_down, s_down = moe_util.problem(1, 1, 3, hidden, inner, group, torch.bfloat16, torch.float32, 34)
+    x, s_up, s_down = ((t.double() * 2.0 ** by).to(t.dtype) for t, by in ((x, rows), (s_up, up), (s_down, down)))
+    weights = torch.rand(tokens, 2, generator=torch.Generator().manual_seed(35)).cuda()
+    y = moe.mlp(x, chosen, weights, moe_util.pack(q_up), s_up, moe_util.pack(q_down), s_down, group)
+    assert bool(y.isfinite().all())
+    moe_util.check_mlp(x, chosen, weights, q_up, s_up, q_down, s_down, group, y, near=True)
