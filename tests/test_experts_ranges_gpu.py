@@ -56,3 +56,22 @@ def test_an_mlp_of_small_values_and_large_scales(rows, up, down, hidden, inner, 
     y = moe.mlp(x, chosen, weights, moe_util.pack(q_up), s_up, moe_util.pack(q_down), s_down, group)
     assert bool(y.isfinite().all())
     moe_util.check_mlp(x, chosen, weights, q_up, s_up, q_down, s_down, group, y, near=True)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("tokens", TOKENS)
+@pytest.mark.parametrize("k,group", [(66, 32), (64, 32), (256, 128)])
+def test_the_largest_scales(k, group, tokens, dtype):
+    """Scales of which eight are no float32 any more, under small rows."""
+    x, chosen, q, s = moe_util.problem(tokens, 2, 3, 40, k, group, dtype, torch.float32, 36)
+    x, s = (x.double() * 2.0 ** (-60 if dtype == torch.bfloat16 else -14)).to(dtype), torch.full_like(s, 2.0 ** (127 if dtype == torch.bfloat16 else 10))
+    y = moe.gemm_experts(x, chosen, moe_util.pack(q), s, group)
+    assert bool(y.isfinite().all())
+    moe_util.check_product(x, chosen, q, s, group, None, y, near=True)
+    _, _, q_down, s_down = moe_util.problem(1, 1, 3, k, 20, group, dtype, torch.float32, 37)
+    s.fill_(2.0 ** (127 if dtype == torch.bfloat16 else 10))
+    x = (x.double() * (2.0 ** -70 if dtype == torch.bfloat16 else 1.0)).to(dtype)
+    weights = torch.rand(tokens, 2, generator=torch.Generator().manual_seed(38)).cuda()
+    y = moe.mlp(x, chosen, weights, moe_util.pack(q), s, moe_util.pack(q_down), s_down, group)
+    assert bool(y.isfinite().all())
+    moe_util.check_mlp(x, chosen, weights, q, s, q_down, s_down, group, y, near=True)
