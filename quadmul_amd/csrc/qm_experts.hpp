@@ -267,6 +267,7 @@ __global__ __launch_bounds__(64 * NW, (ExpertsRowsShape<G, R, C, NW, OUT>::WAVES
                 counts = (unsigned)scalars(p.chosen)[slot] < (unsigned)p.experts;
                 share = __builtin_bit_cast(float, (int)scalars(reinterpret_cast<const int *>(p.shares))[slot]);
             }
+            v4f mine[C] = {};  // SUM: of this run, which is one choice's; share times scale may be less than float32 holds, or more
             const uint8_t *const at = smem + wave * Shape::STAGE;
             uint32_t w_here = w_from, x_here = x_from;
             asm("" : "+v"(w_here), "+v"(x_here));  // (sixteen addresses that do not change would take as many registers)
@@ -301,8 +302,7 @@ __global__ __launch_bounds__(64 * NW, (ExpertsRowsShape<G, R, C, NW, OUT>::WAVES
                 }
                 // (a 16-bit one is in the lower half of its dword)
                 const auto scale_of = [&](const int t, const int i) {
-                    const float own = S == QM_IN_F32 ? __builtin_bit_cast(float, scale[t][i]) : float_of<S == QM_IN_F32 ? QM_IN_F16 : S>((uint16_t)scale[t][i]);
-                    return SUM ? own * share : own;
+                    return S == QM_IN_F32 ? __builtin_bit_cast(float, scale[t][i]) : float_of<S == QM_IN_F32 ? QM_IN_F16 : S>((uint16_t)scale[t][i]);
                 };
                 if (q == 1) {
                     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (all of the run is in registers: its place is free)
@@ -334,7 +334,13 @@ __global__ __launch_bounds__(64 * NW, (ExpertsRowsShape<G, R, C, NW, OUT>::WAVES
 #pragma unroll
                         for (int t = 0; t < C; ++t) part[t] = W::mfma(xs[g * G + i], W::of(w[t][g * G + i]), i == 0 ? start : part[t]);
 #pragma unroll
-                    for (int t = 0; t < C; ++t) total[t] += part[t] * scale_of(t, g);
+                    for (int t = 0; t < C; ++t) (SUM ? mine : total)[t] += part[t] * scale_of(t, g);
+                }
+            }
+            if constexpr (SUM) {
+                if (counts) {
+#pragma unroll
+                    for (int t = 0; t < C; ++t) total[t] += mine[t] * share;
                 }
             }
         }

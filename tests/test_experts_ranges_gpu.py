@@ -75,3 +75,17 @@ def test_the_largest_scales(k, group, tokens, dtype):
     y = moe.mlp(x, chosen, weights, moe_util.pack(q), s, moe_util.pack(q_down), s_down, group)
     assert bool(y.isfinite().all())
     moe_util.check_mlp(x, chosen, weights, q, s, q_down, s_down, group, y, near=True)
+
+
+@pytest.mark.parametrize("tokens", TOKENS)
+@pytest.mark.parametrize("hidden,inner,group", [(256, 96, 32), (384, 320, 64), (384, 128, 128), (34, 6, 32)])
+@pytest.mark.parametrize("rows,down,share", [(40, -100, -50), (-30, 100, 60)])
+def test_weights_of_the_choices_beside_scales(rows, down, share, hidden, inner, group, tokens):
+    """bf16 rows of about 2^rows; the weight of a choice times a scale of the second matrix alone is below float32's normal numbers, or above its largest."""
+    x, chosen, q_up, s_up = moe_util.problem(tokens, 2, 3, 2 * inner, hidden, group, torch.bfloat16, torch.float32, 39)
+    _, _, q_down, s_down = moe_util.problem(1, 1, 3, hidden, inner, group, torch.bfloat16, torch.float32, 40)
+    x, s_down = (x.double() * 2.0 ** rows).to(x.dtype), (s_down.double() * 2.0 ** down).float()
+    weights = ((torch.rand(tokens, 2, generator=torch.Generator().manual_seed(41)).double() + 0.5) * 2.0 ** share).float().cuda()
+    y = moe.mlp(x, chosen, weights, moe_util.pack(q_up), s_up, moe_util.pack(q_down), s_down, group)
+    assert bool(y.isfinite().all())
+    moe_util.check_mlp(x, chosen, weights, q_up, s_up, q_down, s_down, group, y, near=True)
