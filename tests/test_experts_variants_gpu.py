@@ -112,3 +112,54 @@ def test_small_elements_beside_a_large_one_that_no_weight_meets(dtype, tokens):
     x[:, ::64] = 2.0 ** 12 if dtype == torch.bfloat16 else 60000.0
     x[:, 1::2] *= 2.0 ** -8
     moe_util.check_product(x, chosen, q, s, 64, None, moe.gemm_experts(x, chosen, moe_util.pack(q), s, 64), near=True)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("tokens", [1, 6, 40, 300])
+def test_matrices_with_groups_and_scales_of_their_own(dtype, tokens):
+    """The C entry takes groups of another size, and scales of another type, for each of the two matrices."""
+    lib, code, stream = qm.library(), 1 if dtype == torch.float16 else 2, torch.cuda.current_stream().cuda_stream
+    experts, hidden, inner, top_k = 5, 384, 192, 2
+    for (g_up, s_up_type), (g_down, s_down_type) in [((128, dtype), (32, torch.float32)), ((32, torch.float32), (64, dtype)), ((384, torch.float32), (96, torch.float32))]:
+        x, chosen, q_up, s_up = moe_util.problem(tokens, top_k, experts, 2 * inner, hidden, g_up, dtype, s_up_type, 55)
+        _, _, q_down, s_down = moe_util.problem(1, 1, experts, hidden, inner, g_down, dtype, s_down_type, 56)
+        weights = torch.rand(tokens, top_k, generator=torch.Generator().manual_seed(57)).cuda()
+        w_up, w_down = moe_util.pack(q_up), moe_util.pack(q_down)
+        up = qm.ExpertWeights(w_up.data_ptr(), s_up.data_ptr(), None, 3 if s_up_type == torch.float32 else code, experts, 2 * inner, hidden, g_up)
+        down = qm.ExpertWeights(w_down.data_ptr(), s_down.data_ptr(), None, 3 if s_down_type == torch.float32 else code, experts, hidden, inner, g_down)
+        need = lib.qm_moe_mlp_workspace_bytes(ctypes.byref(up), ctypes.byref(down), tokens, top_k)
+        scratch, y = torch.empty(need, dtype=torch.uint8, device="cuda"), torch.empty(tokens, hidden, dtype=dtype, device="cuda")
+        assert lib.qm_moe_mlp_i4(x.data_ptr(), code, hidden, chosen.data_ptr(), weights.data_ptr(), ctypes.byref(up), ctypes.byref(down), y.data_ptr(), tokens, top_k, stream,
+                                 scratch.data_ptr(), need) == 0
+        # (the bounds take one size of groups: scales repeated to that of the smallest common one)
+        s_up, s_down = s_up.repeat_interleave(g_up // 32, dim=2)[..., :-(-hidden // 32)], s_down.repeat_interleave(g_down // 32, dim=2)[..., :-(-inner // 32)]
+        moe_util.check_mlp(x, chosen, weights, q_up, s_up, q_down, s_down, 32, y, near=True)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("tokens", [1, 6, 40, 300])
+def test_rows_in_another_order(dtype, tokens):
+    """A row for each choice, the choices outside the tokens; and rows that all choices of all tokens share."""
+    _, chosen, q, s = moe_util.problem(tokens, 3, 5, 90, 384, 64, dtype, dtype, 58)
+    w, each = moe_util.pack(q), torch.randn(3, tokens, 384, generator=torch.Generator().manual_seed(59)).to(dtype).cuda()
+    for x in (each.transpose(0, 1), each[:, :1].transpose(0, 1).expand(tokens, 3, 384), each[0, 0].expand(tokens, 3, 384)):
+        moe_util.check_product(x, chosen, q, s, 64, None, moe.gemm_experts(x, chosen, w, s, 64), near=True)
+
+
+@pytest.mark.parametrize("tokens", [1, 6, 300])
+def test_weights_of_the_choices_that_are_not_finite(tokens):
+    """They make their own token's row infinite or NaN and no other one's; those of choices without an expert count for nothing."""
+    x, chosen, q, s = moe_util.problem(tokens, 3, 6, 64, 256, 64, torch.bfloat16, torch.bfloat16, 60)
+    _, _, q2, s2 = moe_util.problem(1, 1, 6, 256, 32, 64, torch.bfloat16, torch.bfloat16, 61)
+    weights = torch.rand(tokens, 3, generator=torch.Generator().manual_seed(62)).cuda()
+    call = lambda c, w: moe.mlp(x, c, w, moe_util.pack(q), s, moe_util.pack(q2), s2, 64)  # noqa: E731
+    first, row = call(chosen, weights), tokens // 2
+    others = torch.arange(tokens, device="cuda") != row
+    for bad in (float("inf"), -float("inf"), float("nan")):
+        lost = weights.clone()
+        lost[row, 1] = bad
+        y = call(chosen, lost)
+        assert not y[row].isfinite().any() and torch.equal(y[others], first[others])
+        nobody = chosen.clone()
+        nobody[row, 1] = -1
+        assert call(nobody, lost).isfinite().all()
