@@ -371,9 +371,13 @@ typedef struct qm_expert_weights {
  *   y[t][j][n] = round16( sum_g scale[e][n][g] * sum_{k in g} x[t][j][k] * weight[e][n][k] + bias[e][n] ),  e = chosen[t][j]
  * and 0 where e is none of 0 .. experts - 1 (an expert on another GPU, a token of padding). x is fp16 or bf16, token_stride elements from token to
  * token and choice_stride from choice to choice (0: the same row for all of a token's choices); y [tokens, top_k, n] of its type, not overlapping x.
- * Sums are IEEE single precision, the weights take part as the integers they are; one rounding, at the end. The same expert may be
- * chosen twice by a token. tokens * top_k up to 2^31 - 64. A row of x with an infinity or a NaN has infinities or NaN in all its columns, other rows none of them; a finite element
- * of bf16 above 2^112 may make infinities or NaN of its row's sums.
+ * Sums are IEEE single precision, the products of fp16 with the weights exact; one rounding to 16 bits, at the end. The same expert may be
+ * chosen twice by a token. tokens * top_k up to 2^31 - 64. A row of x with an infinity or a NaN has infinities or NaN in all its columns, other rows none of them.
+ * bf16 comes to the matrix cores in one of two ways, by how many rows there are to an expert (32 and more in the mean: always the second), where k is a multiple of 32:
+ *   few rows     the weights take part as 136 more than they are, and 136 times the sum of x is taken off, as in qm_gemm_grouped_i4: the sum of a part of a group (128 of k at
+ *                most) is off by roundings of sums of (136 + |weight|) |x|, not of |weight| |x|, and a finite element above 2^112 may make infinities or NaN of its row
+ *   many rows    each row is made float16 by a power of two that brings its largest element to 2^14: elements below 2^-28 of that largest are off by up to 2^-39 of it, also where
+ *                the largest meet weights of zero; that power of two makes nothing infinite that sums in single precision hold
  *   workspace    16-byte aligned device memory of qm_gemm_experts_workspace_bytes(...) bytes, used in stream order by the kernels of this call only;
  *                QM_ERR_SCRATCH with less, and nothing is enqueued
  */
@@ -385,9 +389,11 @@ int qm_gemm_experts_i4(const void *x, int dtype, long long token_stride, long lo
  * The gated MLP of each token's experts, their outputs added up by weight:
  *   h[t][j][i] = round16( silu(a[i]) * a[inner + i] ),  a = x[t] * up[e]^T,  e = chosen[t][j];   y[t] = round16( sum_j weights[t][j] * h[t][j] * down[e]^T )
  * silu(a) = a / (1 + exp(-a)); up has n = 2 inner rows of k = hidden, down n = hidden rows of k = inner, neither a bias. Choices whose expert is none of
- * 0 .. experts - 1 add nothing, whatever their weight is. Sums, the gates and the outputs of the experts are in single precision; h is rounded to x's type, of which the second
- * product's operands are, and y once, at the end. x [tokens, hidden] fp16 or bf16, y [tokens, hidden] of its type, not overlapping x; weights [tokens, top_k]
- * float32. Workspace as for qm_gemm_experts_i4, of qm_moe_mlp_workspace_bytes(...) bytes.
+ * 0 .. experts - 1 add nothing, whatever their weight is; another choice's weight that is not finite leaves nothing finite in its token's row. Sums, the gates and the outputs of the experts are in
+ * single precision (a gate below -88.7 gives 0: its exponential is infinite there); h is rounded to x's type, of which the second product's operands are, and y once, at the end. Both
+ * products take bf16 as qm_gemm_experts_i4 does. `up` and `down` may have groups of different sizes and scales of different types. x [tokens, hidden] fp16 or bf16, y [tokens, hidden] of its type, not overlapping x; weights [tokens, top_k]
+ * float32. Workspace as for qm_gemm_experts_i4, of qm_moe_mlp_workspace_bytes(...) bytes: for each choice of a token 2 inner bytes, as many again for many rows, and 4 hidden for each part that the second
+ * product's K is cut into (1, up to 8 where there are few rows).
  */
 size_t qm_moe_mlp_workspace_bytes(const qm_expert_weights *up, const qm_expert_weights *down, int tokens, int top_k);
 int qm_moe_mlp_i4(const void *x, int dtype, long long token_stride, const int *chosen, const float *weights, const qm_expert_weights *up, const qm_expert_weights *down,

@@ -110,7 +110,7 @@ def gemm_experts(x: torch.Tensor, chosen: torch.Tensor, weight: torch.Tensor, we
     no expert.
 
     ``x`` float16 or bfloat16: [tokens, k], a row for all of a token's choices, or [tokens, top_k, k], one for each; ``chosen`` [tokens, top_k] int32;
-    ``bias`` [experts, n] of ``x``'s type. Sums are in float32 and rounded once."""
+    ``bias`` [experts, n] of ``x``'s type. Sums are in float32 and rounded once; what is lost of bf16 on the way to the matrix cores stands at ``qm_gemm_experts_i4``."""
     group_size = int(group_size)
     if _has_extension():
         return _native("gemm_experts", x, chosen, weight, weight_scale, group_size, bias)
