@@ -391,7 +391,6 @@ void gemm_scaled_op(const torch::Tensor &a, const torch::Tensor &b, torch::Tenso
     gemm_scaled(a, b, d, m, n, k, row_scale, col_scale);
 }
 
-// quantize_pack returns new tensors: the Meta form only has to give their shapes and types
 // The mixture of experts (include/qm_abi.h: qm_moe_route, qm_gemm_experts_i4, qm_moe_mlp_i4).
 int check_route(const torch::Tensor &logits, int64_t top_k, const c10::optional<torch::Tensor> &bias, int64_t groups, int64_t top_groups, int64_t group_best)
 {
@@ -511,6 +510,7 @@ torch::Tensor moe_mlp(torch::Tensor x, torch::Tensor chosen, torch::Tensor weigh
     return y;
 }
 
+// quantize_pack returns new tensors: the Meta form only has to give their shapes and types
 std::tuple<torch::Tensor, torch::Tensor> quantize_pack_meta(const torch::Tensor &x)
 {
     TORCH_CHECK(x.dim() == 2 && x.size(1) % 2 == 0, "quadmul.quantize_pack: expects a 2-D tensor with even K");

@@ -1,7 +1,5 @@
 // The kernels of experts' products on one type of activations (QM_EXPERTS_TYPE: QM_IN_F16 or QM_IN_BF16), and which of them runs.
 #include <algorithm>
-#include <cstdio>
-#include <cstdlib>
 
 #include "qm_launch.hpp"
 #include "qm_experts_tile.hpp"
