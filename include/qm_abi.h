@@ -379,7 +379,8 @@ typedef struct qm_expert_weights {
  *   many rows    each row is made float16 by a power of two that brings its largest element to 2^14: elements below 2^-28 of that largest are off by up to 2^-39 of it, also where
  *                the largest meet weights of zero; that power of two makes nothing infinite that sums in single precision hold
  *   workspace    16-byte aligned device memory of qm_gemm_experts_workspace_bytes(...) bytes, used in stream order by the kernels of this call only;
- *                QM_ERR_SCRATCH with less, and nothing is enqueued
+ *                QM_ERR_SCRATCH with less, and nothing is enqueued. The number of bytes goes by the sizes alone (the pointers of `weights` may be NULL still); 0 for sizes
+ *                that the call refuses
  */
 size_t qm_gemm_experts_workspace_bytes(const qm_expert_weights *weights, int tokens, int top_k);
 int qm_gemm_experts_i4(const void *x, int dtype, long long token_stride, long long choice_stride, const int *chosen, const qm_expert_weights *weights, void *y,

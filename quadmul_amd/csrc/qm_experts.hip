@@ -12,11 +12,15 @@
 
 namespace qm {
 
-static int check_weights(const qm_expert_weights *w, const int dtype)
+static int check_sizes(const qm_expert_weights *w, const int dtype)
 {
     if (!w) return QM_ERR_NULL;
     if (w->scale_dtype != QM_IN_F32 && w->scale_dtype != dtype) return QM_ERR_DTYPE;
-    if (w->experts < 0 || w->n < 0 || w->k < 0 || (w->k & 1) || w->group < 32 || w->group % 32 != 0) return QM_ERR_SHAPE;
+    return w->experts < 0 || w->n < 0 || w->k < 0 || (w->k & 1) || w->group < 32 || w->group % 32 != 0 ? QM_ERR_SHAPE : QM_OK;
+}
+static int check_weights(const qm_expert_weights *w, const int dtype)
+{
+    if (const int e = check_sizes(w, dtype); e != QM_OK) return e;
     if (w->experts > 0 && w->n > 0 && w->k > 0 && (!w->weight || !w->scale)) return QM_ERR_NULL;
     return ((uintptr_t)w->scale & (w->scale_dtype == QM_IN_F32 ? 3 : 1)) || ((uintptr_t)w->bias & 1) ? QM_ERR_ALIGN : QM_OK;
 }
@@ -219,7 +223,7 @@ static int check_choices(const int tokens, const int top_k, const int dtype)
 
 QM_EXPORT size_t qm_gemm_experts_workspace_bytes(const qm_expert_weights *weights, int tokens, int top_k)
 {
-    if (check_weights(weights, weights ? weights->scale_dtype : 0) != QM_OK || check_choices(tokens, top_k, QM_IN_F16) != QM_OK) return 0;
+    if (check_sizes(weights, weights ? weights->scale_dtype : 0) != QM_OK || check_choices(tokens, top_k, QM_IN_F16) != QM_OK) return 0;
     return product_plan(weights, tokens, top_k).sorted.bytes;
 }
 
@@ -257,16 +261,16 @@ QM_EXPORT int qm_gemm_experts_i4(const void *x, int dtype, long long token_strid
     return e == hipSuccess ? QM_OK : fail_launch(e);
 }
 
-static int check_mlp(const qm_expert_weights *up, const qm_expert_weights *down, const int dtype)
+static int check_mlp_sizes(const qm_expert_weights *up, const qm_expert_weights *down, const int dtype)
 {
-    if (const int e = check_weights(up, dtype); e != QM_OK) return e;
-    if (const int e = check_weights(down, dtype); e != QM_OK) return e;
+    if (const int e = check_sizes(up, dtype); e != QM_OK) return e;
+    if (const int e = check_sizes(down, dtype); e != QM_OK) return e;
     return (long long)down->k * 2 != up->n || down->n != up->k || up->experts != down->experts || up->bias || down->bias ? QM_ERR_SHAPE : QM_OK;
 }
 
 QM_EXPORT size_t qm_moe_mlp_workspace_bytes(const qm_expert_weights *up, const qm_expert_weights *down, int tokens, int top_k)
 {
-    if (!up || !down || check_mlp(up, down, up->scale_dtype == QM_IN_F32 ? down->scale_dtype : up->scale_dtype) != QM_OK || check_choices(tokens, top_k, QM_IN_F16) != QM_OK) return 0;
+    if (!up || !down || check_mlp_sizes(up, down, up->scale_dtype == QM_IN_F32 ? down->scale_dtype : up->scale_dtype) != QM_OK || check_choices(tokens, top_k, QM_IN_F16) != QM_OK) return 0;
     return mlp_plan(tokens, top_k, up, down).sorted.bytes;
 }
 
@@ -274,7 +278,9 @@ QM_EXPORT int qm_moe_mlp_i4(const void *x, int dtype, long long token_stride, co
                             void *y, int tokens, int top_k, void *stream, void *workspace, size_t workspace_bytes)
 {
     if (const int e = check_choices(tokens, top_k, dtype); e != QM_OK) return e;
-    if (const int e = check_mlp(up, down, dtype); e != QM_OK) return e;
+    if (const int e = check_weights(up, dtype); e != QM_OK) return e;
+    if (const int e = check_weights(down, dtype); e != QM_OK) return e;
+    if (const int e = check_mlp_sizes(up, down, dtype); e != QM_OK) return e;
     if (token_stride < 0) return QM_ERR_SHAPE;
     if (tokens == 0 || down->n == 0) return QM_OK;
     if (!y || !x || (top_k > 0 && (!chosen || !weights))) return QM_ERR_NULL;

@@ -108,3 +108,14 @@ def test_the_most_choices():
         assert lib.qm_gemm_experts_i4(ONE, 1, 128, 0, ONE, w, ONE, tokens, top_k, None, None, 0) == code
         assert lib.qm_moe_mlp_i4(ONE, 1, 128, ONE, ONE, w, down, ONE, tokens, top_k, None, None, 0) == code
         assert (lib.qm_gemm_experts_workspace_bytes(w, tokens, top_k) > 0) == (lib.qm_moe_mlp_workspace_bytes(w, down, tokens, top_k) > 0) == (code == -7)
+
+
+def test_workspaces_go_by_sizes_alone():
+    """A program may ask for them before its weights are anywhere."""
+    lib, nowhere = qm.library(), {"weight": None, "scale": None}
+    for tokens, top_k in ((1, 2), (40, 2), (700, 4)):
+        need = lib.qm_gemm_experts_workspace_bytes(matrices(), tokens, top_k)
+        assert need > 0 and lib.qm_gemm_experts_workspace_bytes(matrices(**nowhere), tokens, top_k) == need
+        need = lib.qm_moe_mlp_workspace_bytes(matrices(), matrices(n=128, k=128), tokens, top_k)
+        assert need > 0 and lib.qm_moe_mlp_workspace_bytes(matrices(**nowhere), matrices(n=128, k=128, **nowhere), tokens, top_k) == need
+    assert lib.qm_gemm_experts_workspace_bytes(matrices(k=127, **nowhere), 3, 2) == 0
