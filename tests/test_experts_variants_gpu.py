@@ -163,3 +163,23 @@ def test_weights_of_the_choices_that_are_not_finite(tokens):
         nobody = chosen.clone()
         nobody[row, 1] = -1
         assert call(nobody, lost).isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("tokens", [1, 3, 40, 300])
+@pytest.mark.parametrize("top_k,experts", [(2, 3), (4, 40)])
+@pytest.mark.parametrize("hidden,inner,group", [(34, 64, 32), (130, 96, 32), (96, 34, 32), (256, 34, 64), (258, 128, 128)])
+def test_one_matrix_for_the_matrix_cores_and_one_not(hidden, inner, group, top_k, experts, tokens, dtype):
+    """A hidden or an inner size that is no multiple of 32: the two products run on kernels of different kinds."""
+    gated(tokens, top_k, experts, hidden, inner, group, dtype, dtype, tokens + hidden, absent=0.2)
+
+
+@pytest.mark.parametrize("tokens", [1, 5, 60, 300])
+@pytest.mark.parametrize("up_off,down_off", [(0, 8), (8, 0)])
+def test_one_matrix_at_sixteen_bytes_and_one_not(up_off, down_off, tokens):
+    x, chosen, q_up, s_up = moe_util.problem(tokens, 2, 5, 128, 256, 64, torch.float16, torch.float16, 63)
+    _, _, q_down, s_down = moe_util.problem(1, 1, 5, 256, 64, 64, torch.float16, torch.float16, 64)
+    at = lambda t, off: torch.zeros(t.numel() + off, dtype=t.dtype, device="cuda")[off:].view(t.shape).copy_(t)  # noqa: E731
+    weights = torch.rand(tokens, 2, generator=torch.Generator().manual_seed(65)).cuda()
+    y = moe.mlp(x, chosen, weights, at(moe_util.pack(q_up), up_off), s_up, at(moe_util.pack(q_down), down_off), s_down, 64)
+    moe_util.check_mlp(x, chosen, weights, q_up, s_up, q_down, s_down, 64, y, near=True)
