@@ -89,3 +89,35 @@ def test_weights_of_the_choices_beside_scales(rows, down, share, hidden, inner, 
     y = moe.mlp(x, chosen, weights, moe_util.pack(q_up), s_up, moe_util.pack(q_down), s_down, group)
     assert bool(y.isfinite().all())
     moe_util.check_mlp(x, chosen, weights, q_up, s_up, q_down, s_down, group, y, near=True)
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("tokens", [70, 300, 1100])
+def test_bits_of_the_rows_beside_sums_made_again(tokens, group):
+    """Every fifth row's sums pass float32's range before its power of two comes off; the others meet the large scales with zeros, and keep their bits."""
+    x, chosen, q, s = moe_util.problem(tokens, 1, 1, 300, 672, group, torch.bfloat16, torch.float32, 42)
+    some = slice(group, 2 * group)  # the second group
+    s[:, :, 1] = 2.0 ** 120
+    x[:, some] = 0.0
+    first = moe.gemm_experts(x, chosen, moe_util.pack(q), s, group)
+    small = torch.arange(tokens, device="cuda") % 5 == 1
+    other = x.clone()
+    other[small] *= 2.0 ** -100
+    other[small, some] = 2.0 ** -100
+    again = moe.gemm_experts(other, chosen, moe_util.pack(q), s, group)
+    assert torch.equal(first[~small], again[~small]) and bool(again.isfinite().all())
+    moe_util.check_product(other, chosen, q, s, group, None, again, near=True)
+
+
+@pytest.mark.parametrize("tokens", TOKENS)
+@pytest.mark.parametrize("hidden,inner,group", [(256, 96, 32), (384, 320, 64), (384, 128, 128), (34, 6, 32)])
+def test_small_weights_of_the_choices_beside_small_scales(hidden, inner, group, tokens):
+    """Gates of ordinary size and large values: the weight of a choice times a scale of the second matrix is nothing in float32, the result is not."""
+    x, chosen, q_up, s_up = moe_util.problem(tokens, 2, 3, 2 * inner, hidden, group, torch.bfloat16, torch.float32, 43)
+    _, _, q_down, s_down = moe_util.problem(1, 1, 3, hidden, inner, group, torch.bfloat16, torch.float32, 44)
+    s_up[:, inner:] *= 2.0 ** 80
+    s_down *= 2.0 ** -100
+    weights = ((torch.rand(tokens, 2, generator=torch.Generator().manual_seed(45)) + 0.5) * 2.0 ** -50).cuda()
+    y = moe.mlp(x, chosen, weights, moe_util.pack(q_up), s_up, moe_util.pack(q_down), s_down, group)
+    assert bool((y != 0.0).any())
+    moe_util.check_mlp(x, chosen, weights, q_up, s_up, q_down, s_down, group, y, near=True)
