@@ -33,7 +33,7 @@ struct ExpertsReady {
     long long token, choice;  // in elements; `per` rows to a token
     int per, rows, K;
     uint16_t *to;             // [rows, K], K filled up with zeros to a multiple of 64
-    float *back;              // [rows]: what sums over a row are multiplied with; not for float16
+    float *back;              // [rows]: what sums over a row are multiplied with, negated where an element is no number or infinite; not for float16
 };
 template <int T>
 __device__ __forceinline__ void experts_ready_rows(const ExpertsReady &p, const long long first, const long long waves)
@@ -46,20 +46,22 @@ __device__ __forceinline__ void experts_ready_rows(const ExpertsReady &p, const 
         if constexpr (T == QM_IN_F16) {
             for (int u = lane; u < units; u += 64) to[u] = paired(*reinterpret_cast<const v4i_half_aligned *>(x + (size_t)u * 8));
         } else {
-            uint32_t most = 0;  // the exponent of the largest element that is a number
+            uint32_t most = 0, top = 0;  // the exponent of the largest element that is a number, and of the largest
             for (int u = lane; u < units; u += 64) {
                 const v4i v = *reinterpret_cast<const v4i_half_aligned *>(x + (size_t)u * 8);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const uint32_t low = (uint32_t)v[i] >> 7 & 0xFF, high = (uint32_t)v[i] >> 23 & 0xFF;
                     most = max(most, max(low == 255 ? 0 : low, high == 255 ? 0 : high));
+                    top = max(top, max(low, high));
                 }
             }
 #pragma unroll
             for (int d = 32; d > 0; d >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, d));
             const uint32_t up = min(268u - most, 253u);  // 2^14 over the largest, as an exponent; and back
             const float factor = __builtin_bit_cast(float, up << 23);
-            if (lane == 0) p.back[row] = __builtin_bit_cast(float, (254u - up) << 23);
+            const uint32_t lost = __ballot(top == 255) != 0 ? 1 : 0;
+            if (lane == 0) p.back[row] = __builtin_bit_cast(float, (254u - up) << 23 | lost << 31);
             for (int u = lane; u < units; u += 64) {
                 const v4i v = paired(*reinterpret_cast<const v4i_half_aligned *>(x + (size_t)u * 8));
                 v4i out;
@@ -237,7 +239,7 @@ __global__ __launch_bounds__(256, 2) void experts_tile_kernel(const ExpertsArgs 
 
     // A bf16 row's power of two comes off its sums after the scales: rows far below 2^14 times scales far above 1 can leave float32's range on the way to a result that does not. Where a
     // wave's sums have, it makes them once more, the power of two in front of the scales: by the same instructions, so what was finite keeps its bits, and straight from memory, as it takes
-    // scales above 2^88 (or a row that is not finite). us without and with this: the MLP of 600 tokens, 8 of 128 of 2048 x 1024, 178.9 and 179.4; a product of 300 tokens, 4 of 32, 2048 x 1024,
+    // scales above 2^88. us without and with this: the MLP of 600 tokens, 8 of 128 of 2048 x 1024, 178.9 and 179.4; a product of 300 tokens, 4 of 32, 2048 x 1024,
     // 25.7 and 26.2; the whole loop over K a second time, which the workgroup's waves would have to agree on, 181.5 and 26.2.
     bool back_done = T == QM_IN_F16;
     if constexpr (T != QM_IN_F16) {
@@ -247,7 +249,16 @@ __global__ __launch_bounds__(256, 2) void experts_tile_kernel(const ExpertsArgs 
         float any = 0.0f;
 #pragma unroll
         for (int i = 0; i < 16; i += 4) any += (all[i] + all[i + 1]) + (all[i + 2] + all[i + 3]);
-        const bool over = !(__builtin_fabsf(any) < __builtin_inff());
+        bool over = !(__builtin_fabsf(any) < __builtin_inff());
+        if (__builtin_expect(__ballot(over) != 0, 0)) {
+            // (rows that are not finite themselves stay so, and a padded batch may be full of them: a tenth of 4096 tokens, 2 of 8 of 4096 x 11008, 2697 us, 7216 with those summed again)
+            over = false;
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    over |= !(__builtin_fabsf(total[m][0][i]) + __builtin_fabsf(total[m][1][i]) < __builtin_inff()) && backs[m * 32 + 8 * (i / 4) + 4 * h + i % 4] > 0.0f;
+        }
         if (__builtin_expect(__ballot(over) != 0, 0)) {
             back_done = true;
             const uint16_t *x_row[MT];
@@ -266,7 +277,7 @@ __global__ __launch_bounds__(256, 2) void experts_tile_kernel(const ExpertsArgs 
 #pragma unroll
                         for (int m = 0; m < MT; ++m)
 #pragma unroll
-                            for (int j = 0; j < 16; ++j) total[m][t][j] += part[m][t][j] * backs[m * 32 + 8 * (j / 4) + 4 * h + j % 4] * scale;
+                            for (int j = 0; j < 16; ++j) total[m][t][j] += part[m][t][j] * __builtin_fabsf(backs[m * 32 + 8 * (j / 4) + 4 * h + j % 4]) * scale;
                     }
                 };
                 // (pieces of a quad and units of a step as `use` has them; the last quad may end with the line)
@@ -308,7 +319,7 @@ __global__ __launch_bounds__(256, 2) void experts_tile_kernel(const ExpertsArgs 
         for (int i = 0; i < 16; ++i) {
             const int row = m * 32 + 8 * (i / 4) + 4 * h + i % 4;
             if (row >= rows) continue;
-            const float back = back_done ? 1.0f : backs[row];
+            const float back = back_done ? 1.0f : __builtin_fabsf(backs[row]);
             if constexpr (PAIRS) {
                 // (ready for the second product, with zeros to the end of its last step)
                 const int stride = p.pairs_out ? ready_stride(columns) : columns;

@@ -121,3 +121,22 @@ def test_small_weights_of_the_choices_beside_small_scales(hidden, inner, group, 
     y = moe.mlp(x, chosen, weights, moe_util.pack(q_up), s_up, moe_util.pack(q_down), s_down, group)
     assert bool((y != 0.0).any())
     moe_util.check_mlp(x, chosen, weights, q_up, s_up, q_down, s_down, group, y, near=True)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("tokens", [70, 300, 1100])
+def test_rows_that_are_not_finite_beside_sums_made_again(tokens, bad):
+    """Padding that is no number, in tiles with and without rows whose sums leave float32's range."""
+    x, chosen, q, s = moe_util.problem(tokens, 1, 1, 300, 672, 64, torch.bfloat16, torch.float32, 46)
+    s[:, :, 1] = 2.0 ** 120
+    x[:, 64:128] = 0.0
+    number = torch.arange(tokens, device="cuda")
+    small, lost = number % 7 == 1, number % 5 == 2
+    x[small & (number > 40)] *= 2.0 ** -100
+    x[small & (number > 40), 64:128] = 2.0 ** -100
+    first = moe.gemm_experts(x, chosen, moe_util.pack(q), s, 64)
+    moe_util.check_product(x, chosen, q, s, 64, None, first, near=True)
+    other = x.clone()
+    other[lost, 100] = bad
+    again = moe.gemm_experts(other, chosen, moe_util.pack(q), s, 64)
+    assert torch.equal(first[~lost], again[~lost]) and not bool(again[lost].isfinite().any())
