@@ -85,6 +85,7 @@ struct ExpertsTileShape {
     static __host__ __device__ constexpr int across(const int columns) { return (columns + COLUMNS - 1) / COLUMNS; }
     static_assert(OUT != EXPERTS_GATED || COLUMNS % 64 == 0, "gated products go on to the end of a step of the second product, which wants zeros there");
     static_assert(X_LOADS >= 1 && W_LOADS >= 1, "every wave loads");
+    static_assert(BM <= 64, "a lane to a row");
 };
 
 template <int T, int S, int G, int MT, ExpertsOut OUT>
@@ -239,17 +240,20 @@ __global__ __launch_bounds__(256, 2) void experts_tile_kernel(const ExpertsArgs 
 
     // A bf16 row's power of two comes off its sums after the scales: rows far below 2^14 times scales far above 1 can leave float32's range on the way to a result that does not. Where a
     // wave's sums have, it makes them once more, the power of two in front of the scales: by the same instructions, so what was finite keeps its bits, and straight from memory, as it takes
-    // scales above 2^88. us without and with this: the MLP of 600 tokens, 8 of 128 of 2048 x 1024, 178.9 and 179.4; a product of 300 tokens, 4 of 32, 2048 x 1024,
-    // 25.7 and 26.2; the whole loop over K a second time, which the workgroup's waves would have to agree on, 181.5 and 26.2.
-    bool back_done = T == QM_IN_F16;
+    // scales above 2^88. us without and with this: the MLP of 600 tokens, 8 of 128 of 2048 x 1024, 174.1 and 174.0, of 2048 tokens 383 and 384; a product of 300 tokens, 4 of 32, 2048 x 1024,
+    // 25.5 and 25.9. The whole loop over K a second time, on which the workgroup's waves have to agree, cost 2 % of the first and the last.
+    const float *last = backs;  // what the sums are multiplied with on their way out
     if constexpr (T != QM_IN_F16) {
-        v16f all = total[0][0] + total[0][1];  // (not finite where one of them is not, and where the next step would not be)
+        float most[4] = {};  // (NaN if one of them is)
 #pragma unroll
-        for (int m = 1; m < MT; ++m) all += total[m][0] + total[m][1];
-        float any = 0.0f;
+        for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int i = 0; i < 16; i += 4) any += (all[i] + all[i + 1]) + (all[i + 2] + all[i + 3]);
-        bool over = !(__builtin_fabsf(any) < __builtin_inff());
+            for (int i = 0; i < 16; ++i) {
+                const float larger = __builtin_elementwise_maximum(__builtin_fabsf(total[m][0][i]), __builtin_fabsf(total[m][1][i]));
+                most[i % 4] = __builtin_elementwise_maximum(most[i % 4], larger);
+            }
+        const float largest = __builtin_elementwise_maximum(__builtin_elementwise_maximum(most[0], most[1]), __builtin_elementwise_maximum(most[2], most[3]));
+        bool over = !(largest < __builtin_inff());
         if (__builtin_expect(__ballot(over) != 0, 0)) {
             // (rows that are not finite themselves stay so, and a padded batch may be full of them: a tenth of 4096 tokens, 2 of 8 of 4096 x 11008, 2697 us, 7216 with those summed again)
             over = false;
@@ -260,7 +264,6 @@ __global__ __launch_bounds__(256, 2) void experts_tile_kernel(const ExpertsArgs 
                     over |= !(__builtin_fabsf(total[m][0][i]) + __builtin_fabsf(total[m][1][i]) < __builtin_inff()) && backs[m * 32 + 8 * (i / 4) + 4 * h + i % 4] > 0.0f;
         }
         if (__builtin_expect(__ballot(over) != 0, 0)) {
-            back_done = true;
             const uint16_t *x_row[MT];
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
@@ -308,6 +311,11 @@ __global__ __launch_bounds__(256, 2) void experts_tile_kernel(const ExpertsArgs 
                 if (G == 2) add(odd);
                 if (G == 4 && (odd || step + 1 == steps)) add(0);
             }
+            // (ones, where this wave's scales were)
+            float *const ones = reinterpret_cast<float *>(smem + Shape::S_AT + wave * 2 * Shape::SCALES * 256);
+            ones[lane] = 1.0f;
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            last = ones;
         }
     }
 
@@ -319,7 +327,7 @@ __global__ __launch_bounds__(256, 2) void experts_tile_kernel(const ExpertsArgs 
         for (int i = 0; i < 16; ++i) {
             const int row = m * 32 + 8 * (i / 4) + 4 * h + i % 4;
             if (row >= rows) continue;
-            const float back = back_done ? 1.0f : __builtin_fabsf(backs[row]);
+            const float back = T == QM_IN_F16 ? 1.0f : __builtin_fabsf(last[row]);
             if constexpr (PAIRS) {
                 // (ready for the second product, with zeros to the end of its last step)
                 const int stride = p.pairs_out ? ready_stride(columns) : columns;
