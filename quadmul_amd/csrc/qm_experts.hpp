@@ -402,13 +402,13 @@ __global__ __launch_bounds__(256) void experts_any_kernel(const ExpertsArgs p)
                     for (int j = lane; j < p.K / 2; j += 64) {
                         const float s = element<S>(p.scale, row * p.groups + 2 * j / p.group);
                         const int byte = (int8_t)b[j];
-                        const float lo = (float)((int)((uint32_t)byte << 28) >> 28), hi = (float)(byte >> 4);
-                        // (the products before the scale: eight times a scale can be more than float32 holds where eight times x's is not)
+                        // Sixteenths of the weights, taken back at the end: eight times a large element, or eight times a large scale, can be more than float32 holds, though the result is not
+                        const float lo = (float)((int)((uint32_t)byte << 28) >> 28) * 0.0625f, hi = (float)(byte >> 4) * 0.0625f;
                         v = __builtin_fmaf(__builtin_fmaf(float_of<T>(x[2 * j + 1]), hi, float_of<T>(x[2 * j]) * lo), s, v);
                     }
 #pragma unroll
                     for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
-                    sum[half] = v;
+                    sum[half] = v * 16.0f;
                 }
             }
             if (lane != 0) continue;

@@ -140,3 +140,14 @@ def test_rows_that_are_not_finite_beside_sums_made_again(tokens, bad):
     other[lost, 100] = bad
     again = moe.gemm_experts(other, chosen, moe_util.pack(q), s, 64)
     assert torch.equal(first[~lost], again[~lost]) and not bool(again[lost].isfinite().any())
+
+
+@pytest.mark.parametrize("tokens,k,group", [(1, 66, 32), (5, 66, 64), (300, 66, 32), (300, 96, 32), (300, 256, 128)])
+@pytest.mark.parametrize("power,up", [(126, -30), (127, -126)])
+def test_the_largest_elements(power, up, k, group, tokens):
+    """bf16 elements of which eight are no float32 any more, under small scales, where the weights take part as they are."""
+    x, chosen, q, s = moe_util.problem(tokens, 2, 3, 40, k, group, torch.bfloat16, torch.float32, 47)
+    x, s = (torch.sign(x.double()) * 2.0 ** power).to(torch.bfloat16), torch.full_like(s, 2.0 ** up)
+    y = moe.gemm_experts(x, chosen, moe_util.pack(q), s, group)
+    assert bool(y.isfinite().all())
+    moe_util.check_product(x, chosen, q, s, group, None, y, near=True)
